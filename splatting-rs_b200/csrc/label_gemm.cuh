@@ -1,0 +1,432 @@
+// The tensor-core pipeline of the label head: D = A B^T over bf16 operands in tiles of 128 x 128
+// per thread block, f32 accumulators in tensor memory, and three endings for a tile:
+//   kStats   the logits' running maximum and sum of exponentials per row (and the target's logit)
+//   kSlopes  the softmax slopes c g (p - [target]), written as bf16 parts
+//   kOut     the tile itself: an output gradient, or a partial sum of one
+//
+// A block is one producer warp (tiled bulk copies into a ring of shared-memory stages), one warp
+// that issues the products, and eight warps that empty one accumulator while the other fills.
+#pragma once
+
+#include "elements.cuh"
+#include "kernels.h"
+#include "tcgen05.cuh"
+
+namespace splat {
+namespace label {
+
+constexpr int kTile = 128;     // rows of A, and of B, per block
+constexpr int kBlockK = 64;    // 128 bytes of bf16
+constexpr int kStages = 6;
+constexpr uint32_t kOperandBytes = kTile * kBlockK * 2;
+constexpr uint32_t kBoxBytes = kOperandBytes / 2;  // a box is 64 x 64 elements
+constexpr int kGemmThreads = 384;
+constexpr int kEpilogueWarps = 8;
+constexpr size_t kGemmSmem = 1024 + (size_t)kStages * 2 * kOperandBytes + 256;
+
+// f32 operands: three bf16 parts each, the six products of parts whose weights sum to 2^-16 or
+// more of the whole, smallest first so that they are added while the sum is small. One hex digit
+// per product, the first in the low one.
+constexpr uint32_t kParts = 3, kPartProducts = 6;
+constexpr uint32_t kPartsOfA = 0x001012, kPartsOfB = 0x010210;
+
+// The rows that have a target, in order: row_of[i] is the i-th one's row. Where `packed`, the
+// features were copied to the workspace in that order; else every row counts and they are read
+// in place.
+struct RowSet {
+    uint32_t count;
+    uint32_t packed;
+    uint32_t status;  // SP_ERR_* raised on the device, kept until it is read
+    uint32_t ticket;  // of the loss sum's blocks
+};
+
+enum Ending { kStats = 0, kSlopes = 1, kOut = 2 };
+
+struct GemmArgs {
+    RowSet* rows;
+    const uint32_t* row_of;
+    uint64_t labels;
+    uint32_t products;     // 1, or kPartProducts
+    uint32_t k_blocks;     // of the inner dimension; kOut with rows_inner: follows the row count
+    uint32_t m_tiles;      // kOut only: where the outer dimension is not the rows
+    uint32_t n_tiles;
+    uint32_t splits;       // kStats, kSlopes: of the label tiles; kOut: of the inner dimension
+    uint32_t first_row, chunk_rows;  // kSlopes, kOut: the rows of this call's slopes
+    uint32_t rows_inner;   // kOut: the inner dimension is the rows (the weight's gradient)
+    float scale, scale2;   // the logits' scale, and times log2(e)
+    const void* targets;
+    int wide;
+    // kStats
+    float2* partials;      // [2 * splits][partial_rows]: maximum and sum
+    uint32_t* partial_labels;  // the maximum's label, or NULL
+    uint64_t partial_rows;
+    float* target_logits;
+    // kSlopes
+    const float* log_normalizers;
+    const float* row_gradient;
+    bf16* slopes;          // [parts][chunk_rows][slope_stride]
+    uint64_t slope_stride;
+    // kOut
+    void* out;             // the gradient itself, or f32 partial sums [splits][out_rows][out_stride]
+    int64_t out_stride;
+    uint64_t out_rows;
+    uint32_t out_columns;
+    int partial;           // out holds partial sums
+    int add;               // ... and this call adds to them
+    int scatter;           // output row i is row_of[first_row + i]
+    int out_packed;        // 16-byte stores are aligned
+};
+
+struct Work {
+    uint32_t m, n0, n1, k0, k1, split;
+};
+
+template <int ENDING>
+struct Schedule {
+    uint32_t items, m_tiles, k_blocks;
+    __device__ Schedule(const GemmArgs& a, uint32_t count) {
+        const uint32_t here = count > a.first_row ? min(count - a.first_row, a.chunk_rows) : 0;
+        k_blocks = a.k_blocks;
+        m_tiles = (here + kTile - 1) / kTile;
+        if (ENDING == kOut && a.rows_inner) {
+            k_blocks = (here + kBlockK - 1) / kBlockK;
+            m_tiles = a.m_tiles;
+        }
+        items = m_tiles * a.splits * (ENDING == kOut ? a.n_tiles : 1);
+    }
+    __device__ Work at(const GemmArgs& a, uint32_t item) const {
+        Work w;
+        w.m = item % m_tiles;
+        uint32_t rest = item / m_tiles;
+        if (ENDING == kOut) {
+            w.n0 = rest % a.n_tiles;
+            w.n1 = w.n0 + 1;
+            w.split = rest / a.n_tiles;
+            w.k0 = (uint32_t)((uint64_t)k_blocks * w.split / a.splits);
+            w.k1 = (uint32_t)((uint64_t)k_blocks * (w.split + 1) / a.splits);
+        } else {
+            w.split = rest;
+            w.n0 = (uint32_t)((uint64_t)a.n_tiles * rest / a.splits);
+            w.n1 = (uint32_t)((uint64_t)a.n_tiles * (rest + 1) / a.splits);
+            w.k0 = 0;
+            w.k1 = k_blocks;
+        }
+        return w;
+    }
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A row's running softmax: the largest logit so far (unscaled), its label, the sum of
+// exp2((z - largest) scale2), and the target's logit once it came past.
+struct RowStats {
+    float largest, sum, target_logit;
+    uint32_t label;
+};
+
+// 32 more logits of a row, labels first..first + 31 (those from `labels` on are absent).
+template <bool LABEL>
+__device__ __forceinline__ void add_logits(RowStats& s, float (&v)[32], uint64_t first, uint64_t labels, float scale2,
+                                           int64_t target) {
+    if (first + 32 > labels) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (first + j >= labels) v[j] = -INFINITY;
+    }
+    float m4[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int j = 4; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], v[j]);
+    const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+    if (m > s.largest) {
+        // exp2(-inf) = 0 clears the sum of a first chunk.
+        s.sum *= exp2_fast((s.largest - m) * scale2);
+        s.largest = m;
+        if (LABEL) {
+#pragma unroll
+            for (int j = 31; j >= 0; --j)
+                if (v[j] == m) s.label = (uint32_t)(first + j);
+        }
+    }
+    const float shift = s.largest == -INFINITY ? 0.0f : -s.largest * scale2;
+    float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < 32; ++j) t[j & 3] += exp2_fast(fmaf(v[j], scale2, shift));
+    s.sum += (t[0] + t[1]) + (t[2] + t[3]);
+    const uint64_t at = (uint64_t)(target - (int64_t)first);
+    if (__any_sync(0xffffffffu, at < 32)) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (at == (uint64_t)j) s.target_logit = v[j];
+    }
+}
+
+// The slopes of 32 logits of a row, in place.
+__device__ __forceinline__ void to_slopes(float (&v)[32], uint64_t first, uint64_t labels, float scale2, float shift,
+                                          float weight, int64_t target) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = exp2_fast(fmaf(v[j], scale2, shift));
+    const uint64_t at = (uint64_t)(target - (int64_t)first);
+    if (__any_sync(0xffffffffu, at < 32)) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (at == (uint64_t)j) v[j] -= 1.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] *= weight;
+    if (first + 32 > labels) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (first + j >= labels) v[j] = 0.0f;
+    }
+}
+
+// 32 values as bf16; what the rounding left stays in v for the next part.
+__device__ __forceinline__ void store_part(bf16* to, float (&v)[32], bool more) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        Pack<bf16, 8> o;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            o.v[j] = __float2bfloat16_rn(v[q * 8 + j]);
+            if (more) v[q * 8 + j] -= __bfloat162float(o.v[j]);
+        }
+        *reinterpret_cast<Pack<bf16, 8>*>(to + q * 8) = o;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_out(T* to, const float (&v)[32], uint32_t columns, bool packed) {
+    constexpr int N = 16 / sizeof(T);
+    if (packed && columns >= 32) {
+#pragma unroll
+        for (int q = 0; q < 32 / N; ++q) {
+            Pack<T, N> o;
+#pragma unroll
+            for (int j = 0; j < N; ++j) o.v[j] = from_float<T>(v[q * N + j]);
+            *reinterpret_cast<Pack<T, N>*>(to + q * N) = o;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if ((uint32_t)j < columns) to[j] = from_float<T>(v[j]);
+    }
+}
+
+template <int ENDING, bool A_TRANSPOSED, bool B_TRANSPOSED, typename T>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+    k_label_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_packed,
+                 const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_b_packed,
+                 const __grid_constant__ GemmArgs a) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem = (tc::smem_address(smem_raw) + 1023u) & ~1023u;
+    const uint32_t barriers = smem + kStages * 2 * kOperandBytes;
+    const uint32_t full = barriers, empty = full + 8 * kStages, done = empty + 8 * kStages, drained = done + 16;
+    const uint32_t tmem_slot = drained + 16;
+    uint8_t* generic_base = smem_raw + (smem - tc::smem_address(smem_raw));
+    const uint32_t warp = threadIdx.x / 32, lane = lane_id();
+
+    if (warp == 0 && lane == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            tc::barrier_init(full + 8 * s, 1);
+            tc::barrier_init(empty + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            tc::barrier_init(done + 8 * b, 1);
+            tc::barrier_init(drained + 8 * b, kEpilogueWarps);
+        }
+        tc::barrier_init_fence();
+    }
+    if (warp == 2) tc::tmem_alloc<false>(tmem_slot, 2 * kTile);
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = *reinterpret_cast<uint32_t*>(generic_base + (tmem_slot - smem));
+    chain_enter();
+
+    const uint32_t count = a.rows->count;
+    const bool packed = a.rows->packed != 0;
+    const Schedule<ENDING> schedule(a, count);
+    bool ok = true;
+
+    if (warp == 0) {
+        if (tc::elect_one()) {
+            const CUtensorMap* pa = packed ? &map_a_packed : &map_a;
+            const CUtensorMap* pb = packed ? &map_b_packed : &map_b;
+            uint32_t stage = 0, phase = 0;
+            // The rows' operand of kOut starts at the chunk's first row in the features, at 0 in the slopes.
+            const int a_rows = ENDING == kOut ? 0 : (int)a.first_row;
+            const int b_rows = ENDING == kOut && B_TRANSPOSED && a.rows_inner ? (int)a.first_row : 0;
+            for (uint32_t item = blockIdx.x; ok && item < schedule.items; item += gridDim.x) {
+                const Work w = schedule.at(a, item);
+                for (uint32_t n = w.n0; ok && n < w.n1; ++n)
+                    for (uint32_t p = 0; ok && p < a.products; ++p) {
+                        const int za = a.products == 1 ? 0 : (int)((kPartsOfA >> (4 * p)) & 15u);
+                        const int zb = a.products == 1 ? 0 : (int)((kPartsOfB >> (4 * p)) & 15u);
+                        for (uint32_t k = w.k0; k < w.k1; ++k) {
+                            if (!(ok = tc::barrier_wait(empty + 8 * stage, phase ^ 1))) break;
+                            const uint32_t bar = full + 8 * stage, to = smem + stage * 2 * kOperandBytes;
+                            tc::barrier_expect(bar, 2 * kOperandBytes);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const int am = (int)w.m * kTile + h * 64, bn = (int)n * kTile + h * 64;
+                                const int kk = (int)k * kBlockK;
+                                if (A_TRANSPOSED) tc::load_box<false>(to + h * kBoxBytes, pa, bar, am, a_rows + kk, za);
+                                else tc::load_box<false>(to + h * kBoxBytes, pa, bar, kk, a_rows + am, za);
+                                if (B_TRANSPOSED)
+                                    tc::load_box<false>(to + kOperandBytes + h * kBoxBytes, pb, bar, bn, b_rows + kk, zb);
+                                else
+                                    tc::load_box<false>(to + kOperandBytes + h * kBoxBytes, pb, bar, kk, bn, zb);
+                            }
+                            if (++stage == kStages) stage = 0, phase ^= 1;
+                        }
+                    }
+            }
+        }
+    } else if (warp == 1) {
+        if (tc::elect_one()) {
+            constexpr uint32_t desc = tc::instruction(kTile, kTile, A_TRANSPOSED, B_TRANSPOSED);
+            uint32_t stage = 0, phase = 0, buffer = 0, buffer_phase = 0;
+            for (uint32_t item = blockIdx.x; ok && item < schedule.items; item += gridDim.x) {
+                const Work w = schedule.at(a, item);
+                const uint32_t steps = (w.k1 - w.k0) * a.products;
+                if (steps == 0) continue;
+                for (uint32_t n = w.n0; ok && n < w.n1; ++n) {
+                    if (!(ok = tc::barrier_wait(drained + 8 * buffer, buffer_phase ^ 1))) break;
+                    tc::fence_after_sync();
+                    for (uint32_t k = 0; k < steps; ++k) {
+                        if (!(ok = tc::barrier_wait(full + 8 * stage, phase))) break;
+                        tc::fence_after_sync();
+                        const uint32_t at = smem + stage * 2 * kOperandBytes;
+#pragma unroll
+                        for (int q = 0; q < kBlockK / 16; ++q) {
+                            // 16 of K: 32 bytes along a row, or 16 rows of 128 bytes.
+                            const uint64_t da = tc::operand(at + q * (A_TRANSPOSED ? 2048 : 32), kBoxBytes);
+                            const uint64_t db = tc::operand(at + kOperandBytes + q * (B_TRANSPOSED ? 2048 : 32), kBoxBytes);
+                            tc::multiply<false>(tmem + buffer * kTile, da, db, desc, k != 0 || q != 0);
+                        }
+                        tc::commit<false>(empty + 8 * stage);
+                        if (++stage == kStages) stage = 0, phase ^= 1;
+                    }
+                    if (!ok) break;
+                    tc::commit<false>(done + 8 * buffer);
+                    if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
+                }
+            }
+        }
+    } else if (warp >= 4) {
+        // Half the tile's columns per warpgroup; thread = row.
+        const uint32_t half = (warp - 4) / 4, quarter = warp % 4;
+        const uint32_t lane_row = quarter * 32 + lane;
+        const uint32_t tmem_at = tmem + ((quarter * 32) << 16) + half * (kTile / 2);
+        uint32_t buffer = 0, buffer_phase = 0;
+        for (uint32_t item = blockIdx.x; ok && item < schedule.items; item += gridDim.x) {
+            const Work w = schedule.at(a, item);
+            const bool empty_sum = w.k0 == w.k1;
+            if (ENDING == kOut && empty_sum && a.add) continue;
+            const uint32_t row = w.m * kTile + lane_row;  // in this call's rows (or labels)
+            const uint32_t compact = a.first_row + row;
+            const bool live = compact < count;
+            RowStats stats{-INFINITY, 0.0f, 0.0f, 0u};
+            int64_t target = -1;
+            float shift = 0.0f, weight = 0.0f;
+            if (ENDING != kOut && live) {
+                const uint32_t original = a.row_of[compact];
+                if (a.targets) target = index_at(a.targets, a.wide, original, a.labels);
+                if (ENDING == kSlopes) {
+                    shift = -a.log_normalizers[original] * 1.44269504088896341f;
+                    weight = a.scale * (a.row_gradient ? a.row_gradient[original] : 1.0f / (float)count);
+                }
+            }
+            for (uint32_t n = w.n0; ok && n < w.n1; ++n) {
+                if (!empty_sum) {
+                    if (!(ok = tc::barrier_wait(done + 8 * buffer, buffer_phase))) break;
+                    tc::fence_after_sync();
+                }
+#pragma unroll
+                for (int c = 0; c < kTile / 64; ++c) {
+                    float v[32];
+                    if (empty_sum) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+                    } else {
+                        __syncwarp();
+                        tc::tmem_load32(tmem_at + buffer * kTile + c * 32, v);
+                        tc::tmem_load_wait();
+                    }
+                    const uint32_t column = n * kTile + half * (kTile / 2) + c * 32;
+                    if constexpr (ENDING == kStats) {
+                        if (a.partial_labels) add_logits<true>(stats, v, column, a.labels, a.scale2, target);
+                        else add_logits<false>(stats, v, column, a.labels, a.scale2, target);
+                    } else if constexpr (ENDING == kSlopes) {
+                        to_slopes(v, column, a.labels, a.scale2, shift, weight, target);
+                        if (!live) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+                        }
+                        bf16* to = a.slopes + (uint64_t)row * a.slope_stride + column;
+                        const uint64_t part = (uint64_t)a.chunk_rows * a.slope_stride;
+                        if (a.products == 1) {
+                            store_part(to, v, false);
+                        } else {
+#pragma unroll
+                            for (int p = 0; p < (int)kParts; ++p) store_part(to + p * part, v, p + 1 < (int)kParts);
+                        }
+                    } else {
+                        const bool inside = (a.rows_inner ? row < a.out_rows : live) && column < a.out_columns;
+                        if (inside) {
+                            const uint32_t columns = a.out_columns - column;
+                            if (a.partial) {
+                                float* to = static_cast<float*>(a.out) +
+                                            ((uint64_t)w.split * a.out_rows + row) * (uint64_t)a.out_stride + column;
+                                if (a.add) {
+#pragma unroll
+                                    for (int j = 0; j < 32; ++j)
+                                        if ((uint32_t)j < columns) v[j] += to[j];
+                                }
+                                store_out<float>(to, v, columns, true);
+                            } else {
+                                const uint64_t r = a.scatter ? a.row_of[compact] : row;
+                                store_out<T>(static_cast<T*>(a.out) + (int64_t)r * a.out_stride + column, v, columns,
+                                             a.out_packed);
+                            }
+                        }
+                    }
+                }
+                if (!empty_sum) {
+                    tc::fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) tc::barrier_arrive_cluster(drained + 8 * buffer);
+                    if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
+                }
+            }
+            if (ENDING == kStats && ok && live) {
+                const uint64_t slot = (uint64_t)(w.split * 2 + half) * a.partial_rows + row;
+                a.partials[slot] = make_float2(stats.largest, stats.sum);
+                if (a.partial_labels) a.partial_labels[slot] = stats.label;
+                // The target is in exactly one thread's columns.
+                const uint64_t t = (uint64_t)target;
+                if (target >= 0 && t / kTile >= w.n0 && t / kTile < w.n1 && (t % kTile) / (kTile / 2) == half)
+                    a.target_logits[row] = stats.target_logit;
+            }
+        }
+    }
+    __syncwarp();
+    if (!ok) {
+        atomicCAS(&a.rows->status, 0u, (uint32_t)SP_ERR_TIMEOUT);
+        // Copies and products issued before the wait that ran out finish meanwhile.
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == 2) {
+        tc::fence_after_sync();
+        tc::tmem_free<false>(tmem, 2 * kTile);
+    }
+}
+
+}  // namespace label
+}  // namespace splat

@@ -1,0 +1,820 @@
+// The label head (splat_labels.h): cross entropy of features against a vocabulary of label rows,
+// its gradient, and prediction, without ever storing the logits.
+//
+//   loss      z = c H W^T in tiles; per row the running maximum m and sum s of 2^((z - m) log2 e);
+//             the tiles' (m, s) are joined: log sum exp z = m + ln s, loss = that - z[target]
+//   gradient  the logits again in tiles, turned into slopes G = c g (exp(z - logsumexp) - [target])
+//             where they are made and written as bf16 parts for a chunk of rows; then
+//             dH = G W and dW = G^T H, the same tile pipeline (label_gemm.cuh)
+//   predict   the loss's pass with the maximum's label kept
+//
+// Rows without a target are left out of every product: their indices are compacted first, and
+// where there are such rows the features are copied in that order (whatever the rows left out
+// hold, NaN included, is never read by a product).
+#include <algorithm>
+#include <cstring>
+#include <new>
+
+#include "label_gemm.cuh"
+#include "objects.h"
+
+using namespace splat;
+using namespace splat::label;
+
+struct sp_label_head {
+    sp_context* ctx = nullptr;
+    uint64_t labels = 0;
+    uint32_t dim = 0;
+    sp_element element = SP_F32;
+    uint64_t max_rows = 0;
+    bool training = false;
+    uint32_t sms = 148;
+    std::vector<void*> allocations;
+    RowSet* rows = nullptr;
+    uint32_t* row_of = nullptr;
+    uint32_t* counts = nullptr;
+    bf16* packed_features = nullptr;
+    bf16* packed_weight = nullptr;
+    float2* partials = nullptr;
+    uint32_t* partial_labels = nullptr;
+    float* target_logits = nullptr;
+    double* loss_sums = nullptr;
+    bf16* slopes = nullptr;
+    float* sums = nullptr;  // partial sums of the output gradients
+
+    uint32_t parts() const { return element == SP_F32 ? kParts : 1; }
+    uint32_t products() const { return element == SP_F32 ? kPartProducts : 1; }
+    uint64_t packed_stride() const { return ((uint64_t)dim + kBlockK - 1) / kBlockK * kBlockK; }
+    uint32_t label_tiles() const { return (uint32_t)((labels + kTile - 1) / kTile); }
+    uint32_t dim_tiles() const { return (dim + kTile - 1) / kTile; }
+};
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr uint32_t kGatherRows = 64;        // rows a block compacts and copies
+constexpr uint32_t kRecountBlocks = 64;     // up to this many blocks each count all targets themselves
+constexpr uint32_t kThreadSlots = 8;        // partials per row one thread joins; more take a warp
+constexpr uint64_t kSlopeBudget = 1ull << 28;  // slope elements kept at once (512 MB)
+
+uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
+
+// ------------------------------------------------------------------ rows and operands
+
+__device__ __forceinline__ bool has_target(const void* targets, int wide, uint64_t i, uint64_t labels) {
+    return !targets || index_at(targets, wide, i, labels) >= 0;
+}
+
+__global__ void __launch_bounds__(kThreads) k_count_targets(const void* __restrict__ targets, int wide, uint64_t n,
+                                                            uint64_t labels, uint32_t* __restrict__ counts) {
+    chain_enter();
+    // One warp per kGatherRows rows.
+    const uint32_t block = blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
+    uint32_t found = 0;
+    for (uint32_t r = lane_id(); r < kGatherRows; r += 32) {
+        const uint64_t i = (uint64_t)block * kGatherRows + r;
+        found += __popc(__ballot_sync(0xffffffffu, i < n && has_target(targets, wide, i, labels)));
+    }
+    if (lane_id() == 0 && (uint64_t)block * kGatherRows < n) counts[block] = found;
+}
+
+__device__ __forceinline__ uint32_t block_sum(uint32_t v) {
+    __shared__ uint32_t warps[kThreads / 32];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if (lane_id() == 0) warps[threadIdx.x / 32] = v;
+    __syncthreads();
+    uint32_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) sum += warps[w];
+    return sum;
+}
+
+// Eight columns of a row as bf16 parts: f32 is hi + mid + lo with each part the rounding of what
+// the earlier ones left (24 bits in all), bf16 is copied.
+template <typename T>
+__device__ __forceinline__ void copy_parts(const T* from, uint32_t columns, bool vector, bf16* to, uint64_t part) {
+    float v[8];
+    if (vector && columns >= 8) {
+        constexpr int N = 16 / sizeof(T);
+#pragma unroll
+        for (int q = 0; q < 8 / N; ++q) {
+            const Pack<T, N> p = *reinterpret_cast<const Pack<T, N>*>(from + q * N);
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[q * N + j] = to_float(p.v[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (uint32_t)j < columns ? to_float(from[j]) : 0.0f;
+    }
+    constexpr int parts = sizeof(T) == 4 ? (int)kParts : 1;
+#pragma unroll
+    for (int p = 0; p < parts; ++p) {
+        Pack<bf16, 8> o;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            o.v[j] = __float2bfloat16_rn(v[j]);
+            v[j] -= __bfloat162float(o.v[j]);
+        }
+        *reinterpret_cast<Pack<bf16, 8>*>(to + p * part) = o;
+    }
+}
+
+// Compacts the rows with targets (row_of), clears the outputs of the others, and copies the
+// features where they cannot be read in place: `in_place` 0, or some rows left out.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    k_gather_rows(const void* __restrict__ targets, int wide, uint64_t n, uint64_t labels,
+                  const uint32_t* __restrict__ counts, const T* __restrict__ features, int64_t stride, uint32_t dim,
+                  int vector, int in_place, RowSet* rows, uint32_t* __restrict__ row_of, bf16* __restrict__ packed,
+                  uint64_t packed_stride, uint64_t part, float* __restrict__ losses, float* __restrict__ normalizers,
+                  T* __restrict__ gradient, int64_t gradient_stride) {
+    chain_enter();
+    __shared__ uint32_t chosen[kGatherRows];
+    __shared__ uint32_t skipped[kGatherRows];
+    __shared__ uint32_t half_count[2];
+    const uint32_t t = threadIdx.x, lane = lane_id();
+    const uint64_t first = (uint64_t)blockIdx.x * kGatherRows;
+    uint32_t before = 0, all = 0;
+    if (!targets) {
+        before = (uint32_t)first;
+        all = (uint32_t)n;
+    } else if (counts) {
+        for (uint32_t b = t; b < gridDim.x; b += kThreads) {
+            const uint32_t c = counts[b];
+            all += c;
+            if (b < blockIdx.x) before += c;
+        }
+        before = block_sum(before);
+        all = block_sum(all);
+    } else {
+        for (uint64_t i = t; i < n; i += kThreads)
+            if (has_target(targets, wide, i, labels)) {
+                ++all;
+                if (i < first) ++before;
+            }
+        before = block_sum(before);
+        all = block_sum(all);
+    }
+    if (blockIdx.x == 0 && t == 0) {
+        rows->count = all;
+        rows->packed = !in_place || all != n;
+    }
+    bool live = false;
+    uint32_t mask = 0;
+    if (t < kGatherRows) {
+        live = first + t < n && has_target(targets, wide, first + t, labels);
+        mask = __ballot_sync(0xffffffffu, live);
+        if (lane == 0) half_count[t / 32] = __popc(mask);
+    }
+    __syncthreads();
+    const uint32_t here = half_count[0] + half_count[1];
+    if (t < kGatherRows) {
+        const uint32_t below = (t >= 32 ? half_count[0] : 0) + __popc(mask & ((1u << lane) - 1u));
+        if (live) {
+            chosen[below] = t;
+            row_of[before + below] = (uint32_t)(first + t);
+        } else {
+            skipped[t - below] = t;
+            if (first + t < n) {
+                if (losses) losses[first + t] = 0.0f;
+                if (normalizers) normalizers[first + t] = 0.0f;
+            }
+        }
+    }
+    __syncthreads();
+    if (gradient) {
+        const uint32_t last = (uint32_t)min((uint64_t)kGatherRows, n - first);
+        for (uint32_t k = 0; k < last - here; ++k)
+            for (uint32_t c = t; c < dim; c += kThreads)
+                gradient[(int64_t)(first + skipped[k]) * gradient_stride + c] = from_float<T>(0.0f);
+    }
+    if (in_place && all == n) return;
+    const uint32_t packs = (uint32_t)(packed_stride / 8);
+    for (uint32_t i = t; i < here * packs; i += kThreads) {
+        const uint32_t r = i / packs, c = (i - r * packs) * 8;
+        copy_parts(features + (int64_t)(first + chosen[r]) * stride + c, c < dim ? dim - c : 0, vector,
+                   packed + (uint64_t)(before + r) * packed_stride + c, part);
+    }
+    // Zero rows up to a whole tile: the weight's gradient sums over them.
+    const uint64_t end = ((uint64_t)all + kTile - 1) / kTile * kTile;
+    for (uint64_t r = all + blockIdx.x; r < end; r += gridDim.x)
+        for (uint32_t c = t * 8; c < packed_stride; c += kThreads * 8)
+            copy_parts(features, 0, false, packed + r * packed_stride + c, part);
+}
+
+// Rows of a matrix as bf16 parts.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_pack_rows(const T* __restrict__ from, int64_t stride, uint64_t rows,
+                                                        uint32_t dim, int vector, bf16* __restrict__ to,
+                                                        uint64_t packed_stride, uint64_t part) {
+    chain_enter();
+    const uint64_t packs = packed_stride / 8;
+    for (uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x; i < rows * packs;
+         i += (uint64_t)gridDim.x * kThreads) {
+        const uint64_t r = i / packs;
+        const uint32_t c = (uint32_t)(i - r * packs) * 8;
+        copy_parts(from + (int64_t)r * stride + c, c < dim ? dim - c : 0, vector, to + r * packed_stride + c, part);
+    }
+}
+
+// ------------------------------------------------------------------ joining
+
+struct Joined {
+    float largest, sum;
+    uint32_t label;
+};
+
+__device__ __forceinline__ Joined join(Joined a, Joined b, float scale2) {
+    Joined r;
+    const bool second = b.largest > a.largest || (b.largest == a.largest && b.label < a.label);
+    r.largest = fmaxf(a.largest, b.largest);
+    r.label = second ? b.label : a.label;
+    const float top = r.largest == -INFINITY ? 0.0f : r.largest;
+    r.sum = a.sum * exp2_fast((a.largest - top) * scale2) + b.sum * exp2_fast((b.largest - top) * scale2);
+    return r;
+}
+
+// `lanes` threads (1 or 32) join a row's partials in slot order within a lane, then across lanes.
+// Prediction (labels_out) takes the maximum; the loss is ln(sum) + c (largest - z[target]), the
+// form without cancellation, and its mean is summed in double: per block, then by the last block.
+template <int LANES>
+__global__ void __launch_bounds__(kThreads)
+    k_join_rows(RowSet* rows, const uint32_t* __restrict__ row_of, const float2* __restrict__ partials,
+                const uint32_t* __restrict__ partial_labels, uint64_t partial_rows, uint32_t slots, float scale,
+                float scale2, const float* __restrict__ target_logits, uint64_t n, float* __restrict__ losses,
+                float* __restrict__ normalizers, int32_t* __restrict__ labels_out, float* __restrict__ log_probability,
+                double* __restrict__ block_sums, float* __restrict__ mean) {
+    chain_enter();
+    const uint32_t count = rows->count;
+    const bool failed = rows->status != 0;
+    const float nan = __int_as_float(0x7fffffff);
+    const uint64_t i = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) / LANES;
+    const uint32_t lane = threadIdx.x % LANES;
+    double loss = 0.0;
+    if (i < count) {
+        Joined all{-INFINITY, 0.0f, 0xffffffffu};
+        for (uint32_t s = lane; s < slots; s += LANES) {
+            const float2 p = partials[s * partial_rows + i];
+            all = join(all, Joined{p.x, p.y, partial_labels ? partial_labels[s * partial_rows + i] : 0u}, scale2);
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) {
+            Joined other;
+            other.largest = __shfl_xor_sync(0xffffffffu, all.largest, o);
+            other.sum = __shfl_xor_sync(0xffffffffu, all.sum, o);
+            other.label = __shfl_xor_sync(0xffffffffu, all.label, o);
+            all = lane & o ? join(other, all, scale2) : join(all, other, scale2);
+        }
+        if (lane == 0) {
+            const uint32_t row = row_of[i];
+            const float log_sum = logf(all.sum);
+            if (labels_out) {
+                labels_out[row] = failed ? -1 : (int32_t)all.label;
+                log_probability[row] = failed ? nan : -log_sum;
+            } else {
+                const float value = failed ? nan : fmaf(scale, all.largest - target_logits[i], log_sum);
+                losses[row] = value;
+                normalizers[row] = failed ? nan : fmaf(scale, all.largest, log_sum);
+                loss = (double)value;
+            }
+        }
+    }
+    if (labels_out) return;
+    __shared__ double shared[kThreads];
+    __shared__ bool last;
+    auto sum_shared = [&]() {
+        for (int half = kThreads / 2; half > 0; half >>= 1) {
+            __syncthreads();
+            if ((int)threadIdx.x < half) shared[threadIdx.x] += shared[threadIdx.x + half];
+        }
+        __syncthreads();
+    };
+    shared[threadIdx.x] = loss;
+    sum_shared();
+    if (threadIdx.x == 0) {
+        block_sums[blockIdx.x] = shared[0];
+        __threadfence();
+        last = atomicAdd(&rows->ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    double sum = 0.0;
+    for (uint32_t b = threadIdx.x; b < gridDim.x; b += kThreads) sum += __ldcg(block_sums + b);
+    __syncthreads();
+    shared[threadIdx.x] = sum;
+    sum_shared();
+    if (threadIdx.x == 0) {
+        *mean = failed ? nan : (float)(shared[0] / (double)max(count, 1u));
+        rows->ticket = 0;
+    }
+}
+
+// A gradient from its f32 partial sums, added in order.
+struct JoinArgs {
+    const float* sums;  // NULL: the gradient is written already
+    uint32_t splits;
+    uint64_t rows, stride;
+    int scatter;  // rows are compact rows from first_row on
+    uint32_t first_row;
+    void* out;
+    int64_t out_stride;
+    uint64_t all_rows;  // rows of the whole gradient
+};
+
+// Both gradients of a chunk; after the last chunk, NaN throughout if a device wait gave up.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_join_gradients(const RowSet* __restrict__ rows,
+                                                             const uint32_t* __restrict__ row_of, uint32_t dim,
+                                                             JoinArgs features, JoinArgs weight) {
+    chain_enter();
+    const bool failed = rows->status != 0;
+    const uint64_t thread = (uint64_t)blockIdx.x * kThreads + threadIdx.x, threads = (uint64_t)gridDim.x * kThreads;
+    const uint32_t quads = (dim + 3) / 4;
+    for (int g = 0; g < 2; ++g) {
+        const JoinArgs& a = g == 0 ? features : weight;
+        T* out = static_cast<T*>(a.out);
+        if (failed) {
+            for (uint64_t i = thread; i < a.all_rows * dim; i += threads)
+                out[(int64_t)(i / dim) * a.out_stride + i % dim] = from_float<T>(__int_as_float(0x7fffffff));
+            continue;
+        }
+        if (!a.sums) continue;
+        uint64_t live = a.rows;
+        if (a.scatter) live = rows->count > a.first_row ? min(a.rows, (uint64_t)(rows->count - a.first_row)) : 0;
+        for (uint64_t i = thread; i < live * quads; i += threads) {
+            const uint64_t r = i / quads;
+            const uint32_t c = (uint32_t)(i - r * quads) * 4;
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (uint32_t s = 0; s < a.splits; ++s) {
+                const float4 v = *reinterpret_cast<const float4*>(a.sums + (s * a.rows + r) * a.stride + c);
+                sum.x += v.x;
+                sum.y += v.y;
+                sum.z += v.z;
+                sum.w += v.w;
+            }
+            const uint64_t row = a.scatter ? row_of[a.first_row + r] : r;
+            T* to = out + (int64_t)row * a.out_stride + c;
+            const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c + j < dim) to[j] = from_float<T>(v[j]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host side
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// cuTensorMapEncodeTiled of the loaded driver (the library does not link libcuda).
+EncodeTiled encode_tiled() {
+    static const EncodeTiled function = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) !=
+                cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return function;
+}
+
+// A bf16 matrix of `parts` planes as 64 x 64 boxes in the 128-byte swizzle; elements outside read
+// as zero.
+sp_status make_map(sp_context* ctx, CUtensorMap* map, const void* base, uint64_t columns, uint64_t rows,
+                   uint64_t stride, uint32_t parts, uint64_t part) {
+    const EncodeTiled encode = encode_tiled();
+    SP_REQUIRE(ctx, encode != nullptr, SP_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    const cuuint64_t dims[3] = {columns, rows, parts};
+    const cuuint64_t strides[2] = {stride * 2, parts > 1 ? part * 2 : stride * 2};
+    const cuuint32_t box[3] = {64, 64, 1}, steps[3] = {1, 1, 1};
+    const CUresult r =
+        encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, steps,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    SP_REQUIRE(ctx, r == CUDA_SUCCESS, SP_ERR_CUDA, "cuTensorMapEncodeTiled: error " + std::to_string((int)r));
+    return SP_OK;
+}
+
+// Tiled copies need a 16-byte base and row pitch (below 2^40 bytes).
+bool in_place(const sp_label_head* h, const void* p, int64_t stride) {
+    return h->element == SP_BF16 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0 &&
+           (uint64_t)stride < (1ull << 39);
+}
+
+bool vector_rows(const sp_label_head* h, const void* p, int64_t stride) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % (16 / (int64_t)element_size(h->element)) == 0;
+}
+
+// Pieces of the label tiles (for `m_tiles` row tiles) that finish soonest: whole waves of blocks
+// times the longest piece. At most four waves of pieces where there is more than one.
+uint32_t stats_splits(uint32_t sms, uint64_t m_tiles, uint32_t n_tiles) {
+    uint32_t best = 1;
+    uint64_t best_cost = ~0ull;
+    for (uint32_t s = 1; s <= n_tiles && (s == 1 || m_tiles * s <= 4ull * sms); ++s) {
+        const uint64_t cost = ((m_tiles * s + sms - 1) / sms) * ((n_tiles + s - 1) / s);
+        if (cost < best_cost) best_cost = cost, best = s;
+    }
+    return best;
+}
+
+// The same for the inner dimension of an output gradient: its pieces go through f32 sums, so one
+// is taken only where it shortens the products by a tenth, and none shorter than 4 steps.
+uint32_t out_splits(uint32_t sms, uint64_t tiles, uint32_t k_blocks) {
+    uint32_t best = 1;
+    double best_cost = 1e300;
+    for (uint32_t s = 1; s == 1 || (tiles * s <= 2ull * sms && k_blocks >= 4 * s); ++s) {
+        const double cost = (double)((tiles * s + sms - 1) / sms) * ((k_blocks + s - 1) / s);
+        if (cost < 0.9 * best_cost) best_cost = cost, best = s;
+    }
+    return best;
+}
+
+uint64_t chunk_limit(const sp_label_head* h) {
+    const uint64_t per_row = (uint64_t)h->label_tiles() * kTile * h->parts();
+    const uint64_t rows = kSlopeBudget / per_row / kTile * kTile;
+    return std::min(std::max<uint64_t>(rows, kTile), round_up(h->max_rows, kTile));
+}
+
+uint64_t sums_stride(const sp_label_head* h) { return ((uint64_t)h->dim + 3) / 4 * 4; }
+
+template <typename T>
+sp_status allocate(sp_label_head* h, T** out, uint64_t count) {
+    void* p = nullptr;
+    SP_CUDA(h->ctx, cudaMalloc(&p, std::max<uint64_t>(count * sizeof(T), 16)));
+    h->allocations.push_back(p);
+    *out = static_cast<T*>(p);
+    return SP_OK;
+}
+
+template <int ENDING, bool A_TRANSPOSED, bool B_TRANSPOSED, typename T>
+cudaError_t run_gemm(const sp_label_head* h, uint64_t items, const CUtensorMap& a, const CUtensorMap& a_packed,
+                     const CUtensorMap& b, const CUtensorMap& b_packed, const GemmArgs& args) {
+    auto kernel = k_label_gemm<ENDING, A_TRANSPOSED, B_TRANSPOSED, T>;
+    static std::atomic<unsigned long long> configured{0};
+    const cudaError_t err = allow_smem_once(kernel, kGemmSmem, configured);
+    if (err != cudaSuccess) return err;
+    const unsigned grid = (unsigned)std::max<uint64_t>(1, std::min<uint64_t>(items, h->sms));
+    return launch_chained(kernel, grid, kGemmThreads, kGemmSmem, h->ctx->stream, a, a_packed, b, b_packed, args);
+}
+
+sp_status check_matrix(sp_context* ctx, const void* p, int64_t stride, uint32_t dim, size_t size, const char* what) {
+    SP_REQUIRE(ctx, p != nullptr, SP_ERR_INVALID, std::string("null ") + what);
+    SP_REQUIRE(ctx, reinterpret_cast<uintptr_t>(p) % size == 0, SP_ERR_INVALID, std::string("misaligned ") + what);
+    SP_REQUIRE(ctx, stride >= (int64_t)dim, SP_ERR_INVALID, std::string("row stride below dim: ") + what);
+    return SP_OK;
+}
+
+// One call's inputs: the compacted rows and the operand maps.
+struct Operands {
+    CUtensorMap features, features_packed, weight;
+    uint64_t row_capacity;
+};
+
+sp_status prepare(sp_label_head* h, const void* features, int64_t feature_stride, const void* weight,
+                  int64_t weight_stride, const void* targets, int wide, uint64_t n, float* losses, float* normalizers,
+                  void* gradient, int64_t gradient_stride, Operands* out) {
+    sp_context* ctx = h->ctx;
+    cudaStream_t st = ctx->stream;
+    const uint64_t stride = h->packed_stride(), capacity = round_up(h->max_rows, kTile);
+    const uint32_t parts = h->parts();
+    const bool features_here = in_place(h, features, feature_stride), weight_here = in_place(h, weight, weight_stride);
+    out->row_capacity = capacity;
+    SP_CHECK(make_map(ctx, &out->features_packed, h->packed_features, h->dim, capacity, stride, parts, capacity * stride));
+    if (features_here) SP_CHECK(make_map(ctx, &out->features, features, h->dim, n, feature_stride, 1, 0));
+    else out->features = out->features_packed;
+    if (weight_here) SP_CHECK(make_map(ctx, &out->weight, weight, h->dim, h->labels, weight_stride, 1, 0));
+    else SP_CHECK(make_map(ctx, &out->weight, h->packed_weight, h->dim, h->labels, stride, parts, h->labels * stride));
+
+    const unsigned blocks = grid_for(n, kGatherRows);
+    const uint32_t* counts = nullptr;
+    if (targets && blocks > kRecountBlocks) {
+        SP_CUDA(ctx, launch_chained(k_count_targets, grid_for(blocks, kThreads / 32), kThreads, 0, st, targets, wide, n,
+                                    h->labels, h->counts));
+        counts = h->counts;
+    }
+    auto gather = [&](auto* typed) {
+        using T = std::remove_pointer_t<decltype(typed)>;
+        cudaError_t err = launch_chained(k_gather_rows<T>, blocks, kThreads, 0, st, targets, wide, n, h->labels, counts,
+                                         static_cast<const T*>(features), feature_stride, h->dim,
+                                         (int)vector_rows(h, features, feature_stride), (int)features_here, h->rows,
+                                         h->row_of, h->packed_features, stride, capacity * stride, losses, normalizers,
+                                         static_cast<T*>(gradient), gradient_stride);
+        if (err == cudaSuccess && !weight_here) {
+            const uint64_t packs = h->labels * (stride / 8);
+            const unsigned grid = (unsigned)std::min<uint64_t>((packs + kThreads - 1) / kThreads, 148 * 16);
+            err = launch_chained(k_pack_rows<T>, grid, kThreads, 0, st, static_cast<const T*>(weight), weight_stride,
+                                 h->labels, h->dim, (int)vector_rows(h, weight, weight_stride), h->packed_weight,
+                                 stride, h->labels * stride);
+        }
+        return err;
+    };
+    const cudaError_t err = h->element == SP_F32 ? gather((float*)nullptr) : gather((bf16*)nullptr);
+    SP_CUDA(ctx, err);
+    return SP_OK;
+}
+
+GemmArgs common_args(const sp_label_head* h, const void* targets, int wide, float scale) {
+    GemmArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.rows = h->rows;
+    a.row_of = h->row_of;
+    a.labels = h->labels;
+    a.products = h->products();
+    a.chunk_rows = 0x80000000u;
+    a.splits = 1;
+    a.scale = scale;
+    a.scale2 = scale * 1.44269504088896341f;
+    a.targets = targets;
+    a.wide = wide;
+    return a;
+}
+
+sp_status check_call(sp_label_head* h, const void* features, int64_t feature_stride, const void* weight,
+                     int64_t weight_stride, uint64_t rows, float scale) {
+    sp_context* ctx = h->ctx;
+    const size_t size = element_size(h->element);
+    SP_REQUIRE(ctx, rows <= h->max_rows, SP_ERR_INVALID, "more rows than the label head was made for");
+    SP_REQUIRE(ctx, scale > 0.0f && scale < INFINITY, SP_ERR_INVALID, "logit_scale must be positive and finite");
+    SP_CHECK(check_matrix(ctx, weight, weight_stride, h->dim, size, "weight"));
+    if (rows > 0) SP_CHECK(check_matrix(ctx, features, feature_stride, h->dim, size, "features"));
+    return SP_OK;
+}
+
+sp_status check_targets(sp_context* ctx, const void* targets, sp_index index) {
+    SP_REQUIRE(ctx, index == SP_INDEX32 || index == SP_INDEX64, SP_ERR_INVALID, "index type");
+    SP_REQUIRE(ctx, targets != nullptr, SP_ERR_INVALID, "null targets");
+    SP_REQUIRE(ctx, reinterpret_cast<uintptr_t>(targets) % (index == SP_INDEX64 ? 8 : 4) == 0, SP_ERR_INVALID,
+               "misaligned targets");
+    return SP_OK;
+}
+
+// The pass over the logits shared by the loss and the prediction.
+sp_status run_stats(sp_label_head* h, const Operands& op, const void* targets, int wide, uint64_t n, float scale,
+                    float* mean, float* losses, float* normalizers, int32_t* labels_out, float* log_probability) {
+    sp_context* ctx = h->ctx;
+    const uint64_t m_tiles = (n + kTile - 1) / kTile;
+    GemmArgs a = common_args(h, targets, wide, scale);
+    a.k_blocks = (h->dim + kBlockK - 1) / kBlockK;
+    a.n_tiles = h->label_tiles();
+    a.splits = stats_splits(h->sms, m_tiles, a.n_tiles);
+    a.partials = h->partials;
+    a.partial_labels = labels_out ? h->partial_labels : nullptr;
+    a.partial_rows = m_tiles * kTile;
+    a.target_logits = h->target_logits;
+    SP_CUDA(ctx, (run_gemm<kStats, false, false, bf16>(h, m_tiles * a.splits, op.features, op.features_packed,
+                                                       op.weight, op.weight, a)));
+    const uint32_t slots = 2 * a.splits;
+    auto join = [&](auto kernel, uint32_t lanes) {
+        return launch_chained(kernel, grid_for(n * lanes, kThreads), kThreads, 0, ctx->stream, h->rows,
+                              static_cast<const uint32_t*>(h->row_of), static_cast<const float2*>(h->partials),
+                              static_cast<const uint32_t*>(a.partial_labels), a.partial_rows, slots, scale, a.scale2,
+                              static_cast<const float*>(h->target_logits), n, losses, normalizers, labels_out,
+                              log_probability, h->loss_sums, mean);
+    };
+    SP_CUDA(ctx, slots <= kThreadSlots ? join(k_join_rows<1>, 1) : join(k_join_rows<32>, 32));
+    return SP_OK;
+}
+
+}  // namespace
+
+// The entries catch whatever the host code may throw (a string or list that finds no memory).
+extern "C" {
+
+sp_status sp_label_head_create(sp_context* ctx, uint64_t labels, uint32_t dim, sp_element element, uint64_t max_rows,
+                               int training, sp_label_head** out) try {
+    if (!ctx || !out) return SP_ERR_INVALID;
+    *out = nullptr;
+    SP_REQUIRE(ctx, labels > 0 && labels < (1ull << 31) - 512, SP_ERR_INVALID, "labels outside [1, 2^31 - 512)");
+    SP_REQUIRE(ctx, dim > 0 && dim < (1u << 20), SP_ERR_INVALID, "dim outside [1, 2^20)");
+    SP_REQUIRE(ctx, element == SP_F32 || element == SP_BF16, SP_ERR_INVALID, "element type");
+    SP_REQUIRE(ctx, max_rows > 0 && max_rows < (1ull << 31) - 512, SP_ERR_INVALID, "max_rows outside [1, 2^31 - 512)");
+    SP_CHECK(select_device(ctx));
+    sp_label_head* h = new (std::nothrow) sp_label_head();
+    SP_REQUIRE(ctx, h != nullptr, SP_ERR_OUT_OF_MEMORY, "host memory");
+    h->ctx = ctx;
+    h->labels = labels;
+    h->dim = dim;
+    h->element = element;
+    h->max_rows = max_rows;
+    h->training = training != 0;
+    sp_status s = SP_OK;
+    auto all = [&]() -> sp_status {
+        int sms = 0;
+        SP_CUDA(ctx, cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, ctx->device));
+        h->sms = (uint32_t)std::max(sms, 1);
+        const uint64_t capacity = round_up(max_rows, kTile), stride = h->packed_stride();
+        SP_CHECK(allocate(h, &h->rows, 1));
+        SP_CUDA(ctx, cudaMemsetAsync(h->rows, 0, sizeof(RowSet), ctx->stream));
+        SP_CHECK(allocate(h, &h->row_of, max_rows));
+        SP_CHECK(allocate(h, &h->counts, (max_rows + kGatherRows - 1) / kGatherRows));
+        SP_CHECK(allocate(h, &h->packed_features, capacity * stride * h->parts()));
+        SP_CHECK(allocate(h, &h->packed_weight, labels * stride * h->parts()));
+        // stats_splits: pieces times row tiles stay within four waves, or one piece.
+        const uint64_t slots = 2 * kTile * std::max<uint64_t>(capacity / kTile, 4ull * h->sms);
+        SP_CHECK(allocate(h, &h->partials, slots));
+        SP_CHECK(allocate(h, &h->partial_labels, slots));
+        SP_CHECK(allocate(h, &h->target_logits, capacity));
+        SP_CHECK(allocate(h, &h->loss_sums, (max_rows * 32 + kThreads - 1) / kThreads));
+        if (h->training) {
+            SP_CHECK(allocate(h, &h->slopes, chunk_limit(h) * h->label_tiles() * kTile * h->parts()));
+            // out_splits: pieces times tiles stay within two waves, or one piece; one piece needs
+            // sums for the weight's gradient alone, over several chunks.
+            const uint64_t tiles = std::max<uint64_t>(2ull * h->sms, h->label_tiles());
+            SP_CHECK(allocate(h, &h->sums, tiles * kTile * sums_stride(h) * 2));
+        }
+        return SP_OK;
+    };
+    if ((s = all()) != SP_OK) {
+        sp_label_head_destroy(h);
+        return s;
+    }
+    *out = h;
+    return SP_OK;
+} catch (...) {
+    return SP_ERR_OUT_OF_MEMORY;
+}
+
+void sp_label_head_destroy(sp_label_head* h) {
+    if (!h) return;
+    cudaSetDevice(h->ctx->device);
+    cudaStreamSynchronize(h->ctx->stream);
+    for (void* p : h->allocations) cudaFree(p);
+    delete h;
+}
+
+sp_status sp_label_head_loss(sp_label_head* h, const void* d_features, int64_t feature_stride, const void* d_weight,
+                             int64_t weight_stride, const void* d_targets, sp_index index, uint64_t rows,
+                             float logit_scale, float* d_mean, float* d_losses, float* d_log_normalizers) try {
+    if (!h) return SP_ERR_INVALID;
+    sp_context* ctx = h->ctx;
+    NvtxRange range("sp_label_head_loss");
+    SP_CHECK(check_call(h, d_features, feature_stride, d_weight, weight_stride, rows, logit_scale));
+    SP_REQUIRE(ctx, d_mean != nullptr, SP_ERR_INVALID, "null mean");
+    SP_CHECK(select_device(ctx));
+    if (rows == 0) {
+        SP_CUDA(ctx, cudaMemsetAsync(d_mean, 0, sizeof(float), ctx->stream));
+        return SP_OK;
+    }
+    SP_CHECK(check_targets(ctx, d_targets, index));
+    SP_REQUIRE(ctx, d_losses != nullptr && d_log_normalizers != nullptr, SP_ERR_INVALID, "null output");
+    Operands op;
+    const int wide = index == SP_INDEX64;
+    SP_CHECK(prepare(h, d_features, feature_stride, d_weight, weight_stride, d_targets, wide, rows, d_losses,
+                     d_log_normalizers, nullptr, 0, &op));
+    return run_stats(h, op, d_targets, wide, rows, logit_scale, d_mean, d_losses, d_log_normalizers, nullptr, nullptr);
+} catch (...) {
+    return SP_ERR_OUT_OF_MEMORY;
+}
+
+sp_status sp_label_head_predict(sp_label_head* h, const void* d_features, int64_t feature_stride,
+                                const void* d_weight, int64_t weight_stride, uint64_t rows, float logit_scale,
+                                int32_t* d_labels, float* d_log_probabilities) try {
+    if (!h) return SP_ERR_INVALID;
+    sp_context* ctx = h->ctx;
+    NvtxRange range("sp_label_head_predict");
+    SP_CHECK(check_call(h, d_features, feature_stride, d_weight, weight_stride, rows, logit_scale));
+    if (rows == 0) return SP_OK;
+    SP_REQUIRE(ctx, d_labels != nullptr && d_log_probabilities != nullptr, SP_ERR_INVALID, "null output");
+    SP_CHECK(select_device(ctx));
+    Operands op;
+    SP_CHECK(prepare(h, d_features, feature_stride, d_weight, weight_stride, nullptr, 0, rows, nullptr, nullptr,
+                     nullptr, 0, &op));
+    return run_stats(h, op, nullptr, 0, rows, logit_scale, nullptr, nullptr, nullptr, d_labels, d_log_probabilities);
+} catch (...) {
+    return SP_ERR_OUT_OF_MEMORY;
+}
+
+sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64_t feature_stride,
+                                 const void* d_weight, int64_t weight_stride, const void* d_targets, sp_index index,
+                                 uint64_t rows, float logit_scale, const float* d_log_normalizers,
+                                 const float* d_row_gradient, void* d_feature_gradient,
+                                 int64_t feature_gradient_stride, void* d_weight_gradient,
+                                 int64_t weight_gradient_stride) try {
+    if (!h) return SP_ERR_INVALID;
+    sp_context* ctx = h->ctx;
+    NvtxRange range("sp_label_head_gradient");
+    const size_t size = element_size(h->element);
+    SP_REQUIRE(ctx, h->training, SP_ERR_INVALID, "the label head was not made for training");
+    SP_CHECK(check_call(h, d_features, feature_stride, d_weight, weight_stride, rows, logit_scale));
+    SP_CHECK(check_matrix(ctx, d_weight_gradient, weight_gradient_stride, h->dim, size, "weight gradient"));
+    SP_CHECK(select_device(ctx));
+    if (rows == 0) {
+        SP_CUDA(ctx, cudaMemset2DAsync(d_weight_gradient, weight_gradient_stride * size, 0, h->dim * size, h->labels,
+                                       ctx->stream));
+        return SP_OK;
+    }
+    SP_CHECK(check_targets(ctx, d_targets, index));
+    SP_REQUIRE(ctx, d_log_normalizers != nullptr, SP_ERR_INVALID, "null log normalizers");
+    SP_CHECK(check_matrix(ctx, d_feature_gradient, feature_gradient_stride, h->dim, size, "feature gradient"));
+    const int wide = index == SP_INDEX64;
+    Operands op;
+    SP_CHECK(prepare(h, d_features, feature_stride, d_weight, weight_stride, d_targets, wide, rows, nullptr, nullptr,
+                     d_feature_gradient, feature_gradient_stride, &op));
+
+    const uint64_t limit = chunk_limit(h), chunks = (rows + limit - 1) / limit;
+    const uint64_t chunk = round_up((rows + chunks - 1) / chunks, kTile);
+    const uint64_t slope_stride = (uint64_t)h->label_tiles() * kTile, sum_stride = sums_stride(h);
+    const uint64_t m_tiles = chunk / kTile;
+    CUtensorMap slopes;
+    SP_CHECK(make_map(ctx, &slopes, h->slopes, slope_stride, chunk, slope_stride, h->parts(), chunk * slope_stride));
+    const uint32_t label_k = (uint32_t)((h->labels + kBlockK - 1) / kBlockK), row_k = (uint32_t)(chunk / kBlockK);
+    const uint32_t feature_splits = out_splits(h->sms, m_tiles * h->dim_tiles(), label_k);
+    const uint32_t weight_splits = out_splits(h->sms, (uint64_t)h->label_tiles() * h->dim_tiles(), row_k);
+    const bool feature_sums = feature_splits > 1, weight_sums = weight_splits > 1 || chunks > 1;
+    float* weight_sum = h->sums;
+    float* feature_sum = h->sums + std::max<uint64_t>(2ull * h->sms, h->label_tiles()) * kTile * sum_stride;
+
+    for (uint64_t c = 0; c < chunks; ++c) {
+        GemmArgs a = common_args(h, d_targets, wide, logit_scale);
+        a.first_row = (uint32_t)(c * chunk);
+        a.chunk_rows = (uint32_t)chunk;
+        a.k_blocks = (h->dim + kBlockK - 1) / kBlockK;
+        a.n_tiles = h->label_tiles();
+        a.splits = stats_splits(h->sms, m_tiles, a.n_tiles);
+        a.log_normalizers = d_log_normalizers;
+        a.row_gradient = d_row_gradient;
+        a.slopes = h->slopes;
+        a.slope_stride = slope_stride;
+        SP_CUDA(ctx, (run_gemm<kSlopes, false, false, bf16>(h, m_tiles * a.splits, op.features, op.features_packed,
+                                                            op.weight, op.weight, a)));
+
+        GemmArgs f = a;  // dH = G W
+        f.k_blocks = label_k;
+        f.n_tiles = h->dim_tiles();
+        f.splits = feature_splits;
+        f.partial = feature_sums;
+        f.out = feature_sums ? (void*)feature_sum : d_feature_gradient;
+        f.out_stride = feature_sums ? (int64_t)sum_stride : feature_gradient_stride;
+        f.out_rows = chunk;
+        f.out_columns = h->dim;
+        f.scatter = !feature_sums;
+        f.out_packed = vector_rows(h, d_feature_gradient, feature_gradient_stride);
+        const uint64_t f_items = m_tiles * f.n_tiles * f.splits;
+        SP_CUDA(ctx, h->element == SP_F32
+                         ? (run_gemm<kOut, false, true, float>(h, f_items, slopes, slopes, op.weight, op.weight, f))
+                         : (run_gemm<kOut, false, true, bf16>(h, f_items, slopes, slopes, op.weight, op.weight, f)));
+
+        GemmArgs w = a;  // dW = G^T H
+        w.rows_inner = 1;
+        w.m_tiles = h->label_tiles();
+        w.n_tiles = h->dim_tiles();
+        w.splits = weight_splits;
+        w.partial = weight_sums;
+        w.add = c > 0;
+        w.out = weight_sums ? (void*)weight_sum : d_weight_gradient;
+        w.out_stride = weight_sums ? (int64_t)sum_stride : weight_gradient_stride;
+        w.out_rows = h->labels;
+        w.out_columns = h->dim;
+        w.out_packed = vector_rows(h, d_weight_gradient, weight_gradient_stride);
+        const uint64_t w_items = (uint64_t)w.m_tiles * w.n_tiles * w.splits;
+        SP_CUDA(ctx, h->element == SP_F32
+                         ? (run_gemm<kOut, true, true, float>(h, w_items, slopes, slopes, op.features,
+                                                              op.features_packed, w))
+                         : (run_gemm<kOut, true, true, bf16>(h, w_items, slopes, slopes, op.features,
+                                                             op.features_packed, w)));
+
+        const bool last = c + 1 == chunks;
+        JoinArgs jf{feature_sums ? feature_sum : nullptr, feature_splits, chunk, sum_stride, 1, a.first_row,
+                    d_feature_gradient, feature_gradient_stride, last ? rows : 0};
+        JoinArgs jw{weight_sums && last ? weight_sum : nullptr, weight_splits, h->labels, sum_stride, 0, 0,
+                    d_weight_gradient, weight_gradient_stride, last ? h->labels : 0};
+        if (!last && !feature_sums) continue;
+        const uint64_t quads = std::max(feature_sums ? chunk * (sum_stride / 4) : 0,
+                                        jw.sums ? h->labels * (sum_stride / 4) : (uint64_t)0);
+        const unsigned grid = (unsigned)std::min<uint64_t>(std::max<uint64_t>((quads + kThreads - 1) / kThreads, 1),
+                                                           148 * 16);
+        SP_CUDA(ctx, h->element == SP_F32
+                         ? launch_chained(k_join_gradients<float>, grid, kThreads, 0, ctx->stream,
+                                          static_cast<const RowSet*>(h->rows), static_cast<const uint32_t*>(h->row_of),
+                                          h->dim, jf, jw)
+                         : launch_chained(k_join_gradients<bf16>, grid, kThreads, 0, ctx->stream,
+                                          static_cast<const RowSet*>(h->rows), static_cast<const uint32_t*>(h->row_of),
+                                          h->dim, jf, jw));
+    }
+    return SP_OK;
+} catch (...) {
+    return SP_ERR_OUT_OF_MEMORY;
+}
+
+sp_status sp_label_head_check(sp_label_head* h) try {
+    if (!h) return SP_ERR_INVALID;
+    sp_context* ctx = h->ctx;
+    SP_CHECK(select_device(ctx));
+    uint32_t status = 0;
+    SP_CUDA(ctx, cudaMemcpyAsync(&status, &h->rows->status, sizeof(status), cudaMemcpyDeviceToHost, ctx->stream));
+    SP_CHECK(sync_stream(ctx));
+    if (status == 0) return SP_OK;
+    SP_CUDA(ctx, cudaMemsetAsync(&h->rows->status, 0, sizeof(status), ctx->stream));
+    return fail(ctx, (sp_status)status, "a device-side wait gave up (label head pipeline)");
+} catch (...) {
+    return SP_ERR_OUT_OF_MEMORY;
+}
+
+}  // extern "C"

@@ -1,0 +1,211 @@
+// The sm_100a instructions the label kernels are built from: mbarriers, tiled bulk copies into
+// shared memory, the fifth-generation tensor-core product and its accumulators in tensor memory.
+// Every wait is bounded: one that runs out returns false, and its caller raises SP_ERR_TIMEOUT
+// and leaves its loops.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace splat {
+namespace tc {
+
+__device__ __forceinline__ uint32_t smem_address(const void* p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t elected;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(elected));
+    return elected != 0;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// The address of `local` (this block's shared memory) in block `rank` of the cluster.
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t local, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
+    return r;
+}
+
+// ---- mbarriers
+
+__device__ __forceinline__ void barrier_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void barrier_init_fence() {
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+
+__device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+// Arrives on a barrier given by its address in the cluster's shared memory.
+__device__ __forceinline__ void barrier_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
+// A wait gives up after this many polls or nanoseconds, whichever comes first: far above any
+// wait of a working pipeline (microseconds).
+constexpr uint32_t kPollLimit = 1u << 26;
+constexpr unsigned long long kWaitLimitNs = 2000000000ull;
+
+__device__ __forceinline__ unsigned long long global_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
+    if (barrier_try(bar, parity)) return true;
+    const unsigned long long start = global_ns();
+    for (uint32_t polls = 1; polls < kPollLimit; ++polls) {
+        if (barrier_try(bar, parity)) return true;
+        if ((polls & 255u) == 0 && global_ns() - start > kWaitLimitNs) return false;
+    }
+    return false;
+}
+
+// ---- tiled bulk copies (TMA)
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
+// One box of a 3-D tensor at (x, y, z) into this block's shared memory. With PAIR the bytes are
+// counted on a barrier of either block of the pair (its cluster address).
+template <bool PAIR>
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+    if constexpr (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+            "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+            "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+            : "memory");
+}
+
+// ---- tensor memory
+
+template <bool PAIR>
+__device__ __forceinline__ void tmem_alloc(uint32_t smem_slot, uint32_t columns) {
+    if constexpr (PAIR)
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_slot),
+                     "r"(columns)
+                     : "memory");
+    else
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_slot),
+                     "r"(columns)
+                     : "memory");
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void tmem_free(uint32_t address, uint32_t columns) {
+    if constexpr (PAIR) {
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns));
+    } else {
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns));
+    }
+}
+
+__device__ __forceinline__ void fence_before_sync() {
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 32 consecutive columns of the calling warp's 32 lanes: thread t gets lane t's 32 words.
+__device__ __forceinline__ void tmem_load32(uint32_t address, float (&v)[32]) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(address));
+}
+__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// ---- products
+
+// Shared-memory operand descriptor: 128-byte swizzle, 8-row groups of 1024 bytes (`stride`);
+// `leading` is the distance between 64-element blocks of an operand whose rows run along K
+// (transposed operands only).
+__device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t leading_bytes) {
+    return (uint64_t)((address & 0x3FFFFu) >> 4) | ((uint64_t)(leading_bytes >> 4) << 16) |
+           ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// bf16 x bf16 products summed in f32; *_transposed: the operand's rows run along K in memory.
+__host__ __device__ constexpr uint32_t instruction(uint32_t m, uint32_t n, bool a_transposed, bool b_transposed) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((a_transposed ? 1u : 0u) << 15) | ((b_transposed ? 1u : 0u) << 16) |
+           ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void multiply(uint32_t accumulator, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+    const uint32_t enable = add ? 1u : 0u;
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(accumulator),
+            "l"(a), "l"(b), "r"(desc), "r"(enable)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(accumulator),
+            "l"(a), "l"(b), "r"(desc), "r"(enable)
+            : "memory");
+}
+
+// Arrives on the barrier (in both blocks of a pair) once every product issued so far is done.
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint32_t bar) {
+    if constexpr (PAIR)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                bar),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+                     : "memory");
+}
+
+}  // namespace tc
+}  // namespace splat

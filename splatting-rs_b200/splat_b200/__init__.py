@@ -7,6 +7,8 @@ over libsplat_b200.so, the B200-native (sm_100a) differentiable Gaussian-splatti
     PoseRefinement instantsplat-rs/src/pose_refinement.rs, camera_pose.rs
     Trainer       instantsplat-rs/src/training.rs (the caller of the path)
     densify       instantsplat-rs/src/densify.rs (on the device)
+    Embedding     codebook features by token, and their gradient (no counterpart)
+    LabelHead     cross entropy, gradient and prediction over a label vocabulary (no counterpart)
 """
 
 from ._lib import SplatError, load as load_library  # noqa: F401
@@ -21,6 +23,7 @@ from .densify import (  # noqa: F401
     densify,
 )
 from .gaussians import GaussianCloud, logit, param_stride, rgb_to_sh_dc, sigmoid  # noqa: F401
+from .labels import Embedding, LabelHead, LabelLoss  # noqa: F401
 from .optimizer import (  # noqa: F401
     Adam,
     LEARNING_RATES_3DGS,

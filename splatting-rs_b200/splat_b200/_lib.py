@@ -1,4 +1,4 @@
-"""ctypes binding of libsplat_b200.so (include/splat.h).
+"""ctypes binding of libsplat_b200.so (include/splat.h, splat_labels.h, splat_io.h).
 
 The library is the product: every call below runs the hand-written sm_100a kernels. There
 is no fallback — importing this module without the built library, or calling into it
@@ -8,7 +8,7 @@ without a CUDA device, raises.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_double, c_float, c_int, c_uint32, c_uint64, c_void_p, c_char_p
+from ctypes import POINTER, c_double, c_float, c_int, c_int64, c_uint32, c_uint64, c_void_p, c_char_p
 from pathlib import Path
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "libsplat_b200.so"
@@ -342,6 +342,22 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "sp_device_poses_step": (c_int, [_P, c_uint32, c_uint32, c_float]),
     "sp_device_poses_download": (c_int, [_P, _P]),
     "sp_train_step_device_poses": (c_int, [_P, _P, _P, c_uint32, c_uint32, c_float, _P]),
+    "sp_embedding_create": (c_int, [_P, c_uint64, c_uint32, c_int, c_uint64, POINTER(_P)]),
+    "sp_embedding_destroy": (None, [_P]),
+    "sp_embedding_lookup": (c_int, [_P, _P, c_int64, _P, c_int, c_uint64, c_float, _P, c_int64]),
+    "sp_embedding_gradient": (c_int, [_P, _P, c_int64, _P, c_int, c_uint64, c_float, _P, c_int64]),
+    "sp_embedding_check": (c_int, [_P]),
+    "sp_label_head_create": (c_int, [_P, c_uint64, c_uint32, c_int, c_uint64, c_int, POINTER(_P)]),
+    "sp_label_head_destroy": (None, [_P]),
+    "sp_label_head_loss": (
+        c_int, [_P, _P, c_int64, _P, c_int64, _P, c_int, c_uint64, c_float, _P, _P, _P]
+    ),
+    "sp_label_head_gradient": (
+        c_int,
+        [_P, _P, c_int64, _P, c_int64, _P, c_int, c_uint64, c_float, _P, _P, _P, c_int64, _P, c_int64],
+    ),
+    "sp_label_head_predict": (c_int, [_P, _P, c_int64, _P, c_int64, c_uint64, c_float, _P, _P]),
+    "sp_label_head_check": (c_int, [_P]),
     "sp_ply_write": (c_int, [c_char_p, _P, c_uint64, c_uint32, c_int]),
     "sp_ply_read_header": (c_int, [c_char_p, POINTER(c_uint64), POINTER(c_uint32)]),
     "sp_ply_read": (c_int, [c_char_p, _P, c_uint64, c_uint32, c_int]),
