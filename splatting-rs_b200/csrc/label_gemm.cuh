@@ -1,11 +1,14 @@
-// The tensor-core pipeline of the label head: D = A B^T over bf16 operands in tiles of 128 x 128
-// per thread block, f32 accumulators in tensor memory, and three endings for a tile:
+// The tensor-core pipeline of the label head: D = A B^T over bf16 operands in tiles of 256 x 256
+// per pair of thread blocks (or 128 x 128 per block), f32 accumulators in tensor memory, and three
+// endings for a tile:
 //   kStats   the logits' running maximum and sum of exponentials per row (and the target's logit)
 //   kSlopes  the softmax slopes c g (p - [target]), written as bf16 parts
 //   kOut     the tile itself: an output gradient, or a partial sum of one
 //
 // A block is one producer warp (tiled bulk copies into a ring of shared-memory stages), one warp
-// that issues the products, and eight warps that empty one accumulator while the other fills.
+// that issues the products, and eight warps that empty one accumulator while the other fills. In a
+// pair each block keeps 128 rows of A and of B and the accumulator of its A rows; the products are
+// issued by the first block and read B from both.
 #pragma once
 
 #include "elements.cuh"
@@ -16,13 +19,17 @@ namespace splat {
 namespace label {
 
 constexpr int kTile = 128;     // rows of A, and of B, per block
+constexpr int kPairTile = 2 * kTile;
 constexpr int kBlockK = 64;    // 128 bytes of bf16
 constexpr int kStages = 6;
 constexpr uint32_t kOperandBytes = kTile * kBlockK * 2;
 constexpr uint32_t kBoxBytes = kOperandBytes / 2;  // a box is 64 x 64 elements
 constexpr int kGemmThreads = 384;
 constexpr int kEpilogueWarps = 8;
-constexpr size_t kGemmSmem = 1024 + (size_t)kStages * 2 * kOperandBytes + 256;
+constexpr uint32_t kStageBytes = 2 * kOperandBytes;
+constexpr uint32_t kStoreBytes = 32 * 128;  // a warp's 32 x 64 slopes on their way out
+// 227 KB of shared memory hold six stages and the outgoing slopes.
+constexpr size_t kGemmSmem = 1024 + (size_t)kStages * kStageBytes + kEpilogueWarps * kStoreBytes + 256;
 
 // f32 operands: three bf16 parts each, the six products of parts whose weights sum to 2^-16 or
 // more of the whole, smallest first so that they are added while the sum is small. One hex digit
@@ -64,8 +71,6 @@ struct GemmArgs {
     // kSlopes
     const float* log_normalizers;
     const float* row_gradient;
-    bf16* slopes;          // [parts][chunk_rows][slope_stride]
-    uint64_t slope_stride;
     // kOut
     void* out;             // the gradient itself, or f32 partial sums [splits][out_rows][out_stride]
     int64_t out_stride;
@@ -81,13 +86,13 @@ struct Work {
     uint32_t m, n0, n1, k0, k1, split;
 };
 
-template <int ENDING>
+template <int ENDING, int TILE>
 struct Schedule {
     uint32_t items, m_tiles, k_blocks;
     __device__ Schedule(const GemmArgs& a, uint32_t count) {
         const uint32_t here = count > a.first_row ? min(count - a.first_row, a.chunk_rows) : 0;
         k_blocks = a.k_blocks;
-        m_tiles = (here + kTile - 1) / kTile;
+        m_tiles = (here + TILE - 1) / TILE;
         if (ENDING == kOut && a.rows_inner) {
             k_blocks = (here + kBlockK - 1) / kBlockK;
             m_tiles = a.m_tiles;
@@ -164,9 +169,9 @@ __device__ __forceinline__ void add_logits(RowStats& s, float (&v)[32], uint64_t
     }
 }
 
-// The slopes of 32 logits of a row, in place.
+// The slopes of 32 logits of a row, in place; zeros past the labels and in rows that do not count.
 __device__ __forceinline__ void to_slopes(float (&v)[32], uint64_t first, uint64_t labels, float scale2, float shift,
-                                          float weight, int64_t target) {
+                                          float weight, int64_t target, bool live) {
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = exp2_fast(fmaf(v[j], scale2, shift));
     const uint64_t at = (uint64_t)(target - (int64_t)first);
@@ -176,7 +181,7 @@ __device__ __forceinline__ void to_slopes(float (&v)[32], uint64_t first, uint64
             if (at == (uint64_t)j) v[j] -= 1.0f;
     }
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] *= weight;
+    for (int j = 0; j < 32; ++j) v[j] = live ? v[j] * weight : 0.0f;
     if (first + 32 > labels) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
@@ -184,17 +189,23 @@ __device__ __forceinline__ void to_slopes(float (&v)[32], uint64_t first, uint64
     }
 }
 
-// 32 values as bf16; what the rounding left stays in v for the next part.
-__device__ __forceinline__ void store_part(bf16* to, float (&v)[32], bool more) {
+// 32 values as bf16 into half a 128-byte row of the swizzled shared tile (16-byte unit u of row r
+// lies at u ^ (r & 7)); what the rounding left stays in v for the next part.
+__device__ __forceinline__ void stage_part(uint32_t tile, uint32_t row, int half, float (&v)[32]) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        Pack<bf16, 8> o;
+        uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            o.v[j] = __float2bfloat16_rn(v[q * 8 + j]);
-            if (more) v[q * 8 + j] -= __bfloat162float(o.v[j]);
+        for (int j = 0; j < 4; ++j) {
+            const __nv_bfloat162 pair = __floats2bfloat162_rn(v[q * 8 + 2 * j], v[q * 8 + 2 * j + 1]);
+            w[j] = reinterpret_cast<const uint32_t&>(pair);
+            v[q * 8 + 2 * j] -= __low2float(pair);
+            v[q * 8 + 2 * j + 1] -= __high2float(pair);
         }
-        *reinterpret_cast<Pack<bf16, 8>*>(to + q * 8) = o;
+        const uint32_t unit = (uint32_t)(half * 4 + q) ^ (row & 7u);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + row * 128 + unit * 16), "r"(w[0]),
+                     "r"(w[1]), "r"(w[2]), "r"(w[3])
+                     : "memory");
     }
 }
 
@@ -216,18 +227,23 @@ __device__ __forceinline__ void store_out(T* to, const float (&v)[32], uint32_t 
     }
 }
 
-template <int ENDING, bool A_TRANSPOSED, bool B_TRANSPOSED, typename T>
+template <int ENDING, bool A_TRANSPOSED, bool B_TRANSPOSED, bool PAIR, typename T>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     k_label_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_packed,
                  const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_b_packed,
-                 const __grid_constant__ GemmArgs a) {
+                 const __grid_constant__ CUtensorMap map_slopes, const __grid_constant__ GemmArgs a) {
+    constexpr int kBlocks = PAIR ? 2 : 1;
+    constexpr int kSide = kTile * kBlocks;  // the pair's tile
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem = (tc::smem_address(smem_raw) + 1023u) & ~1023u;
-    const uint32_t barriers = smem + kStages * 2 * kOperandBytes;
+    const uint32_t store_at = smem + kStages * kStageBytes;
+    const uint32_t barriers = store_at + kEpilogueWarps * kStoreBytes;
     const uint32_t full = barriers, empty = full + 8 * kStages, done = empty + 8 * kStages, drained = done + 16;
     const uint32_t tmem_slot = drained + 16;
     uint8_t* generic_base = smem_raw + (smem - tc::smem_address(smem_raw));
     const uint32_t warp = threadIdx.x / 32, lane = lane_id();
+    const uint32_t rank = PAIR ? tc::cluster_rank() : 0;
+    const uint32_t first_item = blockIdx.x / kBlocks, item_step = gridDim.x / kBlocks;
 
     if (warp == 0 && lane == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -236,20 +252,21 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             tc::barrier_init(done + 8 * b, 1);
-            tc::barrier_init(drained + 8 * b, kEpilogueWarps);
+            tc::barrier_init(drained + 8 * b, kEpilogueWarps * kBlocks);
         }
         tc::barrier_init_fence();
     }
-    if (warp == 2) tc::tmem_alloc<false>(tmem_slot, 2 * kTile);
+    if (warp == 2) tc::tmem_alloc<PAIR>(tmem_slot, 2 * kSide);
     tc::fence_before_sync();
     __syncthreads();
+    if constexpr (PAIR) tc::cluster_sync();  // the other block's barriers are set up too
     tc::fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<uint32_t*>(generic_base + (tmem_slot - smem));
     chain_enter();
 
     const uint32_t count = a.rows->count;
     const bool packed = a.rows->packed != 0;
-    const Schedule<ENDING> schedule(a, count);
+    const Schedule<ENDING, kSide> schedule(a, count);
     bool ok = true;
 
     if (warp == 0) {
@@ -260,37 +277,45 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             // The rows' operand of kOut starts at the chunk's first row in the features, at 0 in the slopes.
             const int a_rows = ENDING == kOut ? 0 : (int)a.first_row;
             const int b_rows = ENDING == kOut && B_TRANSPOSED && a.rows_inner ? (int)a.first_row : 0;
-            for (uint32_t item = blockIdx.x; ok && item < schedule.items; item += gridDim.x) {
+            for (uint32_t item = first_item; ok && item < schedule.items; item += item_step) {
                 const Work w = schedule.at(a, item);
-                for (uint32_t n = w.n0; ok && n < w.n1; ++n)
+                const int am = (int)(w.m * kSide + rank * kTile);
+                for (uint32_t n = w.n0; ok && n < w.n1; ++n) {
+                    const int bn = (int)(n * kSide + rank * kTile);
                     for (uint32_t p = 0; ok && p < a.products; ++p) {
                         const int za = a.products == 1 ? 0 : (int)((kPartsOfA >> (4 * p)) & 15u);
                         const int zb = a.products == 1 ? 0 : (int)((kPartsOfB >> (4 * p)) & 15u);
                         for (uint32_t k = w.k0; k < w.k1; ++k) {
                             if (!(ok = tc::barrier_wait(empty + 8 * stage, phase ^ 1))) break;
-                            const uint32_t bar = full + 8 * stage, to = smem + stage * 2 * kOperandBytes;
-                            tc::barrier_expect(bar, 2 * kOperandBytes);
+                            // Both blocks' copies count on the first one's barrier.
+                            const uint32_t to = smem + stage * kStageBytes;
+                            const uint32_t bar = PAIR ? tc::map_to_rank(full + 8 * stage, 0) : full + 8 * stage;
+                            if (rank == 0) tc::barrier_expect(full + 8 * stage, kStageBytes * kBlocks);
+                            const int kk = (int)k * kBlockK;
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                const int am = (int)w.m * kTile + h * 64, bn = (int)n * kTile + h * 64;
-                                const int kk = (int)k * kBlockK;
-                                if (A_TRANSPOSED) tc::load_box<false>(to + h * kBoxBytes, pa, bar, am, a_rows + kk, za);
-                                else tc::load_box<false>(to + h * kBoxBytes, pa, bar, kk, a_rows + am, za);
-                                if (B_TRANSPOSED)
-                                    tc::load_box<false>(to + kOperandBytes + h * kBoxBytes, pb, bar, bn, b_rows + kk, zb);
-                                else
-                                    tc::load_box<false>(to + kOperandBytes + h * kBoxBytes, pb, bar, kk, bn, zb);
+                                const uint32_t ta = to + h * kBoxBytes, tb = ta + kOperandBytes;
+                                if (A_TRANSPOSED) tc::load_box<PAIR>(ta, pa, bar, am + h * 64, a_rows + kk, za);
+                                else tc::load_box<PAIR>(ta, pa, bar, kk, a_rows + am + h * 64, za);
+                                if (B_TRANSPOSED) tc::load_box<PAIR>(tb, pb, bar, bn + h * 64, b_rows + kk, zb);
+                                else tc::load_box<PAIR>(tb, pb, bar, kk, bn + h * 64, zb);
                             }
                             if (++stage == kStages) stage = 0, phase ^= 1;
                         }
                     }
+                }
+            }
+            // The products' last arrivals reach this block before it may leave.
+            for (int i = 0; ok && i < kStages; ++i) {
+                ok = tc::barrier_wait(empty + 8 * stage, phase ^ 1);
+                if (++stage == kStages) stage = 0, phase ^= 1;
             }
         }
     } else if (warp == 1) {
-        if (tc::elect_one()) {
-            constexpr uint32_t desc = tc::instruction(kTile, kTile, A_TRANSPOSED, B_TRANSPOSED);
+        if (rank == 0 && tc::elect_one()) {
+            constexpr uint32_t desc = tc::instruction(kSide, kSide, A_TRANSPOSED, B_TRANSPOSED);
             uint32_t stage = 0, phase = 0, buffer = 0, buffer_phase = 0;
-            for (uint32_t item = blockIdx.x; ok && item < schedule.items; item += gridDim.x) {
+            for (uint32_t item = first_item; ok && item < schedule.items; item += item_step) {
                 const Work w = schedule.at(a, item);
                 const uint32_t steps = (w.k1 - w.k0) * a.products;
                 if (steps == 0) continue;
@@ -300,19 +325,19 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                     for (uint32_t k = 0; k < steps; ++k) {
                         if (!(ok = tc::barrier_wait(full + 8 * stage, phase))) break;
                         tc::fence_after_sync();
-                        const uint32_t at = smem + stage * 2 * kOperandBytes;
+                        const uint32_t at = smem + stage * kStageBytes;
 #pragma unroll
                         for (int q = 0; q < kBlockK / 16; ++q) {
                             // 16 of K: 32 bytes along a row, or 16 rows of 128 bytes.
                             const uint64_t da = tc::operand(at + q * (A_TRANSPOSED ? 2048 : 32), kBoxBytes);
                             const uint64_t db = tc::operand(at + kOperandBytes + q * (B_TRANSPOSED ? 2048 : 32), kBoxBytes);
-                            tc::multiply<false>(tmem + buffer * kTile, da, db, desc, k != 0 || q != 0);
+                            tc::multiply<PAIR>(tmem + buffer * kSide, da, db, desc, k != 0 || q != 0);
                         }
-                        tc::commit<false>(empty + 8 * stage);
+                        tc::commit<PAIR>(empty + 8 * stage);
                         if (++stage == kStages) stage = 0, phase ^= 1;
                     }
                     if (!ok) break;
-                    tc::commit<false>(done + 8 * buffer);
+                    tc::commit<PAIR>(done + 8 * buffer);
                     if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
                 }
             }
@@ -320,14 +345,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     } else if (warp >= 4) {
         // Half the tile's columns per warpgroup; thread = row.
         const uint32_t half = (warp - 4) / 4, quarter = warp % 4;
-        const uint32_t lane_row = quarter * 32 + lane;
-        const uint32_t tmem_at = tmem + ((quarter * 32) << 16) + half * (kTile / 2);
+        const uint32_t lane_row = rank * kTile + quarter * 32 + lane;
+        const uint32_t tmem_at = tmem + ((quarter * 32) << 16) + half * (kSide / 2);
+        const uint32_t stage_tile = store_at + (warp - 4) * kStoreBytes;
         uint32_t buffer = 0, buffer_phase = 0;
-        for (uint32_t item = blockIdx.x; ok && item < schedule.items; item += gridDim.x) {
+        for (uint32_t item = first_item; ok && item < schedule.items; item += item_step) {
             const Work w = schedule.at(a, item);
             const bool empty_sum = w.k0 == w.k1;
             if (ENDING == kOut && empty_sum && a.add) continue;
-            const uint32_t row = w.m * kTile + lane_row;  // in this call's rows (or labels)
+            const uint32_t row = w.m * kSide + lane_row;  // in this call's rows (or labels)
             const uint32_t compact = a.first_row + row;
             const bool live = compact < count;
             RowStats stats{-INFINITY, 0.0f, 0.0f, 0u};
@@ -346,38 +372,58 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                     if (!(ok = tc::barrier_wait(done + 8 * buffer, buffer_phase))) break;
                     tc::fence_after_sync();
                 }
+                // After the last load the accumulator may fill again.
+                auto drain = [&]() {
+                    tc::fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0)
+                        tc::barrier_arrive_cluster(PAIR ? tc::map_to_rank(drained + 8 * buffer, 0) : drained + 8 * buffer);
+                };
+                const uint32_t accumulator = tmem_at + buffer * kSide, columns_at = n * kSide + half * (kSide / 2);
+                if constexpr (ENDING == kSlopes) {
+                    // 64 columns at a time: each part fills the warp's 32 x 64 tile, which a bulk copy
+                    // writes out while the next is computed.
 #pragma unroll
-                for (int c = 0; c < kTile / 64; ++c) {
-                    float v[32];
-                    if (empty_sum) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-                    } else {
+                    for (int c = 0; c < kSide / 2; c += 64) {
+                        float v[2][32];
                         __syncwarp();
-                        tc::tmem_load32(tmem_at + buffer * kTile + c * 32, v);
+                        tc::tmem_load32(accumulator + c, v[0]);
+                        tc::tmem_load32(accumulator + c + 32, v[1]);
                         tc::tmem_load_wait();
+                        if (c + 64 == kSide / 2) drain();
+#pragma unroll
+                        for (int q = 0; q < 2; ++q)
+                            to_slopes(v[q], columns_at + c + 32 * q, a.labels, a.scale2, shift, weight, target, live);
+                        const int parts = a.products == 1 ? 1 : (int)kParts;
+                        for (int p = 0; p < parts; ++p) {
+                            if (lane == 0) tc::store_wait_read();
+                            __syncwarp();
+                            stage_part(stage_tile, lane, 0, v[0]);
+                            stage_part(stage_tile, lane, 1, v[1]);
+                            tc::fence_async_shared();
+                            __syncwarp();
+                            if (lane == 0)
+                                tc::store_box(&map_slopes, stage_tile, (int)columns_at + c, (int)row, p);
+                        }
                     }
-                    const uint32_t column = n * kTile + half * (kTile / 2) + c * 32;
-                    if constexpr (ENDING == kStats) {
-                        if (a.partial_labels) add_logits<true>(stats, v, column, a.labels, a.scale2, target);
-                        else add_logits<false>(stats, v, column, a.labels, a.scale2, target);
-                    } else if constexpr (ENDING == kSlopes) {
-                        to_slopes(v, column, a.labels, a.scale2, shift, weight, target);
-                        if (!live) {
+                } else {
+#pragma unroll
+                    for (int c = 0; c < kSide / 2; c += 32) {
+                        float v[32];
+                        if (empty_sum) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-                        }
-                        bf16* to = a.slopes + (uint64_t)row * a.slope_stride + column;
-                        const uint64_t part = (uint64_t)a.chunk_rows * a.slope_stride;
-                        if (a.products == 1) {
-                            store_part(to, v, false);
                         } else {
-#pragma unroll
-                            for (int p = 0; p < (int)kParts; ++p) store_part(to + p * part, v, p + 1 < (int)kParts);
+                            __syncwarp();
+                            tc::tmem_load32(accumulator + c, v);
+                            tc::tmem_load_wait();
+                            if (c + 32 == kSide / 2) drain();
                         }
-                    } else {
-                        const bool inside = (a.rows_inner ? row < a.out_rows : live) && column < a.out_columns;
-                        if (inside) {
+                        const uint32_t column = columns_at + c;
+                        if constexpr (ENDING == kStats) {
+                            if (a.partial_labels) add_logits<true>(stats, v, column, a.labels, a.scale2, target);
+                            else add_logits<false>(stats, v, column, a.labels, a.scale2, target);
+                        } else if ((a.rows_inner ? row < a.out_rows : live) && column < a.out_columns) {
                             const uint32_t columns = a.out_columns - column;
                             if (a.partial) {
                                 float* to = static_cast<float*>(a.out) +
@@ -396,12 +442,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                         }
                     }
                 }
-                if (!empty_sum) {
-                    tc::fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) tc::barrier_arrive_cluster(drained + 8 * buffer);
-                    if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
-                }
+                if (!empty_sum && ++buffer == 2) buffer = 0, buffer_phase ^= 1;
             }
             if (ENDING == kStats && ok && live) {
                 const uint64_t slot = (uint64_t)(w.split * 2 + half) * a.partial_rows + row;
@@ -409,10 +450,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 if (a.partial_labels) a.partial_labels[slot] = stats.label;
                 // The target is in exactly one thread's columns.
                 const uint64_t t = (uint64_t)target;
-                if (target >= 0 && t / kTile >= w.n0 && t / kTile < w.n1 && (t % kTile) / (kTile / 2) == half)
+                if (target >= 0 && t / kSide >= w.n0 && t / kSide < w.n1 && (t % kSide) / (kSide / 2) == half)
                     a.target_logits[row] = stats.target_logit;
             }
         }
+        if (ENDING == kSlopes && lane == 0) tc::store_wait();
     }
     __syncwarp();
     if (!ok) {
@@ -422,9 +464,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     }
     tc::fence_before_sync();
     __syncthreads();
+    if constexpr (PAIR) tc::cluster_sync();  // no block leaves while the other may reach into it
     if (warp == 2) {
         tc::fence_after_sync();
-        tc::tmem_free<false>(tmem, 2 * kTile);
+        tc::tmem_free<PAIR>(tmem, 2 * kSide);
     }
 }
 

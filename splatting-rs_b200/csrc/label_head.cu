@@ -45,8 +45,7 @@ struct sp_label_head {
     uint32_t parts() const { return element == SP_F32 ? kParts : 1; }
     uint32_t products() const { return element == SP_F32 ? kPartProducts : 1; }
     uint64_t packed_stride() const { return ((uint64_t)dim + kBlockK - 1) / kBlockK * kBlockK; }
-    uint32_t label_tiles() const { return (uint32_t)((labels + kTile - 1) / kTile); }
-    uint32_t dim_tiles() const { return (dim + kTile - 1) / kTile; }
+    uint64_t slope_stride() const { return (labels + kPairTile - 1) / kPairTile * kPairTile; }
 };
 
 namespace {
@@ -54,6 +53,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr uint32_t kGatherRows = 64;        // rows a block compacts and copies
 constexpr uint32_t kRecountBlocks = 64;     // up to this many blocks each count all targets themselves
+constexpr double kPairCost = 1.4;           // of a 256 x 256 tile, in 128 x 128 tiles of one block
 constexpr uint32_t kThreadSlots = 8;        // partials per row one thread joins; more take a warp
 constexpr uint64_t kSlopeBudget = 1ull << 28;  // slope elements kept at once (512 MB)
 
@@ -385,15 +385,15 @@ EncodeTiled encode_tiled() {
     return function;
 }
 
-// A bf16 matrix of `parts` planes as 64 x 64 boxes in the 128-byte swizzle; elements outside read
+// A bf16 matrix of `parts` planes as 64 x box_rows boxes in the 128-byte swizzle; elements outside read
 // as zero.
 sp_status make_map(sp_context* ctx, CUtensorMap* map, const void* base, uint64_t columns, uint64_t rows,
-                   uint64_t stride, uint32_t parts, uint64_t part) {
+                   uint64_t stride, uint32_t parts, uint64_t part, uint32_t box_rows = 64) {
     const EncodeTiled encode = encode_tiled();
     SP_REQUIRE(ctx, encode != nullptr, SP_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
     const cuuint64_t dims[3] = {columns, rows, parts};
     const cuuint64_t strides[2] = {stride * 2, parts > 1 ? part * 2 : stride * 2};
-    const cuuint32_t box[3] = {64, 64, 1}, steps[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {64, box_rows, 1}, steps[3] = {1, 1, 1};
     const CUresult r =
         encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, steps,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -412,35 +412,60 @@ bool vector_rows(const sp_label_head* h, const void* p, int64_t stride) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % (16 / (int64_t)element_size(h->element)) == 0;
 }
 
-// Pieces of the label tiles (for `m_tiles` row tiles) that finish soonest: whole waves of blocks
-// times the longest piece. At most four waves of pieces where there is more than one.
-uint32_t stats_splits(uint32_t sms, uint64_t m_tiles, uint32_t n_tiles) {
-    uint32_t best = 1;
-    uint64_t best_cost = ~0ull;
-    for (uint32_t s = 1; s <= n_tiles && (s == 1 || m_tiles * s <= 4ull * sms); ++s) {
-        const uint64_t cost = ((m_tiles * s + sms - 1) / sms) * ((n_tiles + s - 1) / s);
-        if (cost < best_cost) best_cost = cost, best = s;
+// How a product is cut up: pairs of blocks or single ones, and the pieces of the label tiles (of
+// the inner dimension, for an output gradient).
+struct Plan {
+    bool pair;
+    uint32_t m_tiles, n_tiles, splits;
+    uint64_t items() const { return (uint64_t)m_tiles * splits; }
+};
+
+uint32_t tiles_of(uint64_t n, bool pair) { return (uint32_t)((n + (pair ? kPairTile : kTile) - 1) / (pair ? kPairTile : kTile)); }
+
+// The cut that finishes soonest: whole waves of blocks times the longest piece, a pair's tile
+// counted as kPairCost single ones (four times the products on two SMs that share their operands).
+// At most four waves of pieces where there is more than one.
+Plan plan_logits(uint32_t sms, uint64_t rows, uint64_t labels) {
+    Plan best{};
+    double best_cost = 1e300;
+    for (int pair = 0; pair < 2; ++pair) {
+        const uint32_t workers = pair ? std::max(sms / 2, 1u) : sms;
+        const uint32_t m = tiles_of(rows, pair), n = tiles_of(labels, pair);
+        for (uint32_t s = 1; s <= n && (s == 1 || (uint64_t)m * s <= 4ull * workers); ++s) {
+            const double cost = (double)(((uint64_t)m * s + workers - 1) / workers) * ((n + s - 1) / s) *
+                                (pair ? kPairCost : 1.0);
+            if (cost < best_cost) best_cost = cost, best = Plan{pair != 0, m, n, s};
+        }
     }
     return best;
 }
 
-// The same for the inner dimension of an output gradient: its pieces go through f32 sums, so one
-// is taken only where it shortens the products by a tenth, and none shorter than 4 steps.
-uint32_t out_splits(uint32_t sms, uint64_t tiles, uint32_t k_blocks) {
-    uint32_t best = 1;
+// The same for an output gradient of m x n. Its pieces go through f32 sums, so more of them are
+// taken only where that shortens the products by a tenth, at most two waves, none below 4 steps.
+Plan plan_out(uint32_t sms, uint64_t rows, uint64_t columns, uint32_t k_blocks) {
+    Plan best{};
     double best_cost = 1e300;
-    for (uint32_t s = 1; s == 1 || (tiles * s <= 2ull * sms && k_blocks >= 4 * s); ++s) {
-        const double cost = (double)((tiles * s + sms - 1) / sms) * ((k_blocks + s - 1) / s);
-        if (cost < 0.9 * best_cost) best_cost = cost, best = s;
+    for (int pair = 0; pair < 2; ++pair) {
+        const uint32_t workers = pair ? std::max(sms / 2, 1u) : sms;
+        const uint32_t m = tiles_of(rows, pair), n = tiles_of(columns, pair);
+        const uint64_t tiles = (uint64_t)m * n;
+        for (uint32_t s = 1; s == 1 || (tiles * s <= 2ull * workers && k_blocks >= 4 * s); ++s) {
+            const double cost = (double)((tiles * s + workers - 1) / workers) * ((k_blocks + s - 1) / s) *
+                                (pair ? kPairCost : 1.0);
+            if (cost < 0.9 * best_cost) best_cost = cost, best = Plan{pair != 0, m, n, s};
+        }
     }
     return best;
 }
 
 uint64_t chunk_limit(const sp_label_head* h) {
-    const uint64_t per_row = (uint64_t)h->label_tiles() * kTile * h->parts();
-    const uint64_t rows = kSlopeBudget / per_row / kTile * kTile;
-    return std::min(std::max<uint64_t>(rows, kTile), round_up(h->max_rows, kTile));
+    const uint64_t rows = kSlopeBudget / (h->slope_stride() * h->parts()) / kPairTile * kPairTile;
+    return std::min(std::max<uint64_t>(rows, kPairTile), round_up(h->max_rows, kPairTile));
 }
+
+// Rows of f32 sums a gradient may need. plan_out: pieces times tiles stay within two waves, or one
+// piece; one piece needs sums for the weight's gradient alone, over several chunks.
+uint64_t sums_rows(const sp_label_head* h) { return std::max<uint64_t>(2ull * h->sms * kTile, h->labels); }
 
 uint64_t sums_stride(const sp_label_head* h) { return ((uint64_t)h->dim + 3) / 4 * 4; }
 
@@ -453,15 +478,38 @@ sp_status allocate(sp_label_head* h, T** out, uint64_t count) {
     return SP_OK;
 }
 
-template <int ENDING, bool A_TRANSPOSED, bool B_TRANSPOSED, typename T>
-cudaError_t run_gemm(const sp_label_head* h, uint64_t items, const CUtensorMap& a, const CUtensorMap& a_packed,
-                     const CUtensorMap& b, const CUtensorMap& b_packed, const GemmArgs& args) {
-    auto kernel = k_label_gemm<ENDING, A_TRANSPOSED, B_TRANSPOSED, T>;
+template <int ENDING, bool A_TRANSPOSED, bool B_TRANSPOSED, bool PAIR, typename T>
+cudaError_t launch_gemm(const sp_label_head* h, uint64_t items, const CUtensorMap& a, const CUtensorMap& a_packed,
+                        const CUtensorMap& b, const CUtensorMap& b_packed, const CUtensorMap& slopes,
+                        const GemmArgs& args) {
+    auto kernel = k_label_gemm<ENDING, A_TRANSPOSED, B_TRANSPOSED, PAIR, T>;
     static std::atomic<unsigned long long> configured{0};
     const cudaError_t err = allow_smem_once(kernel, kGemmSmem, configured);
     if (err != cudaSuccess) return err;
-    const unsigned grid = (unsigned)std::max<uint64_t>(1, std::min<uint64_t>(items, h->sms));
-    return launch_chained(kernel, grid, kGemmThreads, kGemmSmem, h->ctx->stream, a, a_packed, b, b_packed, args);
+    constexpr unsigned blocks = PAIR ? 2 : 1;
+    const unsigned workers = (unsigned)std::max<uint64_t>(1, std::min<uint64_t>(items, h->sms / blocks));
+    cudaLaunchConfig_t config{};
+    config.gridDim = workers * blocks;
+    config.blockDim = kGemmThreads;
+    config.dynamicSmemBytes = kGemmSmem;
+    config.stream = h->ctx->stream;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = blocks;
+    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = 2;
+    return cudaLaunchKernelEx(&config, kernel, a, a_packed, b, b_packed, slopes, args);
+}
+
+template <int ENDING, bool A_TRANSPOSED, bool B_TRANSPOSED, typename T>
+cudaError_t run_gemm(const sp_label_head* h, const Plan& plan, uint64_t items, const CUtensorMap& a,
+                     const CUtensorMap& a_packed, const CUtensorMap& b, const CUtensorMap& b_packed,
+                     const CUtensorMap& slopes, const GemmArgs& args) {
+    return plan.pair ? launch_gemm<ENDING, A_TRANSPOSED, B_TRANSPOSED, true, T>(h, items, a, a_packed, b, b_packed, slopes, args)
+                     : launch_gemm<ENDING, A_TRANSPOSED, B_TRANSPOSED, false, T>(h, items, a, a_packed, b, b_packed, slopes, args);
 }
 
 sp_status check_matrix(sp_context* ctx, const void* p, int64_t stride, uint32_t dim, size_t size, const char* what) {
@@ -482,7 +530,7 @@ sp_status prepare(sp_label_head* h, const void* features, int64_t feature_stride
                   void* gradient, int64_t gradient_stride, Operands* out) {
     sp_context* ctx = h->ctx;
     cudaStream_t st = ctx->stream;
-    const uint64_t stride = h->packed_stride(), capacity = round_up(h->max_rows, kTile);
+    const uint64_t stride = h->packed_stride(), capacity = round_up(h->max_rows, kPairTile);
     const uint32_t parts = h->parts();
     const bool features_here = in_place(h, features, feature_stride), weight_here = in_place(h, weight, weight_stride);
     out->row_capacity = capacity;
@@ -559,16 +607,16 @@ sp_status check_targets(sp_context* ctx, const void* targets, sp_index index) {
 sp_status run_stats(sp_label_head* h, const Operands& op, const void* targets, int wide, uint64_t n, float scale,
                     float* mean, float* losses, float* normalizers, int32_t* labels_out, float* log_probability) {
     sp_context* ctx = h->ctx;
-    const uint64_t m_tiles = (n + kTile - 1) / kTile;
+    const Plan plan = plan_logits(h->sms, n, h->labels);
     GemmArgs a = common_args(h, targets, wide, scale);
     a.k_blocks = (h->dim + kBlockK - 1) / kBlockK;
-    a.n_tiles = h->label_tiles();
-    a.splits = stats_splits(h->sms, m_tiles, a.n_tiles);
+    a.n_tiles = plan.n_tiles;
+    a.splits = plan.splits;
     a.partials = h->partials;
     a.partial_labels = labels_out ? h->partial_labels : nullptr;
-    a.partial_rows = m_tiles * kTile;
+    a.partial_rows = (uint64_t)plan.m_tiles * (plan.pair ? kPairTile : kTile);
     a.target_logits = h->target_logits;
-    SP_CUDA(ctx, (run_gemm<kStats, false, false, bf16>(h, m_tiles * a.splits, op.features, op.features_packed,
+    SP_CUDA(ctx, (run_gemm<kStats, false, false, bf16>(h, plan, plan.items(), op.features, op.features_packed, op.weight,
                                                        op.weight, op.weight, a)));
     const uint32_t slots = 2 * a.splits;
     auto join = [&](auto kernel, uint32_t lanes) {
@@ -609,25 +657,22 @@ sp_status sp_label_head_create(sp_context* ctx, uint64_t labels, uint32_t dim, s
         int sms = 0;
         SP_CUDA(ctx, cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, ctx->device));
         h->sms = (uint32_t)std::max(sms, 1);
-        const uint64_t capacity = round_up(max_rows, kTile), stride = h->packed_stride();
+        const uint64_t capacity = round_up(max_rows, kPairTile), stride = h->packed_stride();
         SP_CHECK(allocate(h, &h->rows, 1));
         SP_CUDA(ctx, cudaMemsetAsync(h->rows, 0, sizeof(RowSet), ctx->stream));
         SP_CHECK(allocate(h, &h->row_of, max_rows));
         SP_CHECK(allocate(h, &h->counts, (max_rows + kGatherRows - 1) / kGatherRows));
         SP_CHECK(allocate(h, &h->packed_features, capacity * stride * h->parts()));
         SP_CHECK(allocate(h, &h->packed_weight, labels * stride * h->parts()));
-        // stats_splits: pieces times row tiles stay within four waves, or one piece.
+        // plan_logits: pieces times row tiles stay within four waves, or one piece.
         const uint64_t slots = 2 * kTile * std::max<uint64_t>(capacity / kTile, 4ull * h->sms);
         SP_CHECK(allocate(h, &h->partials, slots));
         SP_CHECK(allocate(h, &h->partial_labels, slots));
         SP_CHECK(allocate(h, &h->target_logits, capacity));
         SP_CHECK(allocate(h, &h->loss_sums, (max_rows * 32 + kThreads - 1) / kThreads));
         if (h->training) {
-            SP_CHECK(allocate(h, &h->slopes, chunk_limit(h) * h->label_tiles() * kTile * h->parts()));
-            // out_splits: pieces times tiles stay within two waves, or one piece; one piece needs
-            // sums for the weight's gradient alone, over several chunks.
-            const uint64_t tiles = std::max<uint64_t>(2ull * h->sms, h->label_tiles());
-            SP_CHECK(allocate(h, &h->sums, tiles * kTile * sums_stride(h) * 2));
+            SP_CHECK(allocate(h, &h->slopes, chunk_limit(h) * h->slope_stride() * h->parts()));
+            SP_CHECK(allocate(h, &h->sums, sums_rows(h) * sums_stride(h) * 2));
         }
         return SP_OK;
     };
@@ -719,36 +764,36 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
                      d_feature_gradient, feature_gradient_stride, &op));
 
     const uint64_t limit = chunk_limit(h), chunks = (rows + limit - 1) / limit;
-    const uint64_t chunk = round_up((rows + chunks - 1) / chunks, kTile);
-    const uint64_t slope_stride = (uint64_t)h->label_tiles() * kTile, sum_stride = sums_stride(h);
-    const uint64_t m_tiles = chunk / kTile;
-    CUtensorMap slopes;
+    const uint64_t chunk = round_up((rows + chunks - 1) / chunks, kPairTile);
+    const uint64_t slope_stride = h->slope_stride(), sum_stride = sums_stride(h);
+    CUtensorMap slopes, slopes_out;
     SP_CHECK(make_map(ctx, &slopes, h->slopes, slope_stride, chunk, slope_stride, h->parts(), chunk * slope_stride));
-    const uint32_t label_k = (uint32_t)((h->labels + kBlockK - 1) / kBlockK), row_k = (uint32_t)(chunk / kBlockK);
-    const uint32_t feature_splits = out_splits(h->sms, m_tiles * h->dim_tiles(), label_k);
-    const uint32_t weight_splits = out_splits(h->sms, (uint64_t)h->label_tiles() * h->dim_tiles(), row_k);
-    const bool feature_sums = feature_splits > 1, weight_sums = weight_splits > 1 || chunks > 1;
+    SP_CHECK(make_map(ctx, &slopes_out, h->slopes, slope_stride, chunk, slope_stride, h->parts(), chunk * slope_stride, 32));
+    const uint32_t label_k = (uint32_t)((h->labels + kBlockK - 1) / kBlockK);
+    const uint64_t chunk_rows = std::min(chunk, rows);
+    const Plan logits = plan_logits(h->sms, chunk_rows, h->labels);
+    const Plan to_features = plan_out(h->sms, chunk_rows, h->dim, label_k);
+    const Plan to_weight = plan_out(h->sms, h->labels, h->dim, (uint32_t)((chunk_rows + kBlockK - 1) / kBlockK));
+    const bool feature_sums = to_features.splits > 1, weight_sums = to_weight.splits > 1 || chunks > 1;
     float* weight_sum = h->sums;
-    float* feature_sum = h->sums + std::max<uint64_t>(2ull * h->sms, h->label_tiles()) * kTile * sum_stride;
+    float* feature_sum = h->sums + sums_rows(h) * sum_stride;
 
     for (uint64_t c = 0; c < chunks; ++c) {
         GemmArgs a = common_args(h, d_targets, wide, logit_scale);
         a.first_row = (uint32_t)(c * chunk);
         a.chunk_rows = (uint32_t)chunk;
         a.k_blocks = (h->dim + kBlockK - 1) / kBlockK;
-        a.n_tiles = h->label_tiles();
-        a.splits = stats_splits(h->sms, m_tiles, a.n_tiles);
+        a.n_tiles = logits.n_tiles;
+        a.splits = logits.splits;
         a.log_normalizers = d_log_normalizers;
         a.row_gradient = d_row_gradient;
-        a.slopes = h->slopes;
-        a.slope_stride = slope_stride;
-        SP_CUDA(ctx, (run_gemm<kSlopes, false, false, bf16>(h, m_tiles * a.splits, op.features, op.features_packed,
-                                                            op.weight, op.weight, a)));
+        SP_CUDA(ctx, (run_gemm<kSlopes, false, false, bf16>(h, logits, logits.items(), op.features, op.features_packed,
+                                                            op.weight, op.weight, slopes_out, a)));
 
         GemmArgs f = a;  // dH = G W
         f.k_blocks = label_k;
-        f.n_tiles = h->dim_tiles();
-        f.splits = feature_splits;
+        f.n_tiles = to_features.n_tiles;
+        f.splits = to_features.splits;
         f.partial = feature_sums;
         f.out = feature_sums ? (void*)feature_sum : d_feature_gradient;
         f.out_stride = feature_sums ? (int64_t)sum_stride : feature_gradient_stride;
@@ -756,16 +801,17 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
         f.out_columns = h->dim;
         f.scatter = !feature_sums;
         f.out_packed = vector_rows(h, d_feature_gradient, feature_gradient_stride);
-        const uint64_t f_items = m_tiles * f.n_tiles * f.splits;
-        SP_CUDA(ctx, h->element == SP_F32
-                         ? (run_gemm<kOut, false, true, float>(h, f_items, slopes, slopes, op.weight, op.weight, f))
-                         : (run_gemm<kOut, false, true, bf16>(h, f_items, slopes, slopes, op.weight, op.weight, f)));
+        auto run_features = [&](auto* typed) {
+            return run_gemm<kOut, false, true, std::remove_pointer_t<decltype(typed)>>(
+                h, to_features, to_features.items() * f.n_tiles, slopes, slopes, op.weight, op.weight, slopes_out, f);
+        };
+        SP_CUDA(ctx, h->element == SP_F32 ? run_features((float*)nullptr) : run_features((bf16*)nullptr));
 
         GemmArgs w = a;  // dW = G^T H
         w.rows_inner = 1;
-        w.m_tiles = h->label_tiles();
-        w.n_tiles = h->dim_tiles();
-        w.splits = weight_splits;
+        w.m_tiles = to_weight.m_tiles;
+        w.n_tiles = to_weight.n_tiles;
+        w.splits = to_weight.splits;
         w.partial = weight_sums;
         w.add = c > 0;
         w.out = weight_sums ? (void*)weight_sum : d_weight_gradient;
@@ -773,17 +819,16 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
         w.out_rows = h->labels;
         w.out_columns = h->dim;
         w.out_packed = vector_rows(h, d_weight_gradient, weight_gradient_stride);
-        const uint64_t w_items = (uint64_t)w.m_tiles * w.n_tiles * w.splits;
-        SP_CUDA(ctx, h->element == SP_F32
-                         ? (run_gemm<kOut, true, true, float>(h, w_items, slopes, slopes, op.features,
-                                                              op.features_packed, w))
-                         : (run_gemm<kOut, true, true, bf16>(h, w_items, slopes, slopes, op.features,
-                                                             op.features_packed, w)));
+        auto run_weight = [&](auto* typed) {
+            return run_gemm<kOut, true, true, std::remove_pointer_t<decltype(typed)>>(
+                h, to_weight, to_weight.items() * w.n_tiles, slopes, slopes, op.features, op.features_packed, slopes_out, w);
+        };
+        SP_CUDA(ctx, h->element == SP_F32 ? run_weight((float*)nullptr) : run_weight((bf16*)nullptr));
 
         const bool last = c + 1 == chunks;
-        JoinArgs jf{feature_sums ? feature_sum : nullptr, feature_splits, chunk, sum_stride, 1, a.first_row,
+        JoinArgs jf{feature_sums ? feature_sum : nullptr, to_features.splits, chunk, sum_stride, 1, a.first_row,
                     d_feature_gradient, feature_gradient_stride, last ? rows : 0};
-        JoinArgs jw{weight_sums && last ? weight_sum : nullptr, weight_splits, h->labels, sum_stride, 0, 0,
+        JoinArgs jw{weight_sums && last ? weight_sum : nullptr, to_weight.splits, h->labels, sum_stride, 0, 0,
                     d_weight_gradient, weight_gradient_stride, last ? h->labels : 0};
         if (!last && !feature_sums) continue;
         const uint64_t quads = std::max(feature_sums ? chunk * (sum_stride / 4) : 0,

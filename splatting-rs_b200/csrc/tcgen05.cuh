@@ -115,6 +115,20 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, u
             : "memory");
 }
 
+// A box from this block's shared memory to a 3-D tensor. The issuing thread waits for its own
+// stores: store_wait_read until the shared memory may be written again, store_wait until they are
+// complete.
+__device__ __forceinline__ void store_box(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
+                 "r"(src), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// Orders this thread's shared-memory writes before bulk copies that read them.
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 // ---- tensor memory
 
 template <bool PAIR>
