@@ -1,7 +1,8 @@
 // The tensor-core pipeline of the label head: D = A B^T over bf16 operands in tiles of 256 x 256
 // per pair of thread blocks (or 128 x 128 per block), f32 accumulators in tensor memory, and three
 // endings for a tile:
-//   kStats   the logits' running maximum and sum of exponentials per row (and the target's logit)
+//   kStats   the logits' running sum of exponentials per row, and the target's logit or the
+//            largest one and its label
 //   kSlopes  the softmax slopes c g (p - [target]), written as bf16 parts
 //   kOut     the tile itself: an output gradient, or a partial sum of one
 //
@@ -47,12 +48,14 @@ struct RowSet {
     uint32_t ticket;  // of the loss sum's blocks
 };
 
+constexpr uint32_t kNoTarget = 0xffffffffu;  // index_at's -1
+
 enum Ending { kStats = 0, kSlopes = 1, kOut = 2 };
 
 struct GemmArgs {
     RowSet* rows;
     const uint32_t* row_of;
-    uint64_t labels;
+    uint32_t labels;
     uint32_t products;     // 1, or kPartProducts
     uint32_t k_blocks;     // of the inner dimension; kOut with rows_inner: follows the row count
     uint32_t m_tiles;      // kOut only: where the outer dimension is not the rows
@@ -64,7 +67,7 @@ struct GemmArgs {
     const void* targets;
     int wide;
     // kStats
-    float2* partials;      // [2 * splits][partial_rows]: maximum and sum
+    float2* partials;      // [2 * splits][partial_rows]: base (prediction: largest logit) and sum
     uint32_t* partial_labels;  // the maximum's label, or NULL
     uint64_t partial_rows;
     float* target_logits;
@@ -101,18 +104,20 @@ struct Schedule {
     }
     __device__ Work at(const GemmArgs& a, uint32_t item) const {
         Work w;
-        w.m = item % m_tiles;
-        uint32_t rest = item / m_tiles;
         if (ENDING == kOut) {
-            w.n0 = rest % a.n_tiles;
+            // Neighbours share the slopes' tiles, the larger operand.
+            w.n0 = item % a.n_tiles;
             w.n1 = w.n0 + 1;
-            w.split = rest / a.n_tiles;
+            w.m = item / a.n_tiles % m_tiles;
+            w.split = item / a.n_tiles / m_tiles;
             w.k0 = (uint32_t)((uint64_t)k_blocks * w.split / a.splits);
             w.k1 = (uint32_t)((uint64_t)k_blocks * (w.split + 1) / a.splits);
         } else {
-            w.split = rest;
-            w.n0 = (uint32_t)((uint64_t)a.n_tiles * rest / a.splits);
-            w.n1 = (uint32_t)((uint64_t)a.n_tiles * (rest + 1) / a.splits);
+            // Neighbours share the label tiles.
+            w.m = item % m_tiles;
+            w.split = item / m_tiles;
+            w.n0 = (uint32_t)((uint64_t)a.n_tiles * w.split / a.splits);
+            w.n1 = (uint32_t)((uint64_t)a.n_tiles * (w.split + 1) / a.splits);
             w.k0 = 0;
             w.k1 = k_blocks;
         }
@@ -126,59 +131,114 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// A row's running softmax: the largest logit so far (unscaled), its label, the sum of
-// exp2((z - largest) scale2), and the target's logit once it came past.
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+          "l"(reinterpret_cast<unsigned long long&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return d;
+}
+
+// A row's running softmax: sum of 2^(z scale2 - base) over its logits z so far. The loss takes any
+// base that keeps the sum in range; prediction needs the largest logit and its label, and its base is
+// that logit's. The target's logit is picked up when it comes past.
 struct RowStats {
-    float largest, sum, target_logit;
+    float base, sum, target_logit, largest;
     uint32_t label;
 };
 
-// 32 more logits of a row, labels first..first + 31 (those from `labels` on are absent).
+__device__ __forceinline__ float largest_of(const float (&v)[32]) {
+    float m[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int j = 4; j < 32; ++j) m[j & 3] = fmaxf(m[j & 3], v[j]);
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+
+// sum of 2^(v scale2 - base): packed multiply-adds and sums around the exponentials, four sums.
+__device__ __forceinline__ float sum_exp2(const float (&v)[32], float scale2, float base) {
+    const float2 s2 = make_float2(scale2, scale2), b2 = make_float2(-base, -base);
+    float2 t[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+        const float2 x = fma2(make_float2(v[j], v[j + 1]), s2, b2);
+        t[(j / 2) & 1] = add2(t[(j / 2) & 1], make_float2(exp2_fast(x.x), exp2_fast(x.y)));
+    }
+    t[0] = add2(t[0], t[1]);
+    return t[0].x + t[0].y;
+}
+
+// 32 more logits of a row, labels first..first + 31 (those from `labels` on are absent). The loss
+// takes its base from the row's first chunk and looks for the largest logit again only when a sum
+// leaves f32's range (a logit some 127 / log2(e) above the base), so that a chunk's exponentials
+// wait for nothing: the running maximum in every chunk cost a quarter of the pass at width 512.
 template <bool LABEL>
-__device__ __forceinline__ void add_logits(RowStats& s, float (&v)[32], uint64_t first, uint64_t labels, float scale2,
-                                           int64_t target) {
+__device__ __forceinline__ void add_logits(RowStats& s, float (&v)[32], uint32_t first, uint32_t labels, float scale2,
+                                           uint32_t target) {
     if (first + 32 > labels) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
             if (first + j >= labels) v[j] = -INFINITY;
     }
-    float m4[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-    for (int j = 4; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], v[j]);
-    const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-    if (m > s.largest) {
-        // exp2(-inf) = 0 clears the sum of a first chunk.
-        s.sum *= exp2_fast((s.largest - m) * scale2);
-        s.largest = m;
-        if (LABEL) {
+    if (LABEL) {
+        const float m = largest_of(v);
+        if (m > s.largest) {
+            s.largest = m;
+            const float base = __fmul_rn(m, scale2);
+            s.sum *= exp2_fast(s.base - base);  // 0 after a first chunk's base of -inf
+            s.base = base;
 #pragma unroll
             for (int j = 31; j >= 0; --j)
-                if (v[j] == m) s.label = (uint32_t)(first + j);
+                if (v[j] == m) s.label = first + j;
         }
+        // Nothing but -inf so far: any finite base counts that as 0.
+        s.sum += sum_exp2(v, scale2, s.base == -INFINITY ? 0.0f : s.base);
+        return;
     }
-    const float shift = s.largest == -INFINITY ? 0.0f : -s.largest * scale2;
-    float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int j = 0; j < 32; ++j) t[j & 3] += exp2_fast(fmaf(v[j], scale2, shift));
-    s.sum += (t[0] + t[1]) + (t[2] + t[3]);
-    const uint64_t at = (uint64_t)(target - (int64_t)first);
+    if (s.base == -INFINITY) {
+        const float m = largest_of(v);
+        if (m != -INFINITY) s.base = __fmul_rn(m, scale2);  // NaN stays NaN
+    }
+    float base = s.base == -INFINITY ? 0.0f : s.base, sum;
+    for (;;) {
+        sum = s.sum + sum_exp2(v, scale2, base);
+        if (sum != INFINITY) break;
+        const float higher = fmaxf(base, __fmul_rn(largest_of(v), scale2));
+        if (!(higher > base)) break;  // an infinite logit
+        s.sum *= exp2_fast(base - higher);
+        base = s.base = higher;
+    }
+    s.sum = sum;
+    const uint32_t at = target - first;
     if (__any_sync(0xffffffffu, at < 32)) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-            if (at == (uint64_t)j) s.target_logit = v[j];
+            if (at == (uint32_t)j) s.target_logit = v[j];
     }
 }
 
 // The slopes of 32 logits of a row, in place; zeros past the labels and in rows that do not count.
-__device__ __forceinline__ void to_slopes(float (&v)[32], uint64_t first, uint64_t labels, float scale2, float shift,
-                                          float weight, int64_t target, bool live) {
+__device__ __forceinline__ void to_slopes(float (&v)[32], uint32_t first, uint32_t labels, float scale2, float shift,
+                                          float weight, uint32_t target, bool live) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = exp2_fast(fmaf(v[j], scale2, shift));
-    const uint64_t at = (uint64_t)(target - (int64_t)first);
+    for (int j = 0; j < 32; j += 2) {
+        const float2 x = fma2(make_float2(v[j], v[j + 1]), make_float2(scale2, scale2), make_float2(shift, shift));
+        v[j] = exp2_fast(x.x);
+        v[j + 1] = exp2_fast(x.y);
+    }
+    const uint32_t at = target - first;
     if (__any_sync(0xffffffffu, at < 32)) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-            if (at == (uint64_t)j) v[j] -= 1.0f;
+            if (at == (uint32_t)j) v[j] -= 1.0f;
     }
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = live ? v[j] * weight : 0.0f;
@@ -356,12 +416,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             const uint32_t row = w.m * kSide + lane_row;  // in this call's rows (or labels)
             const uint32_t compact = a.first_row + row;
             const bool live = compact < count;
-            RowStats stats{-INFINITY, 0.0f, 0.0f, 0u};
-            int64_t target = -1;
+            RowStats stats{-INFINITY, 0.0f, 0.0f, -INFINITY, 0u};
+            uint32_t target = kNoTarget;
             float shift = 0.0f, weight = 0.0f;
             if (ENDING != kOut && live) {
                 const uint32_t original = a.row_of[compact];
-                if (a.targets) target = index_at(a.targets, a.wide, original, a.labels);
+                if (a.targets) target = (uint32_t)index_at(a.targets, a.wide, original, a.labels);
                 if (ENDING == kSlopes) {
                     shift = -a.log_normalizers[original] * 1.44269504088896341f;
                     weight = a.scale * (a.row_gradient ? a.row_gradient[original] : 1.0f / (float)count);
@@ -406,6 +466,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                                 tc::store_box(&map_slopes, stage_tile, (int)columns_at + c, (int)row, p);
                         }
                     }
+                } else if constexpr (ENDING == kStats) {
+                    // A chunk is reduced while the next one loads. Two chunks a turn: the whole tile
+                    // unrolled overflows the instruction cache.
+                    float v[2][32];
+                    __syncwarp();
+                    tc::tmem_load32(accumulator, v[0]);
+#pragma unroll 1
+                    for (int c = 0; c < kSide / 2; c += 64) {
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            tc::tmem_load_wait();
+                            __syncwarp();
+                            if (q == 0 || c + 64 < kSide / 2) tc::tmem_load32(accumulator + c + 32 * (q + 1), v[1 - q]);
+                            else drain();
+                            const uint32_t column = columns_at + c + 32 * q;
+                            if (a.partial_labels) add_logits<true>(stats, v[q], column, a.labels, a.scale2, target);
+                            else add_logits<false>(stats, v[q], column, a.labels, a.scale2, target);
+                        }
+                    }
                 } else {
 #pragma unroll
                     for (int c = 0; c < kSide / 2; c += 32) {
@@ -420,10 +499,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                             if (c + 32 == kSide / 2) drain();
                         }
                         const uint32_t column = columns_at + c;
-                        if constexpr (ENDING == kStats) {
-                            if (a.partial_labels) add_logits<true>(stats, v, column, a.labels, a.scale2, target);
-                            else add_logits<false>(stats, v, column, a.labels, a.scale2, target);
-                        } else if ((a.rows_inner ? row < a.out_rows : live) && column < a.out_columns) {
+                        if ((a.rows_inner ? row < a.out_rows : live) && column < a.out_columns) {
                             const uint32_t columns = a.out_columns - column;
                             if (a.partial) {
                                 float* to = static_cast<float*>(a.out) +
@@ -446,11 +522,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             }
             if (ENDING == kStats && ok && live) {
                 const uint64_t slot = (uint64_t)(w.split * 2 + half) * a.partial_rows + row;
-                a.partials[slot] = make_float2(stats.largest, stats.sum);
+                a.partials[slot] = make_float2(a.partial_labels ? stats.largest : stats.base, stats.sum);
                 if (a.partial_labels) a.partial_labels[slot] = stats.label;
                 // The target is in exactly one thread's columns.
-                const uint64_t t = (uint64_t)target;
-                if (target >= 0 && t / kSide >= w.n0 && t / kSide < w.n1 && (t % kSide) / (kSide / 2) == half)
+                if (target != kNoTarget && target / kSide >= w.n0 && target / kSide < w.n1 &&
+                    target % kSide / (kSide / 2) == half)
                     a.target_logits[row] = stats.target_logit;
             }
         }

@@ -221,29 +221,34 @@ __global__ void __launch_bounds__(kThreads) k_pack_rows(const T* __restrict__ fr
 
 // ------------------------------------------------------------------ joining
 
+// Partial sums in units of 2^base, joined in double: a part's sum may come close to f32's largest.
 struct Joined {
-    float largest, sum;
+    float base, largest;
+    double sum;
     uint32_t label;
 };
 
-__device__ __forceinline__ Joined join(Joined a, Joined b, float scale2) {
+__device__ __forceinline__ Joined join(Joined a, Joined b) {
     Joined r;
     const bool second = b.largest > a.largest || (b.largest == a.largest && b.label < a.label);
-    r.largest = fmaxf(a.largest, b.largest);
+    r.largest = second ? b.largest : a.largest;
     r.label = second ? b.label : a.label;
-    const float top = r.largest == -INFINITY ? 0.0f : r.largest;
-    r.sum = a.sum * exp2_fast((a.largest - top) * scale2) + b.sum * exp2_fast((b.largest - top) * scale2);
+    r.base = fmaxf(a.base, b.base);
+    const float top = r.base == -INFINITY ? 0.0f : r.base;
+    r.sum = a.sum * (double)exp2f(a.base - top) + b.sum * (double)exp2f(b.base - top);
     return r;
 }
 
 // `lanes` threads (1 or 32) join a row's partials in slot order within a lane, then across lanes.
-// Prediction (labels_out) takes the maximum; the loss is ln(sum) + c (largest - z[target]), the
-// form without cancellation, and its mean is summed in double: per block, then by the last block.
+// In units of ln 2 a row's log sum exp is base + log2(sum), its loss that less z[target] scale2, and
+// its largest log-probability the negative of that with the largest logit, all taken in double so
+// that nothing is lost where they cancel. The loss's mean is summed in double: per block, then by the
+// last block.
 template <int LANES>
 __global__ void __launch_bounds__(kThreads)
     k_join_rows(RowSet* rows, const uint32_t* __restrict__ row_of, const float2* __restrict__ partials,
-                const uint32_t* __restrict__ partial_labels, uint64_t partial_rows, uint32_t slots, float scale,
-                float scale2, const float* __restrict__ target_logits, uint64_t n, float* __restrict__ losses,
+                const uint32_t* __restrict__ partial_labels, uint64_t partial_rows, uint32_t slots, float scale2,
+                const float* __restrict__ target_logits, uint64_t n, float* __restrict__ losses,
                 float* __restrict__ normalizers, int32_t* __restrict__ labels_out, float* __restrict__ log_probability,
                 double* __restrict__ block_sums, float* __restrict__ mean) {
     chain_enter();
@@ -254,29 +259,32 @@ __global__ void __launch_bounds__(kThreads)
     const uint32_t lane = threadIdx.x % LANES;
     double loss = 0.0;
     if (i < count) {
-        Joined all{-INFINITY, 0.0f, 0xffffffffu};
+        Joined all{-INFINITY, -INFINITY, 0.0, 0xffffffffu};
         for (uint32_t s = lane; s < slots; s += LANES) {
             const float2 p = partials[s * partial_rows + i];
-            all = join(all, Joined{p.x, p.y, partial_labels ? partial_labels[s * partial_rows + i] : 0u}, scale2);
+            const uint32_t label = partial_labels ? partial_labels[s * partial_rows + i] : 0u;
+            all = join(all, Joined{partial_labels ? __fmul_rn(p.x, scale2) : p.x, p.x, (double)p.y, label});
         }
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) {
             Joined other;
+            other.base = __shfl_xor_sync(0xffffffffu, all.base, o);
             other.largest = __shfl_xor_sync(0xffffffffu, all.largest, o);
             other.sum = __shfl_xor_sync(0xffffffffu, all.sum, o);
             other.label = __shfl_xor_sync(0xffffffffu, all.label, o);
-            all = lane & o ? join(other, all, scale2) : join(all, other, scale2);
+            all = lane & o ? join(other, all) : join(all, other);
         }
         if (lane == 0) {
             const uint32_t row = row_of[i];
-            const float log_sum = logf(all.sum);
+            const double ln2 = 0.6931471805599453, top = all.base == -INFINITY ? 0.0 : (double)all.base;
+            const double log2_sum = top + log2(all.sum);
             if (labels_out) {
                 labels_out[row] = failed ? -1 : (int32_t)all.label;
-                log_probability[row] = failed ? nan : -log_sum;
+                log_probability[row] = failed ? nan : (float)(((double)all.largest * scale2 - log2_sum) * ln2);
             } else {
-                const float value = failed ? nan : fmaf(scale, all.largest - target_logits[i], log_sum);
+                const float value = failed ? nan : (float)((log2_sum - (double)target_logits[i] * scale2) * ln2);
                 losses[row] = value;
-                normalizers[row] = failed ? nan : fmaf(scale, all.largest, log_sum);
+                normalizers[row] = failed ? nan : (float)(log2_sum * ln2);
                 loss = (double)value;
             }
         }
@@ -573,7 +581,7 @@ GemmArgs common_args(const sp_label_head* h, const void* targets, int wide, floa
     std::memset(&a, 0, sizeof(a));
     a.rows = h->rows;
     a.row_of = h->row_of;
-    a.labels = h->labels;
+    a.labels = (uint32_t)h->labels;
     a.products = h->products();
     a.chunk_rows = 0x80000000u;
     a.splits = 1;
@@ -622,7 +630,7 @@ sp_status run_stats(sp_label_head* h, const Operands& op, const void* targets, i
     auto join = [&](auto kernel, uint32_t lanes) {
         return launch_chained(kernel, grid_for(n * lanes, kThreads), kThreads, 0, ctx->stream, h->rows,
                               static_cast<const uint32_t*>(h->row_of), static_cast<const float2*>(h->partials),
-                              static_cast<const uint32_t*>(a.partial_labels), a.partial_rows, slots, scale, a.scale2,
+                              static_cast<const uint32_t*>(a.partial_labels), a.partial_rows, slots, a.scale2,
                               static_cast<const float*>(h->target_logits), n, losses, normalizers, labels_out,
                               log_probability, h->loss_sums, mean);
     };

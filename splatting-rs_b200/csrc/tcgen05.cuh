@@ -54,15 +54,18 @@ __device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
-// Arrives on a barrier given by its address in the cluster's shared memory.
+// Arrives on a barrier given by its address in the cluster's shared memory. What the arrivals and
+// waits here order are tensor-memory accesses, which their own fences cover, and bulk copies, which
+// the barrier counts; a release at cluster scope would add a memory barrier to each (1.2 of 13
+// stall cycles an instruction in the logits' pass).
 __device__ __forceinline__ void barrier_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
     uint32_t done;
     asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(done)
         : "r"(bar), "r"(parity)
@@ -81,12 +84,16 @@ __device__ __forceinline__ unsigned long long global_ns() {
     return t;
 }
 
+// The clock is read only once many polls have failed: reading it takes longer than most waits.
 __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
-    if (barrier_try(bar, parity)) return true;
-    const unsigned long long start = global_ns();
-    for (uint32_t polls = 1; polls < kPollLimit; ++polls) {
+    unsigned long long start = 0;
+    for (uint32_t polls = 0; polls < kPollLimit; ++polls) {
         if (barrier_try(bar, parity)) return true;
-        if ((polls & 255u) == 0 && global_ns() - start > kWaitLimitNs) return false;
+        if ((polls & 4095u) == 4095u) {
+            const unsigned long long now = global_ns();
+            if (start == 0) start = now;
+            else if (now - start > kWaitLimitNs) return false;
+        }
     }
     return false;
 }
