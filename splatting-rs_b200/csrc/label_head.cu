@@ -45,6 +45,7 @@ struct sp_label_head {
     uint32_t parts() const { return element == SP_F32 ? kParts : 1; }
     uint32_t products() const { return element == SP_F32 ? kPartProducts : 1; }
     uint64_t packed_stride() const { return ((uint64_t)dim + kBlockK - 1) / kBlockK * kBlockK; }
+    uint64_t count_blocks() const { return (max_rows + 63) / 64; }
     uint64_t slope_stride() const { return (labels + kPairTile - 1) / kPairTile * kPairTile; }
 };
 
@@ -52,10 +53,13 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr uint32_t kGatherRows = 64;        // rows a block compacts and copies
-constexpr uint32_t kRecountBlocks = 64;     // up to this many blocks each count all targets themselves
+constexpr uint32_t kCountGroups = 16;       // such blocks' counts are summed this many at a time
+constexpr uint32_t kRecountBlocks = 16;     // up to this many blocks each count all targets themselves
+constexpr uint32_t kLogitWaves = 16, kOutWaves = 4;
+constexpr double kStepUs = 0.19;            // 64 of K of a 128 x 128 tile in a single block
 constexpr double kPairCost = 1.4;           // of a 256 x 256 tile, in 128 x 128 tiles of one block
 constexpr uint32_t kThreadSlots = 8;        // partials per row one thread joins; more take a warp
-constexpr uint64_t kSlopeBudget = 1ull << 28;  // slope elements kept at once (512 MB)
+constexpr uint64_t kSlopeBudget = 5ull << 26;  // slope elements kept at once (640 MB)
 
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
@@ -65,17 +69,30 @@ __device__ __forceinline__ bool has_target(const void* targets, int wide, uint64
     return !targets || index_at(targets, wide, i, labels) >= 0;
 }
 
-__global__ void __launch_bounds__(kThreads) k_count_targets(const void* __restrict__ targets, int wide, uint64_t n,
-                                                            uint64_t labels, uint32_t* __restrict__ counts) {
+// counts[b]: the targets among rows [b, b + 1) kGatherRows; group_counts: of kCountGroups such.
+__global__ void __launch_bounds__(kCountGroups * 32)
+    k_count_targets(const void* __restrict__ targets, int wide, uint64_t n, uint64_t labels,
+                    uint32_t* __restrict__ counts, uint32_t* __restrict__ group_counts) {
     chain_enter();
-    // One warp per kGatherRows rows.
-    const uint32_t block = blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
-    uint32_t found = 0;
-    for (uint32_t r = lane_id(); r < kGatherRows; r += 32) {
-        const uint64_t i = (uint64_t)block * kGatherRows + r;
-        found += __popc(__ballot_sync(0xffffffffu, i < n && has_target(targets, wide, i, labels)));
+    __shared__ uint32_t found[kCountGroups];
+    const uint32_t warp = threadIdx.x / 32, block = blockIdx.x * kCountGroups + warp;
+    uint32_t here = 0;
+#pragma unroll
+    for (uint32_t r = 0; r < kGatherRows; r += 32) {
+        const uint64_t i = (uint64_t)block * kGatherRows + r + lane_id();
+        here += __popc(__ballot_sync(0xffffffffu, i < n && has_target(targets, wide, i, labels)));
     }
-    if (lane_id() == 0 && (uint64_t)block * kGatherRows < n) counts[block] = found;
+    if (lane_id() == 0) {
+        found[warp] = here;
+        if ((uint64_t)block * kGatherRows < n) counts[block] = here;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        uint32_t sum = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kCountGroups; ++w) sum += found[w];
+        group_counts[blockIdx.x] = sum;
+    }
 }
 
 __device__ __forceinline__ uint32_t block_sum(uint32_t v) {
@@ -121,16 +138,37 @@ __device__ __forceinline__ void copy_parts(const T* from, uint32_t columns, bool
     }
 }
 
+// The weight's copy as bf16 parts, where it cannot be read in place (`from` NULL: it can).
+template <typename T>
+struct PackWeight {
+    const T* from;
+    int64_t stride;
+    int vector;
+    bf16* to;
+};
+
 // Compacts the rows with targets (row_of), clears the outputs of the others, and copies the
-// features where they cannot be read in place: `in_place` 0, or some rows left out.
+// features where they cannot be read in place: `in_place` 0, or some rows left out. The first
+// `gather_blocks` blocks do that, the others copy the weight.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    k_gather_rows(const void* __restrict__ targets, int wide, uint64_t n, uint64_t labels,
-                  const uint32_t* __restrict__ counts, const T* __restrict__ features, int64_t stride, uint32_t dim,
-                  int vector, int in_place, RowSet* rows, uint32_t* __restrict__ row_of, bf16* __restrict__ packed,
-                  uint64_t packed_stride, uint64_t part, float* __restrict__ losses, float* __restrict__ normalizers,
-                  T* __restrict__ gradient, int64_t gradient_stride) {
+    k_gather_rows(const void* __restrict__ targets, int wide, uint64_t n, uint64_t labels, uint32_t gather_blocks,
+                  const uint32_t* __restrict__ counts, const uint32_t* __restrict__ group_counts,
+                  const T* __restrict__ features, int64_t stride, uint32_t dim, int vector, int in_place, RowSet* rows,
+                  uint32_t* __restrict__ row_of, bf16* __restrict__ packed, uint64_t packed_stride, uint64_t part,
+                  float* __restrict__ losses, float* __restrict__ normalizers, T* __restrict__ gradient,
+                  int64_t gradient_stride, PackWeight<T> weight) {
     chain_enter();
+    if (blockIdx.x >= gather_blocks) {
+        // A warp per row, eight columns a lane.
+        const uint64_t warps = (uint64_t)(gridDim.x - gather_blocks) * (kThreads / 32);
+        for (uint64_t r = (uint64_t)(blockIdx.x - gather_blocks) * (kThreads / 32) + threadIdx.x / 32; r < labels;
+             r += warps)
+            for (uint32_t c = lane_id() * 8; c < packed_stride; c += 256)
+                copy_parts(weight.from + (int64_t)r * weight.stride + c, c < dim ? dim - c : 0, weight.vector,
+                           weight.to + r * packed_stride + c, labels * packed_stride);
+        return;
+    }
     __shared__ uint32_t chosen[kGatherRows];
     __shared__ uint32_t skipped[kGatherRows];
     __shared__ uint32_t half_count[2];
@@ -141,14 +179,17 @@ __global__ void __launch_bounds__(kThreads)
         before = (uint32_t)first;
         all = (uint32_t)n;
     } else if (counts) {
-        for (uint32_t b = t; b < gridDim.x; b += kThreads) {
-            const uint32_t c = counts[b];
+        const uint32_t group = blockIdx.x / kCountGroups, groups = (gather_blocks + kCountGroups - 1) / kCountGroups;
+        for (uint32_t g = t; g < groups; g += kThreads) {
+            const uint32_t c = group_counts[g];
             all += c;
-            if (b < blockIdx.x) before += c;
+            if (g < group) before += c;
         }
+        if (t < blockIdx.x % kCountGroups) before += counts[group * kCountGroups + t];
         before = block_sum(before);
         all = block_sum(all);
     } else {
+#pragma unroll 4
         for (uint64_t i = t; i < n; i += kThreads)
             if (has_target(targets, wide, i, labels)) {
                 ++all;
@@ -191,32 +232,15 @@ __global__ void __launch_bounds__(kThreads)
                 gradient[(int64_t)(first + skipped[k]) * gradient_stride + c] = from_float<T>(0.0f);
     }
     if (in_place && all == n) return;
-    const uint32_t packs = (uint32_t)(packed_stride / 8);
-    for (uint32_t i = t; i < here * packs; i += kThreads) {
-        const uint32_t r = i / packs, c = (i - r * packs) * 8;
-        copy_parts(features + (int64_t)(first + chosen[r]) * stride + c, c < dim ? dim - c : 0, vector,
-                   packed + (uint64_t)(before + r) * packed_stride + c, part);
-    }
+    for (uint32_t r = t / 32; r < here; r += kThreads / 32)
+        for (uint32_t c = lane * 8; c < packed_stride; c += 256)
+            copy_parts(features + (int64_t)(first + chosen[r]) * stride + c, c < dim ? dim - c : 0, vector,
+                       packed + (uint64_t)(before + r) * packed_stride + c, part);
     // Zero rows up to a whole tile: the weight's gradient sums over them.
     const uint64_t end = ((uint64_t)all + kTile - 1) / kTile * kTile;
-    for (uint64_t r = all + blockIdx.x; r < end; r += gridDim.x)
+    for (uint64_t r = all + blockIdx.x; r < end; r += gather_blocks)
         for (uint32_t c = t * 8; c < packed_stride; c += kThreads * 8)
             copy_parts(features, 0, false, packed + r * packed_stride + c, part);
-}
-
-// Rows of a matrix as bf16 parts.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) k_pack_rows(const T* __restrict__ from, int64_t stride, uint64_t rows,
-                                                        uint32_t dim, int vector, bf16* __restrict__ to,
-                                                        uint64_t packed_stride, uint64_t part) {
-    chain_enter();
-    const uint64_t packs = packed_stride / 8;
-    for (uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x; i < rows * packs;
-         i += (uint64_t)gridDim.x * kThreads) {
-        const uint64_t r = i / packs;
-        const uint32_t c = (uint32_t)(i - r * packs) * 8;
-        copy_parts(from + (int64_t)r * stride + c, c < dim ? dim - c : 0, vector, to + r * packed_stride + c, part);
-    }
 }
 
 // ------------------------------------------------------------------ joining
@@ -290,32 +314,35 @@ __global__ void __launch_bounds__(kThreads)
         }
     }
     if (labels_out) return;
-    __shared__ double shared[kThreads];
+    __shared__ double shared[kThreads / 32];
     __shared__ bool last;
-    auto sum_shared = [&]() {
-        for (int half = kThreads / 2; half > 0; half >>= 1) {
-            __syncthreads();
-            if ((int)threadIdx.x < half) shared[threadIdx.x] += shared[threadIdx.x + half];
+    // The block's sum, in thread 0, added in a fixed order.
+    auto block_total = [&](double v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane_id() == 0) shared[threadIdx.x / 32] = v;
+        __syncthreads();
+        double sum = 0.0;
+        if (threadIdx.x == 0)
+            for (int w = 0; w < kThreads / 32; ++w) sum += shared[w];
+        return sum;
+    };
+    double sum = block_total(loss);
+    if (gridDim.x > 1) {
+        if (threadIdx.x == 0) {
+            block_sums[blockIdx.x] = sum;
+            __threadfence();
+            last = atomicAdd(&rows->ticket, 1u) == gridDim.x - 1;
         }
         __syncthreads();
-    };
-    shared[threadIdx.x] = loss;
-    sum_shared();
-    if (threadIdx.x == 0) {
-        block_sums[blockIdx.x] = shared[0];
+        if (!last) return;
         __threadfence();
-        last = atomicAdd(&rows->ticket, 1u) == gridDim.x - 1;
+        sum = 0.0;
+        for (uint32_t b = threadIdx.x; b < gridDim.x; b += kThreads) sum += __ldcg(block_sums + b);
+        sum = block_total(sum);
     }
-    __syncthreads();
-    if (!last) return;
-    __threadfence();
-    double sum = 0.0;
-    for (uint32_t b = threadIdx.x; b < gridDim.x; b += kThreads) sum += __ldcg(block_sums + b);
-    __syncthreads();
-    shared[threadIdx.x] = sum;
-    sum_shared();
     if (threadIdx.x == 0) {
-        *mean = failed ? nan : (float)(shared[0] / (double)max(count, 1u));
+        *mean = failed ? nan : (float)(sum / (double)max(count, 1u));
         rows->ticket = 0;
     }
 }
@@ -432,15 +459,16 @@ uint32_t tiles_of(uint64_t n, bool pair) { return (uint32_t)((n + (pair ? kPairT
 
 // The cut that finishes soonest: whole waves of blocks times the longest piece, a pair's tile
 // counted as kPairCost single ones (four times the products on two SMs that share their operands).
-// At most four waves of pieces where there is more than one.
+// At most kLogitWaves waves of pieces where there is more than one; starting a piece costs about a tenth
+// of a tile.
 Plan plan_logits(uint32_t sms, uint64_t rows, uint64_t labels) {
     Plan best{};
     double best_cost = 1e300;
     for (int pair = 0; pair < 2; ++pair) {
         const uint32_t workers = pair ? std::max(sms / 2, 1u) : sms;
         const uint32_t m = tiles_of(rows, pair), n = tiles_of(labels, pair);
-        for (uint32_t s = 1; s <= n && (s == 1 || (uint64_t)m * s <= 4ull * workers); ++s) {
-            const double cost = (double)(((uint64_t)m * s + workers - 1) / workers) * ((n + s - 1) / s) *
+        for (uint32_t s = 1; s <= n && (s == 1 || (uint64_t)m * s <= (uint64_t)kLogitWaves * workers); ++s) {
+            const double cost = (double)(((uint64_t)m * s + workers - 1) / workers) * ((n + s - 1) / s + 0.1) *
                                 (pair ? kPairCost : 1.0);
             if (cost < best_cost) best_cost = cost, best = Plan{pair != 0, m, n, s};
         }
@@ -448,21 +476,24 @@ Plan plan_logits(uint32_t sms, uint64_t rows, uint64_t labels) {
     return best;
 }
 
-// The same for an output gradient of m x n. Its pieces go through f32 sums, so more of them are
-// taken only where that shortens the products by a tenth, at most two waves, none below 4 steps.
-Plan plan_out(uint32_t sms, uint64_t rows, uint64_t columns, uint32_t k_blocks) {
+// The same for an output gradient. Its pieces go through f32 sums, written and read at some
+// 6.5 TB/s against kStepUs for a single block's step; at most kOutWaves waves, none below 4 steps.
+// `cost`: in microseconds.
+Plan plan_out(uint32_t sms, uint64_t rows, uint64_t columns, uint32_t k_blocks, double* cost_out = nullptr) {
     Plan best{};
     double best_cost = 1e300;
     for (int pair = 0; pair < 2; ++pair) {
         const uint32_t workers = pair ? std::max(sms / 2, 1u) : sms;
         const uint32_t m = tiles_of(rows, pair), n = tiles_of(columns, pair);
         const uint64_t tiles = (uint64_t)m * n;
-        for (uint32_t s = 1; s == 1 || (tiles * s <= 2ull * workers && k_blocks >= 4 * s); ++s) {
-            const double cost = (double)((tiles * s + workers - 1) / workers) * ((k_blocks + s - 1) / s) *
-                                (pair ? kPairCost : 1.0);
-            if (cost < 0.9 * best_cost) best_cost = cost, best = Plan{pair != 0, m, n, s};
+        for (uint32_t s = 1; s == 1 || (tiles * s <= (uint64_t)kOutWaves * workers && k_blocks >= 4 * s); ++s) {
+            double cost = (double)((tiles * s + workers - 1) / workers) * ((k_blocks + s - 1) / s) * kStepUs *
+                          (pair ? kPairCost : 1.0);
+            if (s > 1) cost += (double)s * rows * columns * 8.0 / 6.5e6;
+            if (cost < best_cost) best_cost = cost, best = Plan{pair != 0, m, n, s};
         }
     }
+    if (cost_out) *cost_out = best_cost;
     return best;
 }
 
@@ -471,9 +502,37 @@ uint64_t chunk_limit(const sp_label_head* h) {
     return std::min(std::max<uint64_t>(rows, kPairTile), round_up(h->max_rows, kPairTile));
 }
 
-// Rows of f32 sums a gradient may need. plan_out: pieces times tiles stay within two waves, or one
-// piece; one piece needs sums for the weight's gradient alone, over several chunks.
-uint64_t sums_rows(const sp_label_head* h) { return std::max<uint64_t>(2ull * h->sms * kTile, h->labels); }
+// The rows of slopes taken at once: all of them, or else of the even cuts and of those that fill the
+// SMs with whole tiles of the features' gradient, the one whose products finish soonest.
+uint64_t chunk_for(const sp_label_head* h, uint64_t rows) {
+    const uint64_t limit = std::min(chunk_limit(h), round_up(rows, kPairTile));
+    if (rows <= limit) return limit;
+    const uint32_t label_k = (uint32_t)((h->labels + kBlockK - 1) / kBlockK);
+    const uint64_t wave = std::max<uint64_t>(h->sms / 2 / tiles_of(h->dim, true), 1) * kPairTile;
+    const uint64_t fewest = (rows + limit - 1) / limit;
+    uint64_t best = 0;
+    double best_cost = 1e300;
+    auto consider = [&](uint64_t chunk) {
+        if (chunk == 0 || chunk > limit) return;
+        double cost = 0.0;
+        const uint64_t whole = rows / chunk, rest = rows % chunk;
+        for (uint64_t part : {chunk, rest}) {
+            if (part == 0) continue;
+            double f = 0.0, w = 0.0;
+            plan_out(h->sms, part, h->dim, label_k, &f);
+            plan_out(h->sms, h->labels, h->dim, (uint32_t)((part + kBlockK - 1) / kBlockK), &w);
+            cost += (f + w) * (part == chunk ? (double)whole : 1.0);
+        }
+        if (cost < best_cost) best_cost = cost, best = chunk;
+    };
+    for (uint64_t chunks = fewest; chunks < fewest + 3; ++chunks) consider(round_up((rows + chunks - 1) / chunks, kPairTile));
+    consider(limit / wave * wave);
+    return best;
+}
+
+// Rows of f32 sums a gradient may need. plan_out: pieces times tiles stay within kOutWaves waves, or
+// one piece; one piece needs sums for the weight's gradient alone, over several chunks.
+uint64_t sums_rows(const sp_label_head* h) { return std::max<uint64_t>((uint64_t)kOutWaves * h->sms * kTile, h->labels); }
 
 uint64_t sums_stride(const sp_label_head* h) { return ((uint64_t)h->dim + 3) / 4 * 4; }
 
@@ -551,25 +610,24 @@ sp_status prepare(sp_label_head* h, const void* features, int64_t feature_stride
     const unsigned blocks = grid_for(n, kGatherRows);
     const uint32_t* counts = nullptr;
     if (targets && blocks > kRecountBlocks) {
-        SP_CUDA(ctx, launch_chained(k_count_targets, grid_for(blocks, kThreads / 32), kThreads, 0, st, targets, wide, n,
-                                    h->labels, h->counts));
+        SP_CUDA(ctx, launch_chained(k_count_targets, grid_for(blocks, kCountGroups), kCountGroups * 32, 0, st, targets,
+                                    wide, n, h->labels, h->counts, h->counts + h->count_blocks()));
         counts = h->counts;
     }
     auto gather = [&](auto* typed) {
         using T = std::remove_pointer_t<decltype(typed)>;
-        cudaError_t err = launch_chained(k_gather_rows<T>, blocks, kThreads, 0, st, targets, wide, n, h->labels, counts,
-                                         static_cast<const T*>(features), feature_stride, h->dim,
-                                         (int)vector_rows(h, features, feature_stride), (int)features_here, h->rows,
-                                         h->row_of, h->packed_features, stride, capacity * stride, losses, normalizers,
-                                         static_cast<T*>(gradient), gradient_stride);
-        if (err == cudaSuccess && !weight_here) {
-            const uint64_t packs = h->labels * (stride / 8);
-            const unsigned grid = (unsigned)std::min<uint64_t>((packs + kThreads - 1) / kThreads, 148 * 16);
-            err = launch_chained(k_pack_rows<T>, grid, kThreads, 0, st, static_cast<const T*>(weight), weight_stride,
-                                 h->labels, h->dim, (int)vector_rows(h, weight, weight_stride), h->packed_weight,
-                                 stride, h->labels * stride);
+        PackWeight<T> pack{nullptr, weight_stride, (int)vector_rows(h, weight, weight_stride), h->packed_weight};
+        unsigned weight_blocks = 0;
+        if (!weight_here) {
+            pack.from = static_cast<const T*>(weight);
+            weight_blocks = (unsigned)std::min<uint64_t>((h->labels + kThreads / 32 - 1) / (kThreads / 32), 148 * 16);
         }
-        return err;
+        return launch_chained(k_gather_rows<T>, blocks + weight_blocks, kThreads, 0, st, targets, wide, n, h->labels,
+                              blocks, counts, static_cast<const uint32_t*>(h->counts + h->count_blocks()),
+                              static_cast<const T*>(features), feature_stride, h->dim,
+                              (int)vector_rows(h, features, feature_stride), (int)features_here, h->rows, h->row_of,
+                              h->packed_features, stride, capacity * stride, losses, normalizers,
+                              static_cast<T*>(gradient), gradient_stride, pack);
     };
     const cudaError_t err = h->element == SP_F32 ? gather((float*)nullptr) : gather((bf16*)nullptr);
     SP_CUDA(ctx, err);
@@ -669,11 +727,11 @@ sp_status sp_label_head_create(sp_context* ctx, uint64_t labels, uint32_t dim, s
         SP_CHECK(allocate(h, &h->rows, 1));
         SP_CUDA(ctx, cudaMemsetAsync(h->rows, 0, sizeof(RowSet), ctx->stream));
         SP_CHECK(allocate(h, &h->row_of, max_rows));
-        SP_CHECK(allocate(h, &h->counts, (max_rows + kGatherRows - 1) / kGatherRows));
+        SP_CHECK(allocate(h, &h->counts, h->count_blocks() + (h->count_blocks() + kCountGroups - 1) / kCountGroups));
         SP_CHECK(allocate(h, &h->packed_features, capacity * stride * h->parts()));
         SP_CHECK(allocate(h, &h->packed_weight, labels * stride * h->parts()));
-        // plan_logits: pieces times row tiles stay within four waves, or one piece.
-        const uint64_t slots = 2 * kTile * std::max<uint64_t>(capacity / kTile, 4ull * h->sms);
+        // plan_logits: pieces times row tiles stay within kLogitWaves waves, or one piece.
+        const uint64_t slots = 2 * kTile * std::max<uint64_t>(capacity / kTile, (uint64_t)kLogitWaves * h->sms);
         SP_CHECK(allocate(h, &h->partials, slots));
         SP_CHECK(allocate(h, &h->partial_labels, slots));
         SP_CHECK(allocate(h, &h->target_logits, capacity));
@@ -771,22 +829,23 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
     SP_CHECK(prepare(h, d_features, feature_stride, d_weight, weight_stride, d_targets, wide, rows, nullptr, nullptr,
                      d_feature_gradient, feature_gradient_stride, &op));
 
-    const uint64_t limit = chunk_limit(h), chunks = (rows + limit - 1) / limit;
-    const uint64_t chunk = round_up((rows + chunks - 1) / chunks, kPairTile);
+    const uint64_t chunk = chunk_for(h, rows), chunks = (rows + chunk - 1) / chunk;
     const uint64_t slope_stride = h->slope_stride(), sum_stride = sums_stride(h);
     CUtensorMap slopes, slopes_out;
     SP_CHECK(make_map(ctx, &slopes, h->slopes, slope_stride, chunk, slope_stride, h->parts(), chunk * slope_stride));
     SP_CHECK(make_map(ctx, &slopes_out, h->slopes, slope_stride, chunk, slope_stride, h->parts(), chunk * slope_stride, 32));
     const uint32_t label_k = (uint32_t)((h->labels + kBlockK - 1) / kBlockK);
-    const uint64_t chunk_rows = std::min(chunk, rows);
-    const Plan logits = plan_logits(h->sms, chunk_rows, h->labels);
-    const Plan to_features = plan_out(h->sms, chunk_rows, h->dim, label_k);
-    const Plan to_weight = plan_out(h->sms, h->labels, h->dim, (uint32_t)((chunk_rows + kBlockK - 1) / kBlockK));
-    const bool feature_sums = to_features.splits > 1, weight_sums = to_weight.splits > 1 || chunks > 1;
+    // One cut of the weight's gradient for every chunk: its pieces' sums go on from one to the next.
+    const Plan to_weight = plan_out(h->sms, h->labels, h->dim, (uint32_t)((std::min(chunk, rows) + kBlockK - 1) / kBlockK));
+    const bool weight_sums = to_weight.splits > 1 || chunks > 1;
     float* weight_sum = h->sums;
     float* feature_sum = h->sums + sums_rows(h) * sum_stride;
 
     for (uint64_t c = 0; c < chunks; ++c) {
+        const uint64_t here = std::min(chunk, rows - c * chunk);
+        const Plan logits = plan_logits(h->sms, here, h->labels);
+        const Plan to_features = plan_out(h->sms, here, h->dim, label_k);
+        const bool feature_sums = to_features.splits > 1;
         GemmArgs a = common_args(h, d_targets, wide, logit_scale);
         a.first_row = (uint32_t)(c * chunk);
         a.chunk_rows = (uint32_t)chunk;
@@ -805,7 +864,7 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
         f.partial = feature_sums;
         f.out = feature_sums ? (void*)feature_sum : d_feature_gradient;
         f.out_stride = feature_sums ? (int64_t)sum_stride : feature_gradient_stride;
-        f.out_rows = chunk;
+        f.out_rows = here;
         f.out_columns = h->dim;
         f.scatter = !feature_sums;
         f.out_packed = vector_rows(h, d_feature_gradient, feature_gradient_stride);
@@ -834,12 +893,12 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
         SP_CUDA(ctx, h->element == SP_F32 ? run_weight((float*)nullptr) : run_weight((bf16*)nullptr));
 
         const bool last = c + 1 == chunks;
-        JoinArgs jf{feature_sums ? feature_sum : nullptr, to_features.splits, chunk, sum_stride, 1, a.first_row,
+        JoinArgs jf{feature_sums ? feature_sum : nullptr, to_features.splits, here, sum_stride, 1, a.first_row,
                     d_feature_gradient, feature_gradient_stride, last ? rows : 0};
         JoinArgs jw{weight_sums && last ? weight_sum : nullptr, to_weight.splits, h->labels, sum_stride, 0, 0,
                     d_weight_gradient, weight_gradient_stride, last ? h->labels : 0};
         if (!last && !feature_sums) continue;
-        const uint64_t quads = std::max(feature_sums ? chunk * (sum_stride / 4) : 0,
+        const uint64_t quads = std::max(feature_sums ? here * (sum_stride / 4) : (uint64_t)0,
                                         jw.sums ? h->labels * (sum_stride / 4) : (uint64_t)0);
         const unsigned grid = (unsigned)std::min<uint64_t>(std::max<uint64_t>((quads + kThreads - 1) / kThreads, 1),
                                                            148 * 16);
