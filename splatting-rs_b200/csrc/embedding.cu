@@ -3,12 +3,15 @@
 // Lookup: out[i] = s T[t_i], a gather of whole rows, bound by the bytes of `out` (the table's
 // rows are re-read from L2).
 //
-// Gradient: dT[v] = s sum_{i: t_i = v} dOut[i], without atomics so that the sums have one order:
-// the (token, position) pairs go through the renderer's stable radix sort (sort.cu), the sorted
-// list is cut into pieces of a fixed length, each piece's runs are summed in f32 registers while
-// dOut's rows stream past once (bound by those bytes), and a token whose run crosses pieces is
-// joined from the pieces' partial sums, in order, by a second kernel, which also writes the zero
-// rows of the tokens nobody has.
+// Gradient: dT[v] = s sum_{i: t_i = v} dOut[i], without atomics on the sums, so that they have one
+// order whatever the scheduling, in one of two ways:
+//  - up to kFewTokens tokens: one kernel whose blocks each own a range of entries, pick their tokens
+//    out of the whole list, order them by entry and position in shared memory and sum the rows
+//    (latency: a sort of the list alone is four launches);
+//  - more: the (token, position) pairs go through the renderer's stable radix sort (sort.cu), each
+//    block sums the runs of a fixed stretch of the sorted list while dOut's rows stream past once
+//    (bound by those bytes), and a token whose run crosses stretches is joined from their partial
+//    sums, in order, by a second kernel, which also writes the zero rows of the tokens nobody has.
 #include <algorithm>
 #include <new>
 
@@ -42,13 +45,23 @@ constexpr int kThreads = 256;
 constexpr int kEmitItems = 8;
 constexpr int kLookupRows = 4;   // rows in flight per thread
 constexpr int kPieceRows = 8;    // rows in flight per thread while summing
-constexpr uint32_t kShortPiece = 16, kLongPiece = 64;
+constexpr int kFewRows = 4;      // ... in blocks of 1024 threads, 64 registers each
+constexpr int kMinLanesLog2 = 2; // at least 4 threads a row while summing
+constexpr uint32_t kShortPiece = 16, kLongPiece = 64, kMostStretch = 2048;
+constexpr uint32_t kFewTokens = 32768;         // 32 warps x 32 x 32 lanes
+constexpr uint64_t kFewReads = 1ull << 24;     // token reads of all blocks together
+constexpr uint32_t kFewThreads = 1024, kMostOwned = 512, kLongRun = 64;
 
-// The sorted positions per piece: long pieces keep the partial sums few, short ones give a small
-// list enough pieces to fill the SMs (148 SMs x 8 warps of pieces either way).
-uint32_t piece_length(uint64_t count) { return count >= (uint64_t)kLongPiece * 148 * 8 ? kLongPiece : kShortPiece; }
+// Sorted positions per group of threads: long pieces make fewer partial sums, short ones give a
+// small list enough groups to fill the SMs (148 SMs x 8 groups of pieces either way).
+uint32_t piece_length(uint64_t count, int lanes_log2) {
+    const uint32_t piece = count >= (uint64_t)kLongPiece * 148 * 8 ? kLongPiece : kShortPiece;
+    return std::min(piece, kMostStretch / ((uint32_t)kThreads >> lanes_log2));
+}
 
-// `lanes` threads (a power of two, at most 32) move one row, N elements at a time.
+// `lanes` threads (a power of two, at most 32) move one row, N elements at a time; kLookupRows rows
+// a thread, the next ones' tokens read meanwhile. The rows are written past the caches' usual
+// residents (the table stays in L2).
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) k_lookup(const T* __restrict__ table, int64_t table_stride,
                                                      const void* __restrict__ tokens, int wide, uint64_t count,
@@ -58,29 +71,37 @@ __global__ void __launch_bounds__(kThreads) k_lookup(const T* __restrict__ table
     const uint32_t lanes = 1u << lanes_log2, lane = threadIdx.x & (lanes - 1);
     const uint64_t rows_per_pass = kThreads >> lanes_log2;
     const uint32_t packs = dim / N;
-    for (uint64_t base = (uint64_t)blockIdx.x * rows_per_pass * kLookupRows; base < count;
-         base += (uint64_t)gridDim.x * rows_per_pass * kLookupRows) {
-        int64_t token[kLookupRows];
-        uint64_t row[kLookupRows];
+    const uint64_t step = (uint64_t)gridDim.x * rows_per_pass * kLookupRows;
+    uint64_t row = (uint64_t)blockIdx.x * rows_per_pass * kLookupRows + (threadIdx.x >> lanes_log2);
+    int64_t next[kLookupRows];
+    auto read_tokens = [&](uint64_t from) {
 #pragma unroll
         for (int k = 0; k < kLookupRows; ++k) {
-            row[k] = base + k * rows_per_pass + (threadIdx.x >> lanes_log2);
-            token[k] = row[k] < count ? index_at(tokens, wide, row[k], entries) : -1;
+            const uint64_t i = from + k * rows_per_pass;
+            next[k] = i < count ? index_at(tokens, wide, i, entries) : -1;
         }
+    };
+    read_tokens(row);
+    for (; row < count; row += step) {
+        int64_t token[kLookupRows];
+#pragma unroll
+        for (int k = 0; k < kLookupRows; ++k) token[k] = next[k];
+        read_tokens(row + step);
         for (uint32_t p = lane; p < packs; p += lanes) {
             Pack<T, N> v[kLookupRows];
 #pragma unroll
             for (int k = 0; k < kLookupRows; ++k)
-                if (token[k] >= 0)
-                    v[k] = *reinterpret_cast<const Pack<T, N>*>(table + token[k] * table_stride + (uint64_t)p * N);
+                if (token[k] >= 0) v[k] = load_pack<T, N>(table + token[k] * table_stride + (uint64_t)p * N);
 #pragma unroll
             for (int k = 0; k < kLookupRows; ++k) {
-                if (row[k] >= count) continue;
-                Pack<T, N> o;
+                const uint64_t i = row + k * rows_per_pass;
+                if (i >= count) continue;
+                float scaled[N];
 #pragma unroll
-                for (int j = 0; j < N; ++j)
-                    o.v[j] = token[k] >= 0 ? from_float<T>(to_float(v[k].v[j]) * scale) : from_float<T>(0.0f);
-                *reinterpret_cast<Pack<T, N>*>(out + (int64_t)row[k] * out_stride + (uint64_t)p * N) = o;
+                for (int j = 0; j < N; ++j) scaled[j] = token[k] >= 0 ? v[k].get(j) * scale : 0.0f;
+                Pack<T, N> o;
+                o.set(scaled);
+                store_streaming(out + (int64_t)i * out_stride + (uint64_t)p * N, o);
             }
         }
     }
@@ -123,10 +144,27 @@ __global__ void __launch_bounds__(kThreads) k_emit_tokens(const void* __restrict
     }
 }
 
-// A piece of the sorted list per group of `lanes` threads, N columns a thread (blockIdx.y: the
-// next lanes * N columns). A run that begins and ends inside its piece is a token's whole sum and
-// is written out; the others leave partial sums: slot 0 of the piece for a run that began before
-// it, slot 1 for one that begins inside and goes on.
+// N columns of a row of sums, scaled and rounded.
+template <typename T, int N>
+__device__ __forceinline__ void store_row(T* to, const float (&sum)[N], float scale, bool packed) {
+    if (packed) {
+        float scaled[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) scaled[j] = sum[j] * scale;
+        Pack<T, N> o;
+        o.set(scaled);
+        store_pack(to, o);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) to[j] = from_float<T>(sum[j] * scale);
+    }
+}
+
+// A stretch of the sorted list per block, a piece of it per group of `lanes` threads, N columns a
+// thread (blockIdx.y: the next lanes * N columns). A run inside its piece is a token's whole sum and
+// is written out. A run over several pieces is added up from their partial sums in shared memory by
+// the piece it begins in; one that crosses stretches leaves partial sums in memory: slot 0 of the
+// stretch for a run that began before it, slot 1 for one that begins inside and goes on.
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads)
     k_sum_pieces(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ positions, uint32_t count,
@@ -135,82 +173,122 @@ __global__ void __launch_bounds__(kThreads)
                  uint32_t partial_stride, uint32_t piece, int lanes_log2, const DeviceMeta* __restrict__ meta) {
     chain_enter();
     if (meta->status != 0) return;  // the list may be out of order: k_join_pieces writes NaN
-    const uint32_t lanes = 1u << lanes_log2;
-    const uint32_t group = blockIdx.x * (kThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
+    __shared__ uint32_t s_key[kMostStretch + 2];  // with the neighbours on both sides
+    __shared__ uint32_t s_position[kMostStretch];
+    __shared__ float s_part[2][kThreads][N];
+    constexpr uint32_t kNobody = 0xffffffffu;
+    const uint32_t lanes = 1u << lanes_log2, groups = kThreads >> lanes_log2;
+    const uint32_t group = threadIdx.x >> lanes_log2, stretch = groups * piece;
+    const uint64_t first = (uint64_t)blockIdx.x * stretch;
+    for (uint32_t i = threadIdx.x; i < stretch + 2; i += kThreads) {
+        const uint64_t at = first + i;  // of the list, plus 1
+        s_key[i] = at >= 1 && at <= count ? keys[at - 1] : kNobody;
+        if (i < stretch && at < count) s_position[i] = positions[at];
+    }
+    __syncthreads();
+    const uint32_t* key = s_key + 1;
+    const uint32_t here = (uint32_t)min((uint64_t)stretch, count - first);
     const uint32_t column = (blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * N;
-    const uint64_t first = (uint64_t)group * piece;
-    if (first >= count || column >= dim) return;
-    const uint32_t begin = (uint32_t)first, end = (uint32_t)min((uint64_t)count, first + piece);
-    float acc[N];
+    const bool inside = column < dim;
+    const uint32_t begin = group * piece, end = min(begin + piece, here);
+    T* const out_column = out + column;
+    bool tail = false;  // the last run begins here and goes on
+    if (inside && begin < here) {
+        float acc[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] = 0.0f;
-    uint32_t current = keys[begin];
-    bool from_before = begin > 0 && keys[begin - 1] == current;
-    auto flush = [&](bool goes_on) {
-        if (current >= entries) return;
-        if (!from_before && !goes_on) {
-            T* to = out + (int64_t)current * out_stride + column;
-            Pack<T, N> o;
+        for (int j = 0; j < N; ++j) acc[j] = 0.0f;
+        uint32_t current = key[begin];
+        bool from_before = key[(int)begin - 1] == current;
+        for (uint32_t i = begin; i < end; i += kPieceRows) {
+            Pack<T, N> v[kPieceRows];
 #pragma unroll
-            for (int j = 0; j < N; ++j) o.v[j] = from_float<T>(acc[j] * scale);
-            if (out_packed) {
-                *reinterpret_cast<Pack<T, N>*>(to) = o;
-            } else {
+            for (int k = 0; k < kPieceRows; ++k)
+                if (i + k < end && key[i + k] < entries)
+                    v[k] = load_pack<T, N>(upstream + (int64_t)s_position[i + k] * upstream_stride + column);
 #pragma unroll
-                for (int j = 0; j < N; ++j) to[j] = o.v[j];
-            }
-        } else {
-            float* to = partials + ((uint64_t)group * 2 + (from_before ? 0 : 1)) * partial_stride + column;
+            for (int k = 0; k < kPieceRows; ++k) {
+                if (i + k >= end) break;
+                const uint32_t now = key[i + k];
+                if (now != current) {
+                    if (from_before) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) to[j] = acc[j];
-        }
-    };
-    for (uint32_t i = begin; i < end; i += kPieceRows) {
-        uint32_t key[kPieceRows];
-        Pack<T, N> v[kPieceRows];
+                        for (int j = 0; j < N; ++j) s_part[0][threadIdx.x][j] = acc[j];
+                    } else if (current < entries) {
+                        store_row<T, N>(out_column + (int64_t)current * out_stride, acc, scale, out_packed);
+                    }
+                    current = now;
+                    from_before = false;
 #pragma unroll
-        for (int k = 0; k < kPieceRows; ++k) {
-            key[k] = entries;
-            if (i + k < end) {
-                key[k] = keys[i + k];
-                if (key[k] < entries)
-                    v[k] = *reinterpret_cast<const Pack<T, N>*>(upstream + (int64_t)positions[i + k] * upstream_stride +
-                                                                column);
+                    for (int j = 0; j < N; ++j) acc[j] = 0.0f;
+                }
+                if (now < entries) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) acc[j] += v[k].get(j);
+                }
             }
         }
+        const bool goes_on = key[end] == current;
+        if (from_before || goes_on) {
+            tail = !from_before;
 #pragma unroll
-        for (int k = 0; k < kPieceRows; ++k) {
-            if (i + k >= end) break;
-            if (key[k] != current) {
-                flush(false);
-                current = key[k];
-                from_before = false;
-#pragma unroll
-                for (int j = 0; j < N; ++j) acc[j] = 0.0f;
-            }
-            if (key[k] < entries) {
-#pragma unroll
-                for (int j = 0; j < N; ++j) acc[j] += to_float(v[k].v[j]);
-            }
+            for (int j = 0; j < N; ++j) s_part[tail ? 1 : 0][threadIdx.x][j] = acc[j];
+        } else if (current < entries) {
+            store_row<T, N>(out_column + (int64_t)current * out_stride, acc, scale, out_packed);
         }
     }
-    flush(end < count && keys[end] == current);
+    __syncthreads();
+    if (!inside || begin >= here) return;
+    // The run that ends piece `from` (its sum so far in `slot`), through the pieces it goes on over.
+    auto follow = [&](uint32_t from, int slot, bool began_before) {
+        const uint32_t token = key[min((from + 1) * piece, here) - 1];
+        if (token >= entries) return;
+        float sum[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) sum[j] = s_part[slot][threadIdx.x][j];
+        uint32_t at = min((from + 1) * piece, here);  // where the run's next row would be
+        for (uint32_t next = from + 1; at < here && key[at] == token; ++next) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) sum[j] += s_part[0][threadIdx.x + (next - group) * lanes][j];
+            at = min((next + 1) * piece, here);
+            if (key[at - 1] != token) break;  // it ended inside piece `next`
+        }
+        const bool beyond = at == here && key[here - 1] == token && key[here] == token;
+        if (!began_before && !beyond) {
+            store_row<T, N>(out_column + (int64_t)token * out_stride, sum, scale, out_packed);
+        } else {
+            float* to = partials + ((uint64_t)blockIdx.x * 2 + (began_before ? 0 : 1)) * partial_stride + column;
+#pragma unroll
+            for (int j = 0; j < N; ++j) to[j] = sum[j];
+        }
+    };
+    if (group == 0 && key[-1] == key[0]) {
+        if (key[end - 1] == key[0]) {
+            follow(0, 0, true);  // all of the first piece, and perhaps more
+        } else if (key[0] < entries) {
+            float* to = partials + (uint64_t)blockIdx.x * 2 * partial_stride + column;
+#pragma unroll
+            for (int j = 0; j < N; ++j) to[j] = s_part[0][threadIdx.x][j];
+        }
+    }
+    if (tail) follow(group, 1, false);
 }
 
 // Per token: zeros where it has no rows, the ordered sum of its partials where its run crosses
-// pieces, nothing where k_sum_pieces wrote it. A warp per token, 4 columns a lane; a token with
-// more than kWarpPieces partials is joined by the block's eight warps together.
-constexpr uint32_t kJoinWarps = kThreads / 32, kWarpPieces = 32;
+// stretches, nothing where k_sum_pieces wrote it. kJoinTokens tokens a warp, 4 columns a lane; a
+// token with more than kWarpParts partials is joined by the block's eight warps together.
+constexpr uint32_t kJoinWarps = kThreads / 32, kJoinTokens = 8, kWarpParts = 16;
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     k_join_pieces(const uint2* __restrict__ ranges, uint32_t entries, uint32_t dim, float scale, T* __restrict__ out,
-                  int64_t out_stride, const float* __restrict__ partials, uint32_t partial_stride, uint32_t piece,
+                  int64_t out_stride, const float* __restrict__ partials, uint32_t partial_stride, uint32_t stretch,
                   const DeviceMeta* __restrict__ meta) {
     chain_enter();
     __shared__ float4 shared[kJoinWarps][32];
-    __shared__ uint2 span[kJoinWarps];
+    __shared__ uint32_t long_tokens[kJoinWarps * kJoinTokens], longs;
+    if (threadIdx.x == 0) longs = 0;
+    __syncthreads();
     const uint32_t warp = threadIdx.x / 32, lane = lane_id();
-    const uint32_t token = blockIdx.x * kJoinWarps + warp;
+    const uint32_t base = (blockIdx.x * kJoinWarps + warp) * kJoinTokens;
     const bool failed = meta->status != 0;
     auto store = [&](uint32_t v, uint32_t column, float4 sum) {
         const float s[4] = {sum.x, sum.y, sum.z, sum.w};
@@ -219,9 +297,9 @@ __global__ void __launch_bounds__(kThreads)
         for (int j = 0; j < 4; ++j)
             if (column + j < dim) to[j] = from_float<T>(s[j] * scale);
     };
-    // Partial p of a run over the sorted positions [s, e): slot 1 of its first piece, then slot 0.
+    // Partials p0..p1 of the run over sorted positions `run`: slot 1 of its first stretch, then slot 0.
     auto sum_of = [&](uint2 run, uint32_t p0, uint32_t p1, uint32_t column) {
-        const uint32_t first = run.x / piece;
+        const uint32_t first = run.x / stretch;
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
         for (uint32_t p = p0; p < p1; ++p) {
@@ -234,40 +312,176 @@ __global__ void __launch_bounds__(kThreads)
         }
         return sum;
     };
-    uint2 run = make_uint2(0u, 0u);
-    uint32_t pieces = 0;
-    if (token < entries) {
-        run = ranges[token];
-        if (run.y > run.x) pieces = (run.y - 1) / piece - run.x / piece + 1;
-        if (failed || pieces == 0) {
+    auto parts_of = [&](uint2 run) { return run.y > run.x ? (run.y - 1) / stretch - run.x / stretch + 1 : 0u; };
+    uint2 mine = make_uint2(0u, 0u);
+    const bool owns = lane < kJoinTokens && base + lane < entries;
+    if (owns && !failed) mine = ranges[base + lane];
+    for (uint32_t left = __ballot_sync(0xffffffffu, owns && parts_of(mine) != 1); left; left &= left - 1) {
+        const uint32_t k = __ffs(left) - 1, token = base + k;
+        const uint2 run = make_uint2(__shfl_sync(0xffffffffu, mine.x, k), __shfl_sync(0xffffffffu, mine.y, k));
+        const uint32_t parts = parts_of(run);
+        if (parts == 0) {
             const float fill = failed ? __int_as_float(0x7fffffff) : 0.0f;
             for (uint32_t c = lane; c < dim; c += 32) out[(int64_t)token * out_stride + c] = from_float<T>(fill);
-        } else if (pieces > 1 && pieces <= kWarpPieces) {
-            for (uint32_t c = lane * 4; c < dim; c += 128) store(token, c, sum_of(run, 0, pieces, c));
+        } else if (parts <= kWarpParts) {
+            for (uint32_t c = lane * 4; c < dim; c += 128) store(token, c, sum_of(run, 0, parts, c));
+        } else if (lane == 0) {
+            long_tokens[atomicAdd(&longs, 1u)] = token;
         }
     }
-    if (lane == 0) span[warp] = !failed && pieces > kWarpPieces ? run : make_uint2(0u, 0u);
     __syncthreads();
-    for (uint32_t w = 0; w < kJoinWarps; ++w) {
-        const uint2 long_run = span[w];
-        if (long_run.y == long_run.x) continue;
-        const uint32_t n = (long_run.y - 1) / piece - long_run.x / piece + 1;
+    for (uint32_t k = 0; k < longs; ++k) {
+        const uint32_t token = long_tokens[k];
+        const uint2 run = ranges[token];
+        const uint32_t n = parts_of(run);
         const uint32_t p0 = (uint32_t)((uint64_t)n * warp / kJoinWarps);
         const uint32_t p1 = (uint32_t)((uint64_t)n * (warp + 1) / kJoinWarps);
         for (uint32_t c0 = 0; c0 < dim; c0 += 128) {
             const uint32_t c = c0 + lane * 4;
-            if (c < dim) shared[warp][lane] = sum_of(long_run, p0, p1, c);
+            if (c < dim) shared[warp][lane] = sum_of(run, p0, p1, c);
             __syncthreads();
             if (warp == 0 && c < dim) {
                 float4 sum = shared[0][lane];
-                for (uint32_t k = 1; k < kJoinWarps; ++k) {
-                    const float4 v = shared[k][lane];
+                for (uint32_t w = 1; w < kJoinWarps; ++w) {
+                    const float4 v = shared[w][lane];
                     sum.x += v.x;
                     sum.y += v.y;
                     sum.z += v.z;
                     sum.w += v.w;
                 }
-                store(blockIdx.x * kJoinWarps + w, c, sum);
+                store(token, c, sum);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// Up to kFewTokens tokens: block b owns entries [b owned, (b + 1) owned). Each warp reads 1/32 of the
+// tokens into registers and counts its entries' ones; the counts give every (entry, warp) its place in
+// a list of positions in shared memory, ordered by entry and then position; the rows are summed from
+// it, a run of at most kLongRun by one group of `lanes` threads in order, a longer one by all groups in
+// equal parts, joined in order.
+template <typename T, int N>
+__global__ void __launch_bounds__(kFewThreads)
+    k_sum_few(const void* __restrict__ tokens, int wide, uint32_t count, uint64_t entries, uint32_t owned,
+              const T* __restrict__ upstream, int64_t upstream_stride, uint32_t dim, float scale, T* __restrict__ out,
+              int64_t out_stride, int out_packed, int lanes_log2) {
+    chain_enter();
+    constexpr uint32_t kWarps = kFewThreads / 32, kItems = kFewTokens / kFewThreads;
+    extern __shared__ float4 few_smem[];
+    __shared__ uint32_t start[kMostOwned + 1], warp_sums[kWarps];
+    float* s_part = reinterpret_cast<float*>(few_smem);  // [kFewThreads][N]
+    uint16_t* placed = reinterpret_cast<uint16_t*>(s_part + kFewThreads * N);  // [kWarps][owned]
+    uint16_t* order = placed + kWarps * owned;                                 // [count]
+    const uint32_t t = threadIdx.x, warp = t / 32, lane = lane_id();
+    const uint32_t section = (count + kFewThreads - 1) / kFewThreads * 32;  // of the tokens, per warp
+    const int64_t first_entry = (int64_t)blockIdx.x * owned;
+
+    uint32_t token[kItems];
+#pragma unroll
+    for (uint32_t k = 0; k < kItems; ++k) {
+        const uint32_t i = warp * section + k * 32 + lane;
+        token[k] = kMostOwned;
+        if (k * 32 < section && i < count) {
+            const int64_t v = index_at(tokens, wide, i, entries) - first_entry;
+            if (v >= 0 && v < (int64_t)owned) token[k] = (uint32_t)v;
+        }
+    }
+    for (uint32_t i = t; i < kWarps * owned; i += kFewThreads) placed[i] = 0;
+    __syncthreads();
+    const uint32_t below = (1u << lane) - 1u;
+    // place(): the next free places of the warp's tokens, equal ones in lane order.
+    uint16_t* mine = placed + warp * owned;
+    auto for_each_place = [&](auto&& place) {
+#pragma unroll
+        for (uint32_t k = 0; k < kItems; ++k) {
+            const bool here = token[k] < kMostOwned;
+            if (!__any_sync(0xffffffffu, here)) continue;
+            const uint32_t peers = __match_any_sync(0xffffffffu, token[k]);
+            const uint32_t before = here ? mine[token[k]] : 0;
+            __syncwarp();
+            if (here) {
+                if ((peers & below) == 0) mine[token[k]] = (uint16_t)(before + __popc(peers));
+                place(before + __popc(peers & below), warp * section + k * 32 + lane);
+            }
+            __syncwarp();
+        }
+    };
+    for_each_place([](uint32_t, uint32_t) {});
+    __syncthreads();
+    // Entry e's total, and in its column the running counts over the warps; then the entries' scan.
+    uint32_t total = 0;
+    if (t < owned)
+        for (uint32_t w = 0; w < kWarps; ++w) {
+            const uint32_t c = placed[w * owned + t];
+            placed[w * owned + t] = (uint16_t)total;
+            total += c;
+        }
+    uint32_t inclusive = total;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, inclusive, o);
+        if (lane >= (uint32_t)o) inclusive += up;
+    }
+    if (lane == 31) warp_sums[warp] = inclusive;
+    __syncthreads();
+    uint32_t offset = 0;
+    for (uint32_t w = 0; w < warp; ++w) offset += warp_sums[w];
+    if (t < owned) {
+        start[t] = offset + inclusive - total;
+        if (t == owned - 1) start[owned] = offset + inclusive;
+        for (uint32_t w = 0; w < kWarps; ++w) placed[w * owned + t] += (uint16_t)start[t];
+    }
+    __syncthreads();
+    for_each_place([&](uint32_t at, uint32_t position) { order[at] = (uint16_t)position; });
+    __syncthreads();
+
+    const uint32_t lanes = 1u << lanes_log2, groups = kFewThreads >> lanes_log2, group = t >> lanes_log2;
+    const uint32_t entries_here = (uint32_t)min((int64_t)owned, (int64_t)entries - first_entry);
+    auto sum_rows = [&](uint32_t from, uint32_t to, uint32_t column, float (&acc)[N]) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] = 0.0f;
+        for (uint32_t i = from; i < to; i += kFewRows) {
+            Pack<T, N> v[kFewRows];
+#pragma unroll
+            for (int k = 0; k < kFewRows; ++k)
+                if (i + k < to) v[k] = load_pack<T, N>(upstream + (int64_t)order[i + k] * upstream_stride + column);
+#pragma unroll
+            for (int k = 0; k < kFewRows; ++k)
+                if (i + k < to) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) acc[j] += v[k].get(j);
+                }
+        }
+    };
+    const uint32_t first_column = (t & (lanes - 1)) * N;
+    for (uint32_t e = group; e < entries_here; e += groups) {
+        const uint32_t from = start[e], to = start[e + 1];
+        if (to - from > kLongRun) continue;
+        for (uint32_t column = first_column; column < dim; column += lanes * N) {
+            float acc[N];
+            sum_rows(from, to, column, acc);
+            store_row<T, N>(out + (first_entry + e) * out_stride + column, acc, scale, out_packed);
+        }
+    }
+    for (uint32_t e = 0; e < entries_here; ++e) {
+        const uint32_t from = start[e], n = start[e + 1] - from;
+        if (n <= kLongRun) continue;
+        for (uint32_t base = 0; base < dim; base += lanes * N) {
+            const uint32_t column = base + first_column;
+            float acc[N];
+            if (column < dim) {
+                sum_rows(from + (uint32_t)((uint64_t)n * group / groups), from + (uint32_t)((uint64_t)n * (group + 1) / groups),
+                         column, acc);
+#pragma unroll
+                for (int j = 0; j < N; ++j) s_part[t * N + j] = acc[j];
+            }
+            __syncthreads();
+            if (group == 0 && column < dim) {
+                for (uint32_t g = 1; g < groups; ++g)
+#pragma unroll
+                    for (int j = 0; j < N; ++j) acc[j] += s_part[(g * lanes + t) * N + j];
+                store_row<T, N>(out + (first_entry + e) * out_stride + column, acc, scale, out_packed);
             }
             __syncthreads();
         }
@@ -283,8 +497,8 @@ sp_status allocate(sp_embedding* e, T** out, uint64_t count) {
     return SP_OK;
 }
 
-int lanes_log2_for(uint32_t packs) {
-    int log2 = 0;
+int lanes_log2_for(uint32_t packs, int least = 0) {
+    int log2 = least;
     while (log2 < 5 && (1u << log2) < packs) ++log2;
     return log2;
 }
@@ -301,26 +515,52 @@ cudaError_t lookup(const sp_embedding* e, const void* table, int64_t table_strid
                    uint64_t count, float scale, void* out, int64_t out_stride) {
     const int log2 = lanes_log2_for(e->dim / N);
     const uint64_t rows_per_block = (uint64_t)(kThreads >> log2) * kLookupRows;
-    const unsigned grid = (unsigned)std::min<uint64_t>((count + rows_per_block - 1) / rows_per_block, 1u << 20);
+    const unsigned grid = (unsigned)std::min<uint64_t>((count + rows_per_block - 1) / rows_per_block, 148 * 8);
     return launch_chained(k_lookup<T, N>, grid, kThreads, 0, e->ctx->stream, static_cast<const T*>(table),
                           table_stride, tokens, wide, count, e->entries, e->dim, scale, static_cast<T*>(out),
                           out_stride, log2);
 }
 
+// How the gradient's rows are laid over threads: N elements a thread, 2^lanes_log2 threads a row.
+struct Rows {
+    const void* upstream;
+    int64_t upstream_stride;
+    float scale;
+    void* out;
+    int64_t out_stride;
+};
+
 template <typename T, int N>
 cudaError_t sum_pieces(const sp_embedding* e, const uint32_t* keys, const uint32_t* positions, uint32_t count,
-                       const void* upstream, int64_t upstream_stride, float scale, void* out, int64_t out_stride,
-                       uint32_t partial_stride, uint32_t piece) {
-    const int log2 = lanes_log2_for(e->dim / N);
-    const uint32_t per_block = kThreads >> log2;
-    const uint32_t pieces = (count + piece - 1) / piece;
-    const uint32_t columns = N << log2;
-    const dim3 grid((pieces + per_block - 1) / per_block, (e->dim + columns - 1) / columns);
-    const int out_packed = pack_width(out, out_stride, e->dim, sizeof(T)) >= N;
+                       const Rows& r, uint32_t partial_stride, uint32_t piece, int lanes_log2) {
+    const uint32_t stretch = (kThreads >> lanes_log2) * piece, columns = N << lanes_log2;
+    const dim3 grid((count + stretch - 1) / stretch, (e->dim + columns - 1) / columns);
+    const int out_packed = pack_width(r.out, r.out_stride, e->dim, sizeof(T)) >= N;
     return launch_chained(k_sum_pieces<T, N>, grid, kThreads, 0, e->ctx->stream, keys, positions, count,
-                          (uint32_t)e->entries, static_cast<const T*>(upstream), upstream_stride, e->dim, scale,
-                          static_cast<T*>(out), out_stride, out_packed, e->partials, partial_stride, piece, log2,
-                          static_cast<const DeviceMeta*>(e->meta));
+                          (uint32_t)e->entries, static_cast<const T*>(r.upstream), r.upstream_stride, e->dim, r.scale,
+                          static_cast<T*>(r.out), r.out_stride, out_packed, e->partials, partial_stride, piece,
+                          lanes_log2, static_cast<const DeviceMeta*>(e->meta));
+}
+
+// Entries per block of k_sum_few, 0 where the sorted list is the better way.
+uint32_t few_owned(uint64_t entries, uint64_t count) {
+    if (count > kFewTokens) return 0;
+    const uint64_t owned = std::min<uint64_t>((entries + 147) / 148, kMostOwned);
+    return (entries + owned - 1) / owned * count <= kFewReads ? (uint32_t)owned : 0;
+}
+
+template <typename T, int N>
+cudaError_t sum_few(const sp_embedding* e, const void* tokens, int wide, uint32_t count, uint32_t owned, const Rows& r,
+                    int lanes_log2) {
+    const size_t smem = kFewThreads * N * sizeof(float) + (kFewThreads / 32 * (size_t)owned + count) * sizeof(uint16_t);
+    static std::atomic<unsigned long long> configured{0};
+    constexpr size_t most = kFewThreads * N * sizeof(float) + (kFewThreads / 32 * kMostOwned + kFewTokens) * sizeof(uint16_t);
+    const cudaError_t err = allow_smem_once(k_sum_few<T, N>, most, configured);
+    if (err != cudaSuccess) return err;
+    const int out_packed = pack_width(r.out, r.out_stride, e->dim, sizeof(T)) >= N;
+    return launch_chained(k_sum_few<T, N>, grid_for(e->entries, owned), kFewThreads, smem, e->ctx->stream, tokens, wide,
+                          count, e->entries, owned, static_cast<const T*>(r.upstream), r.upstream_stride, e->dim,
+                          r.scale, static_cast<T*>(r.out), r.out_stride, out_packed, lanes_log2);
 }
 
 uint32_t partial_stride_of(uint32_t dim) { return (dim + 3) / 4 * 4; }
@@ -350,9 +590,11 @@ sp_status sp_embedding_create(sp_context* ctx, uint64_t entries, uint32_t dim, s
     while ((1ull << bits) <= entries) ++bits;  // keys 0..entries
     e->plan.key_bits = (int)bits;
     e->plan.passes = (int)(bits + 7) / 8;
-    // The most pieces any count up to max_tokens is cut into.
+    // The most stretches any count up to max_tokens is cut into: the shortest is 8 short pieces (32
+    // threads a row), the shortest of a long list 8 long ones.
     const uint64_t most_short = std::min<uint64_t>(max_tokens, (uint64_t)kLongPiece * 148 * 8);
-    const uint64_t pieces = std::max((most_short + kShortPiece - 1) / kShortPiece, (max_tokens + kLongPiece - 1) / kLongPiece);
+    const uint64_t stretches = std::max((most_short + 8 * kShortPiece - 1) / (8 * kShortPiece),
+                                        (max_tokens + 8 * kLongPiece - 1) / (8 * kLongPiece));
     sp_status s = SP_OK;
     auto all = [&]() -> sp_status {
         SP_CHECK(allocate(e, &e->meta, 1));
@@ -364,7 +606,7 @@ sp_status sp_embedding_create(sp_context* ctx, uint64_t entries, uint32_t dim, s
         const uint64_t partitions = (max_tokens + kSortPartition - 1) / kSortPartition;
         SP_CHECK(allocate(e, &e->lookback, partitions * kSortRadix));
         SP_CHECK(allocate(e, &e->ranges, entries));
-        SP_CHECK(allocate(e, &e->partials, pieces * 2 * partial_stride_of(dim)));
+        SP_CHECK(allocate(e, &e->partials, stretches * 2 * partial_stride_of(dim)));
         // The look-back words carry the pass's sequence number: zero is no pass's.
         SP_CUDA(ctx, cudaMemsetAsync(e->lookback, 0, partitions * kSortRadix * sizeof(unsigned long long), ctx->stream));
         SP_CUDA(ctx, cudaMemsetAsync(e->meta, 0, sizeof(DeviceMeta), ctx->stream));
@@ -445,7 +687,32 @@ sp_status sp_embedding_gradient(sp_embedding* e, const void* d_out_gradient, int
     cudaStream_t st = ctx->stream;
     const uint32_t n = (uint32_t)count;
     const int wide = index == SP_INDEX64;
-    const uint32_t piece = piece_length(count), partial_stride = partial_stride_of(e->dim);
+    const Rows r{d_out_gradient, out_gradient_stride, scale, d_table_gradient, table_gradient_stride};
+    // No rows to lay out where there are no tokens (and perhaps no pointer).
+    const int width = n > 0 ? pack_width(d_out_gradient, out_gradient_stride, e->dim, size) : 1;
+    const int lanes_log2 = lanes_log2_for(e->dim / width, kMinLanesLog2);
+    cudaError_t err = cudaErrorInvalidValue;
+#define SPLAT_ROWS(call)                                 \
+    do {                                                 \
+        if (e->element == SP_F32) {                      \
+            if (width == 4) err = call(float, 4);        \
+            else if (width == 2) err = call(float, 2);   \
+            else err = call(float, 1);                   \
+        } else {                                         \
+            if (width == 8) err = call(bf16, 8);         \
+            else if (width == 4) err = call(bf16, 4);    \
+            else if (width == 2) err = call(bf16, 2);    \
+            else err = call(bf16, 1);                    \
+        }                                                \
+    } while (0)
+    if (const uint32_t owned = few_owned(e->entries, count)) {
+#define SPLAT_FEW(T, N) sum_few<T, N>(e, d_tokens, wide, n, owned, r, lanes_log2)
+        SPLAT_ROWS(SPLAT_FEW);
+#undef SPLAT_FEW
+        SP_CUDA(ctx, err);
+        return SP_OK;
+    }
+    const uint32_t piece = piece_length(count, lanes_log2), partial_stride = partial_stride_of(e->dim);
     uint32_t* tickets = e->histograms + kSortMaxPasses * kSortRadix;
     SP_CUDA(ctx, cudaMemsetAsync(e->histograms, 0, (kSortMaxPasses * kSortRadix + kSortMaxPasses) * sizeof(uint32_t), st));
     SP_CUDA(ctx, launch_chained(k_emit_tokens, std::max(1u, grid_for(count, kThreads * kEmitItems)), kThreads, 0, st,
@@ -460,36 +727,25 @@ sp_status sp_embedding_gradient(sp_embedding* e, const void* d_out_gradient, int
     SP_CUDA(ctx, launch_ranges(e->plan, keys, e->meta, std::max<uint64_t>(count, e->entries / 4), e->ranges,
                                (uint32_t)e->entries, st));
     if (n > 0) {
-        const int width = pack_width(d_out_gradient, out_gradient_stride, e->dim, size);
-        cudaError_t err = cudaErrorInvalidValue;
-#define SPLAT_SUM(T, N)                                                                                       \
-    err = sum_pieces<T, N>(e, keys, positions, n, d_out_gradient, out_gradient_stride, scale, d_table_gradient, \
-                           table_gradient_stride, partial_stride, piece)
-        if (e->element == SP_F32) {
-            if (width == 4) SPLAT_SUM(float, 4);
-            else if (width == 2) SPLAT_SUM(float, 2);
-            else SPLAT_SUM(float, 1);
-        } else {
-            if (width == 8) SPLAT_SUM(bf16, 8);
-            else if (width == 4) SPLAT_SUM(bf16, 4);
-            else if (width == 2) SPLAT_SUM(bf16, 2);
-            else SPLAT_SUM(bf16, 1);
-        }
-#undef SPLAT_SUM
+#define SPLAT_PIECES(T, N) sum_pieces<T, N>(e, keys, positions, n, r, partial_stride, piece, lanes_log2)
+        SPLAT_ROWS(SPLAT_PIECES);
+#undef SPLAT_PIECES
         SP_CUDA(ctx, err);
     }
-    const unsigned join_grid = grid_for(e->entries, kJoinWarps);
+#undef SPLAT_ROWS
+    const uint32_t stretch = (kThreads >> lanes_log2) * piece;
+    const unsigned join_grid = grid_for(e->entries, kJoinWarps * kJoinTokens);
     if (e->element == SP_F32)
         SP_CUDA(ctx, launch_chained(k_join_pieces<float>, join_grid, kThreads, 0, st,
                                     static_cast<const uint2*>(e->ranges), (uint32_t)e->entries, e->dim, scale,
                                     static_cast<float*>(d_table_gradient), table_gradient_stride,
-                                    static_cast<const float*>(e->partials), partial_stride, piece,
+                                    static_cast<const float*>(e->partials), partial_stride, stretch,
                                     static_cast<const DeviceMeta*>(e->meta)));
     else
         SP_CUDA(ctx, launch_chained(k_join_pieces<bf16>, join_grid, kThreads, 0, st,
                                     static_cast<const uint2*>(e->ranges), (uint32_t)e->entries, e->dim, scale,
                                     static_cast<bf16*>(d_table_gradient), table_gradient_stride,
-                                    static_cast<const float*>(e->partials), partial_stride, piece,
+                                    static_cast<const float*>(e->partials), partial_stride, stretch,
                                     static_cast<const DeviceMeta*>(e->meta)));
     return SP_OK;
 } catch (...) {

@@ -275,10 +275,12 @@ __device__ __forceinline__ void store_out(T* to, const float (&v)[32], uint32_t 
     if (packed && columns >= 32) {
 #pragma unroll
         for (int q = 0; q < 32 / N; ++q) {
-            Pack<T, N> o;
+            float part[N];
 #pragma unroll
-            for (int j = 0; j < N; ++j) o.v[j] = from_float<T>(v[q * N + j]);
-            *reinterpret_cast<Pack<T, N>*>(to + q * N) = o;
+            for (int j = 0; j < N; ++j) part[j] = v[q * N + j];
+            Pack<T, N> o;
+            o.set(part);
+            store_pack(to + q * N, o);
         }
     } else {
 #pragma unroll

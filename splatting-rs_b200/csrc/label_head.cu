@@ -117,9 +117,9 @@ __device__ __forceinline__ void copy_parts(const T* from, uint32_t columns, bool
         constexpr int N = 16 / sizeof(T);
 #pragma unroll
         for (int q = 0; q < 8 / N; ++q) {
-            const Pack<T, N> p = *reinterpret_cast<const Pack<T, N>*>(from + q * N);
+            const Pack<T, N> p = load_pack<T, N>(from + q * N);
 #pragma unroll
-            for (int j = 0; j < N; ++j) v[q * N + j] = to_float(p.v[j]);
+            for (int j = 0; j < N; ++j) v[q * N + j] = p.get(j);
         }
     } else {
 #pragma unroll
@@ -129,12 +129,10 @@ __device__ __forceinline__ void copy_parts(const T* from, uint32_t columns, bool
 #pragma unroll
     for (int p = 0; p < parts; ++p) {
         Pack<bf16, 8> o;
+        o.set(v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            o.v[j] = __float2bfloat16_rn(v[j]);
-            v[j] -= __bfloat162float(o.v[j]);
-        }
-        *reinterpret_cast<Pack<bf16, 8>*>(to + p * part) = o;
+        for (int j = 0; j < 8; ++j) v[j] -= o.get(j);
+        store_pack(to + p * part, o);
     }
 }
 
