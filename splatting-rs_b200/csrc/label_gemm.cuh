@@ -55,6 +55,7 @@ enum Ending { kStats = 0, kSlopes = 1, kOut = 2 };
 struct GemmArgs {
     RowSet* rows;
     const uint32_t* row_of;
+    uint32_t all_rows;     // not 0: that many rows, all of them count and are read in place
     uint32_t labels;
     uint32_t products;     // 1, or kPartProducts
     uint32_t k_blocks;     // of the inner dimension; kOut with rows_inner: follows the row count
@@ -180,9 +181,10 @@ __device__ __forceinline__ float sum_exp2(const float (&v)[32], float scale2, fl
 // takes its base from the row's first chunk and looks for the largest logit again only when a sum
 // leaves f32's range (a logit some 127 / log2(e) above the base), so that a chunk's exponentials
 // wait for nothing: the running maximum in every chunk cost a quarter of the pass at width 512.
+// `divergent`: not all of the warp's lanes are here.
 template <bool LABEL>
 __device__ __forceinline__ void add_logits(RowStats& s, float (&v)[32], uint32_t first, uint32_t labels, float scale2,
-                                           uint32_t target) {
+                                           uint32_t target, bool divergent = false) {
     if (first + 32 > labels) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
@@ -218,7 +220,7 @@ __device__ __forceinline__ void add_logits(RowStats& s, float (&v)[32], uint32_t
     }
     s.sum = sum;
     const uint32_t at = target - first;
-    if (__any_sync(0xffffffffu, at < 32)) {
+    if (divergent ? at < 32 : __any_sync(0xffffffffu, at < 32)) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
             if (at == (uint32_t)j) s.target_logit = v[j];
@@ -326,8 +328,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const uint32_t tmem = *reinterpret_cast<uint32_t*>(generic_base + (tmem_slot - smem));
     chain_enter();
 
-    const uint32_t count = a.rows->count;
-    const bool packed = a.rows->packed != 0;
+    const uint32_t count = a.all_rows ? a.all_rows : a.rows->count;
+    const bool packed = !a.all_rows && a.rows->packed != 0;
     const Schedule<ENDING, kSide> schedule(a, count);
     bool ok = true;
 
@@ -422,7 +424,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             uint32_t target = kNoTarget;
             float shift = 0.0f, weight = 0.0f;
             if (ENDING != kOut && live) {
-                const uint32_t original = a.row_of[compact];
+                const uint32_t original = a.all_rows ? compact : a.row_of[compact];
                 if (a.targets) target = (uint32_t)index_at(a.targets, a.wide, original, a.labels);
                 if (ENDING == kSlopes) {
                     shift = -a.log_normalizers[original] * 1.44269504088896341f;

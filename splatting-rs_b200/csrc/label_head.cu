@@ -15,7 +15,7 @@
 #include <cstring>
 #include <new>
 
-#include "label_gemm.cuh"
+#include "label_thin.cuh"
 #include "objects.h"
 
 using namespace splat;
@@ -243,66 +243,63 @@ __global__ void __launch_bounds__(kThreads)
 
 // ------------------------------------------------------------------ joining
 
-// Partial sums in units of 2^base, joined in double: a part's sum may come close to f32's largest.
-struct Joined {
-    float base, largest;
-    double sum;
-    uint32_t label;
-};
-
-__device__ __forceinline__ Joined join(Joined a, Joined b) {
-    Joined r;
-    const bool second = b.largest > a.largest || (b.largest == a.largest && b.label < a.label);
-    r.largest = second ? b.largest : a.largest;
-    r.label = second ? b.label : a.label;
-    r.base = fmaxf(a.base, b.base);
-    const float top = r.base == -INFINITY ? 0.0f : r.base;
-    r.sum = a.sum * (double)exp2f(a.base - top) + b.sum * (double)exp2f(b.base - top);
-    return r;
-}
-
-// `lanes` threads (1 or 32) join a row's partials in slot order within a lane, then across lanes.
-// In units of ln 2 a row's log sum exp is base + log2(sum), its loss that less z[target] scale2, and
-// its largest log-probability the negative of that with the largest logit, all taken in double so
-// that nothing is lost where they cancel. The loss's mean is summed in double: per block, then by the
-// last block.
+// `LANES` threads (1 or 32) join a row's partial sums, each in units of 2^base: the highest base
+// (and the largest logit with the lowest label) first, then the sum, in double, since a part may come
+// close to f32's largest. In units of ln 2 a row's log sum exp is base + log2(sum), its loss that less
+// z[target] scale2, and its largest log-probability the negative of that with the largest logit, all
+// taken in double so that nothing is lost where they cancel. The loss's mean is summed in double: per
+// block, then by the last block.
 template <int LANES>
 __global__ void __launch_bounds__(kThreads)
-    k_join_rows(RowSet* rows, const uint32_t* __restrict__ row_of, const float2* __restrict__ partials,
-                const uint32_t* __restrict__ partial_labels, uint64_t partial_rows, uint32_t slots, float scale2,
-                const float* __restrict__ target_logits, uint64_t n, float* __restrict__ losses,
-                float* __restrict__ normalizers, int32_t* __restrict__ labels_out, float* __restrict__ log_probability,
-                double* __restrict__ block_sums, float* __restrict__ mean) {
+    k_join_rows(RowSet* rows, const uint32_t* __restrict__ row_of, uint32_t all_rows,
+                const float2* __restrict__ partials, const uint32_t* __restrict__ partial_labels,
+                uint64_t partial_rows, uint32_t slots, float scale2, const float* __restrict__ target_logits,
+                float* __restrict__ losses, float* __restrict__ normalizers, int32_t* __restrict__ labels_out,
+                float* __restrict__ log_probability, double* __restrict__ block_sums, float* __restrict__ mean) {
     chain_enter();
-    const uint32_t count = rows->count;
+    const uint32_t count = all_rows ? all_rows : rows->count;
     const bool failed = rows->status != 0;
     const float nan = __int_as_float(0x7fffffff);
     const uint64_t i = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) / LANES;
     const uint32_t lane = threadIdx.x % LANES;
     double loss = 0.0;
     if (i < count) {
-        Joined all{-INFINITY, -INFINITY, 0.0, 0xffffffffu};
+        float top = -INFINITY, largest = -INFINITY;
+        uint32_t label = 0xffffffffu;
+#pragma unroll 4
         for (uint32_t s = lane; s < slots; s += LANES) {
-            const float2 p = partials[s * partial_rows + i];
-            const uint32_t label = partial_labels ? partial_labels[s * partial_rows + i] : 0u;
-            all = join(all, Joined{partial_labels ? __fmul_rn(p.x, scale2) : p.x, p.x, (double)p.y, label});
+            const float x = partials[s * partial_rows + i].x;
+            if (partial_labels) {
+                const uint32_t l = partial_labels[s * partial_rows + i];
+                if (x > largest || (x == largest && l < label)) largest = x, label = l;
+                top = fmaxf(top, __fmul_rn(x, scale2));
+            } else {
+                top = fmaxf(top, x);
+            }
         }
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) {
-            Joined other;
-            other.base = __shfl_xor_sync(0xffffffffu, all.base, o);
-            other.largest = __shfl_xor_sync(0xffffffffu, all.largest, o);
-            other.sum = __shfl_xor_sync(0xffffffffu, all.sum, o);
-            other.label = __shfl_xor_sync(0xffffffffu, all.label, o);
-            all = lane & o ? join(other, all) : join(all, other);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float x = __shfl_xor_sync(0xffffffffu, largest, o);
+            const uint32_t l = __shfl_xor_sync(0xffffffffu, label, o);
+            if (x > largest || (x == largest && l < label)) largest = x, label = l;
         }
+        if (top == -INFINITY) top = 0.0f;
+        double sum = 0.0;
+#pragma unroll 4
+        for (uint32_t s = lane; s < slots; s += LANES) {
+            const float2 p = partials[s * partial_rows + i];
+            const float base = partial_labels ? __fmul_rn(p.x, scale2) : p.x;
+            sum += (double)p.y * (double)exp2f(base - top);
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) {
-            const uint32_t row = row_of[i];
-            const double ln2 = 0.6931471805599453, top = all.base == -INFINITY ? 0.0 : (double)all.base;
-            const double log2_sum = top + log2(all.sum);
+            const uint32_t row = all_rows ? (uint32_t)i : row_of[i];
+            const double ln2 = 0.6931471805599453, log2_sum = (double)top + log2(sum);
             if (labels_out) {
-                labels_out[row] = failed ? -1 : (int32_t)all.label;
-                log_probability[row] = failed ? nan : (float)(((double)all.largest * scale2 - log2_sum) * ln2);
+                labels_out[row] = failed ? -1 : (int32_t)label;
+                log_probability[row] = failed ? nan : (float)(((double)largest * scale2 - log2_sum) * ln2);
             } else {
                 const float value = failed ? nan : (float)((log2_sum - (double)target_logits[i] * scale2) * ln2);
                 losses[row] = value;
@@ -577,6 +574,22 @@ cudaError_t run_gemm(const sp_label_head* h, const Plan& plan, uint64_t items, c
                      : launch_gemm<ENDING, A_TRANSPOSED, B_TRANSPOSED, false, T>(h, items, a, a_packed, b, b_packed, slopes, args);
 }
 
+// One call's inputs: the compacted rows and the operand maps.
+struct Operands {
+    CUtensorMap features, features_packed, weight;
+    uint32_t all_rows;  // as in GemmArgs
+};
+
+template <typename T, bool DIRECT>
+cudaError_t launch_thin(const sp_label_head* h, uint32_t blocks, const Operands& op, const ThinArgs& args) {
+    constexpr size_t smem = thin_smem(sizeof(T) == 4);
+    static std::atomic<unsigned long long> configured{0};
+    const cudaError_t err = allow_smem_once(k_label_thin<T, DIRECT>, smem, configured);
+    if (err != cudaSuccess) return err;
+    return launch_chained(k_label_thin<T, DIRECT>, blocks, kThinThreads, smem, h->ctx->stream, op.features,
+                          op.features_packed, op.weight, args);
+}
+
 sp_status check_matrix(sp_context* ctx, const void* p, int64_t stride, uint32_t dim, size_t size, const char* what) {
     SP_REQUIRE(ctx, p != nullptr, SP_ERR_INVALID, std::string("null ") + what);
     SP_REQUIRE(ctx, reinterpret_cast<uintptr_t>(p) % size == 0, SP_ERR_INVALID, std::string("misaligned ") + what);
@@ -584,27 +597,23 @@ sp_status check_matrix(sp_context* ctx, const void* p, int64_t stride, uint32_t 
     return SP_OK;
 }
 
-// One call's inputs: the compacted rows and the operand maps.
-struct Operands {
-    CUtensorMap features, features_packed, weight;
-    uint64_t row_capacity;
-};
-
 sp_status prepare(sp_label_head* h, const void* features, int64_t feature_stride, const void* weight,
                   int64_t weight_stride, const void* targets, int wide, uint64_t n, float* losses, float* normalizers,
-                  void* gradient, int64_t gradient_stride, Operands* out) {
+                  void* gradient, int64_t gradient_stride, bool weight_needed, Operands* out) {
     sp_context* ctx = h->ctx;
     cudaStream_t st = ctx->stream;
     const uint64_t stride = h->packed_stride(), capacity = round_up(h->max_rows, kPairTile);
     const uint32_t parts = h->parts();
     const bool features_here = in_place(h, features, feature_stride), weight_here = in_place(h, weight, weight_stride);
-    out->row_capacity = capacity;
+    // Without targets every row counts: nothing to gather where the operands can be read in place.
+    out->all_rows = !targets && features_here && (weight_here || !weight_needed) ? (uint32_t)n : 0;
     SP_CHECK(make_map(ctx, &out->features_packed, h->packed_features, h->dim, capacity, stride, parts, capacity * stride));
     if (features_here) SP_CHECK(make_map(ctx, &out->features, features, h->dim, n, feature_stride, 1, 0));
     else out->features = out->features_packed;
     if (weight_here) SP_CHECK(make_map(ctx, &out->weight, weight, h->dim, h->labels, weight_stride, 1, 0));
     else SP_CHECK(make_map(ctx, &out->weight, h->packed_weight, h->dim, h->labels, stride, parts, h->labels * stride));
 
+    if (out->all_rows) return SP_OK;
     const unsigned blocks = grid_for(n, kGatherRows);
     const uint32_t* counts = nullptr;
     if (targets && blocks > kRecountBlocks) {
@@ -616,7 +625,7 @@ sp_status prepare(sp_label_head* h, const void* features, int64_t feature_stride
         using T = std::remove_pointer_t<decltype(typed)>;
         PackWeight<T> pack{nullptr, weight_stride, (int)vector_rows(h, weight, weight_stride), h->packed_weight};
         unsigned weight_blocks = 0;
-        if (!weight_here) {
+        if (!weight_here && weight_needed) {
             pack.from = static_cast<const T*>(weight);
             weight_blocks = (unsigned)std::min<uint64_t>((h->labels + kThreads / 32 - 1) / (kThreads / 32), 148 * 16);
         }
@@ -668,26 +677,48 @@ sp_status check_targets(sp_context* ctx, const void* targets, sp_index index) {
 }
 
 // The pass over the logits shared by the loss and the prediction.
-sp_status run_stats(sp_label_head* h, const Operands& op, const void* targets, int wide, uint64_t n, float scale,
+sp_status run_stats(sp_label_head* h, const Operands& op, const void* weight, int64_t weight_stride,
+                    const void* targets, int wide, uint64_t n, float scale,
                     float* mean, float* losses, float* normalizers, int32_t* labels_out, float* log_probability) {
     sp_context* ctx = h->ctx;
-    const Plan plan = plan_logits(h->sms, n, h->labels);
     GemmArgs a = common_args(h, targets, wide, scale);
+    a.all_rows = op.all_rows;
     a.k_blocks = (h->dim + kBlockK - 1) / kBlockK;
-    a.n_tiles = plan.n_tiles;
-    a.splits = plan.splits;
     a.partials = h->partials;
     a.partial_labels = labels_out ? h->partial_labels : nullptr;
-    a.partial_rows = (uint64_t)plan.m_tiles * (plan.pair ? kPairTile : kTile);
     a.target_logits = h->target_logits;
-    SP_CUDA(ctx, (run_gemm<kStats, false, false, bf16>(h, plan, plan.items(), op.features, op.features_packed, op.weight,
-                                                       op.weight, op.weight, a)));
-    const uint32_t slots = 2 * a.splits;
+    uint32_t slots = 0;
+    if (n <= kThinRows) {
+        ThinArgs thin;
+        thin.weight = weight;
+        thin.weight_stride = weight_stride;
+        thin.dim = h->dim;
+        thin.vector = vector_rows(h, weight, weight_stride);
+        thin.columns = (uint32_t)round_up(n, 16);
+        thin.tiles = tiles_of(h->labels, false);
+        const uint32_t blocks = std::min(thin.tiles, h->sms);
+        a.partial_rows = kThinRows;
+        slots = 2 * blocks;
+        thin.g = a;
+        const cudaError_t err = h->element == SP_F32                 ? launch_thin<float, false>(h, blocks, op, thin)
+                                : in_place(h, weight, weight_stride) ? launch_thin<bf16, true>(h, blocks, op, thin)
+                                                                     : launch_thin<bf16, false>(h, blocks, op, thin);
+        SP_CUDA(ctx, err);
+    } else {
+        const Plan plan = plan_logits(h->sms, n, h->labels);
+        a.n_tiles = plan.n_tiles;
+        a.splits = plan.splits;
+        a.partial_rows = (uint64_t)plan.m_tiles * (plan.pair ? kPairTile : kTile);
+        slots = 2 * a.splits;
+        SP_CUDA(ctx, (run_gemm<kStats, false, false, bf16>(h, plan, plan.items(), op.features, op.features_packed,
+                                                           op.weight, op.weight, op.weight, a)));
+    }
     auto join = [&](auto kernel, uint32_t lanes) {
         return launch_chained(kernel, grid_for(n * lanes, kThreads), kThreads, 0, ctx->stream, h->rows,
-                              static_cast<const uint32_t*>(h->row_of), static_cast<const float2*>(h->partials),
+                              static_cast<const uint32_t*>(h->row_of), a.all_rows,
+                              static_cast<const float2*>(h->partials),
                               static_cast<const uint32_t*>(a.partial_labels), a.partial_rows, slots, a.scale2,
-                              static_cast<const float*>(h->target_logits), n, losses, normalizers, labels_out,
+                              static_cast<const float*>(h->target_logits), losses, normalizers, labels_out,
                               log_probability, h->loss_sums, mean);
     };
     SP_CUDA(ctx, slots <= kThreadSlots ? join(k_join_rows<1>, 1) : join(k_join_rows<32>, 32));
@@ -776,8 +807,8 @@ sp_status sp_label_head_loss(sp_label_head* h, const void* d_features, int64_t f
     Operands op;
     const int wide = index == SP_INDEX64;
     SP_CHECK(prepare(h, d_features, feature_stride, d_weight, weight_stride, d_targets, wide, rows, d_losses,
-                     d_log_normalizers, nullptr, 0, &op));
-    return run_stats(h, op, d_targets, wide, rows, logit_scale, d_mean, d_losses, d_log_normalizers, nullptr, nullptr);
+                     d_log_normalizers, nullptr, 0, rows > kThinRows, &op));
+    return run_stats(h, op, d_weight, weight_stride, d_targets, wide, rows, logit_scale, d_mean, d_losses, d_log_normalizers, nullptr, nullptr);
 } catch (...) {
     return SP_ERR_OUT_OF_MEMORY;
 }
@@ -794,8 +825,8 @@ sp_status sp_label_head_predict(sp_label_head* h, const void* d_features, int64_
     SP_CHECK(select_device(ctx));
     Operands op;
     SP_CHECK(prepare(h, d_features, feature_stride, d_weight, weight_stride, nullptr, 0, rows, nullptr, nullptr,
-                     nullptr, 0, &op));
-    return run_stats(h, op, nullptr, 0, rows, logit_scale, nullptr, nullptr, nullptr, d_labels, d_log_probabilities);
+                     nullptr, 0, rows > kThinRows, &op));
+    return run_stats(h, op, d_weight, weight_stride, nullptr, 0, rows, logit_scale, nullptr, nullptr, nullptr, d_labels, d_log_probabilities);
 } catch (...) {
     return SP_ERR_OUT_OF_MEMORY;
 }
@@ -825,7 +856,7 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
     const int wide = index == SP_INDEX64;
     Operands op;
     SP_CHECK(prepare(h, d_features, feature_stride, d_weight, weight_stride, d_targets, wide, rows, nullptr, nullptr,
-                     d_feature_gradient, feature_gradient_stride, &op));
+                     d_feature_gradient, feature_gradient_stride, true, &op));
 
     const uint64_t chunk = chunk_for(h, rows), chunks = (rows + chunk - 1) / chunk;
     const uint64_t slope_stride = h->slope_stride(), sum_stride = sums_stride(h);

@@ -1,0 +1,302 @@
+// The logits' pass for at most kThinRows rows, where the weight's bytes are what it costs: the roles
+// of label_gemm.cuh swapped (128 labels on the accumulator's lanes, the rows its columns), so that
+// the products are no wider than the rows, and the weight read once and in place: bf16 by tiled bulk
+// copies where it is aligned for them, else (f32, odd strides) by eight warps that split it into its
+// bf16 parts on the way into shared memory.
+//
+// The accumulation truncates, so it is spread: even and odd steps of K, and the small products of
+// f32 parts, have accumulators of their own, added in f32 at the end.
+#pragma once
+
+#include "label_gemm.cuh"
+
+namespace splat {
+namespace label {
+
+constexpr int kThinRows = 64;
+constexpr int kThinThreads = 512;
+constexpr int kConvertWarps = 8;
+constexpr int kThinStagesF32 = 2, kThinStagesBf16 = 6;
+constexpr uint32_t kRowsBytes = kThinRows * kBlockK * 2;
+constexpr int kLogitStride = kTile + 1;  // of a row's logits in shared memory: no bank twice
+constexpr uint32_t kThinColumns = 512;
+
+constexpr uint32_t thin_stage_bytes(bool f32) { return (f32 ? kParts : 1) * (kOperandBytes + kRowsBytes); }
+constexpr size_t thin_smem(bool f32) {
+    return 1024 + (size_t)(f32 ? kThinStagesF32 : kThinStagesBf16) * thin_stage_bytes(f32) +
+           kThinRows * kLogitStride * sizeof(float) + 256;
+}
+
+struct ThinArgs {
+    GemmArgs g;
+    const void* weight;
+    int64_t weight_stride;
+    uint32_t dim;
+    int vector;          // 16-byte loads are aligned
+    uint32_t columns;    // of the accumulators: the rows, rounded up to 16
+    uint32_t tiles;      // of 128 labels
+};
+
+__device__ __forceinline__ void tmem_load16(uint32_t address, float (&v)[16]) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(address));
+}
+
+// One thread's eight columns of a weight row on their way to shared memory.
+template <typename T>
+struct RawEight {
+    static constexpr int N = 16 / sizeof(T);
+    Pack<T, N> p[8 / N];
+    __device__ __forceinline__ void load(const T* from, uint32_t columns, bool vector) {
+        if (vector && columns >= 8) {
+#pragma unroll
+            for (int q = 0; q < 8 / N; ++q) p[q] = load_pack<T, N>(from + q * N);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 8 / N; ++q) {
+                float v[N];
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[j] = (uint32_t)(q * N + j) < columns ? to_float(from[q * N + j]) : 0.0f;
+                p[q].set(v);
+            }
+        }
+    }
+};
+
+// DIRECT: the weight arrives by bulk copies; else through the converting warps.
+template <typename T, bool DIRECT>
+__global__ void __launch_bounds__(kThinThreads, 1)
+    k_label_thin(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_rows_packed,
+                 const __grid_constant__ CUtensorMap map_weight, const __grid_constant__ ThinArgs a) {
+    constexpr bool kF32 = sizeof(T) == 4;
+    constexpr int kParted = kF32 ? (int)kParts : 1;
+    constexpr int kRing = kF32 ? kThinStagesF32 : kThinStagesBf16;
+    constexpr uint32_t kBytes = thin_stage_bytes(kF32);
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem = (tc::smem_address(smem_raw) + 1023u) & ~1023u;
+    uint8_t* generic_base = smem_raw + (smem - tc::smem_address(smem_raw));
+    float* logits = reinterpret_cast<float*>(generic_base + kRing * kBytes);
+    const uint32_t barriers = smem + kRing * kBytes + (kThinRows * kLogitStride * sizeof(float) + 15) / 16 * 16;
+    const uint32_t full = barriers, empty = full + 8 * kRing, done = empty + 8 * kRing, drained = done + 16;
+    const uint32_t tmem_slot = drained + 16;
+    const uint32_t warp = threadIdx.x / 32, lane = lane_id();
+
+    if (warp == 0 && lane == 0) {
+        for (int s = 0; s < kRing; ++s) {
+            tc::barrier_init(full + 8 * s, 1 + (DIRECT ? 0 : kConvertWarps));
+            tc::barrier_init(empty + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            tc::barrier_init(done + 8 * b, 1);
+            tc::barrier_init(drained + 8 * b, 4);
+        }
+        tc::barrier_init_fence();
+    }
+    if (warp == 2) tc::tmem_alloc<false>(tmem_slot, kThinColumns);
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = *reinterpret_cast<uint32_t*>(generic_base + (tmem_slot - smem));
+    chain_enter();
+
+    const uint32_t count = a.g.all_rows ? a.g.all_rows : a.g.rows->count;
+    const uint32_t tiles = count ? a.tiles : 0;
+    // A buffer's accumulators: even steps, odd steps, and the products of f32's smaller parts.
+    const uint32_t buffer_columns = 4 * kThinRows;
+    bool ok = true;
+
+    if (warp == 0) {
+        if (tc::elect_one()) {
+            const CUtensorMap* rows = !a.g.all_rows && a.g.rows->packed ? &map_rows_packed : &map_rows;
+            uint32_t stage = 0, phase = 0;
+            for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x)
+                for (uint32_t k = 0; k < a.g.k_blocks; ++k) {
+                    if (!(ok = tc::barrier_wait(empty + 8 * stage, phase ^ 1))) break;
+                    const uint32_t bar = full + 8 * stage, to = smem + stage * kBytes;
+                    tc::barrier_expect(bar, kParted * kRowsBytes + (DIRECT ? kOperandBytes : 0));
+                    if (DIRECT)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            tc::load_box<false>(to + h * kBoxBytes, &map_weight, bar, (int)k * kBlockK,
+                                                (int)tile * kTile + h * 64, 0);
+#pragma unroll
+                    for (int p = 0; p < kParted; ++p)
+                        tc::load_box<false>(to + kParted * kOperandBytes + p * kRowsBytes, rows, bar, (int)k * kBlockK, 0, p);
+                    if (++stage == kRing) stage = 0, phase ^= 1;
+                }
+            for (int i = 0; ok && i < kRing; ++i) {
+                ok = tc::barrier_wait(empty + 8 * stage, phase ^ 1);
+                if (++stage == kRing) stage = 0, phase ^= 1;
+            }
+        }
+    } else if (warp == 1) {
+        if (tc::elect_one()) {
+            const uint32_t desc = tc::instruction(kTile, a.columns, false, false);
+            uint32_t stage = 0, phase = 0, buffer = 0, buffer_phase = 0;
+            for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+                if (!(ok = tc::barrier_wait(drained + 8 * buffer, buffer_phase ^ 1))) break;
+                tc::fence_after_sync();
+                const uint32_t into = tmem + buffer * buffer_columns;
+                for (uint32_t k = 0; k < a.g.k_blocks; ++k) {
+                    if (!(ok = tc::barrier_wait(full + 8 * stage, phase))) break;
+                    tc::fence_after_sync();
+                    const uint32_t w_at = smem + stage * kBytes, r_at = w_at + kParted * kOperandBytes;
+#pragma unroll
+                    for (int p = 0; p < (kF32 ? (int)kPartProducts : 1); ++p) {
+                        const uint32_t pw = kF32 ? (kPartsOfA >> (4 * p)) & 15u : 0, pr = kF32 ? (kPartsOfB >> (4 * p)) & 15u : 0;
+                        const bool small = kF32 && p + 1 < (int)kPartProducts;
+                        const uint32_t accumulator = into + (small ? 2 : k & 1) * kThinRows;
+#pragma unroll
+                        for (int q = 0; q < kBlockK / 16; ++q) {
+                            const bool add = small ? k != 0 || p != 0 || q != 0 : k > 1 || q != 0;
+                            tc::multiply<false>(accumulator, tc::operand(w_at + pw * kOperandBytes + q * 32, kBoxBytes),
+                                                tc::operand(r_at + pr * kRowsBytes + q * 32, kBoxBytes), desc, add);
+                        }
+                    }
+                    tc::commit<false>(empty + 8 * stage);
+                    if (++stage == kRing) stage = 0, phase ^= 1;
+                }
+                if (!ok) break;
+                tc::commit<false>(done + 8 * buffer);
+                if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
+            }
+        }
+    } else if (warp >= 4 && warp < 8) {
+        // The tile's logits turn over in shared memory: a thread reads a label's, then two threads
+        // take half of a row's each.
+        const uint32_t t = threadIdx.x - 128, row = t / 2, half = t % 2;
+        const bool live = row < count;
+        RowStats stats{-INFINITY, 0.0f, 0.0f, -INFINITY, 0u};
+        uint32_t target = kNoTarget;
+        if (live && a.g.targets)
+            target = (uint32_t)index_at(a.g.targets, a.g.wide, a.g.all_rows ? row : a.g.row_of[row], a.g.labels);
+        uint32_t buffer = 0, buffer_phase = 0;
+        for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+            // All four warps agree whether to go on: they meet at barriers below.
+            const bool here = tc::barrier_wait(done + 8 * buffer, buffer_phase);
+            uint32_t all;
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 128, p;\n\t"
+                         "selp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"((uint32_t)here) : "memory");
+            if (!(ok = all != 0)) break;
+            tc::fence_after_sync();
+            const uint32_t from = tmem + buffer * buffer_columns + (((warp - 4) * 32) << 16);
+            for (uint32_t c = 0; c < a.columns; c += 16) {
+                float v[16], w[16];
+                tmem_load16(from + c, v);
+                if (a.g.k_blocks > 1) tmem_load16(from + kThinRows + c, w);
+                tc::tmem_load_wait();
+                if (a.g.k_blocks > 1)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] += w[j];
+                if (kF32) {
+                    tmem_load16(from + 2 * kThinRows + c, w);
+                    tc::tmem_load_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] += w[j];
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) logits[(c + j) * kLogitStride + t] = v[j];
+            }
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::barrier_arrive_cluster(drained + 8 * buffer);
+            asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
+            if (row < a.columns) {
+#pragma unroll 1
+                for (int c = 0; c < kTile / 2; c += 32) {
+                    const uint32_t first = half * (kTile / 2) + c;
+                    float v[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = logits[row * kLogitStride + first + j];
+                    if (a.g.partial_labels) add_logits<true>(stats, v, tile * kTile + first, a.g.labels, a.g.scale2, target, true);
+                    else add_logits<false>(stats, v, tile * kTile + first, a.g.labels, a.g.scale2, target, true);
+                }
+            }
+            asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
+            if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
+        }
+        if (ok && live) {
+            const uint64_t slot = (uint64_t)(blockIdx.x * 2 + half) * a.g.partial_rows + row;
+            a.g.partials[slot] = make_float2(a.g.partial_labels ? stats.largest : stats.base, stats.sum);
+            if (a.g.partial_labels) a.g.partial_labels[slot] = stats.label;
+            if (target != kNoTarget && target / kTile % gridDim.x == blockIdx.x && target % kTile / (kTile / 2) == half)
+                a.g.target_logits[row] = stats.target_logit;
+        }
+    } else if (warp >= 8 && !DIRECT) {
+        // Eight lanes a row of 64 columns, 32 rows a turn; the next two steps' loads are under way.
+        constexpr int kTurns = kTile / 32;
+        const uint32_t t = threadIdx.x - 256, unit = t % 8, first_row = t / 8;
+        const T* weight = static_cast<const T*>(a.weight);
+        RawEight<T> raw[2][kTurns];
+        const uint32_t mine = blockIdx.x < tiles ? (tiles - 1 - blockIdx.x) / gridDim.x + 1 : 0;  // tiles
+        const uint32_t steps = mine * a.g.k_blocks;
+        uint32_t load_tile = blockIdx.x, load_k = 0;
+        auto load_next = [&](RawEight<T> (&to)[kTurns]) {
+            const uint32_t column = load_k * kBlockK + unit * 8;
+            const uint32_t columns = column < a.dim ? a.dim - column : 0;
+#pragma unroll
+            for (int r = 0; r < kTurns; ++r) {
+                const uint32_t label = load_tile * kTile + r * 32 + first_row;
+                const bool there = label < a.g.labels && load_tile < tiles;
+                to[r].load(weight + (there ? (int64_t)label * a.weight_stride + column : 0), there ? columns : 0, a.vector);
+            }
+            if (++load_k == a.g.k_blocks) load_k = 0, load_tile += gridDim.x;
+        };
+        auto convert = [&](RawEight<T> (&from)[kTurns], uint32_t to) {
+#pragma unroll
+            for (int r = 0; r < kTurns; ++r) {
+                float v[8];
+                constexpr int N = RawEight<T>::N;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = from[r].p[j / N].get(j % N);
+                const uint32_t row = r * 32 + first_row, at = to + row * 128 + ((unit ^ (row & 7u)) * 16);
+#pragma unroll
+                for (int p = 0; p < kParted; ++p) {
+                    Pack<bf16, 8> o;
+                    o.set(v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] -= o.get(j);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + p * kOperandBytes), "r"(o.word.x),
+                                 "r"(o.word.y), "r"(o.word.z), "r"(o.word.w)
+                                 : "memory");
+                }
+            }
+        };
+        if (steps > 0) load_next(raw[0]);
+        if (steps > 1) load_next(raw[1]);
+        uint32_t stage = 0, phase = 0;
+        for (uint32_t s = 0; s < steps; s += 2) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                if (s + b >= steps || !ok) break;
+                if (!(ok = tc::barrier_wait(empty + 8 * stage, phase ^ 1))) break;
+                convert(raw[b], smem + stage * kBytes);
+                tc::fence_async_shared();
+                __syncwarp();
+                if (lane == 0) tc::barrier_arrive_cluster(full + 8 * stage);
+                if (s + b + 2 < steps) load_next(raw[b]);
+                if (++stage == kRing) stage = 0, phase ^= 1;
+            }
+            if (!ok) break;
+        }
+    }
+    __syncwarp();
+    if (!ok) {
+        atomicCAS(&a.g.rows->status, 0u, (uint32_t)SP_ERR_TIMEOUT);
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == 2) {
+        tc::fence_after_sync();
+        tc::tmem_free<false>(tmem, kThinColumns);
+    }
+}
+
+}  // namespace label
+}  // namespace splat
