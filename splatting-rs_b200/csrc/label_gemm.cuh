@@ -152,24 +152,27 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 // A row's running softmax: sum of 2^(z scale2 - base) over its logits z so far. The loss takes any
 // base that keeps the sum in range; prediction needs the largest logit and its label, and its base is
 // that logit's. The target's logit is picked up when it comes past.
+constexpr float kLargestSum = 18446744073709551616.0f;  // 2^64
 struct RowStats {
     float base, sum, target_logit, largest;
     uint32_t label;
 };
 
-__device__ __forceinline__ float largest_of(const float (&v)[32]) {
+template <int W>
+__device__ __forceinline__ float largest_of(const float (&v)[W]) {
     float m[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-    for (int j = 4; j < 32; ++j) m[j & 3] = fmaxf(m[j & 3], v[j]);
+    for (int j = 4; j < W; ++j) m[j & 3] = fmaxf(m[j & 3], v[j]);
     return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
 // sum of 2^(v scale2 - base): packed multiply-adds and sums around the exponentials, four sums.
-__device__ __forceinline__ float sum_exp2(const float (&v)[32], float scale2, float base) {
+template <int W>
+__device__ __forceinline__ float sum_exp2(const float (&v)[W], float scale2, float base) {
     const float2 s2 = make_float2(scale2, scale2), b2 = make_float2(-base, -base);
     float2 t[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
+    for (int j = 0; j < W; j += 2) {
         const float2 x = fma2(make_float2(v[j], v[j + 1]), s2, b2);
         t[(j / 2) & 1] = add2(t[(j / 2) & 1], make_float2(exp2_fast(x.x), exp2_fast(x.y)));
     }
@@ -177,17 +180,17 @@ __device__ __forceinline__ float sum_exp2(const float (&v)[32], float scale2, fl
     return t[0].x + t[0].y;
 }
 
-// 32 more logits of a row, labels first..first + 31 (those from `labels` on are absent). The loss
+// W more logits of a row, labels first..first + W - 1 (those from `labels` on are absent). The loss
 // takes its base from the row's first chunk and looks for the largest logit again only when a sum
-// leaves f32's range (a logit some 127 / log2(e) above the base), so that a chunk's exponentials
-// wait for nothing: the running maximum in every chunk cost a quarter of the pass at width 512.
-// `divergent`: not all of the warp's lanes are here.
-template <bool LABEL>
-__device__ __forceinline__ void add_logits(RowStats& s, float (&v)[32], uint32_t first, uint32_t labels, float scale2,
-                                           uint32_t target, bool divergent = false) {
-    if (first + 32 > labels) {
+// passes 2^64 (which leaves room to join sums in f32), so that a chunk's exponentials wait for
+// nothing: the running maximum in every chunk cost a quarter of the pass at width 512. The caller
+// says whether the target is in the chunk of any of the lanes that are here (`near`).
+template <bool LABEL, int W>
+__device__ __forceinline__ void add_logits(RowStats& s, float (&v)[W], uint32_t first, uint32_t labels, float scale2,
+                                           uint32_t target, bool near) {
+    if (first + W > labels) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
+        for (int j = 0; j < W; ++j)
             if (first + j >= labels) v[j] = -INFINITY;
     }
     if (LABEL) {
@@ -198,7 +201,7 @@ __device__ __forceinline__ void add_logits(RowStats& s, float (&v)[32], uint32_t
             s.sum *= exp2_fast(s.base - base);  // 0 after a first chunk's base of -inf
             s.base = base;
 #pragma unroll
-            for (int j = 31; j >= 0; --j)
+            for (int j = W - 1; j >= 0; --j)
                 if (v[j] == m) s.label = first + j;
         }
         // Nothing but -inf so far: any finite base counts that as 0.
@@ -212,17 +215,17 @@ __device__ __forceinline__ void add_logits(RowStats& s, float (&v)[32], uint32_t
     float base = s.base == -INFINITY ? 0.0f : s.base, sum;
     for (;;) {
         sum = s.sum + sum_exp2(v, scale2, base);
-        if (sum != INFINITY) break;
+        if (sum <= kLargestSum) break;
         const float higher = fmaxf(base, __fmul_rn(largest_of(v), scale2));
-        if (!(higher > base)) break;  // an infinite logit
+        if (!(higher > base)) break;  // the sum of many, an infinite logit, or NaN
         s.sum *= exp2_fast(base - higher);
         base = s.base = higher;
     }
     s.sum = sum;
-    const uint32_t at = target - first;
-    if (divergent ? at < 32 : __any_sync(0xffffffffu, at < 32)) {
+    if (near) {
+        const uint32_t at = target - first;
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
+        for (int j = 0; j < W; ++j)
             if (at == (uint32_t)j) s.target_logit = v[j];
     }
 }
@@ -485,8 +488,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                             if (q == 0 || c + 64 < kSide / 2) tc::tmem_load32(accumulator + c + 32 * (q + 1), v[1 - q]);
                             else drain();
                             const uint32_t column = columns_at + c + 32 * q;
-                            if (a.partial_labels) add_logits<true>(stats, v[q], column, a.labels, a.scale2, target);
-                            else add_logits<false>(stats, v[q], column, a.labels, a.scale2, target);
+                            const bool near = __any_sync(0xffffffffu, target - column < 32);
+                            if (a.partial_labels) add_logits<true>(stats, v[q], column, a.labels, a.scale2, target, near);
+                            else add_logits<false>(stats, v[q], column, a.labels, a.scale2, target, near);
                         }
                     }
                 } else {

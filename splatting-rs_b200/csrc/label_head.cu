@@ -58,6 +58,7 @@ constexpr uint32_t kRecountBlocks = 16;     // up to this many blocks each count
 constexpr uint32_t kLogitWaves = 16, kOutWaves = 4;
 constexpr double kStepUs = 0.19;            // 64 of K of a 128 x 128 tile in a single block
 constexpr double kPairCost = 1.4;           // of a 256 x 256 tile, in 128 x 128 tiles of one block
+constexpr int kSlotsAhead = 8;                // partials a thread has under way
 constexpr uint32_t kThreadSlots = 8;        // partials per row one thread joins; more take a warp
 constexpr uint64_t kSlopeBudget = 5ull << 26;  // slope elements kept at once (640 MB)
 
@@ -147,20 +148,23 @@ struct PackWeight {
 
 // Compacts the rows with targets (row_of), clears the outputs of the others, and copies the
 // features where they cannot be read in place: `in_place` 0, or some rows left out. The first
-// `gather_blocks` blocks do that, the others copy the weight.
+// `gather_blocks` * `sharers` blocks do that (`sharers` of them find the same rows and share their
+// copies, the first one writes the lists), the others copy the weight.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     k_gather_rows(const void* __restrict__ targets, int wide, uint64_t n, uint64_t labels, uint32_t gather_blocks,
+                  uint32_t sharers,
                   const uint32_t* __restrict__ counts, const uint32_t* __restrict__ group_counts,
                   const T* __restrict__ features, int64_t stride, uint32_t dim, int vector, int in_place, RowSet* rows,
                   uint32_t* __restrict__ row_of, bf16* __restrict__ packed, uint64_t packed_stride, uint64_t part,
                   float* __restrict__ losses, float* __restrict__ normalizers, T* __restrict__ gradient,
                   int64_t gradient_stride, PackWeight<T> weight) {
     chain_enter();
-    if (blockIdx.x >= gather_blocks) {
+    const uint32_t gathering = gather_blocks * sharers;
+    if (blockIdx.x >= gathering) {
         // A warp per row, eight columns a lane.
-        const uint64_t warps = (uint64_t)(gridDim.x - gather_blocks) * (kThreads / 32);
-        for (uint64_t r = (uint64_t)(blockIdx.x - gather_blocks) * (kThreads / 32) + threadIdx.x / 32; r < labels;
+        const uint64_t warps = (uint64_t)(gridDim.x - gathering) * (kThreads / 32);
+        for (uint64_t r = (uint64_t)(blockIdx.x - gathering) * (kThreads / 32) + threadIdx.x / 32; r < labels;
              r += warps)
             for (uint32_t c = lane_id() * 8; c < packed_stride; c += 256)
                 copy_parts(weight.from + (int64_t)r * weight.stride + c, c < dim ? dim - c : 0, weight.vector,
@@ -171,19 +175,20 @@ __global__ void __launch_bounds__(kThreads)
     __shared__ uint32_t skipped[kGatherRows];
     __shared__ uint32_t half_count[2];
     const uint32_t t = threadIdx.x, lane = lane_id();
-    const uint64_t first = (uint64_t)blockIdx.x * kGatherRows;
+    const uint32_t block = blockIdx.x / sharers, share = blockIdx.x % sharers;
+    const uint64_t first = (uint64_t)block * kGatherRows;
     uint32_t before = 0, all = 0;
     if (!targets) {
         before = (uint32_t)first;
         all = (uint32_t)n;
     } else if (counts) {
-        const uint32_t group = blockIdx.x / kCountGroups, groups = (gather_blocks + kCountGroups - 1) / kCountGroups;
+        const uint32_t group = block / kCountGroups, groups = (gather_blocks + kCountGroups - 1) / kCountGroups;
         for (uint32_t g = t; g < groups; g += kThreads) {
             const uint32_t c = group_counts[g];
             all += c;
             if (g < group) before += c;
         }
-        if (t < blockIdx.x % kCountGroups) before += counts[group * kCountGroups + t];
+        if (t < block % kCountGroups) before += counts[group * kCountGroups + t];
         before = block_sum(before);
         all = block_sum(all);
     } else {
@@ -213,10 +218,10 @@ __global__ void __launch_bounds__(kThreads)
         const uint32_t below = (t >= 32 ? half_count[0] : 0) + __popc(mask & ((1u << lane) - 1u));
         if (live) {
             chosen[below] = t;
-            row_of[before + below] = (uint32_t)(first + t);
+            if (share == 0) row_of[before + below] = (uint32_t)(first + t);
         } else {
             skipped[t - below] = t;
-            if (first + t < n) {
+            if (share == 0 && first + t < n) {
                 if (losses) losses[first + t] = 0.0f;
                 if (normalizers) normalizers[first + t] = 0.0f;
             }
@@ -225,20 +230,26 @@ __global__ void __launch_bounds__(kThreads)
     __syncthreads();
     if (gradient) {
         const uint32_t last = (uint32_t)min((uint64_t)kGatherRows, n - first);
-        for (uint32_t k = 0; k < last - here; ++k)
+        for (uint32_t k = share; k < last - here; k += sharers)
             for (uint32_t c = t; c < dim; c += kThreads)
                 gradient[(int64_t)(first + skipped[k]) * gradient_stride + c] = from_float<T>(0.0f);
     }
     if (in_place && all == n) return;
-    for (uint32_t r = t / 32; r < here; r += kThreads / 32)
-        for (uint32_t c = lane * 8; c < packed_stride; c += 256)
+    // A warp per 256 columns of a row, eight a lane; then zero rows up to a whole tile, which the
+    // weight's gradient sums over.
+    const uint32_t column_parts = (uint32_t)((packed_stride + 255) / 256), warps = kThreads / 32 * sharers;
+    for (uint32_t i = share * (kThreads / 32) + t / 32; i < here * column_parts; i += warps) {
+        const uint32_t r = i / column_parts, c = (i - r * column_parts) * 256 + lane * 8;
+        if (c < packed_stride)
             copy_parts(features + (int64_t)(first + chosen[r]) * stride + c, c < dim ? dim - c : 0, vector,
                        packed + (uint64_t)(before + r) * packed_stride + c, part);
-    // Zero rows up to a whole tile: the weight's gradient sums over them.
-    const uint64_t end = ((uint64_t)all + kTile - 1) / kTile * kTile;
-    for (uint64_t r = all + blockIdx.x; r < end; r += gather_blocks)
-        for (uint32_t c = t * 8; c < packed_stride; c += kThreads * 8)
-            copy_parts(features, 0, false, packed + r * packed_stride + c, part);
+    }
+    const uint64_t padding = ((uint64_t)all + kTile - 1) / kTile * kTile - all;
+    for (uint64_t i = blockIdx.x * (kThreads / 32) + t / 32; i < padding * column_parts; i += (uint64_t)gathering * (kThreads / 32)) {
+        const uint64_t r = i / column_parts;
+        const uint32_t c = (uint32_t)(i - r * column_parts) * 256 + lane * 8;
+        if (c < packed_stride) copy_parts(features, 0, false, packed + (all + r) * packed_stride + c, part);
+    }
 }
 
 // ------------------------------------------------------------------ joining
@@ -266,32 +277,41 @@ __global__ void __launch_bounds__(kThreads)
     if (i < count) {
         float top = -INFINITY, largest = -INFINITY;
         uint32_t label = 0xffffffffu;
-#pragma unroll 4
-        for (uint32_t s = lane; s < slots; s += LANES) {
-            const float x = partials[s * partial_rows + i].x;
-            if (partial_labels) {
-                const uint32_t l = partial_labels[s * partial_rows + i];
-                if (x > largest || (x == largest && l < label)) largest = x, label = l;
-                top = fmaxf(top, __fmul_rn(x, scale2));
-            } else {
-                top = fmaxf(top, x);
+        double sum = 0.0;
+        for (uint32_t s0 = lane; s0 < slots; s0 += LANES * kSlotsAhead) {
+            float2 p[kSlotsAhead];
+            uint32_t l[kSlotsAhead];
+#pragma unroll
+            for (int k = 0; k < kSlotsAhead; ++k) {
+                const uint32_t s = s0 + k * LANES;
+                p[k] = s < slots ? partials[s * partial_rows + i] : make_float2(-INFINITY, 0.0f);
+                l[k] = partial_labels && s < slots ? partial_labels[s * partial_rows + i] : 0xffffffffu;
             }
+            const float before = top;
+#pragma unroll
+            for (int k = 0; k < kSlotsAhead; ++k) {
+                if (partial_labels) {
+                    if (p[k].x > largest || (p[k].x == largest && l[k] < label)) largest = p[k].x, label = l[k];
+                    p[k].x = __fmul_rn(p[k].x, scale2);
+                }
+                top = fmaxf(top, p[k].x);
+            }
+            const float finite = top == -INFINITY ? 0.0f : top;
+            sum *= (double)exp2f(before - finite);
+#pragma unroll
+            for (int k = 0; k < kSlotsAhead; ++k) sum += (double)p[k].y * (double)exp2f(p[k].x - finite);
         }
+        float highest = top;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) {
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, o));
             const float x = __shfl_xor_sync(0xffffffffu, largest, o);
             const uint32_t l = __shfl_xor_sync(0xffffffffu, label, o);
             if (x > largest || (x == largest && l < label)) largest = x, label = l;
         }
-        if (top == -INFINITY) top = 0.0f;
-        double sum = 0.0;
-#pragma unroll 4
-        for (uint32_t s = lane; s < slots; s += LANES) {
-            const float2 p = partials[s * partial_rows + i];
-            const float base = partial_labels ? __fmul_rn(p.x, scale2) : p.x;
-            sum += (double)p.y * (double)exp2f(base - top);
-        }
+        if (highest == -INFINITY) highest = 0.0f;
+        sum *= (double)exp2f(top - highest);
+        top = highest;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) {
@@ -586,7 +606,7 @@ cudaError_t launch_thin(const sp_label_head* h, uint32_t blocks, const Operands&
     static std::atomic<unsigned long long> configured{0};
     const cudaError_t err = allow_smem_once(k_label_thin<T, DIRECT>, smem, configured);
     if (err != cudaSuccess) return err;
-    return launch_chained(k_label_thin<T, DIRECT>, blocks, kThinThreads, smem, h->ctx->stream, op.features,
+    return launch_chained(k_label_thin<T, DIRECT>, blocks, thin_threads(DIRECT), smem, h->ctx->stream, op.features,
                           op.features_packed, op.weight, args);
 }
 
@@ -629,8 +649,10 @@ sp_status prepare(sp_label_head* h, const void* features, int64_t feature_stride
             pack.from = static_cast<const T*>(weight);
             weight_blocks = (unsigned)std::min<uint64_t>((h->labels + kThreads / 32 - 1) / (kThreads / 32), 148 * 16);
         }
-        return launch_chained(k_gather_rows<T>, blocks + weight_blocks, kThreads, 0, st, targets, wide, n, h->labels,
-                              blocks, counts, static_cast<const uint32_t*>(h->counts + h->count_blocks()),
+        // Few blocks of rows share their copies among more, up to a wave of blocks.
+        const uint32_t sharers = std::max(1u, std::min(16u, h->sms / blocks));
+        return launch_chained(k_gather_rows<T>, blocks * sharers + weight_blocks, kThreads, 0, st, targets, wide, n,
+                              h->labels, blocks, sharers, counts, static_cast<const uint32_t*>(h->counts + h->count_blocks()),
                               static_cast<const T*>(features), feature_stride, h->dim,
                               (int)vector_rows(h, features, feature_stride), (int)features_here, h->rows, h->row_of,
                               h->packed_features, stride, capacity * stride, losses, normalizers,
@@ -698,7 +720,7 @@ sp_status run_stats(sp_label_head* h, const Operands& op, const void* weight, in
         thin.tiles = tiles_of(h->labels, false);
         const uint32_t blocks = std::min(thin.tiles, h->sms);
         a.partial_rows = kThinRows;
-        slots = 2 * blocks;
+        slots = blocks;
         thin.g = a;
         const cudaError_t err = h->element == SP_F32                 ? launch_thin<float, false>(h, blocks, op, thin)
                                 : in_place(h, weight, weight_stride) ? launch_thin<bf16, true>(h, blocks, op, thin)

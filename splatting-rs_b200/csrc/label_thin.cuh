@@ -1,11 +1,13 @@
 // The logits' pass for at most kThinRows rows, where the weight's bytes are what it costs: the roles
 // of label_gemm.cuh swapped (128 labels on the accumulator's lanes, the rows its columns), so that
 // the products are no wider than the rows, and the weight read once and in place: bf16 by tiled bulk
-// copies where it is aligned for them, else (f32, odd strides) by eight warps that split it into its
-// bf16 parts on the way into shared memory.
+// copies where it is aligned for them, else (f32, odd strides) by sixteen warps that split it into
+// its bf16 parts on the way into shared memory.
 //
-// The accumulation truncates, so it is spread: even and odd steps of K, and the small products of
-// f32 parts, have accumulators of their own, added in f32 at the end.
+// f32 parts of the rows lie one below the other, so that one product of a weight part covers all the
+// rows' parts it meets: accumulator groups hi hi | hi mid + mid hi | hi lo + mid mid + lo hi. Grouped
+// by size, and hi hi by even and odd steps of K, they also lose less to the tensor cores' truncating
+// additions before they are added in f32.
 #pragma once
 
 #include "label_gemm.cuh"
@@ -14,8 +16,8 @@ namespace splat {
 namespace label {
 
 constexpr int kThinRows = 64;
-constexpr int kThinThreads = 512;
-constexpr int kConvertWarps = 8;
+constexpr int kConvertWarps = 16;
+constexpr int thin_threads(bool direct) { return direct ? 256 : 256 + kConvertWarps * 32; }
 constexpr int kThinStagesF32 = 2, kThinStagesBf16 = 6;
 constexpr uint32_t kRowsBytes = kThinRows * kBlockK * 2;
 constexpr int kLogitStride = kTile + 1;  // of a row's logits in shared memory: no bank twice
@@ -70,7 +72,7 @@ struct RawEight {
 
 // DIRECT: the weight arrives by bulk copies; else through the converting warps.
 template <typename T, bool DIRECT>
-__global__ void __launch_bounds__(kThinThreads, 1)
+__global__ void __launch_bounds__(thin_threads(DIRECT), 1)
     k_label_thin(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_rows_packed,
                  const __grid_constant__ CUtensorMap map_weight, const __grid_constant__ ThinArgs a) {
     constexpr bool kF32 = sizeof(T) == 4;
@@ -106,7 +108,7 @@ __global__ void __launch_bounds__(kThinThreads, 1)
 
     const uint32_t count = a.g.all_rows ? a.g.all_rows : a.g.rows->count;
     const uint32_t tiles = count ? a.tiles : 0;
-    // A buffer's accumulators: even steps, odd steps, and the products of f32's smaller parts.
+    // A buffer's accumulator groups: f32's three, then hi hi (all, for bf16) of the odd steps.
     const uint32_t buffer_columns = 4 * kThinRows;
     bool ok = true;
 
@@ -136,7 +138,6 @@ __global__ void __launch_bounds__(kThinThreads, 1)
         }
     } else if (warp == 1) {
         if (tc::elect_one()) {
-            const uint32_t desc = tc::instruction(kTile, a.columns, false, false);
             uint32_t stage = 0, phase = 0, buffer = 0, buffer_phase = 0;
             for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
                 if (!(ok = tc::barrier_wait(drained + 8 * buffer, buffer_phase ^ 1))) break;
@@ -147,15 +148,25 @@ __global__ void __launch_bounds__(kThinThreads, 1)
                     tc::fence_after_sync();
                     const uint32_t w_at = smem + stage * kBytes, r_at = w_at + kParted * kOperandBytes;
 #pragma unroll
-                    for (int p = 0; p < (kF32 ? (int)kPartProducts : 1); ++p) {
-                        const uint32_t pw = kF32 ? (kPartsOfA >> (4 * p)) & 15u : 0, pr = kF32 ? (kPartsOfB >> (4 * p)) & 15u : 0;
-                        const bool small = kF32 && p + 1 < (int)kPartProducts;
-                        const uint32_t accumulator = into + (small ? 2 : k & 1) * kThinRows;
-#pragma unroll
-                        for (int q = 0; q < kBlockK / 16; ++q) {
-                            const bool add = small ? k != 0 || p != 0 || q != 0 : k > 1 || q != 0;
-                            tc::multiply<false>(accumulator, tc::operand(w_at + pw * kOperandBytes + q * 32, kBoxBytes),
-                                                tc::operand(r_at + pr * kRowsBytes + q * 32, kBoxBytes), desc, add);
+                    for (int q = 0; q < kBlockK / 16; ++q) {
+                        auto product = [&](int weight_part, int rows_part, uint32_t group, uint32_t n, bool add) {
+                            tc::multiply<false>(into + group * kThinRows,
+                                                tc::operand(w_at + weight_part * kOperandBytes + q * 32, kBoxBytes),
+                                                tc::operand(r_at + rows_part * kRowsBytes + q * 32, kBoxBytes),
+                                                tc::instruction(kTile, n, false, false), add);
+                        };
+                        const bool again = k > 1 || q != 0;
+                        if (!kF32) {
+                            product(0, 0, k & 1 ? 3 : 0, a.columns, again);
+                        } else {
+                            if (k & 1) {
+                                product(0, 0, 3, kThinRows, again);
+                                product(0, 1, 1, 2 * kThinRows, true);
+                            } else {
+                                product(0, 0, 0, 3 * kThinRows, again);
+                            }
+                            product(1, 0, 1, 2 * kThinRows, true);
+                            product(2, 0, 2, kThinRows, true);
                         }
                     }
                     tc::commit<false>(empty + 8 * stage);
@@ -167,11 +178,13 @@ __global__ void __launch_bounds__(kThinThreads, 1)
             }
         }
     } else if (warp >= 4 && warp < 8) {
-        // The tile's logits turn over in shared memory: a thread reads a label's, then two threads
-        // take half of a row's each.
-        const uint32_t t = threadIdx.x - 128, row = t / 2, half = t % 2;
+        // The tile's logits turn over in shared memory: a thread reads a label's, then 128 / columns
+        // threads (to a power of two) take a row's, 16 at a time.
+        const uint32_t t = threadIdx.x - 128;
+        const uint32_t split = a.columns <= 16 ? 3 : a.columns <= 32 ? 2 : 1;
+        const uint32_t row = t >> split, part = t & ((1u << split) - 1), span = kTile >> split;
         const bool live = row < count;
-        RowStats stats{-INFINITY, 0.0f, 0.0f, -INFINITY, 0u};
+        RowStats stats{-INFINITY, 0.0f, 0.0f, -INFINITY, 0xffffffffu};
         uint32_t target = kNoTarget;
         if (live && a.g.targets)
             target = (uint32_t)index_at(a.g.targets, a.g.wide, a.g.all_rows ? row : a.g.row_of[row], a.g.labels);
@@ -187,17 +200,18 @@ __global__ void __launch_bounds__(kThinThreads, 1)
             const uint32_t from = tmem + buffer * buffer_columns + (((warp - 4) * 32) << 16);
             for (uint32_t c = 0; c < a.columns; c += 16) {
                 float v[16], w[16];
-                tmem_load16(from + c, v);
-                if (a.g.k_blocks > 1) tmem_load16(from + kThinRows + c, w);
-                tc::tmem_load_wait();
-                if (a.g.k_blocks > 1)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) v[j] += w[j];
-                if (kF32) {
-                    tmem_load16(from + 2 * kThinRows + c, w);
+                auto add_group = [&](uint32_t group) {
+                    tmem_load16(from + group * kThinRows + c, w);
                     tc::tmem_load_wait();
 #pragma unroll
                     for (int j = 0; j < 16; ++j) v[j] += w[j];
+                };
+                tmem_load16(from + c, v);
+                tc::tmem_load_wait();
+                if (a.g.k_blocks > 1) add_group(3);
+                if (kF32) {
+                    add_group(1);
+                    add_group(2);
                 }
 #pragma unroll
                 for (int j = 0; j < 16; ++j) logits[(c + j) * kLogitStride + t] = v[j];
@@ -208,28 +222,41 @@ __global__ void __launch_bounds__(kThinThreads, 1)
             asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
             if (row < a.columns) {
 #pragma unroll 1
-                for (int c = 0; c < kTile / 2; c += 32) {
-                    const uint32_t first = half * (kTile / 2) + c;
-                    float v[32];
+                for (uint32_t c = 0; c < span; c += 16) {
+                    const uint32_t at = part * span + c, first = tile * kTile + at;
+                    float v[16];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = logits[row * kLogitStride + first + j];
-                    if (a.g.partial_labels) add_logits<true>(stats, v, tile * kTile + first, a.g.labels, a.g.scale2, target, true);
-                    else add_logits<false>(stats, v, tile * kTile + first, a.g.labels, a.g.scale2, target, true);
+                    for (int j = 0; j < 16; ++j) v[j] = logits[row * kLogitStride + at + j];
+                    const bool near = target - first < 16;
+                    if (a.g.partial_labels) add_logits<true>(stats, v, first, a.g.labels, a.g.scale2, target, near);
+                    else add_logits<false>(stats, v, first, a.g.labels, a.g.scale2, target, near);
+                    if (near) a.g.target_logits[row] = stats.target_logit;
                 }
             }
             asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
             if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
         }
-        if (ok && live) {
-            const uint64_t slot = (uint64_t)(blockIdx.x * 2 + half) * a.g.partial_rows + row;
+        // The row's parts, in neighbouring lanes, as one.
+        __syncwarp();
+        for (uint32_t o = 1; o < (1u << split); o <<= 1) {
+            const float base = __shfl_xor_sync(0xffffffffu, stats.base, o), sum = __shfl_xor_sync(0xffffffffu, stats.sum, o);
+            const float largest = __shfl_xor_sync(0xffffffffu, stats.largest, o);
+            const uint32_t label = __shfl_xor_sync(0xffffffffu, stats.label, o);
+            const float top = fmaxf(stats.base, base), finite = top == -INFINITY ? 0.0f : top;
+            const float mine = stats.sum * exp2_fast(stats.base - finite), theirs = sum * exp2_fast(base - finite);
+            stats.sum = part & o ? theirs + mine : mine + theirs;
+            stats.base = top;
+            if (largest > stats.largest || (largest == stats.largest && label < stats.label))
+                stats.largest = largest, stats.label = label;
+        }
+        if (ok && live && part == 0) {
+            const uint64_t slot = (uint64_t)blockIdx.x * a.g.partial_rows + row;
             a.g.partials[slot] = make_float2(a.g.partial_labels ? stats.largest : stats.base, stats.sum);
             if (a.g.partial_labels) a.g.partial_labels[slot] = stats.label;
-            if (target != kNoTarget && target / kTile % gridDim.x == blockIdx.x && target % kTile / (kTile / 2) == half)
-                a.g.target_logits[row] = stats.target_logit;
         }
     } else if (warp >= 8 && !DIRECT) {
-        // Eight lanes a row of 64 columns, 32 rows a turn; the next two steps' loads are under way.
-        constexpr int kTurns = kTile / 32;
+        // Eight lanes a row of 64 columns, 64 rows a turn; the next two steps' loads are under way.
+        constexpr int kTurnRows = kConvertWarps * 4, kTurns = kTile / kTurnRows;
         const uint32_t t = threadIdx.x - 256, unit = t % 8, first_row = t / 8;
         const T* weight = static_cast<const T*>(a.weight);
         RawEight<T> raw[2][kTurns];
@@ -241,7 +268,7 @@ __global__ void __launch_bounds__(kThinThreads, 1)
             const uint32_t columns = column < a.dim ? a.dim - column : 0;
 #pragma unroll
             for (int r = 0; r < kTurns; ++r) {
-                const uint32_t label = load_tile * kTile + r * 32 + first_row;
+                const uint32_t label = load_tile * kTile + r * kTurnRows + first_row;
                 const bool there = label < a.g.labels && load_tile < tiles;
                 to[r].load(weight + (there ? (int64_t)label * a.weight_stride + column : 0), there ? columns : 0, a.vector);
             }
@@ -254,7 +281,7 @@ __global__ void __launch_bounds__(kThinThreads, 1)
                 constexpr int N = RawEight<T>::N;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = from[r].p[j / N].get(j % N);
-                const uint32_t row = r * 32 + first_row, at = to + row * 128 + ((unit ^ (row & 7u)) * 16);
+                const uint32_t row = r * kTurnRows + first_row, at = to + row * 128 + ((unit ^ (row & 7u)) * 16);
 #pragma unroll
                 for (int p = 0; p < kParted; ++p) {
                     Pack<bf16, 8> o;
