@@ -4,7 +4,8 @@
 //   kStats   the logits' running sum of exponentials per row, and the target's logit or the
 //            largest one and its label
 //   kSlopes  the softmax slopes c g (p - [target]), written as bf16 parts
-//   kOut     the tile itself: an output gradient, or a partial sum of one
+//   kOut     the tile itself, or a partial sum of it, of the two output gradients dH = G W and
+//            dW = G^T H, in one launch: the tiles of one fill the SMs the other's leave
 //
 // A block is one producer warp (tiled bulk copies into a ring of shared-memory stages), one warp
 // that issues the products, and eight warps that empty one accumulator while the other fills. In a
@@ -52,18 +53,28 @@ constexpr uint32_t kNoTarget = 0xffffffffu;  // index_at's -1
 
 enum Ending { kStats = 0, kSlopes = 1, kOut = 2 };
 
+// One of the output gradients of a chunk of rows.
+struct OutArgs {
+    uint32_t m_tiles, n_tiles, splits;  // m_tiles: dW's; dH's follow the row count
+    uint32_t k_blocks;                  // dH's; dW's follow the row count
+    void* out;            // the gradient itself, or f32 partial sums [splits][rows][stride]
+    int64_t stride;
+    uint64_t rows;        // of the partial sums, or of dW
+    int partial;          // out holds partial sums
+    int add;              // ... and this call adds to them
+    int packed;           // 16-byte stores are aligned
+};
+
 struct GemmArgs {
     RowSet* rows;
     const uint32_t* row_of;
     uint32_t all_rows;     // not 0: that many rows, all of them count and are read in place
-    uint32_t labels;
+    uint32_t labels, dim;
     uint32_t products;     // 1, or kPartProducts
-    uint32_t k_blocks;     // of the inner dimension; kOut with rows_inner: follows the row count
-    uint32_t m_tiles;      // kOut only: where the outer dimension is not the rows
-    uint32_t n_tiles;
-    uint32_t splits;       // kStats, kSlopes: of the label tiles; kOut: of the inner dimension
+    uint32_t k_blocks;     // kStats, kSlopes: of the features' columns
+    uint32_t n_tiles;      // kStats, kSlopes: of the labels
+    uint32_t splits;       // ... and the pieces they are cut into
     uint32_t first_row, chunk_rows;  // kSlopes, kOut: the rows of this call's slopes
-    uint32_t rows_inner;   // kOut: the inner dimension is the rows (the weight's gradient)
     float scale, scale2;   // the logits' scale, and times log2(e)
     const void* targets;
     int wide;
@@ -76,43 +87,47 @@ struct GemmArgs {
     const float* log_normalizers;
     const float* row_gradient;
     // kOut
-    void* out;             // the gradient itself, or f32 partial sums [splits][out_rows][out_stride]
-    int64_t out_stride;
-    uint64_t out_rows;
-    uint32_t out_columns;
-    int partial;           // out holds partial sums
-    int add;               // ... and this call adds to them
-    int scatter;           // output row i is row_of[first_row + i]
-    int out_packed;        // 16-byte stores are aligned
+    OutArgs out[2];        // dH, dW
+    int weight_first;      // dW's tiles, the longer ones, come first
 };
 
 struct Work {
-    uint32_t m, n0, n1, k0, k1, split;
+    uint32_t m, n0, n1, k0, k1, split, which;
 };
 
 template <int ENDING, int TILE>
 struct Schedule {
-    uint32_t items, m_tiles, k_blocks;
+    uint32_t items, m_tiles, k_blocks, row_blocks, before;
     __device__ Schedule(const GemmArgs& a, uint32_t count) {
         const uint32_t here = count > a.first_row ? min(count - a.first_row, a.chunk_rows) : 0;
-        k_blocks = a.k_blocks;
         m_tiles = (here + TILE - 1) / TILE;
-        if (ENDING == kOut && a.rows_inner) {
-            k_blocks = (here + kBlockK - 1) / kBlockK;
-            m_tiles = a.m_tiles;
+        k_blocks = a.k_blocks;
+        row_blocks = (here + kBlockK - 1) / kBlockK;
+        items = m_tiles * a.splits;
+        before = 0;
+        if (ENDING == kOut) {
+            const uint32_t features = m_tiles * a.out[0].n_tiles * a.out[0].splits;
+            const uint32_t weight = a.out[1].m_tiles * a.out[1].n_tiles * a.out[1].splits;
+            items = features + weight;
+            before = a.weight_first ? weight : features;
         }
-        items = m_tiles * a.splits * (ENDING == kOut ? a.n_tiles : 1);
     }
     __device__ Work at(const GemmArgs& a, uint32_t item) const {
         Work w;
+        w.which = 0;
         if (ENDING == kOut) {
+            const bool second = item >= before;
+            if (second) item -= before;
+            w.which = (a.weight_first != 0) != second ? 1 : 0;
+            const OutArgs& o = a.out[w.which];
+            const uint32_t tiles = w.which ? o.m_tiles : m_tiles, blocks = w.which ? row_blocks : o.k_blocks;
             // Neighbours share the slopes' tiles, the larger operand.
-            w.n0 = item % a.n_tiles;
+            w.n0 = item % o.n_tiles;
             w.n1 = w.n0 + 1;
-            w.m = item / a.n_tiles % m_tiles;
-            w.split = item / a.n_tiles / m_tiles;
-            w.k0 = (uint32_t)((uint64_t)k_blocks * w.split / a.splits);
-            w.k1 = (uint32_t)((uint64_t)k_blocks * (w.split + 1) / a.splits);
+            w.m = item / o.n_tiles % tiles;
+            w.split = item / o.n_tiles / tiles;
+            w.k0 = (uint32_t)((uint64_t)blocks * w.split / o.splits);
+            w.k1 = (uint32_t)((uint64_t)blocks * (w.split + 1) / o.splits);
         } else {
             // Neighbours share the label tiles.
             w.m = item % m_tiles;
@@ -294,11 +309,29 @@ __device__ __forceinline__ void store_out(T* to, const float (&v)[32], uint32_t 
     }
 }
 
-template <int ENDING, bool A_TRANSPOSED, bool B_TRANSPOSED, bool PAIR, typename T>
+// Adds to 32 f32 sums in memory where they lie: each has one adder in a launch, so the order of the
+// additions is that of the launches.
+__device__ __forceinline__ void add_out(float* to, const float (&v)[32], uint32_t columns) {
+    if (columns >= 32) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+            asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to + j), "f"(v[j]),
+                         "f"(v[j + 1]), "f"(v[j + 2]), "f"(v[j + 3])
+                         : "memory");
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if ((uint32_t)j < columns) to[j] += v[j];
+    }
+}
+
+// map_slopes: 64 x 64 boxes to read (kOut), 64 x 32 to write (kSlopes).
+template <int ENDING, bool PAIR, typename T>
 __global__ void __launch_bounds__(kGemmThreads, 1)
-    k_label_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_packed,
-                 const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_b_packed,
-                 const __grid_constant__ CUtensorMap map_slopes, const __grid_constant__ GemmArgs a) {
+    k_label_gemm(const __grid_constant__ CUtensorMap map_features,
+                 const __grid_constant__ CUtensorMap map_features_packed,
+                 const __grid_constant__ CUtensorMap map_weight, const __grid_constant__ CUtensorMap map_slopes,
+                 const __grid_constant__ GemmArgs a) {
     constexpr int kBlocks = PAIR ? 2 : 1;
     constexpr int kSide = kTile * kBlocks;  // the pair's tile
     extern __shared__ uint8_t smem_raw[];
@@ -322,6 +355,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             tc::barrier_init(drained + 8 * b, kEpilogueWarps * kBlocks);
         }
         tc::barrier_init_fence();
+        tc::prefetch_map(&map_features);
+        tc::prefetch_map(&map_weight);
     }
     if (warp == 2) tc::tmem_alloc<PAIR>(tmem_slot, 2 * kSide);
     tc::fence_before_sync();
@@ -338,15 +373,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 
     if (warp == 0) {
         if (tc::elect_one()) {
-            const CUtensorMap* pa = packed ? &map_a_packed : &map_a;
-            const CUtensorMap* pb = packed ? &map_b_packed : &map_b;
+            const CUtensorMap* features = packed ? &map_features_packed : &map_features;
             uint32_t stage = 0, phase = 0;
-            // The rows' operand of kOut starts at the chunk's first row in the features, at 0 in the slopes.
-            const int a_rows = ENDING == kOut ? 0 : (int)a.first_row;
-            const int b_rows = ENDING == kOut && B_TRANSPOSED && a.rows_inner ? (int)a.first_row : 0;
             for (uint32_t item = first_item; ok && item < schedule.items; item += item_step) {
                 const Work w = schedule.at(a, item);
-                const int am = (int)(w.m * kSide + rank * kTile);
+                const int am = (int)(w.m * kSide + rank * kTile), first_row = (int)a.first_row;
                 for (uint32_t n = w.n0; ok && n < w.n1; ++n) {
                     const int bn = (int)(n * kSide + rank * kTile);
                     for (uint32_t p = 0; ok && p < a.products; ++p) {
@@ -362,10 +393,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 const uint32_t ta = to + h * kBoxBytes, tb = ta + kOperandBytes;
-                                if (A_TRANSPOSED) tc::load_box<PAIR>(ta, pa, bar, am + h * 64, a_rows + kk, za);
-                                else tc::load_box<PAIR>(ta, pa, bar, kk, a_rows + am + h * 64, za);
-                                if (B_TRANSPOSED) tc::load_box<PAIR>(tb, pb, bar, bn + h * 64, b_rows + kk, zb);
-                                else tc::load_box<PAIR>(tb, pb, bar, kk, bn + h * 64, zb);
+                                const int m = am + h * 64, bm = bn + h * 64;
+                                if (ENDING != kOut) {  // H W^T
+                                    tc::load_box<PAIR>(ta, features, bar, kk, first_row + m, za);
+                                    tc::load_box<PAIR>(tb, &map_weight, bar, kk, bm, zb);
+                                } else if (w.which == 0) {  // G W
+                                    tc::load_box<PAIR>(ta, &map_slopes, bar, kk, m, za);
+                                    tc::load_box<PAIR>(tb, &map_weight, bar, bm, kk, zb);
+                                } else {  // G^T H
+                                    tc::load_box<PAIR>(ta, &map_slopes, bar, m, kk, za);
+                                    tc::load_box<PAIR>(tb, features, bar, bm, first_row + kk, zb);
+                                }
                             }
                             if (++stage == kStages) stage = 0, phase ^= 1;
                         }
@@ -380,12 +418,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
     } else if (warp == 1) {
         if (rank == 0 && tc::elect_one()) {
-            constexpr uint32_t desc = tc::instruction(kSide, kSide, A_TRANSPOSED, B_TRANSPOSED);
             uint32_t stage = 0, phase = 0, buffer = 0, buffer_phase = 0;
             for (uint32_t item = first_item; ok && item < schedule.items; item += item_step) {
                 const Work w = schedule.at(a, item);
                 const uint32_t steps = (w.k1 - w.k0) * a.products;
                 if (steps == 0) continue;
+                // Which operands run along K in memory: W in dH; G and H in dW. 16 of K are 32 bytes along
+                // a row, or 16 rows of 128 bytes.
+                const bool a_transposed = w.which != 0;
+                constexpr bool b_transposed = ENDING == kOut;
+                const uint32_t desc = tc::instruction(kSide, kSide, a_transposed, b_transposed);
+                const uint32_t a_step = a_transposed ? 2048 : 32, b_step = b_transposed ? 2048 : 32;
                 for (uint32_t n = w.n0; ok && n < w.n1; ++n) {
                     if (!(ok = tc::barrier_wait(drained + 8 * buffer, buffer_phase ^ 1))) break;
                     tc::fence_after_sync();
@@ -395,9 +438,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                         const uint32_t at = smem + stage * kStageBytes;
 #pragma unroll
                         for (int q = 0; q < kBlockK / 16; ++q) {
-                            // 16 of K: 32 bytes along a row, or 16 rows of 128 bytes.
-                            const uint64_t da = tc::operand(at + q * (A_TRANSPOSED ? 2048 : 32), kBoxBytes);
-                            const uint64_t db = tc::operand(at + kOperandBytes + q * (B_TRANSPOSED ? 2048 : 32), kBoxBytes);
+                            const uint64_t da = tc::operand(at + q * a_step, kBoxBytes);
+                            const uint64_t db = tc::operand(at + kOperandBytes + q * b_step, kBoxBytes);
                             tc::multiply<PAIR>(tmem + buffer * kSide, da, db, desc, k != 0 || q != 0);
                         }
                         tc::commit<PAIR>(empty + 8 * stage);
@@ -416,10 +458,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         const uint32_t tmem_at = tmem + ((quarter * 32) << 16) + half * (kSide / 2);
         const uint32_t stage_tile = store_at + (warp - 4) * kStoreBytes;
         uint32_t buffer = 0, buffer_phase = 0;
-        for (uint32_t item = first_item; ok && item < schedule.items; item += item_step) {
+        // Output gradients of a call that gave up, here or in a kernel before, are NaN.
+        const bool poisoned = ENDING == kOut && a.rows->status != 0;
+        for (uint32_t item = first_item; (ok || ENDING == kOut) && item < schedule.items; item += item_step) {
             const Work w = schedule.at(a, item);
             const bool empty_sum = w.k0 == w.k1;
-            if (ENDING == kOut && empty_sum && a.add) continue;
+            const OutArgs& o = a.out[w.which];
+            if (ENDING == kOut && empty_sum && o.add) continue;
             const uint32_t row = w.m * kSide + lane_row;  // in this call's rows (or labels)
             const uint32_t compact = a.first_row + row;
             const bool live = compact < count;
@@ -434,9 +479,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                     weight = a.scale * (a.row_gradient ? a.row_gradient[original] : 1.0f / (float)count);
                 }
             }
-            for (uint32_t n = w.n0; ok && n < w.n1; ++n) {
-                if (!empty_sum) {
-                    if (!(ok = tc::barrier_wait(done + 8 * buffer, buffer_phase))) break;
+            for (uint32_t n = w.n0; (ok || ENDING == kOut) && n < w.n1; ++n) {
+                if (!empty_sum && ok) {
+                    ok = __all_sync(0xffffffffu, tc::barrier_wait(done + 8 * buffer, buffer_phase));
+                    if (ENDING != kOut && !ok) break;
                     tc::fence_after_sync();
                 }
                 // After the last load the accumulator may fill again.
@@ -497,7 +543,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
                     for (int c = 0; c < kSide / 2; c += 32) {
                         float v[32];
-                        if (empty_sum) {
+                        if (empty_sum || !ok) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] = 0.0f;
                         } else {
@@ -506,22 +552,21 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                             tc::tmem_load_wait();
                             if (c + 32 == kSide / 2) drain();
                         }
-                        const uint32_t column = columns_at + c;
-                        if ((a.rows_inner ? row < a.out_rows : live) && column < a.out_columns) {
-                            const uint32_t columns = a.out_columns - column;
-                            if (a.partial) {
-                                float* to = static_cast<float*>(a.out) +
-                                            ((uint64_t)w.split * a.out_rows + row) * (uint64_t)a.out_stride + column;
-                                if (a.add) {
+                        if (poisoned || !ok) {
 #pragma unroll
-                                    for (int j = 0; j < 32; ++j)
-                                        if ((uint32_t)j < columns) v[j] += to[j];
-                                }
-                                store_out<float>(to, v, columns, true);
+                            for (int j = 0; j < 32; ++j) v[j] = __int_as_float(0x7fffffff);
+                        }
+                        const uint32_t column = columns_at + c;
+                        if ((w.which ? row < o.rows : live) && column < a.dim) {
+                            const uint32_t columns = a.dim - column;
+                            if (o.partial) {
+                                float* to = static_cast<float*>(o.out) + ((uint64_t)w.split * o.rows + row) * (uint64_t)o.stride +
+                                            column;
+                                if (o.add) add_out(to, v, columns);
+                                else store_out<float>(to, v, columns, true);
                             } else {
-                                const uint64_t r = a.scatter ? a.row_of[compact] : row;
-                                store_out<T>(static_cast<T*>(a.out) + (int64_t)r * a.out_stride + column, v, columns,
-                                             a.out_packed);
+                                const uint64_t r = w.which ? row : a.row_of[compact];
+                                store_out<T>(static_cast<T*>(o.out) + (int64_t)r * o.stride + column, v, columns, o.packed);
                             }
                         }
                     }

@@ -56,10 +56,11 @@ constexpr uint32_t kGatherRows = 64;        // rows a block compacts and copies
 constexpr uint32_t kCountGroups = 16;       // such blocks' counts are summed this many at a time
 constexpr uint32_t kRecountBlocks = 16;     // up to this many blocks each count all targets themselves
 constexpr uint32_t kLogitWaves = 16, kOutWaves = 4;
+constexpr double kLaunchUs = 3.0;           // of a small kernel in the chain
 constexpr double kStepUs = 0.19;            // 64 of K of a 128 x 128 tile in a single block
 constexpr double kPairCost = 1.4;           // of a 256 x 256 tile, in 128 x 128 tiles of one block
 constexpr int kSlotsAhead = 8;                // partials a thread has under way
-constexpr uint32_t kThreadSlots = 8;        // partials per row one thread joins; more take a warp
+constexpr uint32_t kThreadSlots = 8;
 constexpr uint64_t kSlopeBudget = 5ull << 26;  // slope elements kept at once (640 MB)
 
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
@@ -254,7 +255,7 @@ __global__ void __launch_bounds__(kThreads)
 
 // ------------------------------------------------------------------ joining
 
-// `LANES` threads (1 or 32) join a row's partial sums, each in units of 2^base: the highest base
+// LANES threads (1, 8 or 32) join a row's partial sums, each in units of 2^base: the highest base
 // (and the largest logit with the lowest label) first, then the sum, in double, since a part may come
 // close to f32's largest. In units of ln 2 a row's log sum exp is base + log2(sum), its loss that less
 // z[target] scale2, and its largest log-probability the negative of that with the largest logit, all
@@ -274,58 +275,59 @@ __global__ void __launch_bounds__(kThreads)
     const uint64_t i = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) / LANES;
     const uint32_t lane = threadIdx.x % LANES;
     double loss = 0.0;
-    if (i < count) {
-        float top = -INFINITY, largest = -INFINITY;
-        uint32_t label = 0xffffffffu;
-        double sum = 0.0;
-        for (uint32_t s0 = lane; s0 < slots; s0 += LANES * kSlotsAhead) {
-            float2 p[kSlotsAhead];
-            uint32_t l[kSlotsAhead];
+    // Rows past the last go through with no partials: every lane takes part in the shuffles.
+    const uint32_t mine = i < count ? slots : 0;
+    float top = -INFINITY, largest = -INFINITY;
+    uint32_t label = 0xffffffffu;
+    double sum = 0.0;
+    for (uint32_t s0 = lane; s0 < mine; s0 += LANES * kSlotsAhead) {
+        float2 p[kSlotsAhead];
+        uint32_t l[kSlotsAhead];
 #pragma unroll
-            for (int k = 0; k < kSlotsAhead; ++k) {
-                const uint32_t s = s0 + k * LANES;
-                p[k] = s < slots ? partials[s * partial_rows + i] : make_float2(-INFINITY, 0.0f);
-                l[k] = partial_labels && s < slots ? partial_labels[s * partial_rows + i] : 0xffffffffu;
-            }
-            const float before = top;
-#pragma unroll
-            for (int k = 0; k < kSlotsAhead; ++k) {
-                if (partial_labels) {
-                    if (p[k].x > largest || (p[k].x == largest && l[k] < label)) largest = p[k].x, label = l[k];
-                    p[k].x = __fmul_rn(p[k].x, scale2);
-                }
-                top = fmaxf(top, p[k].x);
-            }
-            const float finite = top == -INFINITY ? 0.0f : top;
-            sum *= (double)exp2f(before - finite);
-#pragma unroll
-            for (int k = 0; k < kSlotsAhead; ++k) sum += (double)p[k].y * (double)exp2f(p[k].x - finite);
+        for (int k = 0; k < kSlotsAhead; ++k) {
+            const uint32_t s = s0 + k * LANES;
+            p[k] = s < mine ? partials[s * partial_rows + i] : make_float2(-INFINITY, 0.0f);
+            l[k] = partial_labels && s < mine ? partial_labels[s * partial_rows + i] : 0xffffffffu;
         }
-        float highest = top;
+        const float before = top;
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) {
-            highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, o));
-            const float x = __shfl_xor_sync(0xffffffffu, largest, o);
-            const uint32_t l = __shfl_xor_sync(0xffffffffu, label, o);
-            if (x > largest || (x == largest && l < label)) largest = x, label = l;
-        }
-        if (highest == -INFINITY) highest = 0.0f;
-        sum *= (double)exp2f(top - highest);
-        top = highest;
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) {
-            const uint32_t row = all_rows ? (uint32_t)i : row_of[i];
-            const double ln2 = 0.6931471805599453, log2_sum = (double)top + log2(sum);
-            if (labels_out) {
-                labels_out[row] = failed ? -1 : (int32_t)label;
-                log_probability[row] = failed ? nan : (float)(((double)largest * scale2 - log2_sum) * ln2);
-            } else {
-                const float value = failed ? nan : (float)((log2_sum - (double)target_logits[i] * scale2) * ln2);
-                losses[row] = value;
-                normalizers[row] = failed ? nan : (float)(log2_sum * ln2);
-                loss = (double)value;
+        for (int k = 0; k < kSlotsAhead; ++k) {
+            if (partial_labels) {
+                if (p[k].x > largest || (p[k].x == largest && l[k] < label)) largest = p[k].x, label = l[k];
+                p[k].x = __fmul_rn(p[k].x, scale2);
             }
+            top = fmaxf(top, p[k].x);
+        }
+        const float finite = top == -INFINITY ? 0.0f : top;
+        sum *= (double)exp2f(before - finite);
+#pragma unroll
+        for (int k = 0; k < kSlotsAhead; ++k)
+            if (s0 + k * LANES < mine) sum += (double)p[k].y * (double)exp2f(p[k].x - finite);
+    }
+    float highest = top;
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+        highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, o));
+        const float x = __shfl_xor_sync(0xffffffffu, largest, o);
+        const uint32_t l = __shfl_xor_sync(0xffffffffu, label, o);
+        if (x > largest || (x == largest && l < label)) largest = x, label = l;
+    }
+    if (highest == -INFINITY) highest = 0.0f;
+    sum *= (double)exp2f(top - highest);
+    top = highest;
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (i < count && lane == 0) {
+        const uint32_t row = all_rows ? (uint32_t)i : row_of[i];
+        const double ln2 = 0.6931471805599453, log2_sum = (double)top + log2(sum);
+        if (labels_out) {
+            labels_out[row] = failed ? -1 : (int32_t)label;
+            log_probability[row] = failed ? nan : (float)(((double)largest * scale2 - log2_sum) * ln2);
+        } else {
+            const float value = failed ? nan : (float)((log2_sum - (double)target_logits[i] * scale2) * ln2);
+            losses[row] = value;
+            normalizers[row] = failed ? nan : (float)(log2_sum * ln2);
+            loss = (double)value;
         }
     }
     if (labels_out) return;
@@ -342,22 +344,22 @@ __global__ void __launch_bounds__(kThreads)
             for (int w = 0; w < kThreads / 32; ++w) sum += shared[w];
         return sum;
     };
-    double sum = block_total(loss);
+    double total = block_total(loss);
     if (gridDim.x > 1) {
         if (threadIdx.x == 0) {
-            block_sums[blockIdx.x] = sum;
+            block_sums[blockIdx.x] = total;
             __threadfence();
             last = atomicAdd(&rows->ticket, 1u) == gridDim.x - 1;
         }
         __syncthreads();
         if (!last) return;
         __threadfence();
-        sum = 0.0;
-        for (uint32_t b = threadIdx.x; b < gridDim.x; b += kThreads) sum += __ldcg(block_sums + b);
-        sum = block_total(sum);
+        total = 0.0;
+        for (uint32_t b = threadIdx.x; b < gridDim.x; b += kThreads) total += __ldcg(block_sums + b);
+        total = block_total(total);
     }
     if (threadIdx.x == 0) {
-        *mean = failed ? nan : (float)(sum / (double)max(count, 1u));
+        *mean = failed ? nan : (float)(total / (double)max(count, 1u));
         rows->ticket = 0;
     }
 }
@@ -374,7 +376,8 @@ struct JoinArgs {
     uint64_t all_rows;  // rows of the whole gradient
 };
 
-// Both gradients of a chunk; after the last chunk, NaN throughout if a device wait gave up.
+// Both gradients of a chunk; after the last chunk, NaN throughout if a device wait gave up (a gradient
+// without sums got its own from k_label_gemm).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_join_gradients(const RowSet* __restrict__ rows,
                                                              const uint32_t* __restrict__ row_of, uint32_t dim,
@@ -491,24 +494,48 @@ Plan plan_logits(uint32_t sms, uint64_t rows, uint64_t labels) {
     return best;
 }
 
-// The same for an output gradient. Its pieces go through f32 sums, written and read at some
-// 6.5 TB/s against kStepUs for a single block's step; at most kOutWaves waves, none below 4 steps.
-// `cost`: in microseconds.
-Plan plan_out(uint32_t sms, uint64_t rows, uint64_t columns, uint32_t k_blocks, double* cost_out = nullptr) {
-    Plan best{};
-    double best_cost = 1e300;
+// The same for the two output gradients of a chunk of rows, whose tiles share the SMs, the longer
+// ones first. Their pieces go through f32 sums, written and read at some 6.5 TB/s (and joined by a
+// launch of their own) against kStepUs for a single block's step; at most kOutWaves waves of pieces,
+// none below 4 steps. With `weight_splits` not 0 the weight's gradient is cut as before.
+struct OutPlan {
+    bool pair;
+    uint32_t m_features, m_weight, n, features, weight;  // tiles, and the pieces of either
+    bool weight_first;
+    double us;
+    uint64_t items() const { return ((uint64_t)m_features * features + (uint64_t)m_weight * weight) * n; }
+};
+
+OutPlan plan_out(uint32_t sms, uint64_t rows, uint64_t labels, uint32_t dim, uint32_t parts, bool sums_anyway,
+                 uint32_t weight_splits = 0, int pair_only = -1) {
+    OutPlan best{};
+    best.us = 1e300;
+    const uint32_t label_k = (uint32_t)((labels + kBlockK - 1) / kBlockK), row_k = (uint32_t)((rows + kBlockK - 1) / kBlockK);
+    const double products = parts > 1 ? kPartProducts : 1;
     for (int pair = 0; pair < 2; ++pair) {
+        if (pair_only >= 0 && pair != pair_only) continue;
         const uint32_t workers = pair ? std::max(sms / 2, 1u) : sms;
-        const uint32_t m = tiles_of(rows, pair), n = tiles_of(columns, pair);
-        const uint64_t tiles = (uint64_t)m * n;
-        for (uint32_t s = 1; s == 1 || (tiles * s <= (uint64_t)kOutWaves * workers && k_blocks >= 4 * s); ++s) {
-            double cost = (double)((tiles * s + workers - 1) / workers) * ((k_blocks + s - 1) / s) * kStepUs *
-                          (pair ? kPairCost : 1.0);
-            if (s > 1) cost += (double)s * rows * columns * 8.0 / 6.5e6;
-            if (cost < best_cost) best_cost = cost, best = Plan{pair != 0, m, n, s};
-        }
+        const uint32_t mf = tiles_of(rows, pair), mw = tiles_of(labels, pair), n = tiles_of(dim, pair);
+        auto allowed = [&](uint64_t tiles, uint32_t s, uint32_t k) {
+            return s == 1 || (tiles * s <= (uint64_t)kOutWaves * workers && k >= 4 * s);
+        };
+        for (uint32_t sf = 1; allowed((uint64_t)mf * n, sf, label_k); ++sf)
+            for (uint32_t sw = weight_splits ? weight_splits : 1;
+                 (weight_splits && sw == weight_splits) || (!weight_splits && allowed((uint64_t)mw * n, sw, row_k)); ++sw) {
+                const uint32_t kf = (label_k + sf - 1) / sf, kw = (row_k + sw - 1) / sw;
+                const uint64_t fi = (uint64_t)mf * n * sf, wi = (uint64_t)mw * n * sw;
+                // The first worker has the most pieces, and the most of the long ones.
+                const bool weight_first = kw > kf;
+                const uint64_t longs = ((weight_first ? wi : fi) + workers - 1) / workers;
+                const uint64_t all = (fi + wi + workers - 1) / workers;
+                const double steps = (double)longs * std::max(kf, kw) + (double)(all - longs) * std::min(kf, kw);
+                double us = steps * products * kStepUs * (pair ? kPairCost : 1.0);
+                if (sf > 1) us += (double)sf * rows * dim * 8.0 / 6.5e6;
+                if (sw > 1 || sums_anyway) us += (double)sw * labels * dim * 8.0 / 6.5e6;
+                if ((sf > 1 || sw > 1) && !sums_anyway) us += kLaunchUs;
+                if (us < best.us) best = OutPlan{pair != 0, mf, mw, n, sf, sw, weight_first, us};
+            }
     }
-    if (cost_out) *cost_out = best_cost;
     return best;
 }
 
@@ -522,7 +549,6 @@ uint64_t chunk_limit(const sp_label_head* h) {
 uint64_t chunk_for(const sp_label_head* h, uint64_t rows) {
     const uint64_t limit = std::min(chunk_limit(h), round_up(rows, kPairTile));
     if (rows <= limit) return limit;
-    const uint32_t label_k = (uint32_t)((h->labels + kBlockK - 1) / kBlockK);
     const uint64_t wave = std::max<uint64_t>(h->sms / 2 / tiles_of(h->dim, true), 1) * kPairTile;
     const uint64_t fewest = (rows + limit - 1) / limit;
     uint64_t best = 0;
@@ -531,13 +557,9 @@ uint64_t chunk_for(const sp_label_head* h, uint64_t rows) {
         if (chunk == 0 || chunk > limit) return;
         double cost = 0.0;
         const uint64_t whole = rows / chunk, rest = rows % chunk;
-        for (uint64_t part : {chunk, rest}) {
-            if (part == 0) continue;
-            double f = 0.0, w = 0.0;
-            plan_out(h->sms, part, h->dim, label_k, &f);
-            plan_out(h->sms, h->labels, h->dim, (uint32_t)((part + kBlockK - 1) / kBlockK), &w);
-            cost += (f + w) * (part == chunk ? (double)whole : 1.0);
-        }
+        for (uint64_t part : {chunk, rest})
+            if (part != 0)
+                cost += plan_out(h->sms, part, h->labels, h->dim, h->parts(), true).us * (part == chunk ? (double)whole : 1.0);
         if (cost < best_cost) best_cost = cost, best = chunk;
     };
     for (uint64_t chunks = fewest; chunks < fewest + 3; ++chunks) consider(round_up((rows + chunks - 1) / chunks, kPairTile));
@@ -560,11 +582,16 @@ sp_status allocate(sp_label_head* h, T** out, uint64_t count) {
     return SP_OK;
 }
 
-template <int ENDING, bool A_TRANSPOSED, bool B_TRANSPOSED, bool PAIR, typename T>
-cudaError_t launch_gemm(const sp_label_head* h, uint64_t items, const CUtensorMap& a, const CUtensorMap& a_packed,
-                        const CUtensorMap& b, const CUtensorMap& b_packed, const CUtensorMap& slopes,
+// One call's inputs: the compacted rows and the operand maps.
+struct Operands {
+    CUtensorMap features, features_packed, weight;
+    uint32_t all_rows;  // as in GemmArgs
+};
+
+template <int ENDING, bool PAIR, typename T>
+cudaError_t launch_gemm(const sp_label_head* h, uint64_t items, const Operands& op, const CUtensorMap& slopes,
                         const GemmArgs& args) {
-    auto kernel = k_label_gemm<ENDING, A_TRANSPOSED, B_TRANSPOSED, PAIR, T>;
+    auto kernel = k_label_gemm<ENDING, PAIR, T>;
     static std::atomic<unsigned long long> configured{0};
     const cudaError_t err = allow_smem_once(kernel, kGemmSmem, configured);
     if (err != cudaSuccess) return err;
@@ -583,22 +610,15 @@ cudaError_t launch_gemm(const sp_label_head* h, uint64_t items, const CUtensorMa
     attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
     config.numAttrs = 2;
-    return cudaLaunchKernelEx(&config, kernel, a, a_packed, b, b_packed, slopes, args);
+    return cudaLaunchKernelEx(&config, kernel, op.features, op.features_packed, op.weight, slopes, args);
 }
 
-template <int ENDING, bool A_TRANSPOSED, bool B_TRANSPOSED, typename T>
-cudaError_t run_gemm(const sp_label_head* h, const Plan& plan, uint64_t items, const CUtensorMap& a,
-                     const CUtensorMap& a_packed, const CUtensorMap& b, const CUtensorMap& b_packed,
-                     const CUtensorMap& slopes, const GemmArgs& args) {
-    return plan.pair ? launch_gemm<ENDING, A_TRANSPOSED, B_TRANSPOSED, true, T>(h, items, a, a_packed, b, b_packed, slopes, args)
-                     : launch_gemm<ENDING, A_TRANSPOSED, B_TRANSPOSED, false, T>(h, items, a, a_packed, b, b_packed, slopes, args);
+template <int ENDING, typename T>
+cudaError_t run_gemm(const sp_label_head* h, bool pair, uint64_t items, const Operands& op, const CUtensorMap& slopes,
+                     const GemmArgs& args) {
+    return pair ? launch_gemm<ENDING, true, T>(h, items, op, slopes, args)
+                : launch_gemm<ENDING, false, T>(h, items, op, slopes, args);
 }
-
-// One call's inputs: the compacted rows and the operand maps.
-struct Operands {
-    CUtensorMap features, features_packed, weight;
-    uint32_t all_rows;  // as in GemmArgs
-};
 
 template <typename T, bool DIRECT>
 cudaError_t launch_thin(const sp_label_head* h, uint32_t blocks, const Operands& op, const ThinArgs& args) {
@@ -669,6 +689,7 @@ GemmArgs common_args(const sp_label_head* h, const void* targets, int wide, floa
     a.rows = h->rows;
     a.row_of = h->row_of;
     a.labels = (uint32_t)h->labels;
+    a.dim = h->dim;
     a.products = h->products();
     a.chunk_rows = 0x80000000u;
     a.splits = 1;
@@ -717,13 +738,18 @@ sp_status run_stats(sp_label_head* h, const Operands& op, const void* weight, in
         thin.dim = h->dim;
         thin.vector = vector_rows(h, weight, weight_stride);
         thin.columns = (uint32_t)round_up(n, 16);
-        thin.tiles = tiles_of(h->labels, false);
+        // Whole rounds of tiles over the SMs; converted weights come in tiles of the height that fills
+        // the last round too.
+        const bool direct = in_place(h, weight, weight_stride);
+        const uint64_t rounds = (tiles_of(h->labels, false) + h->sms - 1) / h->sms;
+        thin.tile = direct ? kTile : (uint32_t)round_up((h->labels + rounds * h->sms - 1) / (rounds * h->sms), 8);
+        thin.tiles = (uint32_t)((h->labels + thin.tile - 1) / thin.tile);
         const uint32_t blocks = std::min(thin.tiles, h->sms);
         a.partial_rows = kThinRows;
         slots = blocks;
         thin.g = a;
         const cudaError_t err = h->element == SP_F32                 ? launch_thin<float, false>(h, blocks, op, thin)
-                                : in_place(h, weight, weight_stride) ? launch_thin<bf16, true>(h, blocks, op, thin)
+                                : direct                             ? launch_thin<bf16, true>(h, blocks, op, thin)
                                                                      : launch_thin<bf16, false>(h, blocks, op, thin);
         SP_CUDA(ctx, err);
     } else {
@@ -732,8 +758,7 @@ sp_status run_stats(sp_label_head* h, const Operands& op, const void* weight, in
         a.splits = plan.splits;
         a.partial_rows = (uint64_t)plan.m_tiles * (plan.pair ? kPairTile : kTile);
         slots = 2 * a.splits;
-        SP_CUDA(ctx, (run_gemm<kStats, false, false, bf16>(h, plan, plan.items(), op.features, op.features_packed,
-                                                           op.weight, op.weight, op.weight, a)));
+        SP_CUDA(ctx, (run_gemm<kStats, bf16>(h, plan.pair, plan.items(), op, op.weight, a)));
     }
     auto join = [&](auto kernel, uint32_t lanes) {
         return launch_chained(kernel, grid_for(n * lanes, kThreads), kThreads, 0, ctx->stream, h->rows,
@@ -743,7 +768,10 @@ sp_status run_stats(sp_label_head* h, const Operands& op, const void* weight, in
                               static_cast<const float*>(h->target_logits), losses, normalizers, labels_out,
                               log_probability, h->loss_sums, mean);
     };
-    SP_CUDA(ctx, slots <= kThreadSlots ? join(k_join_rows<1>, 1) : join(k_join_rows<32>, 32));
+        // About kThreadSlots partials a thread, as far as a warp goes.
+    SP_CUDA(ctx, slots <= kThreadSlots       ? join(k_join_rows<1>, 1)
+                 : slots <= 8 * kThreadSlots ? join(k_join_rows<8>, 8)
+                                             : join(k_join_rows<32>, 32));
     return SP_OK;
 }
 
@@ -885,18 +913,18 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
     CUtensorMap slopes, slopes_out;
     SP_CHECK(make_map(ctx, &slopes, h->slopes, slope_stride, chunk, slope_stride, h->parts(), chunk * slope_stride));
     SP_CHECK(make_map(ctx, &slopes_out, h->slopes, slope_stride, chunk, slope_stride, h->parts(), chunk * slope_stride, 32));
-    const uint32_t label_k = (uint32_t)((h->labels + kBlockK - 1) / kBlockK);
     // One cut of the weight's gradient for every chunk: its pieces' sums go on from one to the next.
-    const Plan to_weight = plan_out(h->sms, h->labels, h->dim, (uint32_t)((std::min(chunk, rows) + kBlockK - 1) / kBlockK));
-    const bool weight_sums = to_weight.splits > 1 || chunks > 1;
+    const OutPlan first = plan_out(h->sms, std::min(chunk, rows), h->labels, h->dim, h->parts(), chunks > 1);
+    const bool weight_sums = first.weight > 1 || chunks > 1;
     float* weight_sum = h->sums;
     float* feature_sum = h->sums + sums_rows(h) * sum_stride;
 
     for (uint64_t c = 0; c < chunks; ++c) {
         const uint64_t here = std::min(chunk, rows - c * chunk);
         const Plan logits = plan_logits(h->sms, here, h->labels);
-        const Plan to_features = plan_out(h->sms, here, h->dim, label_k);
-        const bool feature_sums = to_features.splits > 1;
+        const OutPlan plan = c == 0 ? first
+                                    : plan_out(h->sms, here, h->labels, h->dim, h->parts(), true, first.weight);
+        const bool feature_sums = plan.features > 1;
         GemmArgs a = common_args(h, d_targets, wide, logit_scale);
         a.first_row = (uint32_t)(c * chunk);
         a.chunk_rows = (uint32_t)chunk;
@@ -905,54 +933,40 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
         a.splits = logits.splits;
         a.log_normalizers = d_log_normalizers;
         a.row_gradient = d_row_gradient;
-        SP_CUDA(ctx, (run_gemm<kSlopes, false, false, bf16>(h, logits, logits.items(), op.features, op.features_packed,
-                                                            op.weight, op.weight, slopes_out, a)));
+        SP_CUDA(ctx, (run_gemm<kSlopes, bf16>(h, logits.pair, logits.items(), op, slopes_out, a)));
 
-        GemmArgs f = a;  // dH = G W
-        f.k_blocks = label_k;
-        f.n_tiles = to_features.n_tiles;
-        f.splits = to_features.splits;
+        OutArgs& f = a.out[0];
+        f.n_tiles = plan.n;
+        f.splits = plan.features;
+        f.k_blocks = (uint32_t)((h->labels + kBlockK - 1) / kBlockK);
         f.partial = feature_sums;
         f.out = feature_sums ? (void*)feature_sum : d_feature_gradient;
-        f.out_stride = feature_sums ? (int64_t)sum_stride : feature_gradient_stride;
-        f.out_rows = here;
-        f.out_columns = h->dim;
-        f.scatter = !feature_sums;
-        f.out_packed = vector_rows(h, d_feature_gradient, feature_gradient_stride);
-        auto run_features = [&](auto* typed) {
-            return run_gemm<kOut, false, true, std::remove_pointer_t<decltype(typed)>>(
-                h, to_features, to_features.items() * f.n_tiles, slopes, slopes, op.weight, op.weight, slopes_out, f);
-        };
-        SP_CUDA(ctx, h->element == SP_F32 ? run_features((float*)nullptr) : run_features((bf16*)nullptr));
-
-        GemmArgs w = a;  // dW = G^T H
-        w.rows_inner = 1;
-        w.m_tiles = to_weight.m_tiles;
-        w.n_tiles = to_weight.n_tiles;
-        w.splits = to_weight.splits;
+        f.stride = feature_sums ? (int64_t)sum_stride : feature_gradient_stride;
+        f.rows = here;
+        f.packed = vector_rows(h, d_feature_gradient, feature_gradient_stride);
+        OutArgs& w = a.out[1];
+        w.m_tiles = plan.m_weight;
+        w.n_tiles = plan.n;
+        w.splits = plan.weight;
         w.partial = weight_sums;
         w.add = c > 0;
         w.out = weight_sums ? (void*)weight_sum : d_weight_gradient;
-        w.out_stride = weight_sums ? (int64_t)sum_stride : weight_gradient_stride;
-        w.out_rows = h->labels;
-        w.out_columns = h->dim;
-        w.out_packed = vector_rows(h, d_weight_gradient, weight_gradient_stride);
-        auto run_weight = [&](auto* typed) {
-            return run_gemm<kOut, true, true, std::remove_pointer_t<decltype(typed)>>(
-                h, to_weight, to_weight.items() * w.n_tiles, slopes, slopes, op.features, op.features_packed, slopes_out, w);
-        };
-        SP_CUDA(ctx, h->element == SP_F32 ? run_weight((float*)nullptr) : run_weight((bf16*)nullptr));
+        w.stride = weight_sums ? (int64_t)sum_stride : weight_gradient_stride;
+        w.rows = h->labels;
+        w.packed = vector_rows(h, d_weight_gradient, weight_gradient_stride);
+        a.weight_first = plan.weight_first;
+        SP_CUDA(ctx, h->element == SP_F32 ? (run_gemm<kOut, float>(h, plan.pair, plan.items(), op, slopes, a))
+                                          : (run_gemm<kOut, bf16>(h, plan.pair, plan.items(), op, slopes, a)));
 
         const bool last = c + 1 == chunks;
-        JoinArgs jf{feature_sums ? feature_sum : nullptr, to_features.splits, here, sum_stride, 1, a.first_row,
+        JoinArgs jf{feature_sums ? feature_sum : nullptr, plan.features, here, sum_stride, 1, a.first_row,
                     d_feature_gradient, feature_gradient_stride, last ? rows : 0};
-        JoinArgs jw{weight_sums && last ? weight_sum : nullptr, to_weight.splits, h->labels, sum_stride, 0, 0,
+        JoinArgs jw{weight_sums && last ? weight_sum : nullptr, plan.weight, h->labels, sum_stride, 0, 0,
                     d_weight_gradient, weight_gradient_stride, last ? h->labels : 0};
-        if (!last && !feature_sums) continue;
+        if (!jf.sums && !jw.sums) continue;  // written already, NaN included
         const uint64_t quads = std::max(feature_sums ? here * (sum_stride / 4) : (uint64_t)0,
                                         jw.sums ? h->labels * (sum_stride / 4) : (uint64_t)0);
-        const unsigned grid = (unsigned)std::min<uint64_t>(std::max<uint64_t>((quads + kThreads - 1) / kThreads, 1),
-                                                           148 * 16);
+        const unsigned grid = (unsigned)std::min<uint64_t>((quads + kThreads - 1) / kThreads, 148 * 16);
         SP_CUDA(ctx, h->element == SP_F32
                          ? launch_chained(k_join_gradients<float>, grid, kThreads, 0, ctx->stream,
                                           static_cast<const RowSet*>(h->rows), static_cast<const uint32_t*>(h->row_of),

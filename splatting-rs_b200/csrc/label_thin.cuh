@@ -35,8 +35,9 @@ struct ThinArgs {
     int64_t weight_stride;
     uint32_t dim;
     int vector;          // 16-byte loads are aligned
+    uint32_t tile;       // labels per tile: kTile, or for converted weights a multiple of 8
     uint32_t columns;    // of the accumulators: the rows, rounded up to 16
-    uint32_t tiles;      // of 128 labels
+    uint32_t tiles;
 };
 
 __device__ __forceinline__ void tmem_load16(uint32_t address, float (&v)[16]) {
@@ -125,7 +126,7 @@ __global__ void __launch_bounds__(thin_threads(DIRECT), 1)
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
                             tc::load_box<false>(to + h * kBoxBytes, &map_weight, bar, (int)k * kBlockK,
-                                                (int)tile * kTile + h * 64, 0);
+                                                (int)(tile * a.tile) + h * 64, 0);
 #pragma unroll
                     for (int p = 0; p < kParted; ++p)
                         tc::load_box<false>(to + kParted * kOperandBytes + p * kRowsBytes, rows, bar, (int)k * kBlockK, 0, p);
@@ -223,13 +224,15 @@ __global__ void __launch_bounds__(thin_threads(DIRECT), 1)
             if (row < a.columns) {
 #pragma unroll 1
                 for (uint32_t c = 0; c < span; c += 16) {
-                    const uint32_t at = part * span + c, first = tile * kTile + at;
+                    const uint32_t at = part * span + c, first = tile * a.tile + at;
+                    if (at >= a.tile) break;
                     float v[16];
 #pragma unroll
                     for (int j = 0; j < 16; ++j) v[j] = logits[row * kLogitStride + at + j];
-                    const bool near = target - first < 16;
-                    if (a.g.partial_labels) add_logits<true>(stats, v, first, a.g.labels, a.g.scale2, target, near);
-                    else add_logits<false>(stats, v, first, a.g.labels, a.g.scale2, target, near);
+                    const bool near = target - first < min(16u, a.tile - at);
+                    const uint32_t end = min(a.g.labels, (tile + 1) * a.tile);
+                    if (a.g.partial_labels) add_logits<true>(stats, v, first, end, a.g.scale2, target, near);
+                    else add_logits<false>(stats, v, first, end, a.g.scale2, target, near);
                     if (near) a.g.target_logits[row] = stats.target_logit;
                 }
             }
@@ -268,8 +271,8 @@ __global__ void __launch_bounds__(thin_threads(DIRECT), 1)
             const uint32_t columns = column < a.dim ? a.dim - column : 0;
 #pragma unroll
             for (int r = 0; r < kTurns; ++r) {
-                const uint32_t label = load_tile * kTile + r * kTurnRows + first_row;
-                const bool there = label < a.g.labels && load_tile < tiles;
+                const uint32_t in_tile = r * kTurnRows + first_row, label = load_tile * a.tile + in_tile;
+                const bool there = in_tile < a.tile && label < a.g.labels && load_tile < tiles;
                 to[r].load(weight + (there ? (int64_t)label * a.weight_stride + column : 0), there ? columns : 0, a.vector);
             }
             if (++load_k == a.g.k_blocks) load_k = 0, load_tile += gridDim.x;
@@ -277,6 +280,7 @@ __global__ void __launch_bounds__(thin_threads(DIRECT), 1)
         auto convert = [&](RawEight<T> (&from)[kTurns], uint32_t to) {
 #pragma unroll
             for (int r = 0; r < kTurns; ++r) {
+                if (r * kTurnRows + first_row >= a.tile) break;  // those accumulator lanes are not read
                 float v[8];
                 constexpr int N = RawEight<T>::N;
 #pragma unroll

@@ -76,7 +76,7 @@ __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
 // A wait gives up after this many polls or nanoseconds, whichever comes first: far above any
 // wait of a working pipeline (microseconds).
 constexpr uint32_t kPollLimit = 1u << 26;
-constexpr unsigned long long kWaitLimitNs = 2000000000ull;
+constexpr unsigned long long kWaitLimitNs = 1000000000ull;
 
 __device__ __forceinline__ unsigned long long global_ns() {
     unsigned long long t;
@@ -89,7 +89,7 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity) {
     unsigned long long start = 0;
     for (uint32_t polls = 0; polls < kPollLimit; ++polls) {
         if (barrier_try(bar, parity)) return true;
-        if ((polls & 4095u) == 4095u) {
+        if ((polls & 127u) == 127u) {
             const unsigned long long now = global_ns();
             if (start == 0) start = now;
             else if (now - start > kWaitLimitNs) return false;
