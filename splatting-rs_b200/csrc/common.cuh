@@ -91,6 +91,7 @@ struct SortPlan {
     int tile_shift;    // key >> tile_shift = tile index (uncompressed keys)
     int compressed;    // REF20 order in 32-bit keys whose width follows the frame's depth range
     int tile_bits;     // ceil(log2 tiles)
+    int short_partitions;  // partitions of kSortShortPartition 32-bit keys
 };
 
 // bits(0.01f) >> 12 and the largest depth key (NaN included) a visible Gaussian can have:
@@ -102,6 +103,10 @@ constexpr int kSortThreads = 256;
 constexpr int kSortItems = 24;  // measured best of 8-40 keys per thread and 1-4 blocks per SM
 constexpr int kSortBlocksPerSM = 2;
 constexpr int kSortPartition = kSortThreads * kSortItems;  // 6144 keys per partition
+// Lists of some 100,000 to a million keys (the embedding's tokens) leave most of the SMs idle at that
+// size; shorter partitions spread them.
+constexpr int kSortShortItems = 8;
+constexpr int kSortShortPartition = kSortThreads * kSortShortItems;
 constexpr int kSortMaxPasses = 8;
 constexpr int kSortRadix = 256;
 

@@ -44,18 +44,21 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kEmitItems = 8;
 constexpr int kLookupRows = 4;   // rows in flight per thread
-constexpr int kPieceRows = 8;    // rows in flight per thread while summing
+constexpr int kPieceRows = 4;    // rows in flight per thread while summing: 8 and 16 cost more in occupancy
 constexpr int kFewRows = 4;      // ... in blocks of 1024 threads, 64 registers each
 constexpr int kMinLanesLog2 = 2; // at least 4 threads a row while summing
-constexpr uint32_t kShortPiece = 16, kLongPiece = 64, kMostStretch = 2048;
+constexpr uint32_t kShortPiece = 16, kLongPiece = 128, kMostStretch = 2048;
+constexpr uint32_t kGroups = 148 * 16;         // of pieces, where there are enough tokens
 constexpr uint32_t kFewTokens = 32768;         // 32 warps x 32 x 32 lanes
 constexpr uint64_t kFewReads = 1ull << 24;     // token reads of all blocks together
 constexpr uint32_t kFewThreads = 1024, kMostOwned = 512, kLongRun = 64;
 
-// Sorted positions per group of threads: long pieces make fewer partial sums, short ones give a
-// small list enough groups to fill the SMs (148 SMs x 8 groups of pieces either way).
+// Sorted positions per group of threads, a power of two: long pieces make fewer partial sums (500,000
+// bf16 rows of 256: 109 us in pieces of 64, 101 us of 128), short ones give a small list groups enough
+// to fill the SMs.
 uint32_t piece_length(uint64_t count, int lanes_log2) {
-    const uint32_t piece = count >= (uint64_t)kLongPiece * 148 * 8 ? kLongPiece : kShortPiece;
+    uint32_t piece = kShortPiece;
+    while (piece < kLongPiece && count >= (uint64_t)piece * 2 * kGroups) piece *= 2;
     return std::min(piece, kMostStretch / ((uint32_t)kThreads >> lanes_log2));
 }
 
@@ -119,7 +122,7 @@ __global__ void __launch_bounds__(kThreads) k_emit_tokens(const void* __restrict
     for (int p = 0; p < passes; ++p) hist[p][threadIdx.x] = 0;
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         meta->count = count;
-        meta->partitions = (count + kSortPartition - 1) / kSortPartition;
+        meta->partitions = (count + kSortShortPartition - 1) / kSortShortPartition;
         meta->key_shift = 0;
         meta->key_base = 0;
         meta->passes = (uint32_t)passes;
@@ -590,11 +593,10 @@ sp_status sp_embedding_create(sp_context* ctx, uint64_t entries, uint32_t dim, s
     while ((1ull << bits) <= entries) ++bits;  // keys 0..entries
     e->plan.key_bits = (int)bits;
     e->plan.passes = (int)(bits + 7) / 8;
-    // The most stretches any count up to max_tokens is cut into: the shortest is 8 short pieces (32
-    // threads a row), the shortest of a long list 8 long ones.
-    const uint64_t most_short = std::min<uint64_t>(max_tokens, (uint64_t)kLongPiece * 148 * 8);
-    const uint64_t stretches = std::max((most_short + 8 * kShortPiece - 1) / (8 * kShortPiece),
-                                        (max_tokens + 8 * kLongPiece - 1) / (8 * kLongPiece));
+    e->plan.short_partitions = 1;
+    // The most stretches any count up to max_tokens is cut into, at 8 pieces each (32 threads a row): a
+    // count's pieces number below 2 kGroups until they are kLongPiece long.
+    const uint64_t stretches = std::max<uint64_t>(2 * kGroups / 8 + 1, (max_tokens + 8 * kLongPiece - 1) / (8 * kLongPiece));
     sp_status s = SP_OK;
     auto all = [&]() -> sp_status {
         SP_CHECK(allocate(e, &e->meta, 1));
@@ -603,7 +605,7 @@ sp_status sp_embedding_create(sp_context* ctx, uint64_t entries, uint32_t dim, s
             SP_CHECK(allocate(e, &e->values[b], max_tokens));
         }
         SP_CHECK(allocate(e, &e->histograms, kSortMaxPasses * kSortRadix + kSortMaxPasses));
-        const uint64_t partitions = (max_tokens + kSortPartition - 1) / kSortPartition;
+        const uint64_t partitions = (max_tokens + kSortShortPartition - 1) / kSortShortPartition;
         SP_CHECK(allocate(e, &e->lookback, partitions * kSortRadix));
         SP_CHECK(allocate(e, &e->ranges, entries));
         SP_CHECK(allocate(e, &e->partials, stretches * 2 * partial_stride_of(dim)));
@@ -718,7 +720,7 @@ sp_status sp_embedding_gradient(sp_embedding* e, const void* d_out_gradient, int
     SP_CUDA(ctx, launch_chained(k_emit_tokens, std::max(1u, grid_for(count, kThreads * kEmitItems)), kThreads, 0, st,
                                 d_tokens, wide, n, e->entries, e->plan.passes, e->meta, e->keys[0], e->values[0],
                                 e->histograms));
-    const uint32_t partitions = (n + kSortPartition - 1) / kSortPartition;
+    const uint32_t partitions = (n + kSortShortPartition - 1) / kSortShortPartition;
     for (int pass = 0; pass < e->plan.passes && n > 0; ++pass)
         SP_CUDA(ctx, launch_sort_pass(e->plan, pass, ++e->sequence, e->keys[0], e->values[0], e->keys[1], e->values[1],
                                       e->histograms, tickets, e->lookback, partitions, e->meta, st));

@@ -236,15 +236,16 @@ __global__ void __launch_bounds__(kBlock) k_emit(const float4* __restrict__ reco
 }
 
 // One pass of the onesweep sort. A persistent grid: each block takes partitions of
-// kSortPartition keys in ticket order, ranks its keys stably by digit, publishes its digit
+// kSortThreads * ITEMS keys in ticket order, ranks its keys stably by digit, publishes its digit
 // counts, sums its predecessors' (decoupled look-back) and scatters, digit-sorted through
 // shared memory so that the global writes of each digit are contiguous.
-template <typename Key>
+template <typename Key, int ITEMS>
 __global__ void __launch_bounds__(kSortThreads, kSortBlocksPerSM)
     k_sort_pass(int pass, uint32_t sequence, Key* keys0, uint32_t* values0, Key* keys1, uint32_t* values1,
                 const uint32_t* __restrict__ histogram, uint32_t* ticket, unsigned long long* lookback,
                 DeviceMeta* meta) {
     chain_enter();
+    constexpr int kPartition = kSortThreads * ITEMS;
     // Passes past the ones this frame's keys need do nothing; the others ping-pong from the
     // buffer the emission started in.
     if (pass >= (int)meta->passes) return;
@@ -256,7 +257,7 @@ __global__ void __launch_bounds__(kSortThreads, kSortBlocksPerSM)
     uint32_t* __restrict__ values_out = from1 ? values0 : values1;
     extern __shared__ float4 smem4[];
     Key* s_keys = reinterpret_cast<Key*>(smem4);
-    uint32_t* s_values = reinterpret_cast<uint32_t*>(s_keys + kSortPartition);
+    uint32_t* s_values = reinterpret_cast<uint32_t*>(s_keys + kPartition);
     __shared__ uint32_t s_warp[kSortThreads / 32][kSortRadix];
     __shared__ uint32_t s_global_base[kSortRadix];
     __shared__ uint32_t s_block_start[kSortRadix];
@@ -298,15 +299,15 @@ __global__ void __launch_bounds__(kSortThreads, kSortBlocksPerSM)
         __syncthreads();
         const uint32_t part = s_partition;
         if (part >= partitions) break;
-        const uint32_t base = part * kSortPartition;
+        const uint32_t base = part * kPartition;
 
-        // Load: warp w holds keys [base + 32 kSortItems w, base + 32 kSortItems (w + 1)), item k at lane + 32 k,
+        // Load: warp w holds keys [base + 32 ITEMS w, base + 32 ITEMS (w + 1)), item k at lane + 32 k,
         // so (warp, item, lane) order is the keys' original order.
-        Key key[kSortItems];
-        uint32_t value[kSortItems], digit[kSortItems], rank[kSortItems];
+        Key key[ITEMS];
+        uint32_t value[ITEMS], digit[ITEMS], rank[ITEMS];
 #pragma unroll
-        for (int k = 0; k < kSortItems; ++k) {
-            const uint32_t i = base + warp * (32 * kSortItems) + k * 32 + lane;
+        for (int k = 0; k < ITEMS; ++k) {
+            const uint32_t i = base + warp * (32 * ITEMS) + k * 32 + lane;
             const bool valid = i < count;
             key[k] = valid ? keys_in[i] : (Key)0;
             value[k] = valid ? values_in[i] : 0u;
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(kSortThreads, kSortBlocksPerSM)
         }
         // Stable rank within the warp, item by item.
 #pragma unroll
-        for (int k = 0; k < kSortItems; ++k) {
+        for (int k = 0; k < ITEMS; ++k) {
             const uint32_t peers = __match_any_sync(0xffffffffu, digit[k]);
             const bool valid = digit[k] < 256u;
             uint32_t before = 0;
@@ -395,14 +396,14 @@ __global__ void __launch_bounds__(kSortThreads, kSortBlocksPerSM)
         __syncthreads();
         // Digit-sorted order in shared memory.
 #pragma unroll
-        for (int k = 0; k < kSortItems; ++k)
+        for (int k = 0; k < ITEMS; ++k)
             if (digit[k] < 256u) {
                 const uint32_t pos = s_block_start[digit[k]] + s_warp[warp][digit[k]] + rank[k];
                 s_keys[pos] = key[k];
                 s_values[pos] = value[k];
             }
         __syncthreads();
-        const uint32_t valid_here = min((uint32_t)kSortPartition, count - base);
+        const uint32_t valid_here = min((uint32_t)kPartition, count - base);
         for (uint32_t i = t; i < valid_here; i += kSortThreads) {
             const Key k = s_keys[i];
             const uint32_t d = (uint32_t)(k >> shift) & 255u;
@@ -504,22 +505,31 @@ cudaError_t launch_sort_pass(const SortPlan& plan, int pass, uint32_t sequence, 
                              cudaStream_t stream) {
     const unsigned grid = (unsigned)std::min<int>(sort_grid(), (int)std::max<uint32_t>(max_partitions, 1u));
     const uint32_t* hist = sort_histograms + pass * kSortRadix;
-    if (plan.key64) {
+    if (plan.short_partitions) {
+        using K = uint32_t;
+        const size_t smem = kSortShortPartition * (sizeof(K) + sizeof(uint32_t));
+        static std::atomic<unsigned long long> configured{0};
+        const cudaError_t err = allow_smem_once(k_sort_pass<K, kSortShortItems>, smem, configured);
+        if (err != cudaSuccess) return err;
+        launch_chained(k_sort_pass<K, kSortShortItems>, grid, kSortThreads, smem, stream, pass, sequence,
+                       static_cast<K*>(keys0), values0, static_cast<K*>(keys1), values1, hist, sort_tickets + pass,
+                       lookback, meta);
+    } else if (plan.key64) {
         using K = unsigned long long;
         const size_t smem = kSortPartition * (sizeof(K) + sizeof(uint32_t));
         static std::atomic<unsigned long long> configured{0};
-        const cudaError_t err = allow_smem_once(k_sort_pass<K>, smem, configured);
+        const cudaError_t err = allow_smem_once(k_sort_pass<K, kSortItems>, smem, configured);
         if (err != cudaSuccess) return err;
-        launch_chained(k_sort_pass<K>, grid, kSortThreads, smem, stream, pass, sequence, static_cast<K*>(keys0), values0,
+        launch_chained(k_sort_pass<K, kSortItems>, grid, kSortThreads, smem, stream, pass, sequence, static_cast<K*>(keys0), values0,
                                                              static_cast<K*>(keys1), values1, hist,
                                                              sort_tickets + pass, lookback, meta);
     } else {
         using K = uint32_t;
         const size_t smem = kSortPartition * (sizeof(K) + sizeof(uint32_t));
         static std::atomic<unsigned long long> configured{0};
-        const cudaError_t err = allow_smem_once(k_sort_pass<K>, smem, configured);
+        const cudaError_t err = allow_smem_once(k_sort_pass<K, kSortItems>, smem, configured);
         if (err != cudaSuccess) return err;
-        launch_chained(k_sort_pass<K>, grid, kSortThreads, smem, stream, pass, sequence, static_cast<K*>(keys0), values0,
+        launch_chained(k_sort_pass<K, kSortItems>, grid, kSortThreads, smem, stream, pass, sequence, static_cast<K*>(keys0), values0,
                                                              static_cast<K*>(keys1), values1, hist,
                                                              sort_tickets + pass, lookback, meta);
     }
