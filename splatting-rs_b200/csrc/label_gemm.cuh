@@ -8,7 +8,7 @@
 //            dW = G^T H, in one launch: the tiles of one fill the SMs the other's leave
 //
 // A block is one producer warp (tiled bulk copies into a ring of shared-memory stages), one warp
-// that issues the products, and eight warps that empty one accumulator while the other fills. In a
+// that issues the products, and eight or sixteen warps that empty one accumulator while the other fills. In a
 // pair each block keeps 128 rows of A and of B and the accumulator of its A rows; the products are
 // issued by the first block and read B from both.
 #pragma once
@@ -23,15 +23,10 @@ namespace label {
 constexpr int kTile = 128;     // rows of A, and of B, per block
 constexpr int kPairTile = 2 * kTile;
 constexpr int kBlockK = 64;    // 128 bytes of bf16
-constexpr int kStages = 6;
 constexpr uint32_t kOperandBytes = kTile * kBlockK * 2;
 constexpr uint32_t kBoxBytes = kOperandBytes / 2;  // a box is 64 x 64 elements
-constexpr int kGemmThreads = 384;
-constexpr int kEpilogueWarps = 8;
 constexpr uint32_t kStageBytes = 2 * kOperandBytes;
 constexpr uint32_t kStoreBytes = 32 * 128;  // a warp's 32 x 64 slopes on their way out
-// 227 KB of shared memory hold six stages and the outgoing slopes.
-constexpr size_t kGemmSmem = 1024 + (size_t)kStages * kStageBytes + kEpilogueWarps * kStoreBytes + 256;
 
 // f32 operands: three bf16 parts each, the six products of parts whose weights sum to 2^-16 or
 // more of the whole, smallest first so that they are added while the sum is small. One hex digit
@@ -52,6 +47,21 @@ struct RowSet {
 constexpr uint32_t kNoTarget = 0xffffffffu;  // index_at's -1
 
 enum Ending { kStats = 0, kSlopes = 1, kOut = 2 };
+
+// Warps that empty the accumulators: 8, or 16 for a pair's logits of bf16 operands, where the
+// exponentials take as long as the products up to some 256 columns and need more warps to overlap
+// (f32 operands' products are six times as many). 227 KB of shared memory hold the outgoing slopes and
+// as many stages as fit.
+template <int ENDING, bool PAIR, typename T>
+struct Shape {
+    static constexpr int epilogue_warps = ENDING != kOut && PAIR && sizeof(T) == 2 ? 16 : 8;
+    static constexpr int threads = 128 + 32 * epilogue_warps;
+    static constexpr int stages = ENDING == kSlopes && epilogue_warps == 16 ? 5 : 6;
+    static constexpr uint32_t store_bytes = ENDING == kSlopes ? epilogue_warps * kStoreBytes : 0;
+    static constexpr size_t smem = 1024 + (size_t)stages * kStageBytes + store_bytes + 256;
+    static constexpr int column_parts = epilogue_warps / 4;  // of a tile, one per four warps
+    static_assert(smem <= 227 * 1024, "shared memory of a block");
+};
 
 // One of the output gradients of a chunk of rows.
 struct OutArgs {
@@ -79,7 +89,7 @@ struct GemmArgs {
     const void* targets;
     int wide;
     // kStats
-    float2* partials;      // [2 * splits][partial_rows]: base (prediction: largest logit) and sum
+    float2* partials;      // [Shape::column_parts * splits][partial_rows]: base (prediction: largest logit) and sum
     uint32_t* partial_labels;  // the maximum's label, or NULL
     uint64_t partial_rows;
     float* target_logits;
@@ -327,17 +337,19 @@ __device__ __forceinline__ void add_out(float* to, const float (&v)[32], uint32_
 
 // map_slopes: 64 x 64 boxes to read (kOut), 64 x 32 to write (kSlopes).
 template <int ENDING, bool PAIR, typename T>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
     k_label_gemm(const __grid_constant__ CUtensorMap map_features,
                  const __grid_constant__ CUtensorMap map_features_packed,
                  const __grid_constant__ CUtensorMap map_weight, const __grid_constant__ CUtensorMap map_slopes,
                  const __grid_constant__ GemmArgs a) {
     constexpr int kBlocks = PAIR ? 2 : 1;
     constexpr int kSide = kTile * kBlocks;  // the pair's tile
+    using S = Shape<ENDING, PAIR, T>;
+    constexpr int kStages = S::stages, kSpan = kSide / S::column_parts;  // columns per warp
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem = (tc::smem_address(smem_raw) + 1023u) & ~1023u;
     const uint32_t store_at = smem + kStages * kStageBytes;
-    const uint32_t barriers = store_at + kEpilogueWarps * kStoreBytes;
+    const uint32_t barriers = store_at + S::store_bytes;
     const uint32_t full = barriers, empty = full + 8 * kStages, done = empty + 8 * kStages, drained = done + 16;
     const uint32_t tmem_slot = drained + 16;
     uint8_t* generic_base = smem_raw + (smem - tc::smem_address(smem_raw));
@@ -352,7 +364,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             tc::barrier_init(done + 8 * b, 1);
-            tc::barrier_init(drained + 8 * b, kEpilogueWarps * kBlocks);
+            tc::barrier_init(drained + 8 * b, S::epilogue_warps * kBlocks);
         }
         tc::barrier_init_fence();
         tc::prefetch_map(&map_features);
@@ -452,10 +464,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             }
         }
     } else if (warp >= 4) {
-        // Half the tile's columns per warpgroup; thread = row.
-        const uint32_t half = (warp - 4) / 4, quarter = warp % 4;
+        // An equal part of the tile's columns per four warps; thread = row.
+        const uint32_t part = (warp - 4) / 4, quarter = warp % 4;
         const uint32_t lane_row = rank * kTile + quarter * 32 + lane;
-        const uint32_t tmem_at = tmem + ((quarter * 32) << 16) + half * (kSide / 2);
+        const uint32_t tmem_at = tmem + ((quarter * 32) << 16) + part * kSpan;
         const uint32_t stage_tile = store_at + (warp - 4) * kStoreBytes;
         uint32_t buffer = 0, buffer_phase = 0;
         // Output gradients of a call that gave up, here or in a kernel before, are NaN.
@@ -492,56 +504,69 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                     if (lane == 0)
                         tc::barrier_arrive_cluster(PAIR ? tc::map_to_rank(drained + 8 * buffer, 0) : drained + 8 * buffer);
                 };
-                const uint32_t accumulator = tmem_at + buffer * kSide, columns_at = n * kSide + half * (kSide / 2);
+                const uint32_t accumulator = tmem_at + buffer * kSide, columns_at = n * kSide + part * kSpan;
                 if constexpr (ENDING == kSlopes) {
                     // 64 columns at a time: each part fills the warp's 32 x 64 tile, which a bulk copy
                     // writes out while the next is computed.
 #pragma unroll
-                    for (int c = 0; c < kSide / 2; c += 64) {
-                        float v[2][32];
-                        __syncwarp();
-                        tc::tmem_load32(accumulator + c, v[0]);
-                        tc::tmem_load32(accumulator + c + 32, v[1]);
-                        tc::tmem_load_wait();
-                        if (c + 64 == kSide / 2) drain();
-#pragma unroll
-                        for (int q = 0; q < 2; ++q)
-                            to_slopes(v[q], columns_at + c + 32 * q, a.labels, a.scale2, shift, weight, target, live);
-                        const int parts = a.products == 1 ? 1 : (int)kParts;
-                        for (int p = 0; p < parts; ++p) {
+                    for (int c = 0; c < kSpan; c += 64) {
+                        auto reclaim = [&]() {
                             if (lane == 0) tc::store_wait_read();
                             __syncwarp();
-                            stage_part(stage_tile, lane, 0, v[0]);
-                            stage_part(stage_tile, lane, 1, v[1]);
+                        };
+                        auto store = [&](int p) {
                             tc::fence_async_shared();
                             __syncwarp();
-                            if (lane == 0)
-                                tc::store_box(&map_slopes, stage_tile, (int)columns_at + c, (int)row, p);
+                            if (lane == 0) tc::store_box(&map_slopes, stage_tile, (int)columns_at + c, (int)row, p);
+                        };
+                        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                float v[32];
+                                __syncwarp();
+                                tc::tmem_load32(accumulator + c + 32 * q, v);
+                                tc::tmem_load_wait();
+                                if (q == 1 && c + 64 == kSpan) drain();
+                                to_slopes(v, columns_at + c + 32 * q, a.labels, a.scale2, shift, weight, target, live);
+                                if (q == 0) reclaim();
+                                stage_part(stage_tile, lane, q, v);
+                            }
+                            store(0);
+                        } else {
+                            float v[2][32];
+                            __syncwarp();
+                            tc::tmem_load32(accumulator + c, v[0]);
+                            tc::tmem_load32(accumulator + c + 32, v[1]);
+                            tc::tmem_load_wait();
+                            if (c + 64 == kSpan) drain();
+#pragma unroll
+                            for (int q = 0; q < 2; ++q)
+                                to_slopes(v[q], columns_at + c + 32 * q, a.labels, a.scale2, shift, weight, target, live);
+                            for (int p = 0; p < (int)kParts; ++p) {
+                                reclaim();
+                                stage_part(stage_tile, lane, 0, v[0]);
+                                stage_part(stage_tile, lane, 1, v[1]);
+                                store(p);
+                            }
                         }
                     }
                 } else if constexpr (ENDING == kStats) {
-                    // A chunk is reduced while the next one loads. Two chunks a turn: the whole tile
-                    // unrolled overflows the instruction cache.
-                    float v[2][32];
-                    __syncwarp();
-                    tc::tmem_load32(accumulator, v[0]);
+                    // One chunk's code for the whole tile: unrolled it overflows the instruction cache.
 #pragma unroll 1
-                    for (int c = 0; c < kSide / 2; c += 64) {
-#pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            tc::tmem_load_wait();
-                            __syncwarp();
-                            if (q == 0 || c + 64 < kSide / 2) tc::tmem_load32(accumulator + c + 32 * (q + 1), v[1 - q]);
-                            else drain();
-                            const uint32_t column = columns_at + c + 32 * q;
-                            const bool near = __any_sync(0xffffffffu, target - column < 32);
-                            if (a.partial_labels) add_logits<true>(stats, v[q], column, a.labels, a.scale2, target, near);
-                            else add_logits<false>(stats, v[q], column, a.labels, a.scale2, target, near);
-                        }
+                    for (int c = 0; c < kSpan; c += 32) {
+                        float v[32];
+                        __syncwarp();
+                        tc::tmem_load32(accumulator + c, v);
+                        tc::tmem_load_wait();
+                        if (c + 32 == kSpan) drain();
+                        const uint32_t column = columns_at + c;
+                        const bool near = __any_sync(0xffffffffu, target - column < 32);
+                        if (a.partial_labels) add_logits<true>(stats, v, column, a.labels, a.scale2, target, near);
+                        else add_logits<false>(stats, v, column, a.labels, a.scale2, target, near);
                     }
                 } else {
 #pragma unroll
-                    for (int c = 0; c < kSide / 2; c += 32) {
+                    for (int c = 0; c < kSpan; c += 32) {
                         float v[32];
                         if (empty_sum || !ok) {
 #pragma unroll
@@ -550,7 +575,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                             __syncwarp();
                             tc::tmem_load32(accumulator + c, v);
                             tc::tmem_load_wait();
-                            if (c + 32 == kSide / 2) drain();
+                            if (c + 32 == kSpan) drain();
                         }
                         if (poisoned || !ok) {
 #pragma unroll
@@ -574,12 +599,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 if (!empty_sum && ++buffer == 2) buffer = 0, buffer_phase ^= 1;
             }
             if (ENDING == kStats && ok && live) {
-                const uint64_t slot = (uint64_t)(w.split * 2 + half) * a.partial_rows + row;
+                const uint64_t slot = (uint64_t)(w.split * S::column_parts + part) * a.partial_rows + row;
                 a.partials[slot] = make_float2(a.partial_labels ? stats.largest : stats.base, stats.sum);
                 if (a.partial_labels) a.partial_labels[slot] = stats.label;
                 // The target is in exactly one thread's columns.
                 if (target != kNoTarget && target / kSide >= w.n0 && target / kSide < w.n1 &&
-                    target % kSide / (kSide / 2) == half)
+                    target % kSide / kSpan == part)
                     a.target_logits[row] = stats.target_logit;
             }
         }

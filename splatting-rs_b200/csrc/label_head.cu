@@ -593,14 +593,15 @@ cudaError_t launch_gemm(const sp_label_head* h, uint64_t items, const Operands& 
                         const GemmArgs& args) {
     auto kernel = k_label_gemm<ENDING, PAIR, T>;
     static std::atomic<unsigned long long> configured{0};
-    const cudaError_t err = allow_smem_once(kernel, kGemmSmem, configured);
+    using S = Shape<ENDING, PAIR, T>;
+    const cudaError_t err = allow_smem_once(kernel, S::smem, configured);
     if (err != cudaSuccess) return err;
     constexpr unsigned blocks = PAIR ? 2 : 1;
     const unsigned workers = (unsigned)std::max<uint64_t>(1, std::min<uint64_t>(items, h->sms / blocks));
     cudaLaunchConfig_t config{};
     config.gridDim = workers * blocks;
-    config.blockDim = kGemmThreads;
-    config.dynamicSmemBytes = kGemmSmem;
+    config.blockDim = S::threads;
+    config.dynamicSmemBytes = S::smem;
     config.stream = h->ctx->stream;
     cudaLaunchAttribute attributes[2];
     attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -757,8 +758,13 @@ sp_status run_stats(sp_label_head* h, const Operands& op, const void* weight, in
         a.n_tiles = plan.n_tiles;
         a.splits = plan.splits;
         a.partial_rows = (uint64_t)plan.m_tiles * (plan.pair ? kPairTile : kTile);
-        slots = 2 * a.splits;
-        SP_CUDA(ctx, (run_gemm<kStats, bf16>(h, plan.pair, plan.items(), op, op.weight, a)));
+        if (h->element == SP_F32) {
+            slots = (plan.pair ? Shape<kStats, true, float>::column_parts : Shape<kStats, false, float>::column_parts) * a.splits;
+            SP_CUDA(ctx, (run_gemm<kStats, float>(h, plan.pair, plan.items(), op, op.weight, a)));
+        } else {
+            slots = (plan.pair ? Shape<kStats, true, bf16>::column_parts : Shape<kStats, false, bf16>::column_parts) * a.splits;
+            SP_CUDA(ctx, (run_gemm<kStats, bf16>(h, plan.pair, plan.items(), op, op.weight, a)));
+        }
     }
     auto join = [&](auto kernel, uint32_t lanes) {
         return launch_chained(kernel, grid_for(n * lanes, kThreads), kThreads, 0, ctx->stream, h->rows,
@@ -810,7 +816,7 @@ sp_status sp_label_head_create(sp_context* ctx, uint64_t labels, uint32_t dim, s
         SP_CHECK(allocate(h, &h->packed_features, capacity * stride * h->parts()));
         SP_CHECK(allocate(h, &h->packed_weight, labels * stride * h->parts()));
         // plan_logits: pieces times row tiles stay within kLogitWaves waves, or one piece.
-        const uint64_t slots = 2 * kTile * std::max<uint64_t>(capacity / kTile, (uint64_t)kLogitWaves * h->sms);
+        const uint64_t slots = 4 * kTile * std::max<uint64_t>(capacity / kTile, (uint64_t)kLogitWaves * h->sms);
         SP_CHECK(allocate(h, &h->partials, slots));
         SP_CHECK(allocate(h, &h->partial_labels, slots));
         SP_CHECK(allocate(h, &h->target_logits, capacity));
@@ -933,7 +939,8 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
         a.splits = logits.splits;
         a.log_normalizers = d_log_normalizers;
         a.row_gradient = d_row_gradient;
-        SP_CUDA(ctx, (run_gemm<kSlopes, bf16>(h, logits.pair, logits.items(), op, slopes_out, a)));
+        SP_CUDA(ctx, h->element == SP_F32 ? (run_gemm<kSlopes, float>(h, logits.pair, logits.items(), op, slopes_out, a))
+                                          : (run_gemm<kSlopes, bf16>(h, logits.pair, logits.items(), op, slopes_out, a)));
 
         OutArgs& f = a.out[0];
         f.n_tiles = plan.n;
