@@ -277,21 +277,22 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // Per token: zeros where it has no rows, the ordered sum of its partials where its run crosses
-// stretches, nothing where k_sum_pieces wrote it. kJoinTokens tokens a warp, 4 columns a lane; a
-// token with more than kWarpParts partials is joined by the block's eight warps together.
+// stretches, nothing where k_sum_pieces wrote it. Up to kJoinTokens tokens a warp (one where there are
+// few, whose runs are long), 4 columns a lane; a token with more than kWarpParts partials is joined by
+// the block's eight warps together.
 constexpr uint32_t kJoinWarps = kThreads / 32, kJoinTokens = 8, kWarpParts = 16;
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     k_join_pieces(const uint2* __restrict__ ranges, uint32_t entries, uint32_t dim, float scale, T* __restrict__ out,
                   int64_t out_stride, const float* __restrict__ partials, uint32_t partial_stride, uint32_t stretch,
-                  const DeviceMeta* __restrict__ meta) {
+                  uint32_t tokens_per_warp, const DeviceMeta* __restrict__ meta) {
     chain_enter();
     __shared__ float4 shared[kJoinWarps][32];
     __shared__ uint32_t long_tokens[kJoinWarps * kJoinTokens], longs;
     if (threadIdx.x == 0) longs = 0;
     __syncthreads();
     const uint32_t warp = threadIdx.x / 32, lane = lane_id();
-    const uint32_t base = (blockIdx.x * kJoinWarps + warp) * kJoinTokens;
+    const uint32_t base = (blockIdx.x * kJoinWarps + warp) * tokens_per_warp;
     const bool failed = meta->status != 0;
     auto store = [&](uint32_t v, uint32_t column, float4 sum) {
         const float s[4] = {sum.x, sum.y, sum.z, sum.w};
@@ -317,7 +318,7 @@ __global__ void __launch_bounds__(kThreads)
     };
     auto parts_of = [&](uint2 run) { return run.y > run.x ? (run.y - 1) / stretch - run.x / stretch + 1 : 0u; };
     uint2 mine = make_uint2(0u, 0u);
-    const bool owns = lane < kJoinTokens && base + lane < entries;
+    const bool owns = lane < tokens_per_warp && base + lane < entries;
     if (owns && !failed) mine = ranges[base + lane];
     for (uint32_t left = __ballot_sync(0xffffffffu, owns && parts_of(mine) != 1); left; left &= left - 1) {
         const uint32_t k = __ffs(left) - 1, token = base + k;
@@ -363,7 +364,8 @@ __global__ void __launch_bounds__(kThreads)
 // tokens into registers and counts its entries' ones; the counts give every (entry, warp) its place in
 // a list of positions in shared memory, ordered by entry and then position; the rows are summed from
 // it, a run of at most kLongRun by one group of `lanes` threads in order, a longer one by all groups in
-// equal parts, joined in order.
+// equal parts, joined in order. Where the entries make too few blocks for the SMs, blockIdx.y takes
+// every gridDim.y-th tile of columns.
 template <typename T, int N>
 __global__ void __launch_bounds__(kFewThreads)
     k_sum_few(const void* __restrict__ tokens, int wide, uint32_t count, uint64_t entries, uint32_t owned,
@@ -372,7 +374,7 @@ __global__ void __launch_bounds__(kFewThreads)
     chain_enter();
     constexpr uint32_t kWarps = kFewThreads / 32, kItems = kFewTokens / kFewThreads;
     extern __shared__ float4 few_smem[];
-    __shared__ uint32_t start[kMostOwned + 1], warp_sums[kWarps];
+    __shared__ uint32_t start[kMostOwned + 1], warp_sums[kWarps], longs[kMostOwned], long_count;
     float* s_part = reinterpret_cast<float*>(few_smem);  // [kFewThreads][N]
     uint16_t* placed = reinterpret_cast<uint16_t*>(s_part + kFewThreads * N);  // [kWarps][owned]
     uint16_t* order = placed + kWarps * owned;                                 // [count]
@@ -391,6 +393,7 @@ __global__ void __launch_bounds__(kFewThreads)
         }
     }
     for (uint32_t i = t; i < kWarps * owned; i += kFewThreads) placed[i] = 0;
+    if (t == 0) long_count = 0;
     __syncthreads();
     const uint32_t below = (1u << lane) - 1u;
     // place(): the next free places of the warp's tokens, equal ones in lane order.
@@ -457,20 +460,24 @@ __global__ void __launch_bounds__(kFewThreads)
                 }
         }
     };
-    const uint32_t first_column = (t & (lanes - 1)) * N;
+    const uint32_t first_column = (t & (lanes - 1)) * N, tile = lanes * N;
     for (uint32_t e = group; e < entries_here; e += groups) {
         const uint32_t from = start[e], to = start[e + 1];
-        if (to - from > kLongRun) continue;
-        for (uint32_t column = first_column; column < dim; column += lanes * N) {
+        if (to - from > kLongRun) {
+            if ((t & (lanes - 1)) == 0) longs[atomicAdd(&long_count, 1u)] = e;
+            continue;
+        }
+        for (uint32_t column = blockIdx.y * tile + first_column; column < dim; column += gridDim.y * tile) {
             float acc[N];
             sum_rows(from, to, column, acc);
             store_row<T, N>(out + (first_entry + e) * out_stride + column, acc, scale, out_packed);
         }
     }
-    for (uint32_t e = 0; e < entries_here; ++e) {
-        const uint32_t from = start[e], n = start[e + 1] - from;
-        if (n <= kLongRun) continue;
-        for (uint32_t base = 0; base < dim; base += lanes * N) {
+    __syncthreads();
+    // In whatever order they were noted: each is summed by itself.
+    for (uint32_t k = 0; k < long_count; ++k) {
+        const uint32_t e = longs[k], from = start[e], n = start[e + 1] - from;
+        for (uint32_t base = blockIdx.y * tile; base < dim; base += gridDim.y * tile) {
             const uint32_t column = base + first_column;
             float acc[N];
             if (column < dim) {
@@ -545,10 +552,12 @@ cudaError_t sum_pieces(const sp_embedding* e, const uint32_t* keys, const uint32
                           lanes_log2, static_cast<const DeviceMeta*>(e->meta));
 }
 
-// Entries per block of k_sum_few, 0 where the sorted list is the better way.
+// Entries per block of k_sum_few, 0 where the sorted list is the better way: a block an SM, or two where
+// they have many rows to write (60,000 rows of 64 f32: 41 us in one, 17 us in two; 1000 rows 12 and 14).
 uint32_t few_owned(uint64_t entries, uint64_t count) {
     if (count > kFewTokens) return 0;
-    const uint64_t owned = std::min<uint64_t>((entries + 147) / 148, kMostOwned);
+    const uint64_t blocks = entries >= 148 * 128 ? 296 : 148;
+    const uint64_t owned = std::min<uint64_t>((entries + blocks - 1) / blocks, kMostOwned);
     return (entries + owned - 1) / owned * count <= kFewReads ? (uint32_t)owned : 0;
 }
 
@@ -561,7 +570,12 @@ cudaError_t sum_few(const sp_embedding* e, const void* tokens, int wide, uint32_
     const cudaError_t err = allow_smem_once(k_sum_few<T, N>, most, configured);
     if (err != cudaSuccess) return err;
     const int out_packed = pack_width(r.out, r.out_stride, e->dim, sizeof(T)) >= N;
-    return launch_chained(k_sum_few<T, N>, grid_for(e->entries, owned), kFewThreads, smem, e->ctx->stream, tokens, wide,
+    // Fewer threads a row where that makes column tiles for idle SMs.
+    const unsigned blocks = grid_for(e->entries, owned);
+    auto tiles = [&]() { return (e->dim + (N << lanes_log2) - 1) / (N << lanes_log2); };
+    while (lanes_log2 > kMinLanesLog2 && blocks * tiles() < 148) --lanes_log2;
+    const dim3 grid(blocks, std::max(1u, std::min(tiles(), 148 / blocks)));
+    return launch_chained(k_sum_few<T, N>, grid, kFewThreads, smem, e->ctx->stream, tokens, wide,
                           count, e->entries, owned, static_cast<const T*>(r.upstream), r.upstream_stride, e->dim,
                           r.scale, static_cast<T*>(r.out), r.out_stride, out_packed, lanes_log2);
 }
@@ -736,19 +750,20 @@ sp_status sp_embedding_gradient(sp_embedding* e, const void* d_out_gradient, int
     }
 #undef SPLAT_ROWS
     const uint32_t stretch = (kThreads >> lanes_log2) * piece;
-    const unsigned join_grid = grid_for(e->entries, kJoinWarps * kJoinTokens);
+    const uint32_t tokens_per_warp = e->entries >= 148 * kJoinWarps * kJoinTokens ? kJoinTokens : 1;
+    const unsigned join_grid = grid_for(e->entries, kJoinWarps * tokens_per_warp);
     if (e->element == SP_F32)
         SP_CUDA(ctx, launch_chained(k_join_pieces<float>, join_grid, kThreads, 0, st,
                                     static_cast<const uint2*>(e->ranges), (uint32_t)e->entries, e->dim, scale,
                                     static_cast<float*>(d_table_gradient), table_gradient_stride,
                                     static_cast<const float*>(e->partials), partial_stride, stretch,
-                                    static_cast<const DeviceMeta*>(e->meta)));
+                                    tokens_per_warp, static_cast<const DeviceMeta*>(e->meta)));
     else
         SP_CUDA(ctx, launch_chained(k_join_pieces<bf16>, join_grid, kThreads, 0, st,
                                     static_cast<const uint2*>(e->ranges), (uint32_t)e->entries, e->dim, scale,
                                     static_cast<bf16*>(d_table_gradient), table_gradient_stride,
                                     static_cast<const float*>(e->partials), partial_stride, stretch,
-                                    static_cast<const DeviceMeta*>(e->meta)));
+                                    tokens_per_warp, static_cast<const DeviceMeta*>(e->meta)));
     return SP_OK;
 } catch (...) {
     return SP_ERR_OUT_OF_MEMORY;

@@ -96,6 +96,11 @@ struct GemmArgs {
     // kSlopes
     const float* log_normalizers;
     const float* row_gradient;
+    // bf16 operands: what rounding left of each row's target slope, by far the row's largest. dH takes it
+    // in in f32 from the weight's rows, which undoes most of the slopes' rounding there.
+    float* residuals;
+    const bf16* weight;
+    int64_t weight_stride;
     // kOut
     OutArgs out[2];        // dH, dW
     int weight_first;      // dW's tiles, the longer ones, come first
@@ -255,9 +260,10 @@ __device__ __forceinline__ void add_logits(RowStats& s, float (&v)[W], uint32_t 
     }
 }
 
-// The slopes of 32 logits of a row, in place; zeros past the labels and in rows that do not count.
+// The slopes of 32 logits of a row, in place; zeros past the labels and in rows that do not count. The
+// target's, if it is among them, also in `target_slope`.
 __device__ __forceinline__ void to_slopes(float (&v)[32], uint32_t first, uint32_t labels, float scale2, float shift,
-                                          float weight, uint32_t target, bool live) {
+                                          float weight, uint32_t target, bool live, float& target_slope) {
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
         const float2 x = fma2(make_float2(v[j], v[j + 1]), make_float2(scale2, scale2), make_float2(shift, shift));
@@ -268,7 +274,10 @@ __device__ __forceinline__ void to_slopes(float (&v)[32], uint32_t first, uint32
     if (__any_sync(0xffffffffu, at < 32)) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-            if (at == (uint32_t)j) v[j] -= 1.0f;
+            if (at == (uint32_t)j) {
+                v[j] -= 1.0f;
+                target_slope = v[j] * weight;
+            }
     }
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = live ? v[j] * weight : 0.0f;
@@ -316,6 +325,22 @@ __device__ __forceinline__ void store_out(T* to, const float (&v)[32], uint32_t 
 #pragma unroll
         for (int j = 0; j < 32; ++j)
             if ((uint32_t)j < columns) to[j] = from_float<T>(v[j]);
+    }
+}
+
+// v += factor * (a row's 32 columns, of which `columns` exist), rows being 16-byte aligned.
+__device__ __forceinline__ void add_scaled(float (&v)[32], float factor, const bf16* row, uint32_t columns) {
+    if (columns >= 32) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const Pack<bf16, 8> p = load_pack<bf16, 8>(row + q * 8);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[q * 8 + j] = fmaf(factor, p.get(j), v[q * 8 + j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if ((uint32_t)j < columns) v[j] = fmaf(factor, to_float(row[j]), v[j]);
     }
 }
 
@@ -483,6 +508,11 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
             RowStats stats{-INFINITY, 0.0f, 0.0f, -INFINITY, 0u};
             uint32_t target = kNoTarget;
             float shift = 0.0f, weight = 0.0f;
+            float residual = 0.0f;
+            if (ENDING == kOut && sizeof(T) == 2 && live && w.which == 0) {
+                target = (uint32_t)index_at(a.targets, a.wide, a.row_of[compact], a.labels);
+                residual = a.residuals[row];
+            }
             if (ENDING != kOut && live) {
                 const uint32_t original = a.all_rows ? compact : a.row_of[compact];
                 if (a.targets) target = (uint32_t)index_at(a.targets, a.wide, original, a.labels);
@@ -527,13 +557,17 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                                 tc::tmem_load32(accumulator + c + 32 * q, v);
                                 tc::tmem_load_wait();
                                 if (q == 1 && c + 64 == kSpan) drain();
-                                to_slopes(v, columns_at + c + 32 * q, a.labels, a.scale2, shift, weight, target, live);
+                                const uint32_t column = columns_at + c + 32 * q;
+                                float slope = 0.0f;
+                                to_slopes(v, column, a.labels, a.scale2, shift, weight, target, live, slope);
+                                if (target - column < 32)
+                                    a.residuals[row] = slope - __bfloat162float(__float2bfloat16_rn(slope));
                                 if (q == 0) reclaim();
                                 stage_part(stage_tile, lane, q, v);
                             }
                             store(0);
                         } else {
-                            float v[2][32];
+                            float v[2][32], unused;
                             __syncwarp();
                             tc::tmem_load32(accumulator + c, v[0]);
                             tc::tmem_load32(accumulator + c + 32, v[1]);
@@ -541,7 +575,8 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                             if (c + 64 == kSpan) drain();
 #pragma unroll
                             for (int q = 0; q < 2; ++q)
-                                to_slopes(v[q], columns_at + c + 32 * q, a.labels, a.scale2, shift, weight, target, live);
+                                to_slopes(v[q], columns_at + c + 32 * q, a.labels, a.scale2, shift, weight, target, live,
+                                          unused);
                             for (int p = 0; p < (int)kParts; ++p) {
                                 reclaim();
                                 stage_part(stage_tile, lane, 0, v[0]);
@@ -584,6 +619,8 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                         const uint32_t column = columns_at + c;
                         if ((w.which ? row < o.rows : live) && column < a.dim) {
                             const uint32_t columns = a.dim - column;
+                            if (sizeof(T) == 2 && w.which == 0 && w.k0 == 0)
+                                add_scaled(v, residual, a.weight + (int64_t)target * a.weight_stride + column, columns);
                             if (o.partial) {
                                 float* to = static_cast<float*>(o.out) + ((uint64_t)w.split * o.rows + row) * (uint64_t)o.stride +
                                             column;

@@ -56,6 +56,7 @@ constexpr uint32_t kGatherRows = 64;        // rows a block compacts and copies
 constexpr uint32_t kCountGroups = 16;       // such blocks' counts are summed this many at a time
 constexpr uint32_t kRecountBlocks = 16;     // up to this many blocks each count all targets themselves
 constexpr uint32_t kLogitWaves = 16, kOutWaves = 4;
+constexpr uint32_t kLongestSum = 32;         // steps of 64 of K
 constexpr double kLaunchUs = 3.0;           // of a small kernel in the chain
 constexpr double kStepUs = 0.19;            // 64 of K of a 128 x 128 tile in a single block
 constexpr double kPairCost = 1.4;           // of a 256 x 256 tile, in 128 x 128 tiles of one block
@@ -516,12 +517,16 @@ OutPlan plan_out(uint32_t sms, uint64_t rows, uint64_t labels, uint32_t dim, uin
         if (pair_only >= 0 && pair != pair_only) continue;
         const uint32_t workers = pair ? std::max(sms / 2, 1u) : sms;
         const uint32_t mf = tiles_of(rows, pair), mw = tiles_of(labels, pair), n = tiles_of(dim, pair);
-        auto allowed = [&](uint64_t tiles, uint32_t s, uint32_t k) {
-            return s == 1 || (tiles * s <= (uint64_t)kOutWaves * workers && k >= 4 * s);
+        const double step_us = products * kStepUs * (pair ? kPairCost : 1.0);
+        // f32 operands' sums are cut at kLongestSum steps: the tensor cores' additions truncate.
+        const uint32_t least_f = parts > 1 ? (label_k + kLongestSum - 1) / kLongestSum : 1;
+        const uint32_t least_w = parts > 1 ? (row_k + kLongestSum - 1) / kLongestSum : 1;
+        auto allowed = [&](uint64_t tiles, uint32_t s, uint32_t least, uint32_t k) {
+            return s == least || (tiles * s <= (uint64_t)kOutWaves * workers && k >= 4 * s);
         };
-        for (uint32_t sf = 1; allowed((uint64_t)mf * n, sf, label_k); ++sf)
-            for (uint32_t sw = weight_splits ? weight_splits : 1;
-                 (weight_splits && sw == weight_splits) || (!weight_splits && allowed((uint64_t)mw * n, sw, row_k)); ++sw) {
+        for (uint32_t sf = least_f; allowed((uint64_t)mf * n, sf, least_f, label_k); ++sf)
+            for (uint32_t sw = weight_splits ? weight_splits : least_w;
+                 (weight_splits && sw == weight_splits) || (!weight_splits && allowed((uint64_t)mw * n, sw, least_w, row_k)); ++sw) {
                 const uint32_t kf = (label_k + sf - 1) / sf, kw = (row_k + sw - 1) / sw;
                 const uint64_t fi = (uint64_t)mf * n * sf, wi = (uint64_t)mw * n * sw;
                 // The first worker has the most pieces, and the most of the long ones.
@@ -529,7 +534,7 @@ OutPlan plan_out(uint32_t sms, uint64_t rows, uint64_t labels, uint32_t dim, uin
                 const uint64_t longs = ((weight_first ? wi : fi) + workers - 1) / workers;
                 const uint64_t all = (fi + wi + workers - 1) / workers;
                 const double steps = (double)longs * std::max(kf, kw) + (double)(all - longs) * std::min(kf, kw);
-                double us = steps * products * kStepUs * (pair ? kPairCost : 1.0);
+                double us = steps * step_us;
                 if (sf > 1) us += (double)sf * rows * dim * 8.0 / 6.5e6;
                 if (sw > 1 || sums_anyway) us += (double)sw * labels * dim * 8.0 / 6.5e6;
                 if ((sf > 1 || sw > 1) && !sums_anyway) us += kLaunchUs;
@@ -568,8 +573,14 @@ uint64_t chunk_for(const sp_label_head* h, uint64_t rows) {
 }
 
 // Rows of f32 sums a gradient may need. plan_out: pieces times tiles stay within kOutWaves waves, or
-// one piece; one piece needs sums for the weight's gradient alone, over several chunks.
-uint64_t sums_rows(const sp_label_head* h) { return std::max<uint64_t>((uint64_t)kOutWaves * h->sms * kTile, h->labels); }
+// there is one piece, which needs sums for the weight's gradient alone, over several chunks; or f32's
+// least pieces, of which a gradient of r rows over an inner n has at most n / (64 kLongestSum) + 1: r n
+// is at most the slope budget, and r at most the labels or, with more labels than one piece takes, the
+// budget over those.
+uint64_t sums_rows(const sp_label_head* h) {
+    const uint64_t f32 = h->parts() > 1 ? 2 * (kSlopeBudget / kParts / (kLongestSum * kBlockK)) : 0;
+    return std::max<uint64_t>((uint64_t)kOutWaves * h->sms * kTile, h->labels + f32);
+}
 
 uint64_t sums_stride(const sp_label_head* h) { return ((uint64_t)h->dim + 3) / 4 * 4; }
 
@@ -931,6 +942,9 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
         const OutPlan plan = c == 0 ? first
                                     : plan_out(h->sms, here, h->labels, h->dim, h->parts(), true, first.weight);
         const bool feature_sums = plan.features > 1;
+        SP_REQUIRE(ctx, (!feature_sums || plan.features * here <= sums_rows(h)) &&
+                            (!weight_sums || plan.weight * h->labels <= sums_rows(h)),
+                   SP_ERR_OVERFLOW, "the gradients' sums exceed their workspace");
         GemmArgs a = common_args(h, d_targets, wide, logit_scale);
         a.first_row = (uint32_t)(c * chunk);
         a.chunk_rows = (uint32_t)chunk;
@@ -939,6 +953,10 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
         a.splits = logits.splits;
         a.log_normalizers = d_log_normalizers;
         a.row_gradient = d_row_gradient;
+        a.residuals = h->target_logits;  // free in a gradient
+        const bool weight_here = in_place(h, d_weight, weight_stride);
+        a.weight = weight_here ? static_cast<const bf16*>(d_weight) : h->packed_weight;
+        a.weight_stride = weight_here ? weight_stride : (int64_t)h->packed_stride();
         SP_CUDA(ctx, h->element == SP_F32 ? (run_gemm<kSlopes, float>(h, logits.pair, logits.items(), op, slopes_out, a))
                                           : (run_gemm<kSlopes, bf16>(h, logits.pair, logits.items(), op, slopes_out, a)));
 
