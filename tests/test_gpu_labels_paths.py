@@ -1,0 +1,189 @@
+"""The label operators where they change the way they go, and the example that runs them together:
+sizes on both sides of each rule, operands that cannot be read in place, offsets past 32 bits, a
+context with a stream of its own. Against plain 64-bit results, with the bounds of test_gpu_labels."""
+
+from __future__ import annotations
+
+import sys
+from pathlib import Path
+
+import pytest
+import torch
+
+import splat_b200 as sb
+from test_gpu_labels import A, TYPES, U, Bounds, close, matrix, tokens_for
+
+pytestmark = pytest.mark.gpu
+
+
+def gradient_bound(upstream, tokens, entries, scale):
+    """(table gradient, error bound) as in test_embedding_gradient."""
+    held = (tokens >= 0) & (tokens < entries)
+    at, rows = tokens[held].long(), upstream[held].double()
+    dim = upstream.shape[1]
+    want = torch.zeros(entries, dim, dtype=torch.float64, device="cuda").index_add_(0, at, rows)
+    size = torch.zeros(entries, dim, dtype=torch.float64, device="cuda").index_add_(0, at, rows.abs())
+    count = torch.bincount(at, minlength=entries)[:, None]
+    return want * scale, scale * (size * (count + 1) * A + want.abs() * U[upstream.dtype]) * (1 + 1e-3)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize(
+    "n,entries,dim,kind",
+    [(32_768, 40, 24, "some"), (32_769, 40, 24, "some"),  # one kernel, and the sorted list
+     (32_768, 3, 200, "all"), (40_000, 30, 200, "all"),   # few entries: column tiles, a warp per join
+     (64, 1, 64, "all"), (65, 1, 64, "all"),              # a run of one group, and of all of them
+     (500, 20_000, 40, "some"), (2000, 90_000, 16, "all"),  # many entries a block, mostly without rows
+     (75_775, 7, 33, "skewed"), (75_776, 7, 33, "skewed"),  # pieces of 16 and of 32
+     (151_552, 500, 12, "skewed"), (303_104, 2, 16, "skewed"), (310_000, 70_000, 8, "some")],
+)
+def test_embedding_gradient_paths(ctx, n, entries, dim, kind, dtype):
+    e = sb.Embedding(ctx, entries, dim, dtype, n)
+    upstream, tokens = matrix(n, dim, dtype, 3), tokens_for(kind, n, entries, torch.int32, 4)
+    want, bound = gradient_bound(upstream, tokens, entries, 1.0)
+    got = e.gradient(upstream, tokens)
+    close(got, want, bound)
+    assert torch.equal(got, e.gradient(upstream, tokens))
+    e.check()
+
+
+def test_one_handle_for_calls_of_all_sizes(ctx):
+    """Workspaces are shared by the calls of a handle, whatever way each goes."""
+    entries, dim = 300, 64
+    e = sb.Embedding(ctx, entries, dim, torch.float32, 200_000)
+    for n in (200_000, 10, 33_000, 0, 160_000, 32_768, 1):
+        upstream, tokens = matrix(n, dim, torch.float32, n), tokens_for("skewed", n, entries, torch.int64, n + 1)
+        want, bound = gradient_bound(upstream, tokens, entries, 1.0)
+        close(e.gradient(upstream, tokens), want, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [16, 17, 64, 65, 128, 129])
+@pytest.mark.parametrize("pad,shift,dim", [(0, 0, 72), (1, 0, 72), (0, 1, 64), (3, 5, 200)])
+def test_predict_and_loss_around_the_few_row_pass(ctx, rows, pad, shift, dim, dtype):
+    labels = 1500
+    head = sb.LabelHead(ctx, labels, dim, dtype, 200, training=False)
+    features = matrix(rows, dim, dtype, 1, pad, shift, spread=dim**-0.25)
+    weight = matrix(labels, dim, dtype, 2, shift=0 if shift == 1 else shift, pad=pad, spread=dim**-0.25)
+    b = Bounds(features, weight, None, 1.3)
+    got, log_probabilities = head.predict(features, weight, 1.3)
+    best = b.z.amax(1)
+    close(log_probabilities, best - b.normalizers, 2 * b.z_error + b.exp_error + 4 * A * b.normalizers.abs())
+    assert (best - b.z.gather(1, got.long()[:, None])[:, 0] <= 2 * b.z_error).all()
+    targets = tokens_for("some", rows, labels, torch.int32, 3)
+    b = Bounds(features, weight, targets, 1.3)
+    loss = head.loss(features, weight, targets, 1.3)
+    close(loss.losses, b.losses, b.loss_error)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,labels,dim", [(1030, 20_000, 40), (3000, 259, 33), (20_500, 130, 16), (66, 40_000, 16)])
+def test_loss_and_gradient_in_pieces(ctx, rows, labels, dim, dtype):
+    """Label tiles cut into pieces, row targets counted by groups, gradients summed from pieces."""
+    head = sb.LabelHead(ctx, labels, dim, dtype, rows)
+    features, weight = matrix(rows, dim, dtype, 1, spread=0.5), matrix(labels, dim, dtype, 2, spread=0.5)
+    targets = tokens_for("some", rows, labels, torch.int64, 3)
+    b = Bounds(features, weight, targets, 1.0)
+    loss = head.loss(features, weight, targets)
+    close(loss.losses, b.losses, b.loss_error)
+    assert abs(loss.mean.double() - b.losses.sum() / len(b.rows)) <= b.loss_error.sum() / len(b.rows) + A * abs(loss.mean)
+    to_features, to_weight = head.gradient(features, weight, targets, loss.log_normalizers)
+    close(to_features, b.to_features, b.features_error)
+    close(to_weight, b.to_weight, b.weight_error)
+
+
+def test_logits_that_grow_along_the_vocabulary(ctx):
+    """Each label tile raises the largest logit by more than the sums' range: the base moves on."""
+    rows, labels, dim = 130, 2000, 16
+    for dtype in TYPES:
+        head = sb.LabelHead(ctx, labels, dim, dtype, rows)
+        features = torch.ones(rows, dim, dtype=dtype, device="cuda")
+        weight = torch.arange(labels, device="cuda")[:, None].expand(labels, dim).to(dtype).contiguous()
+        targets = tokens_for("all", rows, labels, torch.int32, 3)
+        for few in (False, True):
+            some = slice(0, 40) if few else slice(0, rows)
+            b = Bounds(features[some], weight, targets[some], 1.0)
+            loss = head.loss(features[some], weight, targets[some])
+            close(loss.losses, b.losses, b.loss_error)
+
+
+def test_lowest_values_of_the_type_as_labels_out_of_use(ctx):
+    """Label rows that push their logits to the type's lowest values have probability 0 and no gradient."""
+    rows, labels, dim = 200, 300, 32
+    head = sb.LabelHead(ctx, labels, dim, torch.bfloat16, rows)
+    features, weight = matrix(rows, dim, torch.bfloat16, 1), matrix(labels, dim, torch.bfloat16, 2)
+    features[:, 0] = 1.0
+    off = torch.arange(0, labels, 3, device="cuda")
+    weight[off] = 0
+    weight[off, 0] = torch.finfo(torch.bfloat16).min
+    keep = torch.ones(labels, dtype=torch.bool, device="cuda")
+    keep[off] = False
+    targets = torch.nonzero(keep)[:, 0][torch.randint(0, int(keep.sum()), (rows,), device="cuda")]
+    b = Bounds(features, weight[keep], torch.searchsorted(torch.nonzero(keep)[:, 0], targets), 1.0)
+    loss = head.loss(features, weight, targets)
+    close(loss.losses, b.losses, b.loss_error)
+    _, to_weight = head.gradient(features, weight, targets, loss.log_normalizers)
+    assert to_weight[off].count_nonzero() == 0
+    close(to_weight[keep], b.to_weight, b.weight_error)
+
+
+def test_offsets_past_32_bits(ctx):
+    """Rows further apart than 2^31 elements in all."""
+    rows, stride, dim = 70_000, 32_768, 16
+    wide = torch.zeros(rows, stride, dtype=torch.bfloat16, device="cuda")
+    far = wide[:, :dim]
+    far.copy_(torch.randn(rows, dim, device="cuda"))
+    packed = far.contiguous()
+    tokens = tokens_for("some", 4000, rows, torch.int64, 1)
+    e = sb.Embedding(ctx, rows, dim, torch.bfloat16, 4000)
+    found = e.lookup(packed, tokens)
+    assert torch.equal(e.lookup(far, tokens), found)
+    want = e.gradient(found, tokens).clone()
+    e.gradient(found, tokens, out=far)
+    assert torch.equal(far, want)
+    far.copy_(packed)
+    head = sb.LabelHead(ctx, 64, dim, torch.bfloat16, rows)
+    weight, targets = matrix(64, dim, torch.bfloat16, 2), tokens_for("some", rows, 64, torch.int32, 3)
+    near, away = head.loss(packed, weight, targets), head.loss(far, weight, targets)
+    assert torch.equal(near.losses, away.losses)
+    to_near, _ = head.gradient(packed, weight, targets, near.log_normalizers)
+    head.gradient(packed, weight, targets, near.log_normalizers, feature_gradient=far)
+    assert torch.equal(far, to_near)
+    targets = tokens_for("all", 90, rows, torch.int32, 4)
+    codes = sb.LabelHead(ctx, rows, dim, torch.bfloat16, 90)
+    far.copy_(packed)
+    assert torch.equal(codes.loss(packed[:90], far, targets).losses, codes.loss(packed[:90], packed, targets).losses)
+
+
+def test_a_context_with_a_stream_of_its_own():
+    stream = torch.cuda.Stream()
+    own = sb.Context(0, stream=stream.cuda_stream)
+    rows, labels, dim = 300, 400, 64
+    weight, targets = matrix(labels, dim, torch.float32, 2), tokens_for("some", rows, labels, torch.int32, 3)
+    head, e = sb.LabelHead(own, labels, dim, torch.float32, rows), sb.Embedding(own, labels, dim, torch.float32, rows)
+    for _ in range(5):
+        torch.cuda._sleep(200_000)  # the operands are late on the current stream
+        table = weight * 1
+        features = e.lookup(table, targets)
+        loss = head.loss(features, table, targets)
+        to_features, _ = head.gradient(features, table, targets, loss.log_normalizers)
+        back = e.gradient(to_features, targets) * 1
+        b = Bounds(features, weight, targets, 1.0)
+        close(loss.losses, b.losses, b.loss_error)
+        close(to_features, b.to_features, b.features_error)
+        want, bound = gradient_bound(to_features, targets, labels, 1.0)
+        close(back, want, bound)
+    e.close(), head.close()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_example_learns_its_scene(dtype):
+    sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "examples"))
+    import label_scene
+
+    result = label_scene.train(steps=60, dtype=dtype, scale=0.1)
+    # It starts at the loss of a uniform guess among 100 labels (small random weights: within 0.1 of
+    # ln 100) and ends far below it; a token's Gaussians mostly share their region.
+    assert abs(result["first_loss"] - 4.605) < 0.1
+    assert result["last_loss"] < 0.5 * result["first_loss"]
+    assert result["accuracy"] > 0.5
