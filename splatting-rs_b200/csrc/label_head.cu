@@ -749,6 +749,7 @@ sp_status run_stats(sp_label_head* h, const Operands& op, const void* weight, in
         thin.weight_stride = weight_stride;
         thin.dim = h->dim;
         thin.vector = vector_rows(h, weight, weight_stride);
+        thin.known_rows = targets || op.all_rows ? 0 : (uint32_t)n;
         thin.columns = (uint32_t)round_up(n, 16);
         // Whole rounds of tiles over the SMs; converted weights come in tiles of the height that fills
         // the last round too.

@@ -36,6 +36,7 @@ struct ThinArgs {
     uint32_t dim;
     int vector;          // 16-byte loads are aligned
     uint32_t tile;       // labels per tile: kTile, or for converted weights a multiple of 8
+    uint32_t known_rows; // not 0: the rows' count, known before the launch that gathers them is done
     uint32_t columns;    // of the accumulators: the rows, rounded up to 16
     uint32_t tiles;
 };
@@ -105,9 +106,11 @@ __global__ void __launch_bounds__(thin_threads(DIRECT), 1)
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<uint32_t*>(generic_base + (tmem_slot - smem));
-    chain_enter();
+    // The gathering launch before this one has itself waited for all that came earlier, the weight among
+    // it: the converting warps need not wait for the rows.
+    if (DIRECT || warp < 8 || a.known_rows == 0) chain_enter();
 
-    const uint32_t count = a.g.all_rows ? a.g.all_rows : a.g.rows->count;
+    const uint32_t count = a.known_rows ? a.known_rows : a.g.all_rows ? a.g.all_rows : a.g.rows->count;
     const uint32_t tiles = count ? a.tiles : 0;
     // A buffer's accumulator groups: f32's three, then hi hi (all, for bf16) of the odd steps.
     const uint32_t buffer_columns = 4 * kThinRows;

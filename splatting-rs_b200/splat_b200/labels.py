@@ -50,24 +50,25 @@ class _Handle:
 
     def _matrix(self, x, columns: int, what: str, rows: int | None = None) -> tuple[int, int]:
         """(pointer, row stride) of a matrix argument."""
-        if x.dtype is not self.dtype or x.dim() != 2 or x.size(1) != columns or (rows is not None and x.size(0) != rows):
+        shape = x.shape
+        if x.dtype is not self.dtype or len(shape) != 2 or shape[1] != columns or (rows is not None and shape[0] != rows):
             raise ValueError(f"{what}: a {self.dtype} matrix of {'any' if rows is None else rows} x {columns}, "
-                             f"got {x.dtype} {tuple(x.shape)}")
+                             f"got {x.dtype} {tuple(shape)}")
         if x.get_device() != self.ctx.device:
             raise ValueError(f"{what}: on cuda:{self.ctx.device}, got {x.device}")
         row_stride, column_stride = x.stride()
         if column_stride != 1 and columns > 1:
             raise ValueError(f"{what}: unit column stride, got {x.stride()}")
-        if row_stride < columns and x.size(0) <= 1:
+        if row_stride < columns and shape[0] <= 1:
             row_stride = columns
         return x.data_ptr(), row_stride
 
     def _vector(self, x, what: str, count: int | None = None, dtype=None) -> int:
-        if x.dim() != 1 or not x.is_contiguous() or (dtype is not None and x.dtype is not dtype) or (
-            count is not None and x.size(0) != count
-        ):
+        shape = x.shape
+        if (len(shape) != 1 or not x.is_contiguous() or (dtype is not None and x.dtype is not dtype)
+                or (count is not None and shape[0] != count)):
             raise ValueError(f"{what}: a contiguous vector of {'any number of' if count is None else count} "
-                             f"{'values' if dtype is None else dtype}, got {x.dtype} {tuple(x.shape)}")
+                             f"{'values' if dtype is None else dtype}, got {x.dtype} {tuple(shape)}")
         if x.get_device() != self.ctx.device:
             raise ValueError(f"{what}: on cuda:{self.ctx.device}, got {x.device}")
         return x.data_ptr()
@@ -122,7 +123,7 @@ class Embedding(_Handle):
         """scale * table[tokens], in the element type."""
         table_at, table_stride = self._matrix(table, self.dim, "table", self.entries)
         tokens_at, index = self._index(tokens, "tokens")
-        count = tokens.size(0)
+        count = tokens.shape[0]
         if out is None:
             out = table.new_empty((count, self.dim))
             out_at, out_stride = out.data_ptr(), self.dim
@@ -134,7 +135,7 @@ class Embedding(_Handle):
     def gradient(self, out_gradient, tokens, scale: float = 1.0, out=None):
         """The gradient of the table from that of `lookup`'s result: every entry's row written."""
         tokens_at, index = self._index(tokens, "tokens")
-        count = tokens.size(0)
+        count = tokens.shape[0]
         gradient_at, gradient_stride = self._matrix(out_gradient, self.dim, "out_gradient", count)
         if out is None:
             out = out_gradient.new_empty((self.entries, self.dim))
@@ -174,20 +175,20 @@ class LabelHead(_Handle):
     def loss(self, features, weight, targets, logit_scale: float = 1.0) -> LabelLoss:
         """Cross entropy of softmax(logit_scale * features @ weight.T) at each row's target."""
         inputs = self._inputs(features, weight)
-        rows = features.size(0)
+        rows = features.shape[0]
         targets_at, index = self._index(targets, "targets", rows)
-        # One allocation: losses, log normalizers, mean.
-        out = features.new_empty(2 * rows + 1, dtype=self._torch.float32)
-        at = out.data_ptr()
-        self._call("sp_label_head_loss", *inputs, targets_at, index, rows, logit_scale, at + 8 * rows, at, at + 4 * rows)
-        return LabelLoss(out[2 * rows], out[:rows], out[rows : 2 * rows])
+        losses = features.new_empty(rows, dtype=self._torch.float32)
+        normalizers, mean = self._torch.empty_like(losses), losses.new_empty(())
+        self._call("sp_label_head_loss", *inputs, targets_at, index, rows, logit_scale, mean.data_ptr(),
+                   losses.data_ptr(), normalizers.data_ptr())
+        return LabelLoss(mean, losses, normalizers)
 
     def gradient(self, features, weight, targets, log_normalizers, logit_scale: float = 1.0, row_gradient=None,
                  feature_gradient=None, weight_gradient=None):
         """(gradient of the features, of the weight) of the mean loss, or with `row_gradient` (one
         float32 per row) of sum(row_gradient * losses). `log_normalizers` as `loss` returned them."""
         inputs = self._inputs(features, weight)
-        rows = features.size(0)
+        rows = features.shape[0]
         targets_at, index = self._index(targets, "targets", rows)
         float32 = self._torch.float32
         normalizers_at = self._vector(log_normalizers, "log_normalizers", rows, float32)
@@ -204,7 +205,7 @@ class LabelHead(_Handle):
     def predict(self, features, weight, logit_scale: float = 1.0):
         """(label int32, log-probability float32) of each row's most probable label."""
         inputs = self._inputs(features, weight)
-        rows = features.size(0)
+        rows = features.shape[0]
         labels = features.new_empty(rows, dtype=self._torch.int32)
         log_probabilities = features.new_empty(rows, dtype=self._torch.float32)
         self._call("sp_label_head_predict", *inputs, rows, logit_scale, labels.data_ptr(), log_probabilities.data_ptr())
