@@ -927,10 +927,11 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
                      d_feature_gradient, feature_gradient_stride, true, &op));
 
     const uint64_t chunk = chunk_for(h, rows), chunks = (rows + chunk - 1) / chunk;
-    const uint64_t slope_stride = h->slope_stride(), sum_stride = sums_stride(h);
+    const uint64_t sum_stride = sums_stride(h);
     CUtensorMap slopes, slopes_out;
-    SP_CHECK(make_map(ctx, &slopes, h->slopes, slope_stride, chunk, slope_stride, h->parts(), chunk * slope_stride));
-    SP_CHECK(make_map(ctx, &slopes_out, h->slopes, slope_stride, chunk, slope_stride, h->parts(), chunk * slope_stride, 32));
+    const uint32_t panels = (uint32_t)(h->slope_stride() / 64);
+    SP_CHECK(make_map(ctx, &slopes, h->slopes, 64, chunk, 64, panels * h->parts(), chunk * 64));
+    SP_CHECK(make_map(ctx, &slopes_out, h->slopes, 64, chunk, 64, panels * h->parts(), chunk * 64, 32));
     // One cut of the weight's gradient for every chunk: its pieces' sums go on from one to the next.
     const OutPlan first = plan_out(h->sms, std::min(chunk, rows), h->labels, h->dim, h->parts(), chunks > 1);
     const bool weight_sums = first.weight > 1 || chunks > 1;
@@ -954,6 +955,7 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
         a.splits = logits.splits;
         a.log_normalizers = d_log_normalizers;
         a.row_gradient = d_row_gradient;
+        a.panels = panels;
         a.residuals = h->target_logits;  // free in a gradient
         const bool weight_here = in_place(h, d_weight, weight_stride);
         a.weight = weight_here ? static_cast<const bf16*>(d_weight) : h->packed_weight;
