@@ -372,74 +372,80 @@ __global__ void __launch_bounds__(kFewThreads)
               const T* __restrict__ upstream, int64_t upstream_stride, uint32_t dim, float scale, T* __restrict__ out,
               int64_t out_stride, int out_packed, int lanes_log2) {
     chain_enter();
-    constexpr uint32_t kWarps = kFewThreads / 32, kItems = kFewTokens / kFewThreads;
+    constexpr uint32_t kWarps = kFewThreads / 32;
     extern __shared__ float4 few_smem[];
     __shared__ uint32_t start[kMostOwned + 1], warp_sums[kWarps], longs[kMostOwned], long_count;
     float* s_part = reinterpret_cast<float*>(few_smem);  // [kFewThreads][N]
     uint16_t* placed = reinterpret_cast<uint16_t*>(s_part + kFewThreads * N);  // [kWarps][owned]
-    uint16_t* order = placed + kWarps * owned;                                 // [count]
+    uint16_t* order = placed + kWarps * owned;                                 // [count], then the entries
     const uint32_t t = threadIdx.x, warp = t / 32, lane = lane_id();
     const uint32_t section = (count + kFewThreads - 1) / kFewThreads * 32;  // of the tokens, per warp
     const int64_t first_entry = (int64_t)blockIdx.x * owned;
 
-    uint32_t token[kItems];
-#pragma unroll
-    for (uint32_t k = 0; k < kItems; ++k) {
-        const uint32_t i = warp * section + k * 32 + lane;
-        token[k] = kMostOwned;
-        if (k * 32 < section && i < count) {
+    // The warp's tokens as entries of this block (kMostOwned: another block's).
+    uint16_t* entry_of = order + count + warp * section;
+#pragma unroll 8
+    for (uint32_t k = lane; k < section; k += 32) {
+        const uint32_t i = warp * section + k;
+        uint32_t entry = kMostOwned;
+        if (i < count) {
             const int64_t v = index_at(tokens, wide, i, entries) - first_entry;
-            if (v >= 0 && v < (int64_t)owned) token[k] = (uint32_t)v;
+            if (v >= 0 && v < (int64_t)owned) entry = (uint32_t)v;
         }
+        entry_of[k] = (uint16_t)entry;
     }
     for (uint32_t i = t; i < kWarps * owned; i += kFewThreads) placed[i] = 0;
     if (t == 0) long_count = 0;
     __syncthreads();
     const uint32_t below = (1u << lane) - 1u;
-    // place(): the next free places of the warp's tokens, equal ones in lane order.
+    // place(entry, at, position): the warp's tokens, each `at` its next place in its entry, equal ones in
+    // lane order.
     uint16_t* mine = placed + warp * owned;
     auto for_each_place = [&](auto&& place) {
-#pragma unroll
-        for (uint32_t k = 0; k < kItems; ++k) {
-            const bool here = token[k] < kMostOwned;
+#pragma unroll 2
+        for (uint32_t k = lane; k < section; k += 32) {
+            const uint32_t entry = entry_of[k];
+            const bool here = entry < kMostOwned;
             if (!__any_sync(0xffffffffu, here)) continue;
-            const uint32_t peers = __match_any_sync(0xffffffffu, token[k]);
-            const uint32_t before = here ? mine[token[k]] : 0;
+            const uint32_t peers = __match_any_sync(0xffffffffu, entry);
+            const uint32_t before = here ? mine[entry] : 0;
             __syncwarp();
             if (here) {
-                if ((peers & below) == 0) mine[token[k]] = (uint16_t)(before + __popc(peers));
-                place(before + __popc(peers & below), warp * section + k * 32 + lane);
+                if ((peers & below) == 0) mine[entry] = (uint16_t)(before + __popc(peers));
+                place(entry, before + __popc(peers & below), warp * section + k);
             }
             __syncwarp();
         }
     };
-    for_each_place([](uint32_t, uint32_t) {});
+    for_each_place([](uint32_t, uint32_t, uint32_t) {});
     __syncthreads();
-    // Entry e's total, and in its column the running counts over the warps; then the entries' scan.
-    uint32_t total = 0;
-    if (t < owned)
-        for (uint32_t w = 0; w < kWarps; ++w) {
-            const uint32_t c = placed[w * owned + t];
-            placed[w * owned + t] = (uint16_t)total;
-            total += c;
-        }
-    uint32_t inclusive = total;
+    // Entry e's total, and in its column the running counts over the warps (a warp per entry); then the
+    // entries' scan.
+    auto scan = [&](uint32_t v) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, inclusive, o);
-        if (lane >= (uint32_t)o) inclusive += up;
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t up = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= (uint32_t)o) v += up;
+        }
+        return v;
+    };
+    for (uint32_t e = warp; e < owned; e += kWarps) {
+        const uint32_t c = placed[lane * owned + e], inclusive = scan(c);
+        placed[lane * owned + e] = (uint16_t)(inclusive - c);
+        if (lane == 31) start[e] = inclusive;
     }
+    __syncthreads();
+    const uint32_t total = t < owned ? start[t] : 0, inclusive = scan(total);
     if (lane == 31) warp_sums[warp] = inclusive;
     __syncthreads();
-    uint32_t offset = 0;
-    for (uint32_t w = 0; w < warp; ++w) offset += warp_sums[w];
+    const uint32_t before_warp = scan(warp_sums[lane]) - warp_sums[lane];
+    const uint32_t offset = __shfl_sync(0xffffffffu, before_warp, warp);
     if (t < owned) {
         start[t] = offset + inclusive - total;
         if (t == owned - 1) start[owned] = offset + inclusive;
-        for (uint32_t w = 0; w < kWarps; ++w) placed[w * owned + t] += (uint16_t)start[t];
     }
     __syncthreads();
-    for_each_place([&](uint32_t at, uint32_t position) { order[at] = (uint16_t)position; });
+    for_each_place([&](uint32_t entry, uint32_t at, uint32_t position) { order[start[entry] + at] = (uint16_t)position; });
     __syncthreads();
 
     const uint32_t lanes = 1u << lanes_log2, groups = kFewThreads >> lanes_log2, group = t >> lanes_log2;
@@ -461,39 +467,46 @@ __global__ void __launch_bounds__(kFewThreads)
         }
     };
     const uint32_t first_column = (t & (lanes - 1)) * N, tile = lanes * N;
-    for (uint32_t e = group; e < entries_here; e += groups) {
-        const uint32_t from = start[e], to = start[e + 1];
-        if (to - from > kLongRun) {
-            if ((t & (lanes - 1)) == 0) longs[atomicAdd(&long_count, 1u)] = e;
-            continue;
-        }
-        for (uint32_t column = blockIdx.y * tile + first_column; column < dim; column += gridDim.y * tile) {
-            float acc[N];
-            sum_rows(from, to, column, acc);
-            store_row<T, N>(out + (first_entry + e) * out_stride + column, acc, scale, out_packed);
-        }
-    }
-    __syncthreads();
-    // In whatever order they were noted: each is summed by itself.
-    for (uint32_t k = 0; k < long_count; ++k) {
-        const uint32_t e = longs[k], from = start[e], n = start[e + 1] - from;
+    // An entry's run goes to a team of groups in equal parts, joined in order: as many groups as there
+    // are to each entry, all of them for runs longer than kLongRun a group.
+    const uint32_t groups_log2 = 31 - __clz(groups);
+    uint32_t usual_log2 = 0;
+    while (((uint32_t)2 << usual_log2) * entries_here <= groups) ++usual_log2;
+    auto sum_entry = [&](uint32_t e, uint32_t team_log2, bool takes) {
+        const uint32_t team = 1u << team_log2, member = group & (team - 1);
+        const uint32_t from = takes ? start[e] : 0, n = takes ? start[e + 1] - from : 0;
         for (uint32_t base = blockIdx.y * tile; base < dim; base += gridDim.y * tile) {
             const uint32_t column = base + first_column;
             float acc[N];
-            if (column < dim) {
-                sum_rows(from + (uint32_t)((uint64_t)n * group / groups), from + (uint32_t)((uint64_t)n * (group + 1) / groups),
-                         column, acc);
+            if (takes && column < dim) {
+                sum_rows(from + (n * member >> team_log2), from + (n * (member + 1) >> team_log2), column, acc);
+                if (member != 0)
 #pragma unroll
-                for (int j = 0; j < N; ++j) s_part[t * N + j] = acc[j];
+                    for (int j = 0; j < N; ++j) s_part[t * N + j] = acc[j];
             }
-            __syncthreads();
-            if (group == 0 && column < dim) {
-                for (uint32_t g = 1; g < groups; ++g)
+            if (team > 1) __syncthreads();
+            if (takes && member == 0 && column < dim) {
+                for (uint32_t m = 1; m < team; ++m)
 #pragma unroll
-                    for (int j = 0; j < N; ++j) acc[j] += s_part[(g * lanes + t) * N + j];
+                    for (int j = 0; j < N; ++j) acc[j] += s_part[(t + m * lanes) * N + j];
                 store_row<T, N>(out + (first_entry + e) * out_stride + column, acc, scale, out_packed);
             }
+            if (team > 1) __syncthreads();
+        }
+    };
+    // The teams' entries, then the long runs that were noted, each by itself: whatever their order.
+    const uint32_t teams_log2 = groups_log2 - usual_log2, turns = (entries_here + (1u << teams_log2) - 1) >> teams_log2;
+    for (uint32_t k = 0, long_runs = 0; k < turns + long_runs; ++k) {
+        const bool all = k >= turns;
+        const uint32_t e = all ? longs[k - turns] : (k << teams_log2) + (group >> usual_log2);
+        const bool is_long = !all && usual_log2 < groups_log2 && e < entries_here &&
+                             start[e + 1] - start[e] > kLongRun << usual_log2;
+        if (is_long && (group & ((1u << usual_log2) - 1)) == 0 && (t & (lanes - 1)) == 0)
+            longs[atomicAdd(&long_count, 1u)] = e;
+        sum_entry(e, all ? groups_log2 : usual_log2, e < entries_here && !is_long);
+        if (k + 1 == turns) {
             __syncthreads();
+            long_runs = long_count;
         }
     }
 }
@@ -564,9 +577,10 @@ uint32_t few_owned(uint64_t entries, uint64_t count) {
 template <typename T, int N>
 cudaError_t sum_few(const sp_embedding* e, const void* tokens, int wide, uint32_t count, uint32_t owned, const Rows& r,
                     int lanes_log2) {
-    const size_t smem = kFewThreads * N * sizeof(float) + (kFewThreads / 32 * (size_t)owned + count) * sizeof(uint16_t);
+    const size_t smem = kFewThreads * N * sizeof(float) +
+                        (kFewThreads / 32 * (size_t)owned + count + (count + kFewThreads - 1) / kFewThreads * kFewThreads) * sizeof(uint16_t);
     static std::atomic<unsigned long long> configured{0};
-    constexpr size_t most = kFewThreads * N * sizeof(float) + (kFewThreads / 32 * kMostOwned + kFewTokens) * sizeof(uint16_t);
+    constexpr size_t most = kFewThreads * N * sizeof(float) + (kFewThreads / 32 * kMostOwned + 2 * kFewTokens) * sizeof(uint16_t);
     const cudaError_t err = allow_smem_once(k_sum_few<T, N>, most, configured);
     if (err != cudaSuccess) return err;
     const int out_packed = pack_width(r.out, r.out_stride, e->dim, sizeof(T)) >= N;
