@@ -64,12 +64,13 @@ sp_status sp_label_head_create(sp_context* ctx, uint64_t labels, uint32_t dim, s
                                int training, sp_label_head** out);
 void sp_label_head_destroy(sp_label_head* h);
 /* Cross entropy of each row's target: losses[i] = log_normalizers[i] - z[i][targets[i]] with
- * log_normalizers[i] = log sum_v exp z[i][v]; *mean = the mean over the rows with a target (0 when
+ * log_normalizers[i] = log sum_v exp z[i][v] (f64: a confident row's slope is the small difference of
+ * its target's logit and this); *mean = the mean over the rows with a target (0 when
  * there is none). A row without a target is skipped, whatever its features hold: 0 in both
  * outputs. logit_scale > 0 and finite. */
 sp_status sp_label_head_loss(sp_label_head* h, const void* d_features, int64_t feature_stride, const void* d_weight,
                              int64_t weight_stride, const void* d_targets, sp_index index, uint64_t rows,
-                             float logit_scale, float* d_mean, float* d_losses, float* d_log_normalizers);
+                             float logit_scale, float* d_mean, float* d_losses, double* d_log_normalizers);
 /* The gradient of sum_i g[i] losses[i], g = d_row_gradient (rows floats), or with NULL of the mean
  * (g[i] = 1 / rows with a target). Both gradients are overwritten; a row without a target gets a
  * zero row and adds nothing to the weight's. `d_log_normalizers` are those of sp_label_head_loss
@@ -77,7 +78,7 @@ sp_status sp_label_head_loss(sp_label_head* h, const void* d_features, int64_t f
  * slopes are rounded to the element type (f32: kept to 24 bits) before the second products. */
 sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64_t feature_stride,
                                  const void* d_weight, int64_t weight_stride, const void* d_targets, sp_index index,
-                                 uint64_t rows, float logit_scale, const float* d_log_normalizers,
+                                 uint64_t rows, float logit_scale, const double* d_log_normalizers,
                                  const float* d_row_gradient, void* d_feature_gradient,
                                  int64_t feature_gradient_stride, void* d_weight_gradient,
                                  int64_t weight_gradient_stride);

@@ -94,7 +94,7 @@ struct GemmArgs {
     uint64_t partial_rows;
     float* target_logits;
     // kSlopes
-    const float* log_normalizers;
+    const double* log_normalizers;
     const float* row_gradient;
     uint32_t panels;       // of 64 labels in a part of the slopes
     // bf16 operands: what rounding left of each row's target slope, by far the row's largest. dH takes it
@@ -180,9 +180,10 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
-// A row's running softmax: sum of 2^(z scale2 - base) over its logits z so far. The loss takes any
-// base that keeps the sum in range; prediction needs the largest logit and its label, and its base is
-// that logit's. The target's logit is picked up when it comes past.
+// A row's running softmax: sum of 2^(z scale2 - base) over its logits z so far, without the one that
+// matters: the target's for the loss, the largest for prediction. What is left of 1 after its probability
+// is then known to full precision however near 1 that is. The loss takes any base that keeps the sum in
+// range; prediction's is that of the largest logit.
 constexpr float kLargestSum = 18446744073709551616.0f;  // 2^64
 struct RowStats {
     float base, sum, target_logit, largest;
@@ -227,17 +228,32 @@ __device__ __forceinline__ void add_logits(RowStats& s, float (&v)[W], uint32_t 
     if (LABEL) {
         const float m = largest_of(v);
         if (m > s.largest) {
-            s.largest = m;
+            // The one that was the largest joins the others (exp2(-inf) = 0 where there was none).
             const float base = __fmul_rn(m, scale2);
-            s.sum *= exp2_fast(s.base - base);  // 0 after a first chunk's base of -inf
+            s.sum = (s.sum + 1.0f) * exp2_fast(s.base - base);
             s.base = base;
+            s.largest = m;
+            uint32_t place = 0;
 #pragma unroll
             for (int j = W - 1; j >= 0; --j)
-                if (v[j] == m) s.label = first + j;
+                if (v[j] == m) place = j;
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+                if (place == (uint32_t)j) v[j] = -INFINITY;
+            s.label = first + place;
         }
         // Nothing but -inf so far: any finite base counts that as 0.
         s.sum += sum_exp2(v, scale2, s.base == -INFINITY ? 0.0f : s.base);
         return;
+    }
+    if (near) {
+        const uint32_t at = target - first;
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+            if (at == (uint32_t)j) {
+                s.target_logit = v[j];
+                v[j] = -INFINITY;
+            }
     }
     if (s.base == -INFINITY) {
         const float m = largest_of(v);
@@ -253,32 +269,36 @@ __device__ __forceinline__ void add_logits(RowStats& s, float (&v)[W], uint32_t 
         base = s.base = higher;
     }
     s.sum = sum;
-    if (near) {
-        const uint32_t at = target - first;
-#pragma unroll
-        for (int j = 0; j < W; ++j)
-            if (at == (uint32_t)j) s.target_logit = v[j];
-    }
 }
 
-// The slopes of 32 logits of a row, in place; zeros past the labels and in rows that do not count. The
-// target's, if it is among them, also in `target_slope`.
+// The slopes of 32 logits of a row, in place (the target's only if PLACE); zeros past the labels and in rows that do not count. The
+// target's, if it is among them, also in `target_slope`: p - 1 from the difference of its logit and the
+// normalizer, -(shift + shift_low) to twice f32's precision, since p itself may round to 1.
+template <bool PLACE>
 __device__ __forceinline__ void to_slopes(float (&v)[32], uint32_t first, uint32_t labels, float scale2, float shift,
-                                          float weight, uint32_t target, bool live, float& target_slope) {
+                                          float weight, uint32_t target, bool live, float shift_low, float& target_slope) {
+    const uint32_t at = target - first;
+    const bool near = __any_sync(0xffffffffu, at < 32);
+    float logit = 0.0f;
+    if (near) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (at == (uint32_t)j) logit = v[j];
+    }
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
         const float2 x = fma2(make_float2(v[j], v[j + 1]), make_float2(scale2, scale2), make_float2(shift, shift));
         v[j] = exp2_fast(x.x);
         v[j + 1] = exp2_fast(x.y);
     }
-    const uint32_t at = target - first;
-    if (__any_sync(0xffffffffu, at < 32)) {
+    if (near) {
+        const float slope = expm1f((fmaf(logit, scale2, shift) + shift_low) * 0.693147181f);
+        if (at < 32) target_slope = slope * weight;
+        if (PLACE) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (at == (uint32_t)j) {
-                v[j] -= 1.0f;
-                target_slope = v[j] * weight;
-            }
+            for (int j = 0; j < 32; ++j)
+                if (at == (uint32_t)j) v[j] = slope;
+        }
     }
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = live ? v[j] * weight : 0.0f;
@@ -307,6 +327,12 @@ __device__ __forceinline__ void stage_part(uint32_t tile, uint32_t row, int half
                      "r"(w[1]), "r"(w[2]), "r"(w[3])
                      : "memory");
     }
+}
+
+// Column `column` of that row.
+__device__ __forceinline__ void stage_one(uint32_t tile, uint32_t row, uint32_t column, bf16 v) {
+    const uint32_t at = tile + row * 128 + ((column / 8) ^ (row & 7u)) * 16 + column % 8 * 2;
+    asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"(__bfloat16_as_ushort(v)) : "memory");
 }
 
 template <typename T>
@@ -510,7 +536,7 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
             const bool live = compact < count;
             RowStats stats{-INFINITY, 0.0f, 0.0f, -INFINITY, 0u};
             uint32_t target = kNoTarget;
-            float shift = 0.0f, weight = 0.0f;
+            float shift = 0.0f, shift_low = 0.0f, weight = 0.0f;
             float residual = 0.0f;
             if (ENDING == kOut && sizeof(T) == 2 && live && w.which == 0) {
                 target = (uint32_t)index_at(a.targets, a.wide, a.row_of[compact], a.labels);
@@ -520,7 +546,9 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                 const uint32_t original = a.all_rows ? compact : a.row_of[compact];
                 if (a.targets) target = (uint32_t)index_at(a.targets, a.wide, original, a.labels);
                 if (ENDING == kSlopes) {
-                    shift = -a.log_normalizers[original] * 1.44269504088896341f;
+                    const double exact_shift = a.log_normalizers[original] * -1.4426950408889634;
+                    shift = (float)exact_shift;
+                    shift_low = (float)(exact_shift - (double)shift);
                     weight = a.scale * (a.row_gradient ? a.row_gradient[original] : 1.0f / (float)count);
                 }
             }
@@ -562,11 +590,14 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                                 if (q == 1 && c + 64 == kSpan) drain();
                                 const uint32_t column = columns_at + c + 32 * q;
                                 float slope = 0.0f;
-                                to_slopes(v, column, a.labels, a.scale2, shift, weight, target, live, slope);
-                                if (target - column < 32)
-                                    a.residuals[row] = slope - __bfloat162float(__float2bfloat16_rn(slope));
+                                to_slopes<false>(v, column, a.labels, a.scale2, shift, weight, target, live, shift_low, slope);
                                 if (q == 0) reclaim();
                                 stage_part(stage_tile, lane, q, v);
+                                if (target - column < 32) {
+                                    const bf16 rounded = __float2bfloat16_rn(slope);
+                                    stage_one(stage_tile, lane, 32 * q + target - column, rounded);
+                                    a.residuals[row] = slope - __bfloat162float(rounded);
+                                }
                             }
                             store(0);
                         } else {
@@ -578,8 +609,8 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                             if (c + 64 == kSpan) drain();
 #pragma unroll
                             for (int q = 0; q < 2; ++q)
-                                to_slopes(v[q], columns_at + c + 32 * q, a.labels, a.scale2, shift, weight, target, live,
-                                          unused);
+                                to_slopes<true>(v[q], columns_at + c + 32 * q, a.labels, a.scale2, shift, weight, target, live,
+                                          shift_low, unused);
                             for (int p = 0; p < (int)kParts; ++p) {
                                 reclaim();
                                 stage_part(stage_tile, lane, 0, v[0]);

@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kThreads)
                   const uint32_t* __restrict__ counts, const uint32_t* __restrict__ group_counts,
                   const T* __restrict__ features, int64_t stride, uint32_t dim, int vector, int in_place, RowSet* rows,
                   uint32_t* __restrict__ row_of, bf16* __restrict__ packed, uint64_t packed_stride, uint64_t part,
-                  float* __restrict__ losses, float* __restrict__ normalizers, T* __restrict__ gradient,
+                  float* __restrict__ losses, double* __restrict__ normalizers, T* __restrict__ gradient,
                   int64_t gradient_stride, PackWeight<T> weight) {
     chain_enter();
     const uint32_t gathering = gather_blocks * sharers;
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kThreads)
             skipped[t - below] = t;
             if (share == 0 && first + t < n) {
                 if (losses) losses[first + t] = 0.0f;
-                if (normalizers) normalizers[first + t] = 0.0f;
+                if (normalizers) normalizers[first + t] = 0.0;
             }
         }
     }
@@ -258,16 +258,15 @@ __global__ void __launch_bounds__(kThreads)
 
 // LANES threads (1, 8 or 32) join a row's partial sums, each in units of 2^base: the highest base
 // (and the largest logit with the lowest label) first, then the sum, in double, since a part may come
-// close to f32's largest. In units of ln 2 a row's log sum exp is base + log2(sum), its loss that less
-// z[target] scale2, and its largest log-probability the negative of that with the largest logit, all
-// taken in double so that nothing is lost where they cancel. The loss's mean is summed in double: per
-// block, then by the last block.
+// close to f32's largest. With the rest, the sum without the target's logit (the largest's), in units of
+// the latter's exponential, the loss (the negative log-probability) is log1p(rest): nothing cancels. The
+// loss's mean is summed in double: per block, then by the last block.
 template <int LANES>
 __global__ void __launch_bounds__(kThreads)
     k_join_rows(RowSet* rows, const uint32_t* __restrict__ row_of, uint32_t all_rows,
                 const float2* __restrict__ partials, const uint32_t* __restrict__ partial_labels,
                 uint64_t partial_rows, uint32_t slots, float scale2, const float* __restrict__ target_logits,
-                float* __restrict__ losses, float* __restrict__ normalizers, int32_t* __restrict__ labels_out,
+                float* __restrict__ losses, double* __restrict__ normalizers, int32_t* __restrict__ labels_out,
                 float* __restrict__ log_probability, double* __restrict__ block_sums, float* __restrict__ mean) {
     chain_enter();
     const uint32_t count = all_rows ? all_rows : rows->count;
@@ -281,6 +280,9 @@ __global__ void __launch_bounds__(kThreads)
     float top = -INFINITY, largest = -INFINITY;
     uint32_t label = 0xffffffffu;
     double sum = 0.0;
+    // Prediction: each part's largest goes into the sum here, and the row's out of it again (a 1 in units
+    // of 2^top, to double's precision).
+    const double one = partial_labels ? 1.0 : 0.0;
     for (uint32_t s0 = lane; s0 < mine; s0 += LANES * kSlotsAhead) {
         float2 p[kSlotsAhead];
         uint32_t l[kSlotsAhead];
@@ -303,7 +305,7 @@ __global__ void __launch_bounds__(kThreads)
         sum *= (double)exp2f(before - finite);
 #pragma unroll
         for (int k = 0; k < kSlotsAhead; ++k)
-            if (s0 + k * LANES < mine) sum += (double)p[k].y * (double)exp2f(p[k].x - finite);
+            if (s0 + k * LANES < mine) sum += ((double)p[k].y + one) * (double)exp2f(p[k].x - finite);
     }
     float highest = top;
 #pragma unroll
@@ -320,15 +322,25 @@ __global__ void __launch_bounds__(kThreads)
     for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (i < count && lane == 0) {
         const uint32_t row = all_rows ? (uint32_t)i : row_of[i];
-        const double ln2 = 0.6931471805599453, log2_sum = (double)top + log2(sum);
+        const double ln2 = 0.6931471805599453;
         if (labels_out) {
             labels_out[row] = failed ? -1 : (int32_t)label;
-            log_probability[row] = failed ? nan : (float)(((double)largest * scale2 - log2_sum) * ln2);
+            // An infinite largest logit has no softmax.
+            log_probability[row] = failed || !(fabsf(largest) < INFINITY) ? nan : (float)-log1p(sum - 1.0);
         } else {
-            const float value = failed ? nan : (float)((log2_sum - (double)target_logits[i] * scale2) * ln2);
-            losses[row] = value;
-            normalizers[row] = failed ? nan : (float)(log2_sum * ln2);
-            loss = (double)value;
+            const double target2 = (double)target_logits[i] * scale2;
+            const double rest = sum == 0.0 ? 0.0 : sum * exp2((double)top - target2);
+            double value, normalizer;
+            if (rest <= 1.0) {
+                value = log1p(rest);
+                normalizer = target2 * ln2 + value;
+            } else {
+                normalizer = (double)top * ln2 + log(sum) + log1p(1.0 / rest);
+                value = normalizer - target2 * ln2;
+            }
+            losses[row] = failed || target2 == INFINITY ? nan : (float)value;
+            normalizers[row] = failed ? (double)nan : normalizer;
+            loss = (double)losses[row];
         }
     }
     if (labels_out) return;
@@ -650,7 +662,7 @@ sp_status check_matrix(sp_context* ctx, const void* p, int64_t stride, uint32_t 
 }
 
 sp_status prepare(sp_label_head* h, const void* features, int64_t feature_stride, const void* weight,
-                  int64_t weight_stride, const void* targets, int wide, uint64_t n, float* losses, float* normalizers,
+                  int64_t weight_stride, const void* targets, int wide, uint64_t n, float* losses, double* normalizers,
                   void* gradient, int64_t gradient_stride, bool weight_needed, Operands* out) {
     sp_context* ctx = h->ctx;
     cudaStream_t st = ctx->stream;
@@ -731,10 +743,17 @@ sp_status check_targets(sp_context* ctx, const void* targets, sp_index index) {
     return SP_OK;
 }
 
+// Whether the few-row pass takes a call. Not a training head's loss: its gradient makes the logits again
+// in the other pass, and a confident row's slope is the small difference of the two passes' numbers, which
+// have to be rounded alike.
+bool few_rows(const sp_label_head* h, uint64_t n, const void* targets) {
+    return n <= kThinRows && !(targets && h->training);
+}
+
 // The pass over the logits shared by the loss and the prediction.
 sp_status run_stats(sp_label_head* h, const Operands& op, const void* weight, int64_t weight_stride,
                     const void* targets, int wide, uint64_t n, float scale,
-                    float* mean, float* losses, float* normalizers, int32_t* labels_out, float* log_probability) {
+                    float* mean, float* losses, double* normalizers, int32_t* labels_out, float* log_probability) {
     sp_context* ctx = h->ctx;
     GemmArgs a = common_args(h, targets, wide, scale);
     a.all_rows = op.all_rows;
@@ -743,7 +762,7 @@ sp_status run_stats(sp_label_head* h, const Operands& op, const void* weight, in
     a.partial_labels = labels_out ? h->partial_labels : nullptr;
     a.target_logits = h->target_logits;
     uint32_t slots = 0;
-    if (n <= kThinRows) {
+    if (few_rows(h, n, targets)) {
         ThinArgs thin;
         thin.weight = weight;
         thin.weight_stride = weight_stride;
@@ -859,7 +878,7 @@ void sp_label_head_destroy(sp_label_head* h) {
 
 sp_status sp_label_head_loss(sp_label_head* h, const void* d_features, int64_t feature_stride, const void* d_weight,
                              int64_t weight_stride, const void* d_targets, sp_index index, uint64_t rows,
-                             float logit_scale, float* d_mean, float* d_losses, float* d_log_normalizers) try {
+                             float logit_scale, float* d_mean, float* d_losses, double* d_log_normalizers) try {
     if (!h) return SP_ERR_INVALID;
     sp_context* ctx = h->ctx;
     NvtxRange range("sp_label_head_loss");
@@ -875,7 +894,7 @@ sp_status sp_label_head_loss(sp_label_head* h, const void* d_features, int64_t f
     Operands op;
     const int wide = index == SP_INDEX64;
     SP_CHECK(prepare(h, d_features, feature_stride, d_weight, weight_stride, d_targets, wide, rows, d_losses,
-                     d_log_normalizers, nullptr, 0, rows > kThinRows, &op));
+                     d_log_normalizers, nullptr, 0, !few_rows(h, rows, d_targets), &op));
     return run_stats(h, op, d_weight, weight_stride, d_targets, wide, rows, logit_scale, d_mean, d_losses, d_log_normalizers, nullptr, nullptr);
 } catch (...) {
     return SP_ERR_OUT_OF_MEMORY;
@@ -893,7 +912,7 @@ sp_status sp_label_head_predict(sp_label_head* h, const void* d_features, int64_
     SP_CHECK(select_device(ctx));
     Operands op;
     SP_CHECK(prepare(h, d_features, feature_stride, d_weight, weight_stride, nullptr, 0, rows, nullptr, nullptr,
-                     nullptr, 0, rows > kThinRows, &op));
+                     nullptr, 0, !few_rows(h, rows, nullptr), &op));
     return run_stats(h, op, d_weight, weight_stride, nullptr, 0, rows, logit_scale, nullptr, nullptr, nullptr, d_labels, d_log_probabilities);
 } catch (...) {
     return SP_ERR_OUT_OF_MEMORY;
@@ -901,7 +920,7 @@ sp_status sp_label_head_predict(sp_label_head* h, const void* d_features, int64_
 
 sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64_t feature_stride,
                                  const void* d_weight, int64_t weight_stride, const void* d_targets, sp_index index,
-                                 uint64_t rows, float logit_scale, const float* d_log_normalizers,
+                                 uint64_t rows, float logit_scale, const double* d_log_normalizers,
                                  const float* d_row_gradient, void* d_feature_gradient,
                                  int64_t feature_gradient_stride, void* d_weight_gradient,
                                  int64_t weight_gradient_stride) try {

@@ -242,18 +242,21 @@ __global__ void __launch_bounds__(thin_threads(DIRECT), 1)
             asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
             if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
         }
-        // The row's parts, in neighbouring lanes, as one.
+        // The row's parts, in neighbouring lanes, as one; of prediction's two largest logits the one that
+        // is not joins the sum.
         __syncwarp();
         for (uint32_t o = 1; o < (1u << split); o <<= 1) {
             const float base = __shfl_xor_sync(0xffffffffu, stats.base, o), sum = __shfl_xor_sync(0xffffffffu, stats.sum, o);
             const float largest = __shfl_xor_sync(0xffffffffu, stats.largest, o);
             const uint32_t label = __shfl_xor_sync(0xffffffffu, stats.label, o);
+            const bool other = largest > stats.largest || (largest == stats.largest && label < stats.label);
+            const float one = a.g.partial_labels ? 1.0f : 0.0f;
             const float top = fmaxf(stats.base, base), finite = top == -INFINITY ? 0.0f : top;
-            const float mine = stats.sum * exp2_fast(stats.base - finite), theirs = sum * exp2_fast(base - finite);
+            const float mine = (stats.sum + (other ? one : 0.0f)) * exp2_fast(stats.base - finite);
+            const float theirs = (sum + (other ? 0.0f : one)) * exp2_fast(base - finite);
             stats.sum = part & o ? theirs + mine : mine + theirs;
             stats.base = top;
-            if (largest > stats.largest || (largest == stats.largest && label < stats.label))
-                stats.largest = largest, stats.label = label;
+            if (other) stats.largest = largest, stats.label = label;
         }
         if (ok && live && part == 0) {
             const uint64_t slot = (uint64_t)blockIdx.x * a.g.partial_rows + row;

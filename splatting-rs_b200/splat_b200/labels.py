@@ -150,7 +150,7 @@ class Embedding(_Handle):
 @dataclass
 class LabelLoss:
     """`LabelHead.loss`: the mean over the rows with a target (a 0-d tensor), and per row the loss
-    and log sum exp of the logits (0 for a row without a target)."""
+    and, in float64, the log sum exp of the logits (0 for a row without a target)."""
 
     mean: object
     losses: object
@@ -178,7 +178,7 @@ class LabelHead(_Handle):
         rows = features.shape[0]
         targets_at, index = self._index(targets, "targets", rows)
         losses = features.new_empty(rows, dtype=self._torch.float32)
-        normalizers, mean = self._torch.empty_like(losses), losses.new_empty(())
+        normalizers, mean = losses.new_empty(rows, dtype=self._torch.float64), losses.new_empty(())
         self._call("sp_label_head_loss", *inputs, targets_at, index, rows, logit_scale, mean.data_ptr(),
                    losses.data_ptr(), normalizers.data_ptr())
         return LabelLoss(mean, losses, normalizers)
@@ -191,7 +191,7 @@ class LabelHead(_Handle):
         rows = features.shape[0]
         targets_at, index = self._index(targets, "targets", rows)
         float32 = self._torch.float32
-        normalizers_at = self._vector(log_normalizers, "log_normalizers", rows, float32)
+        normalizers_at = self._vector(log_normalizers, "log_normalizers", rows, self._torch.float64)
         row_at = None if row_gradient is None else self._vector(row_gradient, "row_gradient", rows, float32)
         if feature_gradient is None:
             feature_gradient = features.new_empty((rows, self.dim))

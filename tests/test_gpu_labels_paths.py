@@ -187,3 +187,35 @@ def test_the_example_learns_its_scene(dtype):
     assert abs(result["first_loss"] - 4.605) < 0.1
     assert result["last_loss"] < 0.5 * result["first_loss"]
     assert result["accuracy"] > 0.5
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,labels,dim", [(5, 20, 256), (300, 40, 300), (700, 900, 64), (3000, 30, 128)])
+def test_confident_rows_keep_their_small_losses_and_slopes(ctx, rows, labels, dim, dtype):
+    """Targets of probability close to 1: the loss and the slopes are what the other labels leave, and
+    keep their relative precision (f32: a few roundings of logits of size 20, exp makes them relative)."""
+    weight = matrix(labels, dim, dtype, 2)
+    weight /= weight.float().norm(dim=1, keepdim=True).to(dtype)
+    targets = tokens_for("all", rows, labels, torch.int32, 3)
+    features = (weight[targets.long()].float() + 0.05 * torch.randn(rows, dim, device="cuda") / dim**0.5).to(dtype)
+    scale = 20.0
+    exact = Bounds(features, weight, targets, scale)
+    p = torch.exp(-exact.losses)
+    assert (p > 0.9).float().mean() > 0.5
+    head = sb.LabelHead(ctx, labels, dim, dtype, rows)
+    loss = head.loss(features, weight, targets, scale)
+    # Each other label's share of the loss: exp of a difference of two logits.
+    products = 6 if dtype == torch.float32 else 1
+    each = 2 * A * 2 * (products * (dim / 16 + 1) + 4) * scale * (features.double().abs() @ weight.double().abs().T).amax(1)
+    each = each + 8 * A * 20 * 2 + 2.0**-20
+    close(loss.losses, exact.losses, exact.losses * each * 2)
+    to_features, to_weight = head.gradient(features, weight, targets, loss.log_normalizers, scale)
+    if dtype == torch.float32:
+        for got, want in ((to_features, exact.to_features), (to_weight, exact.to_weight)):
+            error = float((got.double() - want).norm() / want.norm())
+            assert error <= float(2 * each.max()), f"relative error {error:.1e}"
+    probe = sb.LabelHead(ctx, labels, dim, dtype, rows, training=False)
+    close(probe.loss(features, weight, targets, scale).losses, exact.losses, exact.losses * each * 2)
+    labels_found, log_probabilities = probe.predict(features, weight, scale)
+    assert torch.equal(labels_found, targets)
+    close(log_probabilities, -exact.losses, exact.losses * each * 2)
