@@ -193,13 +193,19 @@ class LabelHead(_Handle):
         float32 = self._torch.float32
         normalizers_at = self._vector(log_normalizers, "log_normalizers", rows, self._torch.float64)
         row_at = None if row_gradient is None else self._vector(row_gradient, "row_gradient", rows, float32)
+        # Fresh gradients are dense; only the caller's own are checked.
         if feature_gradient is None:
             feature_gradient = features.new_empty((rows, self.dim))
+            to_features = feature_gradient.data_ptr(), self.dim
+        else:
+            to_features = self._matrix(feature_gradient, self.dim, "feature_gradient", rows)
         if weight_gradient is None:
             weight_gradient = weight.new_empty((self.labels, self.dim))
+            to_weight = weight_gradient.data_ptr(), self.dim
+        else:
+            to_weight = self._matrix(weight_gradient, self.dim, "weight_gradient", self.labels)
         self._call("sp_label_head_gradient", *inputs, targets_at, index, rows, logit_scale, normalizers_at, row_at,
-                   *self._matrix(feature_gradient, self.dim, "feature_gradient", rows),
-                   *self._matrix(weight_gradient, self.dim, "weight_gradient", self.labels))
+                   *to_features, *to_weight)
         return feature_gradient, weight_gradient
 
     def predict(self, features, weight, logit_scale: float = 1.0):
