@@ -62,7 +62,10 @@ constexpr double kStepUs = 0.19;            // 64 of K of a 128 x 128 tile in a 
 constexpr double kPairCost = 1.4;           // of a 256 x 256 tile, in 128 x 128 tiles of one block
 constexpr int kSlotsAhead = 8;                // partials a thread has under way
 constexpr uint32_t kThreadSlots = 8;
-constexpr uint64_t kSlopeBudget = 5ull << 26;  // slope elements kept at once (640 MB)
+// Slope elements kept at once (1.25 GiB). More rows go in chunks; their weight's gradient is summed over
+// those, and a short last chunk fills few waves: 20,000 x 32,768 x 512 took 2036 us in chunks of a half
+// of this, 1970 in one piece.
+constexpr uint64_t kSlopeBudget = 5ull << 27;
 
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 

@@ -219,3 +219,33 @@ def test_confident_rows_keep_their_small_losses_and_slopes(ctx, rows, labels, di
     labels_found, log_probabilities = probe.predict(features, weight, scale)
     assert torch.equal(labels_found, targets)
     close(log_probabilities, -exact.losses, exact.losses * each * 2)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["all", "some", "none after row 200"])
+def test_gradient_of_more_slopes_than_the_workspace_holds(ctx, dtype, kind):
+    """Above 671 million slopes (f32: a third of that) the rows go in chunks, and the weight's gradient is
+    summed over them; a chunk without targets adds nothing."""
+    rows, labels, dim = (10_300, 70_000, 24) if dtype == torch.bfloat16 else (3700, 70_000, 24)
+    head = sb.LabelHead(ctx, labels, dim, dtype, rows)
+    features, weight = matrix(rows, dim, dtype, 1), matrix(labels, dim, dtype, 2)
+    targets = tokens_for("some" if kind == "some" else "all", rows, labels, torch.int64, 3)
+    if kind == "none after row 200":
+        targets[200:] = -1
+    loss = head.loss(features, weight, targets, 0.3)
+    to_features, to_weight = head.gradient(features, weight, targets, loss.log_normalizers, 0.3)
+    count = int(((targets >= 0) & (targets < labels)).sum())
+    want_weight = torch.zeros(labels, dim, dtype=torch.float64, device="cuda")
+    weight_error = torch.zeros_like(want_weight)
+    for first in range(0, rows, 1000):
+        part = slice(first, min(rows, first + 1000))
+        g = torch.full((part.stop - first,), 1.0 / count, device="cuda")
+        b = Bounds(features[part], weight, targets[part], 0.3, g)
+        want_weight += b.to_weight
+        weight_error += b.weight_error
+        close(loss.losses[part], b.losses, b.loss_error)
+        close(to_features[part], b.to_features, b.features_error)
+    close(to_weight, want_weight, weight_error * 1.1)  # the chunks' sums add f32 roundings
+    again = head.gradient(features, weight, targets, loss.log_normalizers, 0.3)
+    assert torch.equal(again[0], to_features) and torch.equal(again[1], to_weight)
+    head.check()
