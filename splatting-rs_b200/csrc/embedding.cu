@@ -11,7 +11,8 @@
 //  - more: the (token, position) pairs go through the renderer's stable radix sort (sort.cu), each
 //    block sums the runs of a fixed stretch of the sorted list while dOut's rows stream past once
 //    (bound by those bytes), and a token whose run crosses stretches is joined from their partial
-//    sums, in order, by a second kernel, which also writes the zero rows of the tokens nobody has.
+//    sums, in order, by a second kernel. The kernel that makes the pairs zeroes the gradient first,
+//    for the tokens nobody has.
 #include <algorithm>
 #include <new>
 
@@ -35,7 +36,6 @@ struct sp_embedding {
     uint32_t* values[2] = {nullptr, nullptr};
     uint32_t* histograms = nullptr;  // kSortMaxPasses * kSortRadix digit counts, then the tickets
     unsigned long long* lookback = nullptr;
-    uint2* ranges = nullptr;
     float* partials = nullptr;
 };
 
@@ -53,9 +53,9 @@ constexpr uint32_t kFewTokens = 32768;         // 32 warps x 32 x 32 lanes
 constexpr uint64_t kFewReads = 1ull << 24;     // token reads of all blocks together
 constexpr uint32_t kFewThreads = 1024, kMostOwned = 512, kLongRun = 64;
 
-// Sorted positions per group of threads, a power of two: long pieces make fewer partial sums (500,000
-// bf16 rows of 256: 109 us in pieces of 64, 101 us of 128), short ones give a small list groups enough
-// to fill the SMs.
+// Sorted positions per group of threads, a power of two: long pieces make fewer partial sums (the
+// gradient of 500,000 bf16 rows of 256: 102 us in pieces of 64, 94 us of 128), short ones give a small
+// list groups enough to fill the SMs.
 uint32_t piece_length(uint64_t count, int lanes_log2) {
     uint32_t piece = kShortPiece;
     while (piece < kLongPiece && count >= (uint64_t)piece * 2 * kGroups) piece *= 2;
@@ -112,11 +112,15 @@ __global__ void __launch_bounds__(kThreads) k_lookup(const T* __restrict__ table
 
 // The sort's input: key = token (entries for none, which sorts last), value = position, with every
 // pass's digit histogram; block 0 sets the sort's bookkeeping. The device status is left alone:
-// it stays raised until it is read.
+// it stays raised until it is read. The blocks also zero the gradient's `zero_rows` rows of `zero_units`
+// U each (dense rows are one), so that entries without tokens need no look at the sorted list.
+template <typename U>
 __global__ void __launch_bounds__(kThreads) k_emit_tokens(const void* __restrict__ tokens, int wide, uint32_t count,
                                                           uint64_t entries, int passes, DeviceMeta* meta,
                                                           uint32_t* __restrict__ keys, uint32_t* __restrict__ values,
-                                                          uint32_t* __restrict__ histograms) {
+                                                          uint32_t* __restrict__ histograms,
+                                                          U* __restrict__ zero, uint64_t zero_rows,
+                                                          uint64_t zero_units, int64_t zero_stride) {
     chain_enter();
     __shared__ uint32_t hist[4][kSortRadix];
     for (int p = 0; p < passes; ++p) hist[p][threadIdx.x] = 0;
@@ -127,6 +131,13 @@ __global__ void __launch_bounds__(kThreads) k_emit_tokens(const void* __restrict
         meta->key_base = 0;
         meta->passes = (uint32_t)passes;
         meta->first_buffer = 0;
+    }
+    const uint64_t thread = (uint64_t)blockIdx.x * kThreads + threadIdx.x, threads = (uint64_t)gridDim.x * kThreads;
+    if (zero_rows == 1) {
+        for (uint64_t i = thread; i < zero_units; i += threads) zero[i] = U{};
+    } else {
+        for (uint64_t row = thread / 32; row < zero_rows; row += threads / 32)
+            for (uint64_t i = lane_id(); i < zero_units; i += 32) zero[(int64_t)row * zero_stride + i] = U{};
     }
     __syncthreads();
     const uint32_t base = blockIdx.x * kThreads * kEmitItems;
@@ -177,7 +188,7 @@ __global__ void __launch_bounds__(kThreads)
     chain_enter();
     if (meta->status != 0) return;  // the list may be out of order: k_join_pieces writes NaN
     __shared__ uint32_t s_key[kMostStretch + 2];  // with the neighbours on both sides
-    __shared__ uint32_t s_position[kMostStretch];
+    __shared__ alignas(16) uint32_t s_position[kMostStretch];
     __shared__ float s_part[2][kThreads][N];
     constexpr uint32_t kNobody = 0xffffffffu;
     const uint32_t lanes = 1u << lanes_log2, groups = kThreads >> lanes_log2;
@@ -202,12 +213,34 @@ __global__ void __launch_bounds__(kThreads)
         for (int j = 0; j < N; ++j) acc[j] = 0.0f;
         uint32_t current = key[begin];
         bool from_before = key[(int)begin - 1] == current;
-        for (uint32_t i = begin; i < end; i += kPieceRows) {
-            Pack<T, N> v[kPieceRows];
+        // Rows of a batch that is whole and has tokens throughout (the list is sorted) need no tests.
+        auto load = [&](uint32_t i, Pack<T, N> (&v)[kPieceRows]) {
+            if (i + kPieceRows <= end && key[i + kPieceRows - 1] < entries) {
+                uint32_t at[kPieceRows];
 #pragma unroll
-            for (int k = 0; k < kPieceRows; ++k)
-                if (i + k < end && key[i + k] < entries)
-                    v[k] = load_pack<T, N>(upstream + (int64_t)s_position[i + k] * upstream_stride + column);
+                for (int k = 0; k < kPieceRows; k += 4) {
+                    const uint4 four = *reinterpret_cast<const uint4*>(s_position + i + k);
+                    at[k] = four.x, at[k + 1] = four.y, at[k + 2] = four.z, at[k + 3] = four.w;
+                }
+#pragma unroll
+                for (int k = 0; k < kPieceRows; ++k)
+                    v[k] = load_pack<T, N>(upstream + (int64_t)at[k] * upstream_stride + column);
+            } else {
+#pragma unroll
+                for (int k = 0; k < kPieceRows; ++k)
+                    if (i + k < end && key[i + k] < entries)
+                        v[k] = load_pack<T, N>(upstream + (int64_t)s_position[i + k] * upstream_stride + column);
+            }
+        };
+        auto add = [&](uint32_t i, const Pack<T, N> (&v)[kPieceRows]) {
+            if (i + kPieceRows <= end && key[i + kPieceRows - 1] == current) {
+                if (current >= entries) return;
+#pragma unroll
+                for (int k = 0; k < kPieceRows; ++k)
+#pragma unroll
+                    for (int j = 0; j < N; ++j) acc[j] += v[k].get(j);
+                return;
+            }
 #pragma unroll
             for (int k = 0; k < kPieceRows; ++k) {
                 if (i + k >= end) break;
@@ -229,6 +262,11 @@ __global__ void __launch_bounds__(kThreads)
                     for (int j = 0; j < N; ++j) acc[j] += v[k].get(j);
                 }
             }
+        };
+        for (uint32_t i = begin; i < end; i += kPieceRows) {
+            Pack<T, N> v[kPieceRows];
+            load(i, v);
+            add(i, v);
         }
         const bool goes_on = key[end] == current;
         if (from_before || goes_on) {
@@ -276,24 +314,26 @@ __global__ void __launch_bounds__(kThreads)
     if (tail) follow(group, 1, false);
 }
 
-// Per token: zeros where it has no rows, the ordered sum of its partials where its run crosses
-// stretches, nothing where k_sum_pieces wrote it. Up to kJoinTokens tokens a warp (one where there are
-// few, whose runs are long), 4 columns a lane; a token with more than kWarpParts partials is joined by
-// the block's eight warps together.
-constexpr uint32_t kJoinWarps = kThreads / 32, kJoinTokens = 8, kWarpParts = 16;
+// The runs that cross stretches: a warp looks whether one begins in its stretch and goes on, finds in
+// how many stretches (the sorted list's keys at their starts), and adds up their partial sums in order,
+// 4 columns a lane; a run with more than kWarpParts of them is joined by the block's eight warps
+// together. blockIdx.y takes every gridDim.y-th 128 columns. If the sort failed, NaN throughout.
+constexpr uint32_t kJoinWarps = kThreads / 32, kWarpParts = 16;
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    k_join_pieces(const uint2* __restrict__ ranges, uint32_t entries, uint32_t dim, float scale, T* __restrict__ out,
-                  int64_t out_stride, const float* __restrict__ partials, uint32_t partial_stride, uint32_t stretch,
-                  uint32_t tokens_per_warp, const DeviceMeta* __restrict__ meta) {
+    k_join_pieces(const uint32_t* __restrict__ keys, uint32_t count, uint32_t entries, uint32_t dim, float scale,
+                  T* __restrict__ out, int64_t out_stride, const float* __restrict__ partials, uint32_t partial_stride,
+                  uint32_t stretch, const DeviceMeta* __restrict__ meta) {
     chain_enter();
     __shared__ float4 shared[kJoinWarps][32];
-    __shared__ uint32_t long_tokens[kJoinWarps * kJoinTokens], longs;
-    if (threadIdx.x == 0) longs = 0;
-    __syncthreads();
+    __shared__ uint2 long_runs[kJoinWarps];  // the stretch it begins in, its partial sums
     const uint32_t warp = threadIdx.x / 32, lane = lane_id();
-    const uint32_t base = (blockIdx.x * kJoinWarps + warp) * tokens_per_warp;
-    const bool failed = meta->status != 0;
+    if (meta->status != 0) {
+        const uint64_t block = (uint64_t)blockIdx.y * gridDim.x + blockIdx.x, blocks = (uint64_t)gridDim.x * gridDim.y;
+        for (uint64_t row = block * kJoinWarps + warp; row < entries; row += blocks * kJoinWarps)
+            for (uint32_t c = lane; c < dim; c += 32) out[(int64_t)row * out_stride + c] = from_float<T>(__int_as_float(0x7fffffff));
+        return;
+    }
     auto store = [&](uint32_t v, uint32_t column, float4 sum) {
         const float s[4] = {sum.x, sum.y, sum.z, sum.w};
         T* to = out + (int64_t)v * out_stride + column;
@@ -301,9 +341,8 @@ __global__ void __launch_bounds__(kThreads)
         for (int j = 0; j < 4; ++j)
             if (column + j < dim) to[j] = from_float<T>(s[j] * scale);
     };
-    // Partials p0..p1 of the run over sorted positions `run`: slot 1 of its first stretch, then slot 0.
-    auto sum_of = [&](uint2 run, uint32_t p0, uint32_t p1, uint32_t column) {
-        const uint32_t first = run.x / stretch;
+    // Partial sums p0..p1 of the run that begins in stretch `first`: its slot 1, then the next ones' slot 0.
+    auto sum_of = [&](uint32_t first, uint32_t p0, uint32_t p1, uint32_t column) {
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
         for (uint32_t p = p0; p < p1; ++p) {
@@ -316,33 +355,43 @@ __global__ void __launch_bounds__(kThreads)
         }
         return sum;
     };
-    auto parts_of = [&](uint2 run) { return run.y > run.x ? (run.y - 1) / stretch - run.x / stretch + 1 : 0u; };
-    uint2 mine = make_uint2(0u, 0u);
-    const bool owns = lane < tokens_per_warp && base + lane < entries;
-    if (owns && !failed) mine = ranges[base + lane];
-    for (uint32_t left = __ballot_sync(0xffffffffu, owns && parts_of(mine) != 1); left; left &= left - 1) {
-        const uint32_t k = __ffs(left) - 1, token = base + k;
-        const uint2 run = make_uint2(__shfl_sync(0xffffffffu, mine.x, k), __shfl_sync(0xffffffffu, mine.y, k));
-        const uint32_t parts = parts_of(run);
-        if (parts == 0) {
-            const float fill = failed ? __int_as_float(0x7fffffff) : 0.0f;
-            for (uint32_t c = lane; c < dim; c += 32) out[(int64_t)token * out_stride + c] = from_float<T>(fill);
-        } else if (parts <= kWarpParts) {
-            for (uint32_t c = lane * 4; c < dim; c += 128) store(token, c, sum_of(run, 0, parts, c));
-        } else if (lane == 0) {
-            long_tokens[atomicAdd(&longs, 1u)] = token;
-        }
+    const uint32_t stretches = (count + stretch - 1) / stretch, mine = blockIdx.x * kJoinWarps + warp;
+    uint32_t token = 0, parts = 0;
+    if (mine + 1 < stretches) {
+        const uint64_t next = (uint64_t)(mine + 1) * stretch;
+        token = keys[next];
+        const bool begins = mine == 0 || keys[next - stretch - 1] != token;
+        if (token < entries && keys[next - 1] == token && begins) parts = 2;
     }
+    // How far it goes: the last of `found` stretches is one of the run's; those from `end` on are not.
+    // (The same in all of a warp's lanes.)
+    if (parts != 0) {
+        uint32_t found = mine + 1, end = stretches, step = 1;
+        while (end - found > 1) {
+            const uint64_t at = (uint64_t)found + (uint64_t)(lane + 1) * step;
+            const bool in = at < end && keys[at * stretch] == token;
+            const uint32_t many = __popc(__ballot_sync(0xffffffffu, in));  // the list is sorted: the first lanes
+            const uint64_t beyond = (uint64_t)found + (uint64_t)(many + 1) * step;
+            found += many * step;
+            if (many < 32) end = (uint32_t)min((uint64_t)end, beyond);
+            step = max((end - found) / 32, 1u);
+        }
+        parts = found - mine + 1;
+    }
+    if (lane == 0) long_runs[warp] = make_uint2(mine, parts > kWarpParts ? parts : 0u);
+    const uint32_t first_column = blockIdx.y * 128 + lane * 4, step = gridDim.y * 128;
+    if (parts != 0 && parts <= kWarpParts)
+        for (uint32_t c = first_column; c < dim; c += step) store(token, c, sum_of(mine, 0, parts, c));
     __syncthreads();
-    for (uint32_t k = 0; k < longs; ++k) {
-        const uint32_t token = long_tokens[k];
-        const uint2 run = ranges[token];
-        const uint32_t n = parts_of(run);
+    for (uint32_t k = 0; k < kJoinWarps; ++k) {
+        const uint32_t first = long_runs[k].x, n = long_runs[k].y;
+        if (n == 0) continue;
         const uint32_t p0 = (uint32_t)((uint64_t)n * warp / kJoinWarps);
         const uint32_t p1 = (uint32_t)((uint64_t)n * (warp + 1) / kJoinWarps);
-        for (uint32_t c0 = 0; c0 < dim; c0 += 128) {
+        const uint32_t long_token = keys[(uint64_t)(first + 1) * stretch];
+        for (uint32_t c0 = blockIdx.y * 128; c0 < dim; c0 += step) {
             const uint32_t c = c0 + lane * 4;
-            if (c < dim) shared[warp][lane] = sum_of(run, p0, p1, c);
+            if (c < dim) shared[warp][lane] = sum_of(first, p0, p1, c);
             __syncthreads();
             if (warp == 0 && c < dim) {
                 float4 sum = shared[0][lane];
@@ -353,7 +402,7 @@ __global__ void __launch_bounds__(kThreads)
                     sum.z += v.z;
                     sum.w += v.w;
                 }
-                store(token, c, sum);
+                store(long_token, c, sum);
             }
             __syncthreads();
         }
@@ -635,7 +684,6 @@ sp_status sp_embedding_create(sp_context* ctx, uint64_t entries, uint32_t dim, s
         SP_CHECK(allocate(e, &e->histograms, kSortMaxPasses * kSortRadix + kSortMaxPasses));
         const uint64_t partitions = (max_tokens + kSortShortPartition - 1) / kSortShortPartition;
         SP_CHECK(allocate(e, &e->lookback, partitions * kSortRadix));
-        SP_CHECK(allocate(e, &e->ranges, entries));
         SP_CHECK(allocate(e, &e->partials, stretches * 2 * partial_stride_of(dim)));
         // The look-back words carry the pass's sequence number: zero is no pass's.
         SP_CUDA(ctx, cudaMemsetAsync(e->lookback, 0, partitions * kSortRadix * sizeof(unsigned long long), ctx->stream));
@@ -745,39 +793,44 @@ sp_status sp_embedding_gradient(sp_embedding* e, const void* d_out_gradient, int
     const uint32_t piece = piece_length(count, lanes_log2), partial_stride = partial_stride_of(e->dim);
     uint32_t* tickets = e->histograms + kSortMaxPasses * kSortRadix;
     SP_CUDA(ctx, cudaMemsetAsync(e->histograms, 0, (kSortMaxPasses * kSortRadix + kSortMaxPasses) * sizeof(uint32_t), st));
-    SP_CUDA(ctx, launch_chained(k_emit_tokens, std::max(1u, grid_for(count, kThreads * kEmitItems)), kThreads, 0, st,
-                                d_tokens, wide, n, e->entries, e->plan.passes, e->meta, e->keys[0], e->values[0],
-                                e->histograms));
+    // The gradient's rows as 16-byte units where they are whole ones, 4-byte or 2-byte ones otherwise.
+    const bool dense = table_gradient_stride == (int64_t)e->dim;
+    const uint64_t zero_rows = dense ? 1 : e->entries, zero_bytes = (dense ? e->entries : 1) * e->dim * size;
+    const uint64_t alignment = reinterpret_cast<uintptr_t>(d_table_gradient) | zero_bytes |
+                               (dense ? 0 : (uint64_t)table_gradient_stride * size);
+    const unsigned emit_grid = std::max(grid_for(count, kThreads * kEmitItems),
+                                        (unsigned)std::min<uint64_t>(148 * 8, zero_rows * zero_bytes / (kThreads * 256)));
+#define SPLAT_EMIT(U)                                                                                                  \
+    SP_CUDA(ctx, launch_chained(k_emit_tokens<U>, emit_grid, kThreads, 0, st, d_tokens, wide, n, e->entries,          \
+                                e->plan.passes, e->meta, e->keys[0], e->values[0], e->histograms,                     \
+                                static_cast<U*>(d_table_gradient), zero_rows, zero_bytes / sizeof(U),                  \
+                                (int64_t)(table_gradient_stride * size / sizeof(U))))
+    if (alignment % 16 == 0) SPLAT_EMIT(uint4);
+    else if (alignment % 4 == 0) SPLAT_EMIT(uint32_t);
+    else SPLAT_EMIT(uint16_t);
+#undef SPLAT_EMIT
     const uint32_t partitions = (n + kSortShortPartition - 1) / kSortShortPartition;
-    for (int pass = 0; pass < e->plan.passes && n > 0; ++pass)
+    for (int pass = 0; pass < e->plan.passes; ++pass)
         SP_CUDA(ctx, launch_sort_pass(e->plan, pass, ++e->sequence, e->keys[0], e->values[0], e->keys[1], e->values[1],
                                       e->histograms, tickets, e->lookback, partitions, e->meta, st));
     const uint32_t* keys = e->keys[e->plan.passes & 1];
     const uint32_t* positions = e->values[e->plan.passes & 1];
-    SP_CUDA(ctx, launch_ranges(e->plan, keys, e->meta, std::max<uint64_t>(count, e->entries / 4), e->ranges,
-                               (uint32_t)e->entries, st));
-    if (n > 0) {
 #define SPLAT_PIECES(T, N) sum_pieces<T, N>(e, keys, positions, n, r, partial_stride, piece, lanes_log2)
-        SPLAT_ROWS(SPLAT_PIECES);
+    SPLAT_ROWS(SPLAT_PIECES);
 #undef SPLAT_PIECES
-        SP_CUDA(ctx, err);
-    }
 #undef SPLAT_ROWS
+    SP_CUDA(ctx, err);
     const uint32_t stretch = (kThreads >> lanes_log2) * piece;
-    const uint32_t tokens_per_warp = e->entries >= 148 * kJoinWarps * kJoinTokens ? kJoinTokens : 1;
-    const unsigned join_grid = grid_for(e->entries, kJoinWarps * tokens_per_warp);
-    if (e->element == SP_F32)
-        SP_CUDA(ctx, launch_chained(k_join_pieces<float>, join_grid, kThreads, 0, st,
-                                    static_cast<const uint2*>(e->ranges), (uint32_t)e->entries, e->dim, scale,
-                                    static_cast<float*>(d_table_gradient), table_gradient_stride,
-                                    static_cast<const float*>(e->partials), partial_stride, stretch,
-                                    tokens_per_warp, static_cast<const DeviceMeta*>(e->meta)));
-    else
-        SP_CUDA(ctx, launch_chained(k_join_pieces<bf16>, join_grid, kThreads, 0, st,
-                                    static_cast<const uint2*>(e->ranges), (uint32_t)e->entries, e->dim, scale,
-                                    static_cast<bf16*>(d_table_gradient), table_gradient_stride,
-                                    static_cast<const float*>(e->partials), partial_stride, stretch,
-                                    tokens_per_warp, static_cast<const DeviceMeta*>(e->meta)));
+    const unsigned join_blocks = grid_for((n + stretch - 1) / stretch, kJoinWarps);
+    const dim3 join_grid(join_blocks, std::max(1u, std::min((e->dim + 127) / 128, 148 * 4 / join_blocks)));
+#define SPLAT_JOIN(T)                                                                                                 \
+    SP_CUDA(ctx, launch_chained(k_join_pieces<T>, join_grid, kThreads, 0, st, keys, n, (uint32_t)e->entries, e->dim,  \
+                                scale, static_cast<T*>(d_table_gradient), table_gradient_stride,                      \
+                                static_cast<const float*>(e->partials), partial_stride, stretch,                      \
+                                static_cast<const DeviceMeta*>(e->meta)))
+    if (e->element == SP_F32) SPLAT_JOIN(float);
+    else SPLAT_JOIN(bf16);
+#undef SPLAT_JOIN
     return SP_OK;
 } catch (...) {
     return SP_ERR_OUT_OF_MEMORY;

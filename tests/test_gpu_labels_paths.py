@@ -249,3 +249,41 @@ def test_gradient_of_more_slopes_than_the_workspace_holds(ctx, dtype, kind):
     again = head.gradient(features, weight, targets, loss.log_normalizers, 0.3)
     assert torch.equal(again[0], to_features) and torch.equal(again[1], to_weight)
     head.check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,pad,shift", [(45, 0, 0), (45, 3, 1), (64, 0, 1), (64, 8, 0), (6, 2, 2), (300, 4, 0)])
+def test_embedding_gradient_writes_every_row_and_nothing_else(ctx, dim, pad, shift, dtype):
+    """The sorted list's way: rows of zeros for entries without tokens, in 16-byte, 4-byte and 2-byte
+    units, dense or not; what lies between the rows and around them stays."""
+    n, entries = 40_000, 999
+    e = sb.Embedding(ctx, entries, dim, dtype, n)
+    upstream, tokens = matrix(n, dim, dtype, 3), tokens_for("some", n, entries, torch.int32, 4)
+    tokens[(tokens > 300) & (tokens < 700)] = -1  # a gap, and ones at both ends
+    tokens[(tokens < 5) | (tokens > 990)] = 9
+    whole = torch.full((shift + entries * (dim + pad) + 8,), -7.0, dtype=dtype, device="cuda")
+    out = whole[shift:shift + entries * (dim + pad)].view(entries, dim + pad)[:, :dim]
+    want, bound = gradient_bound(upstream, tokens, entries, 0.5)
+    close(e.gradient(upstream, tokens, 0.5, out=out), want, bound)
+    assert out[301:700].count_nonzero() == 0 and out[:5].count_nonzero() == 0 and out[991:].count_nonzero() == 0
+    out.zero_()
+    assert (whole == -7).sum() == whole.numel() - entries * dim, "wrote outside its rows"
+    e.check()
+
+
+@pytest.mark.parametrize("n", [40_000, 75_000, 400_000])
+def test_embedding_gradient_of_runs_over_many_stretches(ctx, n):
+    """One token for nearly all rows, at the list's begin, middle or end, and runs that begin and end at
+    the stretches' borders."""
+    entries, dim = 64, 24
+    e = sb.Embedding(ctx, entries, dim, torch.float32, n)
+    upstream = matrix(n, dim, torch.float32, 5)
+    place = torch.arange(n, device="cuda")
+    cases = [torch.full((n,), v, device="cuda") for v in (0, 31, 63)]
+    cases += [place // length % entries for length in (512, 1024, 2048, 4096)]
+    cases += [torch.where(place < k, 3, 40) for k in (1, 2047, 2048, 2049, n - 1)]
+    cases += [torch.where(place < n // 2, 7, -1), torch.full((n,), -1, device="cuda")]
+    for tokens in cases:
+        want, bound = gradient_bound(upstream, tokens, entries, 1.0)
+        close(e.gradient(upstream, tokens), want, bound)
+    e.check()
