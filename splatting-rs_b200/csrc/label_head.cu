@@ -710,6 +710,9 @@ sp_status prepare(sp_label_head* h, const void* features, int64_t feature_stride
     return SP_OK;
 }
 
+// The scale of logits that took `additions`, in powers of 2.
+float scale2_for(float scale, uint32_t additions) { return (float)(scale * 1.4426950408889634 * given_back(additions)); }
+
 GemmArgs common_args(const sp_label_head* h, const void* targets, int wide, float scale) {
     GemmArgs a;
     std::memset(&a, 0, sizeof(a));
@@ -721,7 +724,7 @@ GemmArgs common_args(const sp_label_head* h, const void* targets, int wide, floa
     a.chunk_rows = 0x80000000u;
     a.splits = 1;
     a.scale = scale;
-    a.scale2 = scale * 1.44269504088896341f;
+    a.scale2 = scale2_for(scale, (h->dim + 15) / 16);
     a.targets = targets;
     a.wide = wide;
     return a;
@@ -782,6 +785,7 @@ sp_status run_stats(sp_label_head* h, const Operands& op, const void* weight, in
         const uint32_t blocks = std::min(thin.tiles, h->sms);
         a.partial_rows = kThinRows;
         slots = blocks;
+        a.scale2 = scale2_for(scale, ((h->dim + 15) / 16 + 1) / 2);  // two accumulators
         thin.g = a;
         const cudaError_t err = h->element == SP_F32                 ? launch_thin<float, false>(h, blocks, op, thin)
                                 : direct                             ? launch_thin<bf16, true>(h, blocks, op, thin)
