@@ -555,11 +555,17 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                     const double exact_shift = a.log_normalizers[original] * -1.4426950408889634;
                     shift = (float)exact_shift;
                     shift_low = (float)(exact_shift - (double)shift);
-                    weight = a.scale * (a.row_gradient ? a.row_gradient[original] : 1.0f / (float)count);
+                    weight = a.row_gradient ? a.scale * a.row_gradient[original] : 1.0f;
                 }
             }
-            // bf16 gradients lose more than this in their last rounding.
-            const float correction = ENDING == kOut ? (float)given_back((w.k1 - w.k0) * (kBlockK / 16)) : 1.0f;
+            // The mean's factor comes after the sums: the target's slope p - 1, by far the largest, is then near
+            // -1 and loses little where it is rounded to bf16 (the factor in it, all rows' lost the same up to
+            // 2^-9, which adds up in dW). bf16 gradients lose more than the truncation in their last rounding.
+            float factor = 1.0f;
+            if (ENDING == kOut) {
+                if (!a.row_gradient) factor = a.scale / (float)max(count, 1u);
+                if (sizeof(T) == 4) factor *= (float)given_back((w.k1 - w.k0) * (kBlockK / 16));
+            }
             for (uint32_t n = w.n0; (ok || ENDING == kOut) && n < w.n1; ++n) {
                 if (!empty_sum && ok) {
                     ok = __all_sync(0xffffffffu, tc::barrier_wait(done + 8 * buffer, buffer_phase));
@@ -654,10 +660,6 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                             tc::tmem_load_wait();
                             if (c + 32 == kSpan) drain();
                         }
-                        if (sizeof(T) == 4) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] *= correction;
-                        }
                         if (poisoned || !ok) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] = __int_as_float(0x7fffffff);
@@ -667,6 +669,8 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                             const uint32_t columns = a.dim - column;
                             if (sizeof(T) == 2 && w.which == 0 && w.k0 == 0)
                                 add_scaled(v, residual, a.weight + (int64_t)target * a.weight_stride + column, columns);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] *= factor;
                             if (o.partial) {
                                 float* to = static_cast<float*>(o.out) + ((uint64_t)w.split * o.rows + row) * (uint64_t)o.stride +
                                             column;
