@@ -80,7 +80,10 @@ struct GemmArgs {
     const uint32_t* row_of;
     uint32_t all_rows;     // not 0: that many rows, all of them count and are read in place
     uint32_t labels, dim;
-    uint32_t products;     // 1, or kPartProducts
+    uint32_t products;     // 1, or more for operands in parts: those of the p-th product are the p-th hex
+    uint32_t parts_a, parts_b;  // digits of these
+    uint32_t slope_parts;  // kSlopes
+    uint32_t only_weight;  // kOut: so many first products are dW's alone
     uint32_t k_blocks;     // kStats, kSlopes: of the features' columns
     uint32_t n_tiles;      // kStats, kSlopes: of the labels
     uint32_t splits;       // ... and the pieces they are cut into
@@ -452,9 +455,8 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                 const int am = (int)(w.m * kSide + rank * kTile), first_row = (int)a.first_row;
                 for (uint32_t n = w.n0; ok && n < w.n1; ++n) {
                     const int bn = (int)(n * kSide + rank * kTile);
-                    for (uint32_t p = 0; ok && p < a.products; ++p) {
-                        const int za = a.products == 1 ? 0 : (int)((kPartsOfA >> (4 * p)) & 15u);
-                        const int zb = a.products == 1 ? 0 : (int)((kPartsOfB >> (4 * p)) & 15u);
+                    for (uint32_t p = ENDING == kOut && w.which == 0 ? a.only_weight : 0; ok && p < a.products; ++p) {
+                        const int za = (int)((a.parts_a >> (4 * p)) & 15u), zb = (int)((a.parts_b >> (4 * p)) & 15u);
                         for (uint32_t k = w.k0; k < w.k1; ++k) {
                             if (!(ok = tc::barrier_wait(empty + 8 * stage, phase ^ 1))) break;
                             // Both blocks' copies count on the first one's barrier.
@@ -493,7 +495,7 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
             uint32_t stage = 0, phase = 0, buffer = 0, buffer_phase = 0;
             for (uint32_t item = first_item; ok && item < schedule.items; item += item_step) {
                 const Work w = schedule.at(a, item);
-                const uint32_t steps = (w.k1 - w.k0) * a.products;
+                const uint32_t steps = (w.k1 - w.k0) * (a.products - (ENDING == kOut && w.which == 0 ? a.only_weight : 0));
                 if (steps == 0) continue;
                 // Which operands run along K in memory: W in dH; G and H in dW. 16 of K are 32 bytes along
                 // a row, or 16 rows of 128 bytes.
@@ -594,7 +596,7 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                             __syncwarp();
                             if (lane == 0) tc::store_box(&map_slopes, stage_tile, 0, (int)row, (int)(p * a.panels + (columns_at + c) / 64));
                         };
-                        if constexpr (sizeof(T) == 2) {
+                        if (sizeof(T) == 2 && (PAIR || a.slope_parts == 1)) {
 #pragma unroll
                             for (int q = 0; q < 2; ++q) {
                                 float v[32];
@@ -614,7 +616,7 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                                 }
                             }
                             store(0);
-                        } else {
+                        } else if constexpr (sizeof(T) == 4 || !PAIR) {
                             float v[2][32], unused;
                             __syncwarp();
                             tc::tmem_load32(accumulator + c, v[0]);
@@ -625,11 +627,18 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                             for (int q = 0; q < 2; ++q)
                                 to_slopes<true>(v[q], columns_at + c + 32 * q, a.labels, a.scale2, shift, weight, target, live,
                                           shift_low, unused);
-                            for (int p = 0; p < (int)kParts; ++p) {
+                            for (int p = 0; p < (int)a.slope_parts; ++p) {
                                 reclaim();
                                 stage_part(stage_tile, lane, 0, v[0]);
                                 stage_part(stage_tile, lane, 1, v[1]);
                                 store(p);
+                                if (sizeof(T) == 2 && p == 0 && target - columns_at - c < 64) {
+                                    float left = 0.0f;
+#pragma unroll
+                                    for (int j = 0; j < 64; ++j)
+                                        if (target - columns_at - c == (uint32_t)j) left = v[j / 32][j % 32];
+                                    a.residuals[row] = left;
+                                }
                             }
                         }
                     }

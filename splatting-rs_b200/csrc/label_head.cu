@@ -44,6 +44,11 @@ struct sp_label_head {
 
     uint32_t parts() const { return element == SP_F32 ? kParts : 1; }
     uint32_t products() const { return element == SP_F32 ? kPartProducts : 1; }
+    // Parts of the slopes: f32's three, and two for bf16 operands where the rows are few. One rounding to
+    // bf16 is then as much of the weight's gradient as its own last one (2.4e-3 of its norm in all, 1.7e-3 with
+    // two parts), and two parts cost the gradient of 128 x 65,536 x 512 13 of 88 us. With more rows a label's
+    // sums average it out, and a second part would double the bytes and half of the products.
+    uint32_t slope_parts(uint64_t rows) const { return element == SP_F32 ? kParts : rows <= kTile ? 2 : 1; }
     uint64_t packed_stride() const { return ((uint64_t)dim + kBlockK - 1) / kBlockK * kBlockK; }
     uint64_t count_blocks() const { return (max_rows + 63) / 64; }
     uint64_t slope_stride() const { return (labels + kPairTile - 1) / kPairTile * kPairTile; }
@@ -498,7 +503,7 @@ uint32_t tiles_of(uint64_t n, bool pair) { return (uint32_t)((n + (pair ? kPairT
 Plan plan_logits(uint32_t sms, uint64_t rows, uint64_t labels) {
     Plan best{};
     double best_cost = 1e300;
-    for (int pair = 0; pair < 2; ++pair) {
+    for (int pair = 0; pair < (rows <= kTile ? 1 : 2); ++pair) {  // no pair for half a pair's tile
         const uint32_t workers = pair ? std::max(sms / 2, 1u) : sms;
         const uint32_t m = tiles_of(rows, pair), n = tiles_of(labels, pair);
         for (uint32_t s = 1; s <= n && (s == 1 || (uint64_t)m * s <= (uint64_t)kLogitWaves * workers); ++s) {
@@ -721,6 +726,8 @@ GemmArgs common_args(const sp_label_head* h, const void* targets, int wide, floa
     a.labels = (uint32_t)h->labels;
     a.dim = h->dim;
     a.products = h->products();
+    a.parts_a = h->element == SP_F32 ? kPartsOfA : 0;
+    a.parts_b = h->element == SP_F32 ? kPartsOfB : 0;
     a.chunk_rows = 0x80000000u;
     a.splits = 1;
     a.scale = scale;
@@ -952,12 +959,13 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
     SP_CHECK(prepare(h, d_features, feature_stride, d_weight, weight_stride, d_targets, wide, rows, nullptr, nullptr,
                      d_feature_gradient, feature_gradient_stride, true, &op));
 
-    const uint64_t chunk = chunk_for(h, rows), chunks = (rows + chunk - 1) / chunk;
+    const uint32_t slope_parts = h->slope_parts(rows);
+    const uint64_t chunk = slope_parts == 2 ? kTile : chunk_for(h, rows), chunks = (rows + chunk - 1) / chunk;
     const uint64_t sum_stride = sums_stride(h);
     CUtensorMap slopes, slopes_out;
     const uint32_t panels = (uint32_t)(h->slope_stride() / 64);
-    SP_CHECK(make_map(ctx, &slopes, h->slopes, 64, chunk, 64, panels * h->parts(), chunk * 64));
-    SP_CHECK(make_map(ctx, &slopes_out, h->slopes, 64, chunk, 64, panels * h->parts(), chunk * 64, 32));
+    SP_CHECK(make_map(ctx, &slopes, h->slopes, 64, chunk, 64, panels * slope_parts, chunk * 64));
+    SP_CHECK(make_map(ctx, &slopes_out, h->slopes, 64, chunk, 64, panels * slope_parts, chunk * 64, 32));
     // One cut of the weight's gradient for every chunk: its pieces' sums go on from one to the next.
     const OutPlan first = plan_out(h->sms, std::min(chunk, rows), h->labels, h->dim, h->parts(), chunks > 1);
     const bool weight_sums = first.weight > 1 || chunks > 1;
@@ -982,6 +990,7 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
         a.log_normalizers = d_log_normalizers;
         a.row_gradient = d_row_gradient;
         a.panels = panels;
+        a.slope_parts = slope_parts;
         a.residuals = h->target_logits;  // free in a gradient
         const bool weight_here = in_place(h, d_weight, weight_stride);
         a.weight = weight_here ? static_cast<const bf16*>(d_weight) : h->packed_weight;
@@ -989,6 +998,7 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
         SP_CUDA(ctx, h->element == SP_F32 ? (run_gemm<kSlopes, float>(h, logits.pair, logits.items(), op, slopes_out, a))
                                           : (run_gemm<kSlopes, bf16>(h, logits.pair, logits.items(), op, slopes_out, a)));
 
+        if (slope_parts == 2) a.products = 2, a.only_weight = 1, a.parts_a = 0x01;  // the small part first
         OutArgs& f = a.out[0];
         f.n_tiles = plan.n;
         f.splits = plan.features;

@@ -287,3 +287,24 @@ def test_embedding_gradient_of_runs_over_many_stretches(ctx, n):
         want, bound = gradient_bound(upstream, tokens, entries, 1.0)
         close(e.gradient(upstream, tokens), want, bound)
     e.check()
+
+
+@pytest.mark.parametrize("rows,labels,dim", [(1, 700, 40), (2, 21, 242), (15, 1186, 33), (90, 5117, 156), (128, 398, 64)])
+def test_bf16_weight_gradient_of_few_rows_is_rounded_once(ctx, rows, labels, dim):
+    """Each value is within half a unit in the last place (8 bits) of its exact sum, give or take 2^-15 of
+    the sum's terms: a slope in two parts is off by 2^-17, and by as much again where its logit is (logits up
+    to 16, f32 sums over at most 256 columns, exponentials to 2^-21). One rounding of the slopes to bf16 would
+    be 2^-9 of the terms."""
+    head = sb.LabelHead(ctx, labels, dim, torch.bfloat16, rows)
+    features, weight = matrix(rows, dim, torch.bfloat16, 1), matrix(labels, dim, torch.bfloat16, 2)
+    targets = tokens_for("all", rows, labels, torch.int64, 3)
+    loss = head.loss(features, weight, targets, 0.2)
+    _, to_weight = head.gradient(features, weight, targets, loss.log_normalizers, 0.2)
+    h, w = features.double(), weight.double()
+    logits = 0.2 * h @ w.T
+    assert logits.abs().max() < 16
+    slopes = torch.softmax(logits, 1)
+    slopes[torch.arange(rows), targets] -= 1
+    want, terms = 0.2 / rows * slopes.T @ h, 0.2 / rows * slopes.T.abs() @ h.abs()
+    half = torch.ldexp(torch.ones_like(want), torch.frexp(want).exponent - 9)
+    assert (((to_weight.double() - want).abs() - half) <= 2.0**-15 * terms).all()
