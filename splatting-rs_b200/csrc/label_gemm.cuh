@@ -418,7 +418,12 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
     uint8_t* generic_base = smem_raw + (smem - tc::smem_address(smem_raw));
     const uint32_t warp = threadIdx.x / 32, lane = lane_id();
     const uint32_t rank = PAIR ? tc::cluster_rank() : 0;
-    const uint32_t first_item = blockIdx.x / kBlocks, item_step = gridDim.x / kBlocks;
+    // Workers take the items round by round. The output gradients', the long ones first, go in turns from
+    // either end, so that the workers with one long item more have a short one less.
+    auto item_of = [](uint32_t round) {
+        const uint32_t worker = blockIdx.x / kBlocks, workers = gridDim.x / kBlocks;
+        return round * workers + (ENDING == kOut && round % 2 ? workers - 1 - worker : worker);
+    };
 
     if (warp == 0 && lane == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -450,8 +455,8 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
         if (tc::elect_one()) {
             const CUtensorMap* features = packed ? &map_features_packed : &map_features;
             uint32_t stage = 0, phase = 0;
-            for (uint32_t item = first_item; ok && item < schedule.items; item += item_step) {
-                const Work w = schedule.at(a, item);
+            for (uint32_t round = 0; ok && item_of(round) < schedule.items; ++round) {
+                const Work w = schedule.at(a, item_of(round));
                 const int am = (int)(w.m * kSide + rank * kTile), first_row = (int)a.first_row;
                 for (uint32_t n = w.n0; ok && n < w.n1; ++n) {
                     const int bn = (int)(n * kSide + rank * kTile);
@@ -493,8 +498,8 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
     } else if (warp == 1) {
         if (rank == 0 && tc::elect_one()) {
             uint32_t stage = 0, phase = 0, buffer = 0, buffer_phase = 0;
-            for (uint32_t item = first_item; ok && item < schedule.items; item += item_step) {
-                const Work w = schedule.at(a, item);
+            for (uint32_t round = 0; ok && item_of(round) < schedule.items; ++round) {
+                const Work w = schedule.at(a, item_of(round));
                 const uint32_t steps = (w.k1 - w.k0) * (a.products - (ENDING == kOut && w.which == 0 ? a.only_weight : 0));
                 if (steps == 0) continue;
                 // Which operands run along K in memory: W in dH; G and H in dW. 16 of K are 32 bytes along
@@ -534,8 +539,8 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
         uint32_t buffer = 0, buffer_phase = 0;
         // Output gradients of a call that gave up, here or in a kernel before, are NaN.
         const bool poisoned = ENDING == kOut && a.rows->status != 0;
-        for (uint32_t item = first_item; (ok || ENDING == kOut) && item < schedule.items; item += item_step) {
-            const Work w = schedule.at(a, item);
+        for (uint32_t round = 0; (ok || ENDING == kOut) && item_of(round) < schedule.items; ++round) {
+            const Work w = schedule.at(a, item_of(round));
             const bool empty_sum = w.k0 == w.k1;
             const OutArgs& o = a.out[w.which];
             if (ENDING == kOut && empty_sum && o.add) continue;
