@@ -1,11 +1,12 @@
 // The label head (splat_labels.h): cross entropy of features against a vocabulary of label rows,
 // its gradient, and prediction, without ever storing the logits.
 //
-//   loss      z = c H W^T in tiles; per row the running maximum m and sum s of 2^((z - m) log2 e);
-//             the tiles' (m, s) are joined: log sum exp z = m + ln s, loss = that - z[target]
-//   gradient  the logits again in tiles, turned into slopes G = c g (exp(z - logsumexp) - [target])
+//   loss      z = c H W^T in tiles; per row the sum s of 2^(z log2 e - base) over all labels but the
+//             target, base following the largest; the tiles' (base, s) are joined, and with the target's
+//             z: loss = log1p(s 2^base / e^z[target]), log sum exp z = z[target] + loss
+//   gradient  the logits again in tiles, turned into slopes G = exp(z - logsumexp) - [target]
 //             where they are made and written as bf16 parts for a chunk of rows; then
-//             dH = G W and dW = G^T H, the same tile pipeline (label_gemm.cuh)
+//             dH = c g G W and dW = c g G^T H, the same tile pipeline (label_gemm.cuh)
 //   predict   the loss's pass with the maximum's label kept
 //
 // Rows without a target are left out of every product: their indices are compacted first, and

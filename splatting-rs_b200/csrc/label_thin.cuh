@@ -4,6 +4,10 @@
 // copies where it is aligned for them, else (f32, odd strides) by sixteen warps that split it into
 // its bf16 parts on the way into shared memory.
 //
+// One bf16 row against 65,536 labels of 512 takes 20 us, 67 MB at 3.3 TB/s: four tiles a block at most, so the
+// first copies' latency and the last tile's sums are a good part. 60 f32 rows against 20,011 labels of 768 take 36
+// us for 62 MB: bound by the blocks' conversion and the shared memory that it and the products share.
+//
 // f32 parts of the rows lie one below the other, so that one product of a weight part covers all the
 // rows' parts it meets: accumulator groups hi hi | hi mid + mid hi | hi lo + mid mid + lo hi. Grouped
 // by size, and hi hi by even and odd steps of K, they also lose less to the tensor cores' truncating
