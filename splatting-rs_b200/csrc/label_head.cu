@@ -787,7 +787,7 @@ sp_status run_stats(sp_label_head* h, const Operands& op, const void* weight, in
         // Whole rounds of tiles over the SMs; converted weights come in tiles of the height that fills
         // the last round too.
         const bool direct = in_place(h, weight, weight_stride);
-        const uint64_t rounds = (tiles_of(h->labels, false) + h->sms - 1) / h->sms;
+        const uint64_t round = (uint64_t)(direct ? kTile : kConvertTile) * h->sms, rounds = (h->labels + round - 1) / round;
         thin.tile = direct ? kTile : (uint32_t)round_up((h->labels + rounds * h->sms - 1) / (rounds * h->sms), 8);
         thin.tiles = (uint32_t)((h->labels + thin.tile - 1) / thin.tile);
         const uint32_t blocks = std::min(thin.tiles, h->sms);

@@ -1,12 +1,13 @@
 // The logits' pass for at most kThinRows rows, where the weight's bytes are what it costs: the roles
 // of label_gemm.cuh swapped (128 labels on the accumulator's lanes, the rows its columns), so that
 // the products are no wider than the rows, and the weight read once and in place: bf16 by tiled bulk
-// copies where it is aligned for them, else (f32, odd strides) by sixteen warps that split it into
+// copies where it is aligned for them, else (f32, odd strides) by 24 warps that split it into
 // its bf16 parts on the way into shared memory.
 //
 // One bf16 row against 65,536 labels of 512 takes 20 us, 67 MB at 3.3 TB/s: four tiles a block at most, so the
-// first copies' latency and the last tile's sums are a good part. 60 f32 rows against 20,011 labels of 768 take 36
-// us for 62 MB: bound by the blocks' conversion and the shared memory that it and the products share.
+// first copies' latency and the last tile's sums are a good part. 60 f32 rows against 20,011 labels of 768 take 32
+// us for 62 MB: bound by the instructions of the conversion and its hand-over from stage to stage (without the
+// loads it takes 25).
 //
 // f32 parts of the rows lie one below the other, so that one product of a weight part covers all the
 // rows' parts it meets: accumulator groups hi hi | hi mid + mid hi | hi lo + mid mid + lo hi. Grouped
@@ -20,7 +21,9 @@ namespace splat {
 namespace label {
 
 constexpr int kThinRows = 64;
-constexpr int kConvertWarps = 16;
+constexpr int kConvertWarps = 24;
+constexpr uint32_t kConvertTile = kConvertWarps * 4;  // labels of a converted tile, at most: eight threads a row
+constexpr int kConvertAhead = 5;                      // steps whose loads a thread has under way
 constexpr int thin_threads(bool direct) { return direct ? 256 : 256 + kConvertWarps * 32; }
 constexpr int kThinStagesF32 = 2, kThinStagesBf16 = 6;
 constexpr uint32_t kRowsBytes = kThinRows * kBlockK * 2;
@@ -39,7 +42,7 @@ struct ThinArgs {
     int64_t weight_stride;
     uint32_t dim;
     int vector;          // 16-byte loads are aligned
-    uint32_t tile;       // labels per tile: kTile, or for converted weights a multiple of 8
+    uint32_t tile;       // labels per tile: kTile, or for converted weights a multiple of 8 up to kConvertTile
     uint32_t known_rows; // not 0: the rows' count, known before the launch that gathers them is done
     uint32_t columns;    // of the accumulators: the rows, rounded up to 16
     uint32_t tiles;
@@ -268,59 +271,54 @@ __global__ void __launch_bounds__(thin_threads(DIRECT), 1)
             if (a.g.partial_labels) a.g.partial_labels[slot] = stats.label;
         }
     } else if (warp >= 8 && !DIRECT) {
-        // Eight lanes a row of 64 columns, 64 rows a turn; the next two steps' loads are under way.
-        constexpr int kTurnRows = kConvertWarps * 4, kTurns = kTile / kTurnRows;
-        const uint32_t t = threadIdx.x - 256, unit = t % 8, first_row = t / 8;
+        // Eight lanes a row of 64 columns, a tile a turn; the next steps' loads are under way: 60 rows, 20,011
+        // labels, 768 columns take 38 us with gather and join, 39 with three steps', 45 with seven (more code
+        // than the instruction caches like); 41 with sixteen warps, two turns and two steps'.
+        const uint32_t t = threadIdx.x - 256, unit = t % 8, in_tile = t / 8;
         const T* weight = static_cast<const T*>(a.weight);
-        RawEight<T> raw[2][kTurns];
+        RawEight<T> raw[kConvertAhead];
         const uint32_t mine = blockIdx.x < tiles ? (tiles - 1 - blockIdx.x) / gridDim.x + 1 : 0;  // tiles
         const uint32_t steps = mine * a.g.k_blocks;
         uint32_t load_tile = blockIdx.x, load_k = 0;
-        auto load_next = [&](RawEight<T> (&to)[kTurns]) {
-            const uint32_t column = load_k * kBlockK + unit * 8;
+        auto load_next = [&](RawEight<T>& to) {
+            const uint32_t column = load_k * kBlockK + unit * 8, label = load_tile * a.tile + in_tile;
             const uint32_t columns = column < a.dim ? a.dim - column : 0;
-#pragma unroll
-            for (int r = 0; r < kTurns; ++r) {
-                const uint32_t in_tile = r * kTurnRows + first_row, label = load_tile * a.tile + in_tile;
-                const bool there = in_tile < a.tile && label < a.g.labels && load_tile < tiles;
-                to[r].load(weight + (there ? (int64_t)label * a.weight_stride + column : 0), there ? columns : 0, a.vector);
-            }
+            const bool there = in_tile < a.tile && label < a.g.labels && load_tile < tiles;
+            to.load(weight + (there ? (int64_t)label * a.weight_stride + column : 0), there ? columns : 0, a.vector);
             if (++load_k == a.g.k_blocks) load_k = 0, load_tile += gridDim.x;
         };
-        auto convert = [&](RawEight<T> (&from)[kTurns], uint32_t to) {
+        auto convert = [&](const RawEight<T>& from, uint32_t to) {
+            if (in_tile >= a.tile) return;  // those accumulator lanes are not read
+            float v[8];
+            constexpr int N = RawEight<T>::N;
 #pragma unroll
-            for (int r = 0; r < kTurns; ++r) {
-                if (r * kTurnRows + first_row >= a.tile) break;  // those accumulator lanes are not read
-                float v[8];
-                constexpr int N = RawEight<T>::N;
+            for (int j = 0; j < 8; ++j) v[j] = from.p[j / N].get(j % N);
+            const uint32_t at = to + in_tile * 128 + ((unit ^ (in_tile & 7u)) * 16);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = from[r].p[j / N].get(j % N);
-                const uint32_t row = r * kTurnRows + first_row, at = to + row * 128 + ((unit ^ (row & 7u)) * 16);
+            for (int p = 0; p < kParted; ++p) {
+                Pack<bf16, 8> o;
+                o.set(v);
 #pragma unroll
-                for (int p = 0; p < kParted; ++p) {
-                    Pack<bf16, 8> o;
-                    o.set(v);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] -= o.get(j);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + p * kOperandBytes), "r"(o.word.x),
-                                 "r"(o.word.y), "r"(o.word.z), "r"(o.word.w)
-                                 : "memory");
-                }
+                for (int j = 0; j < 8; ++j) v[j] -= o.get(j);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + p * kOperandBytes), "r"(o.word.x),
+                             "r"(o.word.y), "r"(o.word.z), "r"(o.word.w)
+                             : "memory");
             }
         };
-        if (steps > 0) load_next(raw[0]);
-        if (steps > 1) load_next(raw[1]);
-        uint32_t stage = 0, phase = 0;
-        for (uint32_t s = 0; s < steps; s += 2) {
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < kConvertAhead; ++b)
+            if ((uint32_t)b < steps) load_next(raw[b]);
+        uint32_t stage = 0, phase = 0;
+        for (uint32_t s = 0; s < steps; s += kConvertAhead) {
+#pragma unroll
+            for (int b = 0; b < kConvertAhead; ++b) {
                 if (s + b >= steps || !ok) break;
                 if (!(ok = tc::barrier_wait(empty + 8 * stage, phase ^ 1))) break;
                 convert(raw[b], smem + stage * kBytes);
                 tc::fence_async_shared();
                 __syncwarp();
                 if (lane == 0) tc::barrier_arrive_cluster(full + 8 * stage);
-                if (s + b + 2 < steps) load_next(raw[b]);
+                if (s + b + kConvertAhead < steps) load_next(raw[b]);
                 if (++stage == kRing) stage = 0, phase ^= 1;
             }
             if (!ok) break;
