@@ -56,8 +56,9 @@ sp_status sp_embedding_check(sp_embedding* e);
 
 /* Logits z[i][v] = logit_scale * <features[i], weight[v]> over `labels` labels, never stored: the
  * products run in tiles on the tensor cores, and each tile is reduced (or turned into its gradient)
- * where it was made. f32 operands are split into three bf16 parts each and their six largest
- * partial products are summed, which keeps f32 accuracy. `max_rows` bounds the rows of one call
+ * where it was made. f32 operands are split into three bf16 parts each (24 bits for
+ * magnitudes from 2^-110 on, any finite or infinite value) and their six largest partial products are
+ * summed; an infinite feature that meets an infinite weight gives NaN. `max_rows` bounds the rows of one call
  * (below 2^31 - 512); `training` != 0 also reserves the gradient's workspace. */
 typedef struct sp_label_head sp_label_head;
 sp_status sp_label_head_create(sp_context* ctx, uint64_t labels, uint32_t dim, sp_element element, uint64_t max_rows,

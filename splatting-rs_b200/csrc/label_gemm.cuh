@@ -40,6 +40,25 @@ constexpr uint32_t kStoreBytes = 32 * 128;  // a warp's 32 x 64 slopes on their 
 constexpr uint32_t kParts = 3, kPartProducts = 6;
 constexpr uint32_t kPartsOfA = 0x001012, kPartsOfB = 0x010210;
 
+// The next part of eight f32 operands, what it leaves stays in v: the upper 16 bits, then those of the rest,
+// then (`last`) the other 8 bits, exact to 24 bits in all for magnitudes from 2^-110 on. Truncated, not rounded:
+// no part of a finite value is infinite, and all have its sign, so that no two products of one pair of values
+// overflow in opposite directions. The products left out are then 6e-8 of a logit (rounded parts: 6e-9), a
+// third of what the sums lose. An infinite value is infinite in its last part alone, which meets only the other
+// operand's first: against a part of 0 it would make NaN.
+__device__ __forceinline__ Pack<bf16, 8> take_part(float (&v)[8], bool last) {
+    Pack<bf16, 8> o;
+    uint32_t* two = reinterpret_cast<uint32_t*>(&o.word);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (last) asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(two[j]) : "f"(v[2 * j + 1]), "f"(v[2 * j]));
+        else asm("cvt.rz.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(two[j]) : "f"(v[2 * j + 1]), "f"(v[2 * j]));
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] -= o.get(j);
+    return o;
+}
+
 // The rows that have a target, in order: row_of[i] is the i-th one's row. Where `packed`, the
 // features were copied to the workspace in that order; else every row counts and they are read
 // in place.

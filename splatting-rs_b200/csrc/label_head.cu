@@ -120,8 +120,7 @@ __device__ __forceinline__ uint32_t block_sum(uint32_t v) {
     return sum;
 }
 
-// Eight columns of a row as bf16 parts: f32 is hi + mid + lo with each part the rounding of what
-// the earlier ones left (24 bits in all), bf16 is copied.
+// Eight columns of a row as bf16 parts: f32 in three (take_part), bf16 is copied.
 template <typename T>
 __device__ __forceinline__ void copy_parts(const T* from, uint32_t columns, bool vector, bf16* to, uint64_t part) {
     float v[8];
@@ -139,13 +138,7 @@ __device__ __forceinline__ void copy_parts(const T* from, uint32_t columns, bool
     }
     constexpr int parts = sizeof(T) == 4 ? (int)kParts : 1;
 #pragma unroll
-    for (int p = 0; p < parts; ++p) {
-        Pack<bf16, 8> o;
-        o.set(v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] -= o.get(j);
-        store_pack(to + p * part, o);
-    }
+    for (int p = 0; p < parts; ++p) store_pack(to + p * part, take_part(v, p == parts - 1));
 }
 
 // The weight's copy as bf16 parts, where it cannot be read in place (`from` NULL: it can).

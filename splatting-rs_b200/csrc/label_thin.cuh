@@ -296,10 +296,7 @@ __global__ void __launch_bounds__(thin_threads(DIRECT), 1)
             const uint32_t at = to + in_tile * 128 + ((unit ^ (in_tile & 7u)) * 16);
 #pragma unroll
             for (int p = 0; p < kParted; ++p) {
-                Pack<bf16, 8> o;
-                o.set(v);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] -= o.get(j);
+                const Pack<bf16, 8> o = take_part(v, p == kParted - 1);
                 asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + p * kOperandBytes), "r"(o.word.x),
                              "r"(o.word.y), "r"(o.word.z), "r"(o.word.w)
                              : "memory");
