@@ -68,7 +68,9 @@ void sp_label_head_destroy(sp_label_head* h);
  * log_normalizers[i] = log sum_v exp z[i][v] (f64: a confident row's slope is the small difference of
  * its target's logit and this); *mean = the mean over the rows with a target (0 when
  * there is none). A row without a target is skipped, whatever its features hold: 0 in both
- * outputs. logit_scale > 0 and finite. */
+ * outputs. A label whose logit is -inf, or as low as the element type goes, has probability 0 beside
+ * others; a row with a logit of NaN or +inf, or with all of them -inf, gets NaN. logit_scale > 0 and
+ * finite. */
 sp_status sp_label_head_loss(sp_label_head* h, const void* d_features, int64_t feature_stride, const void* d_weight,
                              int64_t weight_stride, const void* d_targets, sp_index index, uint64_t rows,
                              float logit_scale, float* d_mean, float* d_losses, double* d_log_normalizers);
@@ -83,7 +85,8 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
                                  const float* d_row_gradient, void* d_feature_gradient,
                                  int64_t feature_gradient_stride, void* d_weight_gradient,
                                  int64_t weight_gradient_stride);
-/* Each row's most probable label (the lowest of equal ones) and its log-probability. */
+/* Each row's most probable label (the lowest of equal ones) and its log-probability, NaN where the loss
+ * is. */
 sp_status sp_label_head_predict(sp_label_head* h, const void* d_features, int64_t feature_stride,
                                 const void* d_weight, int64_t weight_stride, uint64_t rows, float logit_scale,
                                 int32_t* d_labels, float* d_log_probabilities);

@@ -117,7 +117,7 @@ struct GemmArgs {
     const void* targets;
     int wide;
     // kStats
-    float2* partials;      // [Shape::column_parts * splits][partial_rows]: base (prediction: largest logit) and sum
+    float2* partials;      // [Shape::column_parts * splits][partial_rows]: base and sum
     uint32_t* partial_labels;  // the maximum's label, or NULL
     uint64_t partial_rows;
     float* target_logits;
@@ -214,15 +214,28 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
-// A row's running softmax: sum of 2^(z scale2 - base) over its logits z so far, without the one that
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return d;
+}
+
+// A row's running softmax: sum of 2^((z - base) scale2) over its logits z so far, without the one that
 // matters: the target's for the loss, the largest for prediction. What is left of 1 after its probability
-// is then known to full precision however near 1 that is. The loss takes any base that keeps the sum in
-// range; prediction's is that of the largest logit.
+// is then known to full precision however near 1 that is. The loss takes any logit as base that keeps the sum
+// in range; prediction's is the largest. The difference comes before the scale: 2^(z scale2 - base scale2) in
+// one operation is off by a whole rounding of base scale2 in the exponent, which passes f32's range at logits
+// of 2^31 (the type's lowest values, as masks), and so does base scale2 itself near the largest.
 constexpr float kLargestSum = 18446744073709551616.0f;  // 2^64
 struct RowStats {
     float base, sum, target_logit, largest;
     uint32_t label;
 };
+
+// base, or for one of -inf (no logits so far, or none above it) any that counts those as 0.
+__device__ __forceinline__ float finite_base(float base) { return base == -INFINITY ? 0.0f : base; }
 
 template <int W>
 __device__ __forceinline__ float largest_of(const float (&v)[W]) {
@@ -232,14 +245,14 @@ __device__ __forceinline__ float largest_of(const float (&v)[W]) {
     return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
-// sum of 2^(v scale2 - base): packed multiply-adds and sums around the exponentials, four sums.
+// sum of 2^((v - base) scale2): packed operations around the exponentials, four sums.
 template <int W>
 __device__ __forceinline__ float sum_exp2(const float (&v)[W], float scale2, float base) {
-    const float2 s2 = make_float2(scale2, scale2), b2 = make_float2(-base, -base);
+    const float2 s2 = make_float2(scale2, scale2), below = make_float2(-base, -base);
     float2 t[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
     for (int j = 0; j < W; j += 2) {
-        const float2 x = fma2(make_float2(v[j], v[j + 1]), s2, b2);
+        const float2 x = mul2(add2(make_float2(v[j], v[j + 1]), below), s2);
         t[(j / 2) & 1] = add2(t[(j / 2) & 1], make_float2(exp2_fast(x.x), exp2_fast(x.y)));
     }
     t[0] = add2(t[0], t[1]);
@@ -263,10 +276,8 @@ __device__ __forceinline__ void add_logits(RowStats& s, float (&v)[W], uint32_t 
         const float m = largest_of(v);
         if (m > s.largest) {
             // The one that was the largest joins the others (exp2(-inf) = 0 where there was none).
-            const float base = __fmul_rn(m, scale2);
-            s.sum = (s.sum + 1.0f) * exp2_fast(s.base - base);
-            s.base = base;
-            s.largest = m;
+            s.sum = (s.sum + 1.0f) * exp2_fast((s.base - m) * scale2);
+            s.base = s.largest = m;
             uint32_t place = 0;
 #pragma unroll
             for (int j = W - 1; j >= 0; --j)
@@ -276,8 +287,7 @@ __device__ __forceinline__ void add_logits(RowStats& s, float (&v)[W], uint32_t 
                 if (place == (uint32_t)j) v[j] = -INFINITY;
             s.label = first + place;
         }
-        // Nothing but -inf so far: any finite base counts that as 0.
-        s.sum += sum_exp2(v, scale2, s.base == -INFINITY ? 0.0f : s.base);
+        s.sum += sum_exp2(v, scale2, finite_base(s.base));
         return;
     }
     if (near) {
@@ -291,15 +301,15 @@ __device__ __forceinline__ void add_logits(RowStats& s, float (&v)[W], uint32_t 
     }
     if (s.base == -INFINITY) {
         const float m = largest_of(v);
-        if (m != -INFINITY) s.base = __fmul_rn(m, scale2);  // NaN stays NaN
+        if (m != -INFINITY) s.base = m;  // NaN stays NaN
     }
-    float base = s.base == -INFINITY ? 0.0f : s.base, sum;
+    float base = finite_base(s.base), sum;
     for (;;) {
         sum = s.sum + sum_exp2(v, scale2, base);
         if (sum <= kLargestSum) break;
-        const float higher = fmaxf(base, __fmul_rn(largest_of(v), scale2));
+        const float higher = fmaxf(base, largest_of(v));
         if (!(higher > base)) break;  // the sum of many, an infinite logit, or NaN
-        s.sum *= exp2_fast(base - higher);
+        s.sum *= exp2_fast((base - higher) * scale2);
         base = s.base = higher;
     }
     s.sum = sum;
@@ -307,10 +317,11 @@ __device__ __forceinline__ void add_logits(RowStats& s, float (&v)[W], uint32_t 
 
 // The slopes of 32 logits of a row, in place (the target's only if PLACE); zeros past the labels and in rows that do not count. The
 // target's, if it is among them, also in `target_slope`: p - 1 from the difference of its logit and the
-// normalizer, -(shift + shift_low) to twice f32's precision, since p itself may round to 1.
+// normalizer, since p itself may round to 1. The normalizer over the scale is `normalizer`, to f32's precision,
+// less shift_low / scale2.
 template <bool PLACE>
-__device__ __forceinline__ void to_slopes(float (&v)[32], uint32_t first, uint32_t labels, float scale2, float shift,
-                                          float weight, uint32_t target, bool live, float shift_low, float& target_slope) {
+__device__ __forceinline__ void to_slopes(float (&v)[32], uint32_t first, uint32_t labels, float scale2,
+                                          float normalizer, float weight, uint32_t target, bool live, float shift_low, float& target_slope) {
     const uint32_t at = target - first;
     const bool near = __any_sync(0xffffffffu, at < 32);
     float logit = 0.0f;
@@ -321,12 +332,13 @@ __device__ __forceinline__ void to_slopes(float (&v)[32], uint32_t first, uint32
     }
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
-        const float2 x = fma2(make_float2(v[j], v[j + 1]), make_float2(scale2, scale2), make_float2(shift, shift));
+        const float2 x = fma2(add2(make_float2(v[j], v[j + 1]), make_float2(-normalizer, -normalizer)),
+                              make_float2(scale2, scale2), make_float2(shift_low, shift_low));
         v[j] = exp2_fast(x.x);
         v[j + 1] = exp2_fast(x.y);
     }
     if (near) {
-        const float slope = expm1f((fmaf(logit, scale2, shift) + shift_low) * 0.693147181f);
+        const float slope = expm1f(fmaf(logit - normalizer, scale2, shift_low) * 0.693147181f);
         if (at < 32) target_slope = slope * weight;
         if (PLACE) {
 #pragma unroll
@@ -574,7 +586,7 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
             const bool live = compact < count;
             RowStats stats{-INFINITY, 0.0f, 0.0f, -INFINITY, 0u};
             uint32_t target = kNoTarget;
-            float shift = 0.0f, shift_low = 0.0f, weight = 0.0f;
+            float normalizer = 0.0f, shift_low = 0.0f, weight = 0.0f;
             float residual = 0.0f;
             if (ENDING == kOut && sizeof(T) == 2 && live && w.which == 0) {
                 target = (uint32_t)index_at(a.targets, a.wide, a.row_of[compact], a.labels);
@@ -584,9 +596,9 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                 const uint32_t original = a.all_rows ? compact : a.row_of[compact];
                 if (a.targets) target = (uint32_t)index_at(a.targets, a.wide, original, a.labels);
                 if (ENDING == kSlopes) {
-                    const double exact_shift = a.log_normalizers[original] * -1.4426950408889634;
-                    shift = (float)exact_shift;
-                    shift_low = (float)(exact_shift - (double)shift);
+                    const double exact = a.log_normalizers[original] * 1.4426950408889634 / a.scale2;
+                    normalizer = (float)exact;
+                    shift_low = (float)(((double)normalizer - exact) * a.scale2);
                     weight = a.row_gradient ? a.scale * a.row_gradient[original] : 1.0f;
                 }
             }
@@ -636,7 +648,7 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                                 if (q == 1 && c + 64 == kSpan) drain();
                                 const uint32_t column = columns_at + c + 32 * q;
                                 float slope = 0.0f;
-                                to_slopes<false>(v, column, a.labels, a.scale2, shift, weight, target, live, shift_low, slope);
+                                to_slopes<false>(v, column, a.labels, a.scale2, normalizer, weight, target, live, shift_low, slope);
                                 if (q == 0) reclaim();
                                 stage_part(stage_tile, lane, q, v);
                                 if (target - column < 32) {
@@ -655,7 +667,7 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                             if (c + 64 == kSpan) drain();
 #pragma unroll
                             for (int q = 0; q < 2; ++q)
-                                to_slopes<true>(v[q], columns_at + c + 32 * q, a.labels, a.scale2, shift, weight, target, live,
+                                to_slopes<true>(v[q], columns_at + c + 32 * q, a.labels, a.scale2, normalizer, weight, target, live,
                                           shift_low, unused);
                             for (int p = 0; p < (int)a.slope_parts; ++p) {
                                 reclaim();
@@ -726,7 +738,7 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
             }
             if (ENDING == kStats && ok && live) {
                 const uint64_t slot = (uint64_t)(w.split * S::column_parts + part) * a.partial_rows + row;
-                a.partials[slot] = make_float2(a.partial_labels ? stats.largest : stats.base, stats.sum);
+                a.partials[slot] = make_float2(stats.base, stats.sum);
                 if (a.partial_labels) a.partial_labels[slot] = stats.label;
                 // The target is in exactly one thread's columns.
                 if (target != kNoTarget && target / kSide >= w.n0 && target / kSide < w.n1 &&

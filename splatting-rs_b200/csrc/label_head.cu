@@ -1,9 +1,9 @@
 // The label head (splat_labels.h): cross entropy of features against a vocabulary of label rows,
 // its gradient, and prediction, without ever storing the logits.
 //
-//   loss      z = c H W^T in tiles; per row the sum s of 2^(z log2 e - base) over all labels but the
-//             target, base following the largest; the tiles' (base, s) are joined, and with the target's
-//             z: loss = log1p(s 2^base / e^z[target]), log sum exp z = z[target] + loss
+//   loss      z = c H W^T in tiles; per row the sum s of e^(z - base) over all labels but the target, base
+//             following the largest; the tiles' (base, s) are joined, and with the target's
+//             z: loss = log1p(s e^base / e^z[target]), log sum exp z = z[target] + loss
 //   gradient  the logits again in tiles, turned into slopes G = exp(z - logsumexp) - [target]
 //             where they are made and written as bf16 parts for a chunk of rows; then
 //             dH = c g G W and dW = c g G^T H, the same tile pipeline (label_gemm.cuh)
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kThreads)
 
 // ------------------------------------------------------------------ joining
 
-// LANES threads (1, 8 or 32) join a row's partial sums, each in units of 2^base: the highest base
+// LANES threads (1, 8 or 32) join a row's partial sums, each in units of its base's exponential: the highest base
 // (and the largest logit with the lowest label) first, then the sum, in double, since a part may come
 // close to f32's largest. With the rest, the sum without the target's logit (the largest's), in units of
 // the latter's exponential, the loss (the negative log-probability) is log1p(rest): nothing cancels. The
@@ -282,8 +282,8 @@ __global__ void __launch_bounds__(kThreads)
     float top = -INFINITY, largest = -INFINITY;
     uint32_t label = 0xffffffffu;
     double sum = 0.0;
-    // Prediction: each part's largest goes into the sum here, and the row's out of it again (a 1 in units
-    // of 2^top, to double's precision).
+    // Prediction: each part's largest goes into the sum here, and the row's out of it again (a 1, to double's
+    // precision).
     const double one = partial_labels ? 1.0 : 0.0;
     for (uint32_t s0 = lane; s0 < mine; s0 += LANES * kSlotsAhead) {
         float2 p[kSlotsAhead];
@@ -299,15 +299,14 @@ __global__ void __launch_bounds__(kThreads)
         for (int k = 0; k < kSlotsAhead; ++k) {
             if (partial_labels) {
                 if (p[k].x > largest || (p[k].x == largest && l[k] < label)) largest = p[k].x, label = l[k];
-                p[k].x = __fmul_rn(p[k].x, scale2);
             }
             top = fmaxf(top, p[k].x);
         }
-        const float finite = top == -INFINITY ? 0.0f : top;
-        sum *= (double)exp2f(before - finite);
+        const float finite = finite_base(top);
+        sum *= (double)exp2f((before - finite) * scale2);
 #pragma unroll
         for (int k = 0; k < kSlotsAhead; ++k)
-            if (s0 + k * LANES < mine) sum += ((double)p[k].y + one) * (double)exp2f(p[k].x - finite);
+            if (s0 + k * LANES < mine) sum += ((double)p[k].y + one) * (double)exp2f((p[k].x - finite) * scale2);
     }
     float highest = top;
 #pragma unroll
@@ -317,8 +316,8 @@ __global__ void __launch_bounds__(kThreads)
         const uint32_t l = __shfl_xor_sync(0xffffffffu, label, o);
         if (x > largest || (x == largest && l < label)) largest = x, label = l;
     }
-    if (highest == -INFINITY) highest = 0.0f;
-    sum *= (double)exp2f(top - highest);
+    highest = finite_base(highest);
+    sum *= (double)exp2f((top - highest) * scale2);
     top = highest;
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -330,18 +329,21 @@ __global__ void __launch_bounds__(kThreads)
             // An infinite largest logit has no softmax.
             log_probability[row] = failed || !(fabsf(largest) < INFINITY) ? nan : (float)-log1p(sum - 1.0);
         } else {
-            const double target2 = (double)target_logits[i] * scale2;
-            const double rest = sum == 0.0 ? 0.0 : sum * exp2((double)top - target2);
+            const double target = target_logits[i], unit = (double)scale2 * ln2;
+            const double rest = sum == 0.0 ? 0.0 : sum * exp2(((double)top - target) * scale2);
             double value, normalizer;
             if (rest <= 1.0) {
                 value = log1p(rest);
-                normalizer = target2 * ln2 + value;
+                normalizer = target * unit + value;
             } else {
-                normalizer = (double)top * ln2 + log(sum) + log1p(1.0 / rest);
-                value = normalizer - target2 * ln2;
+                const double others = log(sum) + log1p(1.0 / rest);
+                normalizer = (double)top * unit + others;
+                value = ((double)top - target) * unit + others;
             }
-            losses[row] = failed || target2 == INFINITY ? nan : (float)value;
-            normalizers[row] = failed ? (double)nan : normalizer;
+            // No softmax: the target's logit is infinite, or all are -inf.
+            if (failed || target == INFINITY || (target == -INFINITY && sum == 0.0)) value = normalizer = nan;
+            losses[row] = (float)value;
+            normalizers[row] = normalizer;
             loss = (double)losses[row];
         }
     }

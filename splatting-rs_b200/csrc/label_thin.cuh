@@ -258,16 +258,16 @@ __global__ void __launch_bounds__(thin_threads(DIRECT), 1)
             const uint32_t label = __shfl_xor_sync(0xffffffffu, stats.label, o);
             const bool other = largest > stats.largest || (largest == stats.largest && label < stats.label);
             const float one = a.g.partial_labels ? 1.0f : 0.0f;
-            const float top = fmaxf(stats.base, base), finite = top == -INFINITY ? 0.0f : top;
-            const float mine = (stats.sum + (other ? one : 0.0f)) * exp2_fast(stats.base - finite);
-            const float theirs = (sum + (other ? 0.0f : one)) * exp2_fast(base - finite);
+            const float top = fmaxf(stats.base, base), finite = finite_base(top);
+            const float mine = (stats.sum + (other ? one : 0.0f)) * exp2_fast((stats.base - finite) * a.g.scale2);
+            const float theirs = (sum + (other ? 0.0f : one)) * exp2_fast((base - finite) * a.g.scale2);
             stats.sum = part & o ? theirs + mine : mine + theirs;
             stats.base = top;
             if (other) stats.largest = largest, stats.label = label;
         }
         if (ok && live && part == 0) {
             const uint64_t slot = (uint64_t)blockIdx.x * a.g.partial_rows + row;
-            a.g.partials[slot] = make_float2(a.g.partial_labels ? stats.largest : stats.base, stats.sum);
+            a.g.partials[slot] = make_float2(stats.base, stats.sum);
             if (a.g.partial_labels) a.g.partial_labels[slot] = stats.label;
         }
     } else if (warp >= 8 && !DIRECT) {

@@ -78,3 +78,81 @@ def test_f32_operands_up_to_the_largest_value(ctx, rows, training, which):
     _, log_probabilities = head.predict(features, weight, scale)
     close(log_probabilities, b.z.amax(1) - b.normalizers, 2 * b.z_error + b.exp_error + 4 * A * b.normalizers.abs())
     head.check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,training", PASSES)
+@pytest.mark.parametrize("scale", [1.0, 0.3, 0.45, 0.05, 7.0])
+def test_blocks_of_labels_out_of_use(ctx, rows, training, scale, dtype):
+    """Every label that a thread sees first, or last, is out of use: whatever the scale makes of the type's
+    lowest value (in units of 2 it may pass f32's range, or be off by a rounding of 1e31)."""
+    labels, dim = 700, 32
+    off = torch.cat([torch.arange(0, 70), torch.arange(256, 400), torch.arange(600, 700)]).cuda()
+    features, weight, targets, kept, _ = labels_out_of_use(rows, labels, dim, dtype, off, torch.finfo(dtype).min, 1.0)
+    b = Bounds(features, weight[kept], torch.searchsorted(kept, targets), scale)
+    head = sb.LabelHead(ctx, labels, dim, dtype, rows, training=training)
+    loss = head.loss(features, weight, targets, scale)
+    close(loss.losses, b.losses, b.loss_error)
+    if training:
+        to_features, to_weight = head.gradient(features, weight, targets, loss.log_normalizers, scale)
+        assert to_weight[off].count_nonzero() == 0
+        close(to_weight[kept], b.to_weight, b.weight_error)
+        close(to_features, b.to_features, b.features_error)
+    best = b.z.amax(1)
+    got, log_probabilities = head.predict(features, weight, scale)
+    close(log_probabilities, best - b.normalizers, 2 * b.z_error + b.exp_error + 4 * A * b.normalizers.abs())
+    assert torch.isin(got, kept.int()).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,training", PASSES)
+@pytest.mark.parametrize("scale", [1.0, 0.3, 0.45])
+@pytest.mark.parametrize("logit", [1e6, -1e6, 3e9, -3e9, 1e30, "lowest", "largest"])
+def test_equal_logits_of_any_size(ctx, rows, training, scale, logit, dtype):
+    """All labels' logits are one value, up to the type's lowest (every label out of use): the loss is ln
+    labels and the slopes are 1 / labels, as far as the normalizer in 64 bits still tells them apart."""
+    labels, dim = 500, 40
+    ends = {"lowest": torch.finfo(dtype).min, "largest": torch.finfo(dtype).max}
+    features, weight = matrix(rows, dim, dtype, 1), torch.zeros(labels, dim, dtype=dtype, device="cuda")
+    features[:, 3], weight[:, 3] = 1.0, ends.get(logit, logit)
+    targets = tokens_for("all", rows, labels, torch.int32, 3)
+    head = sb.LabelHead(ctx, labels, dim, dtype, rows, training=training)
+    loss = head.loss(features, weight, targets, scale)
+    want = torch.full((rows,), float(labels), dtype=torch.float64, device="cuda").log()
+    # The sum of the labels' ones is exact; the exponentials of 0 are good to 2^-21, the loss is rounded.
+    close(loss.losses, want, 2.0**-20 + 4 * A * want)
+    got, log_probabilities = head.predict(features, weight, scale)
+    close(log_probabilities, -want, 2.0**-20 + 4 * A * want)
+    assert got.count_nonzero() == 0
+    if training and isinstance(logit, float) and abs(logit) < 1e10:
+        _, to_weight = head.gradient(features, weight, targets, loss.log_normalizers, scale)
+        # The normalizers are good to 2^-53 of 3e9 and of ln labels; then as in Bounds, with logits that are exact.
+        slopes = torch.full((rows, labels), 1.0 / labels, dtype=torch.float64, device="cuda")
+        slopes[torch.arange(rows, device="cuda"), targets.long()] -= 1.0
+        slopes *= float(torch.tensor(scale)) / rows
+        h, element = features.double(), 2.0**-24 if dtype == torch.float32 else 2.0**-8
+        products = 6 if dtype == torch.float32 else 1
+        each = element + 2.0**-20 + 2 * A * (products * (rows / 16 + 1) + 8)
+        close(to_weight, slopes.T @ h, slopes.abs().T @ h.abs() * each + (slopes.T @ h).abs() * element * 1.01)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,training", PASSES)
+def test_rows_without_any_logit_have_no_softmax(ctx, rows, training, dtype):
+    """Every logit of a row is -inf, as after a mask that leaves nothing: NaN, in that row alone."""
+    labels, dim = 500, 40
+    features, weight = matrix(rows, dim, dtype, 1), matrix(labels, dim, dtype, 2)
+    features[:, 0], weight[:, 0] = 0.0, torch.finfo(dtype).min
+    bare = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    bare[::7] = True
+    features[bare] = 0.0
+    features[bare, 0] = 3.0  # past f32's range
+    targets = tokens_for("all", rows, labels, torch.int32, 3)
+    b = Bounds(features, weight, targets, 1.0)
+    head = sb.LabelHead(ctx, labels, dim, dtype, rows, training=training)
+    loss = head.loss(features, weight, targets)
+    assert loss.losses[bare].isnan().all() and loss.log_normalizers[bare].isnan().all() and loss.mean.isnan()
+    close(loss.losses[~bare], b.losses[~bare], b.loss_error[~bare])
+    _, log_probabilities = head.predict(features, weight)
+    assert log_probabilities[bare].isnan().all()
+    assert log_probabilities[~bare].isfinite().all()
