@@ -85,8 +85,8 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
                                  const float* d_row_gradient, void* d_feature_gradient,
                                  int64_t feature_gradient_stride, void* d_weight_gradient,
                                  int64_t weight_gradient_stride);
-/* Each row's most probable label (the lowest of equal ones) and its log-probability, NaN where the loss
- * is. */
+/* Each row's most probable label (the lowest of equal ones) and its log-probability. A row with a logit of NaN or
+ * +inf, or with all of them -inf, gets the label of its largest that is a number (0 without one) and NaN. */
 sp_status sp_label_head_predict(sp_label_head* h, const void* d_features, int64_t feature_stride,
                                 const void* d_weight, int64_t weight_stride, uint64_t rows, float logit_scale,
                                 int32_t* d_labels, float* d_log_probabilities);

@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(thin_threads(DIRECT), 1)
         const uint32_t split = a.columns <= 16 ? 3 : a.columns <= 32 ? 2 : 1;
         const uint32_t row = t >> split, part = t & ((1u << split) - 1), span = kTile >> split;
         const bool live = row < count;
-        RowStats stats{-INFINITY, 0.0f, 0.0f, -INFINITY, 0xffffffffu};
+        RowStats stats{-INFINITY, 0.0f, 0.0f, -INFINITY, 0u};
         uint32_t target = kNoTarget;
         if (live && a.g.targets)
             target = (uint32_t)index_at(a.g.targets, a.g.wide, a.g.all_rows ? row : a.g.row_of[row], a.g.labels);

@@ -156,3 +156,28 @@ def test_rows_without_any_logit_have_no_softmax(ctx, rows, training, dtype):
     _, log_probabilities = head.predict(features, weight)
     assert log_probabilities[bare].isnan().all()
     assert log_probabilities[~bare].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [5, 20, 40, 64, 65, 300])
+def test_predicted_labels_are_labels(ctx, rows, dtype):
+    """Rows of NaN, of logits all -inf and of an infinite logit: the label of the largest that is a number, 0
+    if there is none, and a log-probability of NaN."""
+    labels, dim = 500, 40
+    features, weight = matrix(rows, dim, dtype, 1), matrix(labels, dim, dtype, 2)
+    features[:, 0], weight[:, 0] = 0.0, torch.finfo(dtype).min
+    features[0] = float("nan")
+    features[2], features[2, 0] = 0.0, 3.0  # -inf throughout
+    weight[:, 1] = -1.0
+    weight[[77, 402], 1] = 1.0
+    features[4], features[4, 1] = 0.0, float("inf")  # +inf twice, -inf elsewhere
+    head = sb.LabelHead(ctx, labels, dim, dtype, rows, training=False)
+    got, log_probabilities = head.predict(features, weight)
+    assert got[[0, 2, 4]].tolist() == [0, 0, 77]
+    assert log_probabilities[[0, 2, 4]].isnan().all()
+    ordinary = torch.ones(rows, dtype=torch.bool, device="cuda")
+    ordinary[[0, 2, 4]] = False
+    want = Bounds(features[ordinary], weight, None, 1.0)
+    picked = want.z.gather(1, got[ordinary].long()[:, None])[:, 0]
+    assert (want.z.amax(1) - picked <= 2 * want.z_error).all()
+    assert log_probabilities[ordinary].isfinite().all()
