@@ -32,7 +32,7 @@ typedef enum sp_index { SP_INDEX32 = 0, SP_INDEX64 = 1 } sp_index;
 /* ------------------------------------------------------------------ embedding */
 
 /* A table of `entries` rows of `dim` features looked up by token, and the gradient of its rows.
- * `max_tokens` bounds the tokens of one call (below 2^30); entries and dim below 2^31. */
+ * `max_tokens` bounds the tokens of one call (below 2^30); entries below 2^31, dim below 2^20. */
 typedef struct sp_embedding sp_embedding;
 sp_status sp_embedding_create(sp_context* ctx, uint64_t entries, uint32_t dim, sp_element element,
                               uint64_t max_tokens, sp_embedding** out);
@@ -58,8 +58,8 @@ sp_status sp_embedding_check(sp_embedding* e);
  * products run in tiles on the tensor cores, and each tile is reduced (or turned into its gradient)
  * where it was made. f32 operands are split into three bf16 parts each (24 bits for
  * magnitudes from 2^-110 on, any finite or infinite value) and their six largest partial products are
- * summed; an infinite feature that meets an infinite weight gives NaN. `max_rows` bounds the rows of one call
- * (below 2^31 - 512); `training` != 0 also reserves the gradient's workspace. */
+ * summed; an infinite feature that meets an infinite weight gives NaN. `max_rows` bounds the rows of one call;
+ * it and labels are below 2^31 - 512, dim below 2^20. `training` != 0 also reserves the gradient's workspace. */
 typedef struct sp_label_head sp_label_head;
 sp_status sp_label_head_create(sp_context* ctx, uint64_t labels, uint32_t dim, sp_element element, uint64_t max_rows,
                                int training, sp_label_head** out);

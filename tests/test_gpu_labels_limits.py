@@ -181,3 +181,19 @@ def test_predicted_labels_are_labels(ctx, rows, dtype):
     picked = want.z.gather(1, got[ordinary].long()[:, None])[:, 0]
     assert (want.z.amax(1) - picked <= 2 * want.z_error).all()
     assert log_probabilities[ordinary].isfinite().all()
+
+
+def test_sizes_as_the_header_states_them(ctx):
+    """The largest dim goes through, the next ones are refused, as are counts past theirs."""
+    f32, dim = torch.float32, (1 << 20) - 1
+    e = sb.Embedding(ctx, 3, dim, f32, 4)
+    table, tokens = matrix(3, dim, f32, 1), torch.tensor([2, 0, 2, -1], device="cuda")
+    assert torch.equal(e.lookup(table, tokens, 2.0)[:3], 2.0 * table[tokens[:3]])
+    upstream = matrix(4, dim, f32, 2)
+    assert torch.equal(e.gradient(upstream, tokens), torch.stack([upstream[1], 0 * upstream[1], upstream[0] + upstream[2]]))
+    for sizes in ((3, 1 << 20, 4), (1 << 31, 4, 4), (3, 4, 1 << 30)):
+        with pytest.raises(sb.SplatError):
+            sb.Embedding(ctx, sizes[0], sizes[1], f32, sizes[2])
+    for sizes in ((3, 1 << 20, 4), ((1 << 31) - 512, 4, 4), (3, 4, (1 << 31) - 512)):
+        with pytest.raises(sb.SplatError):
+            sb.LabelHead(ctx, sizes[0], sizes[1], f32, sizes[2])
