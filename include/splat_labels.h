@@ -76,8 +76,10 @@ sp_status sp_label_head_loss(sp_label_head* h, const void* d_features, int64_t f
                              float logit_scale, float* d_mean, float* d_losses, double* d_log_normalizers);
 /* The gradient of sum_i g[i] losses[i], g = d_row_gradient (rows floats), or with NULL of the mean
  * (g[i] = 1 / rows with a target). Both gradients are overwritten; a row without a target gets a
- * zero row and adds nothing to the weight's. `d_log_normalizers` are those of sp_label_head_loss
- * for the same features, weight, targets and scale. Needs a handle made for training. The softmax
+ * zero row and adds nothing to the weight's. `d_log_normalizers` are those of this
+ * handle's sp_label_head_loss for the same features, weight, targets and scale: a confident row's slope is the
+ * difference of its logit and its normalizer, which have to come from logits of the same rounding (another
+ * handle, not made for training, may sum them in another order). Needs a handle made for training. The softmax
  * slopes are rounded to the element type (f32: kept to 24 bits) before the second products. */
 sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64_t feature_stride,
                                  const void* d_weight, int64_t weight_stride, const void* d_targets, sp_index index,

@@ -186,7 +186,8 @@ class LabelHead(_Handle):
     def gradient(self, features, weight, targets, log_normalizers, logit_scale: float = 1.0, row_gradient=None,
                  feature_gradient=None, weight_gradient=None):
         """(gradient of the features, of the weight) of the mean loss, or with `row_gradient` (one
-        float32 per row) of sum(row_gradient * losses). `log_normalizers` as `loss` returned them."""
+        float32 per row) of sum(row_gradient * losses). `log_normalizers` as `loss` of this head returned
+        them (those of a head not made for training may be of differently rounded logits)."""
         inputs = self._inputs(features, weight)
         rows = features.shape[0]
         targets_at, index = self._index(targets, "targets", rows)
