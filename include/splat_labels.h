@@ -79,8 +79,9 @@ sp_status sp_label_head_loss(sp_label_head* h, const void* d_features, int64_t f
  * zero row and adds nothing to the weight's. `d_log_normalizers` are those of this
  * handle's sp_label_head_loss for the same features, weight, targets and scale: a confident row's slope is the
  * difference of its logit and its normalizer, which have to come from logits of the same rounding (another
- * handle, not made for training, may sum them in another order). Needs a handle made for training. The softmax
- * slopes are rounded to the element type (f32: kept to 24 bits) before the second products. */
+ * handle, not made for training, may sum them in another order). Needs a handle made for training. Before the
+ * second products the softmax slopes are kept to 24 bits (f32) or rounded to bf16, without the mean's factor;
+ * the weight's gradient takes them to 16 bits where there are at most 128 rows or d_row_gradient. */
 sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64_t feature_stride,
                                  const void* d_weight, int64_t weight_stride, const void* d_targets, sp_index index,
                                  uint64_t rows, float logit_scale, const double* d_log_normalizers,

@@ -315,13 +315,14 @@ __device__ __forceinline__ void add_logits(RowStats& s, float (&v)[W], uint32_t 
     s.sum = sum;
 }
 
-// The slopes of 32 logits of a row, in place (the target's only if PLACE); zeros past the labels and in rows that do not count. The
-// target's, if it is among them, also in `target_slope`: p - 1 from the difference of its logit and the
+// The slopes of 32 logits of a row, in place (the target's only if PLACE); zeros past the labels and in rows that
+// do not count. The target's, if it is among them, also in `target_slope`: p - 1 from the difference of its logit and the
 // normalizer, since p itself may round to 1. The normalizer over the scale is `normalizer`, to f32's precision,
 // less shift_low / scale2.
 template <bool PLACE>
 __device__ __forceinline__ void to_slopes(float (&v)[32], uint32_t first, uint32_t labels, float scale2,
-                                          float normalizer, float weight, uint32_t target, bool live, float shift_low, float& target_slope) {
+                                          float normalizer, float weight, uint32_t target, bool live,
+                                          float shift_low, float& target_slope) {
     const uint32_t at = target - first;
     const bool near = __any_sync(0xffffffffu, at < 32);
     float logit = 0.0f;
@@ -372,6 +373,16 @@ __device__ __forceinline__ void stage_part(uint32_t tile, uint32_t row, int half
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + row * 128 + unit * 16), "r"(w[0]),
                      "r"(w[1]), "r"(w[2]), "r"(w[3])
                      : "memory");
+    }
+}
+
+// What the first part leaves of 32 values.
+__device__ __forceinline__ void round_off(float (&v)[32]) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+        const __nv_bfloat162 pair = __floats2bfloat162_rn(v[j], v[j + 1]);
+        v[j] -= __low2float(pair);
+        v[j + 1] -= __high2float(pair);
     }
 }
 
@@ -638,27 +649,34 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                             __syncwarp();
                             if (lane == 0) tc::store_box(&map_slopes, stage_tile, 0, (int)row, (int)(p * a.panels + (columns_at + c) / 64));
                         };
-                        if (sizeof(T) == 2 && (PAIR || a.slope_parts == 1)) {
+                        if constexpr (sizeof(T) == 2) {
+                            // A second part takes the slopes from the accumulator again: 64 of them and what
+                            // the first one left do not fit a thread's registers.
+#pragma unroll 1
+                            for (uint32_t p = 0; p < a.slope_parts; ++p) {
 #pragma unroll
-                            for (int q = 0; q < 2; ++q) {
-                                float v[32];
-                                __syncwarp();
-                                tc::tmem_load32(accumulator + c + 32 * q, v);
-                                tc::tmem_load_wait();
-                                if (q == 1 && c + 64 == kSpan) drain();
-                                const uint32_t column = columns_at + c + 32 * q;
-                                float slope = 0.0f;
-                                to_slopes<false>(v, column, a.labels, a.scale2, normalizer, weight, target, live, shift_low, slope);
-                                if (q == 0) reclaim();
-                                stage_part(stage_tile, lane, q, v);
-                                if (target - column < 32) {
-                                    const bf16 rounded = __float2bfloat16_rn(slope);
-                                    stage_one(stage_tile, lane, 32 * q + target - column, rounded);
-                                    a.residuals[row] = slope - __bfloat162float(rounded);
+                                for (int q = 0; q < 2; ++q) {
+                                    float v[32];
+                                    __syncwarp();
+                                    tc::tmem_load32(accumulator + c + 32 * q, v);
+                                    tc::tmem_load_wait();
+                                    if (q == 1 && c + 64 == kSpan && p + 1 == a.slope_parts) drain();
+                                    const uint32_t column = columns_at + c + 32 * q;
+                                    float slope = 0.0f;
+                                    to_slopes<false>(v, column, a.labels, a.scale2, normalizer, weight, target, live, shift_low, slope);
+                                    if (p != 0) round_off(v);
+                                    if (q == 0) reclaim();
+                                    stage_part(stage_tile, lane, q, v);
+                                    if (target - column < 32) {
+                                        const bf16 rounded = __float2bfloat16_rn(slope);
+                                        const float left = slope - __bfloat162float(rounded);
+                                        stage_one(stage_tile, lane, 32 * q + target - column, p == 0 ? rounded : __float2bfloat16_rn(left));
+                                        a.residuals[row] = left;
+                                    }
                                 }
+                                store(p);
                             }
-                            store(0);
-                        } else if constexpr (sizeof(T) == 4 || !PAIR) {
+                        } else {
                             float v[2][32], unused;
                             __syncwarp();
                             tc::tmem_load32(accumulator + c, v[0]);
@@ -667,20 +685,13 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                             if (c + 64 == kSpan) drain();
 #pragma unroll
                             for (int q = 0; q < 2; ++q)
-                                to_slopes<true>(v[q], columns_at + c + 32 * q, a.labels, a.scale2, normalizer, weight, target, live,
-                                          shift_low, unused);
+                                to_slopes<true>(v[q], columns_at + c + 32 * q, a.labels, a.scale2, normalizer, weight, target,
+                                                live, shift_low, unused);
                             for (int p = 0; p < (int)a.slope_parts; ++p) {
                                 reclaim();
                                 stage_part(stage_tile, lane, 0, v[0]);
                                 stage_part(stage_tile, lane, 1, v[1]);
                                 store(p);
-                                if (sizeof(T) == 2 && p == 0 && target - columns_at - c < 64) {
-                                    float left = 0.0f;
-#pragma unroll
-                                    for (int j = 0; j < 64; ++j)
-                                        if (target - columns_at - c == (uint32_t)j) left = v[j / 32][j % 32];
-                                    a.residuals[row] = left;
-                                }
                             }
                         }
                     }

@@ -48,8 +48,13 @@ struct sp_label_head {
     // Parts of the slopes: f32's three, and two for bf16 operands where the rows are few. One rounding to
     // bf16 is then as much of the weight's gradient as its own last one (2.4e-3 of its norm in all, 1.7e-3 with
     // two parts), and two parts cost the gradient of 128 x 65,536 x 512 13 of 88 us. With more rows a label's
-    // sums average it out, and a second part would double the bytes and half of the products.
-    uint32_t slope_parts(uint64_t rows) const { return element == SP_F32 ? kParts : rows <= kTile ? 2 : 1; }
+    // sums average it out, and a second part would double the bytes and half of the products. Not where the rows
+    // have factors of their own, which are in their slopes: the targets' slopes of rows of one factor, near
+    // minus that, are all rounded the same way (1.1e-3 of the weight's gradient at 20,000 x 32,768 x 512, which
+    // takes 2.3 ms with two parts and 1.5 with one).
+    uint32_t slope_parts(uint64_t rows, bool own_factors) const {
+        return element == SP_F32 ? kParts : rows <= kTile || own_factors ? 2 : 1;
+    }
     uint64_t packed_stride() const { return ((uint64_t)dim + kBlockK - 1) / kBlockK * kBlockK; }
     uint64_t count_blocks() const { return (max_rows + 63) / 64; }
     uint64_t slope_stride() const { return (labels + kPairTile - 1) / kPairTile * kPairTile; }
@@ -560,15 +565,20 @@ OutPlan plan_out(uint32_t sms, uint64_t rows, uint64_t labels, uint32_t dim, uin
     return best;
 }
 
-uint64_t chunk_limit(const sp_label_head* h) {
+// Rows whose slopes in one part (f32: in three) the workspace holds: all, twice where they may have two parts,
+// or what the budget has room for, but a pair's tile of the most parts.
+uint64_t slope_rows(const sp_label_head* h) {
     const uint64_t rows = kSlopeBudget / (h->slope_stride() * h->parts()) / kPairTile * kPairTile;
-    return std::min(std::max<uint64_t>(rows, kPairTile), round_up(h->max_rows, kPairTile));
+    const uint64_t twice = h->element == SP_BF16 && h->max_rows > kTile ? 2 : 1;
+    return std::max(std::min(rows, twice * round_up(h->max_rows, kPairTile)), twice * kPairTile);
 }
 
-// The rows of slopes taken at once: all of them, or else of the even cuts and of those that fill the
+// The rows of slopes of `parts` taken at once: all of them, or else of the even cuts and of those that fill the
 // SMs with whole tiles of the features' gradient, the one whose products finish soonest.
-uint64_t chunk_for(const sp_label_head* h, uint64_t rows) {
-    const uint64_t limit = std::min(chunk_limit(h), round_up(rows, kPairTile));
+uint64_t chunk_for(const sp_label_head* h, uint64_t rows, uint32_t parts) {
+    if (rows <= kTile) return parts == 2 ? kTile : kPairTile;  // two parts: what fits where one of a pair's tile does
+    const uint64_t room = slope_rows(h) * h->parts() / parts / kPairTile * kPairTile;
+    const uint64_t limit = std::min(room, round_up(rows, kPairTile));
     if (rows <= limit) return limit;
     const uint64_t wave = std::max<uint64_t>(h->sms / 2 / tiles_of(h->dim, true), 1) * kPairTile;
     const uint64_t fewest = (rows + limit - 1) / limit;
@@ -863,7 +873,7 @@ sp_status sp_label_head_create(sp_context* ctx, uint64_t labels, uint32_t dim, s
         SP_CHECK(allocate(h, &h->target_logits, capacity));
         SP_CHECK(allocate(h, &h->loss_sums, (max_rows * 32 + kThreads - 1) / kThreads));
         if (h->training) {
-            SP_CHECK(allocate(h, &h->slopes, chunk_limit(h) * h->slope_stride() * h->parts()));
+            SP_CHECK(allocate(h, &h->slopes, slope_rows(h) * h->slope_stride() * h->parts()));
             SP_CHECK(allocate(h, &h->sums, sums_rows(h) * sums_stride(h) * 2));
         }
         return SP_OK;
@@ -955,8 +965,8 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
     SP_CHECK(prepare(h, d_features, feature_stride, d_weight, weight_stride, d_targets, wide, rows, nullptr, nullptr,
                      d_feature_gradient, feature_gradient_stride, true, &op));
 
-    const uint32_t slope_parts = h->slope_parts(rows);
-    const uint64_t chunk = slope_parts == 2 ? kTile : chunk_for(h, rows), chunks = (rows + chunk - 1) / chunk;
+    const uint32_t slope_parts = h->slope_parts(rows, d_row_gradient != nullptr);
+    const uint64_t chunk = chunk_for(h, rows, slope_parts), chunks = (rows + chunk - 1) / chunk;
     const uint64_t sum_stride = sums_stride(h);
     CUtensorMap slopes, slopes_out;
     const uint32_t panels = (uint32_t)(h->slope_stride() / 64);

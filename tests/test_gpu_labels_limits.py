@@ -197,3 +197,82 @@ def test_sizes_as_the_header_states_them(ctx):
     for sizes in ((3, 1 << 20, 4), ((1 << 31) - 512, 4, 4), (3, 4, (1 << 31) - 512)):
         with pytest.raises(sb.SplatError):
             sb.LabelHead(ctx, sizes[0], sizes[1], f32, sizes[2])
+
+
+@pytest.mark.parametrize("rows,labels,dim,factor", [(129, 300, 64, "uniform"), (256, 1000, 64, "uniform"),
+                                                    (1000, 300, 72, "random"), (1000, 300, 72, "uniform"),
+                                                    (3001, 65, 200, "by label")])
+def test_bf16_weight_gradient_of_weighted_rows_is_rounded_once(ctx, rows, labels, dim, factor):
+    """Each value is within half a unit in the last place (8 bits) of its exact sum, give or take its terms'
+    2^-15 (a slope in two parts is off by 2^-17, and by as much again where its logit is, with logits up to 16)
+    and the f32 sum of both parts over the rows. One rounding of slopes of one factor would be up to 2^-9 of the
+    terms, all of one sign."""
+    head = sb.LabelHead(ctx, labels, dim, torch.bfloat16, rows)
+    features, weight = matrix(rows, dim, torch.bfloat16, 1), matrix(labels, dim, torch.bfloat16, 2)
+    targets = tokens_for("some", rows, labels, torch.int64, 3)
+    held = (targets >= 0) & (targets < labels)
+    at = targets.clamp(0, labels - 1)
+    factors = {"uniform": torch.full((rows,), 1.0 / rows, device="cuda"),
+               "random": torch.rand(rows, device="cuda", generator=torch.Generator("cuda").manual_seed(4)) - 0.3,
+               "by label": torch.rand(labels, device="cuda", generator=torch.Generator("cuda").manual_seed(5))[at]}
+    loss = head.loss(features, weight, targets, 0.2)
+    to_features, to_weight = head.gradient(features, weight, targets, loss.log_normalizers, 0.2, factors[factor])
+    h, w = features.double(), weight.double()
+    logits = 0.2 * h @ w.T
+    assert logits.abs().max() < 16
+    slopes = torch.softmax(logits, 1)
+    slopes[torch.arange(rows, device="cuda"), at] -= 1
+    slopes *= (float(torch.tensor(0.2)) * factors[factor].double() * held)[:, None]
+    want, terms = slopes.T @ h, slopes.T.abs() @ h.abs()
+    half = torch.ldexp(torch.ones_like(want), torch.frexp(want).exponent - 9)
+    assert (((to_weight.double() - want).abs() - half) <= (2.0**-15 + 2 * A * (2 * (rows / 16 + 1) + 8)) * terms).all()
+    b = Bounds(features, weight, targets, 0.2, factors[factor])
+    close(to_features, b.to_features, b.features_error)
+    again = head.gradient(features, weight, targets, loss.log_normalizers, 0.2, factors[factor])
+    assert torch.equal(again[0], to_features) and torch.equal(again[1], to_weight)
+
+
+@pytest.mark.parametrize("rows", [100, 129, 700])
+def test_confident_weighted_rows_keep_their_slopes(ctx, rows):
+    """As test_confident_rows_keep_their_small_losses_and_slopes, bf16 with a factor a row: the slopes are made in
+    tiles of another shape than the loss's, of the same logits bit for bit."""
+    labels, dim, scale = 40, 256, 20.0
+    weight = matrix(labels, dim, torch.bfloat16, 2)
+    weight /= weight.float().norm(dim=1, keepdim=True).to(torch.bfloat16)
+    targets = tokens_for("all", rows, labels, torch.int32, 3)
+    features = (weight[targets.long()].float() + 0.05 * matrix(rows, dim, torch.float32, 4) / dim**0.5).bfloat16()
+    factors = matrix(1, rows, torch.float32, 5)[0].contiguous()
+    exact = Bounds(features, weight, targets, scale, factors)
+    assert (torch.exp(-exact.losses) > 0.999).float().mean() > 0.5
+    head = sb.LabelHead(ctx, labels, dim, torch.bfloat16, rows)
+    loss = head.loss(features, weight, targets, scale)
+    to_features, to_weight = head.gradient(features, weight, targets, loss.log_normalizers, scale, factors)
+    # Two roundings to bf16 (slopes, result), each at most 2^-9 of a value; the logits' errors are far below.
+    for got, want in ((to_features, exact.to_features), (to_weight, exact.to_weight)):
+        assert float((got.double() - want).norm() / want.norm()) <= 2.0**-8
+
+
+@pytest.mark.parametrize("kind", ["all", "some", "none after row 200"])
+def test_weighted_rows_in_chunks(ctx, kind):
+    """Slopes in two parts of half as many rows a time: several chunks of rows with factors of their own."""
+    rows, labels, dim = 6200, 70_000, 24
+    head = sb.LabelHead(ctx, labels, dim, torch.bfloat16, rows)
+    features, weight = matrix(rows, dim, torch.bfloat16, 1), matrix(labels, dim, torch.bfloat16, 2)
+    targets = tokens_for("some" if kind == "some" else "all", rows, labels, torch.int64, 3)
+    if kind == "none after row 200":
+        targets[200:] = -1
+    factors = matrix(1, rows, torch.float32, 5)[0].contiguous()
+    loss = head.loss(features, weight, targets, 0.3)
+    to_features, to_weight = head.gradient(features, weight, targets, loss.log_normalizers, 0.3, factors)
+    want_weight = torch.zeros(labels, dim, dtype=torch.float64, device="cuda")
+    weight_error = torch.zeros_like(want_weight)
+    for first in range(0, rows, 1000):
+        part = slice(first, min(rows, first + 1000))
+        b = Bounds(features[part], weight, targets[part], 0.3, factors[part])
+        want_weight += b.to_weight
+        weight_error += b.weight_error
+        close(to_features[part], b.to_features, b.features_error)
+    close(to_weight, want_weight, weight_error * 1.1)  # the chunks' sums add f32 roundings
+    again = head.gradient(features, weight, targets, loss.log_normalizers, 0.3, factors)
+    assert torch.equal(again[0], to_features) and torch.equal(again[1], to_weight)
+    head.check()
