@@ -81,7 +81,8 @@ sp_status sp_label_head_loss(sp_label_head* h, const void* d_features, int64_t f
  * difference of its logit and its normalizer, which have to come from logits of the same rounding (another
  * handle, not made for training, may sum them in another order). Needs a handle made for training. Before the
  * second products the softmax slopes are kept to 24 bits (f32) or rounded to bf16, without the mean's factor;
- * the weight's gradient takes them to 16 bits where there are at most 128 rows or d_row_gradient. */
+ * the weight's gradient takes them to 16 bits where rows are at most 128, or rows times labels at most 2^21, or
+ * with d_row_gradient. */
 sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64_t feature_stride,
                                  const void* d_weight, int64_t weight_stride, const void* d_targets, sp_index index,
                                  uint64_t rows, float logit_scale, const double* d_log_normalizers,

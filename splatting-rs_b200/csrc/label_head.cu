@@ -22,6 +22,10 @@
 using namespace splat;
 using namespace splat::label;
 
+namespace {
+constexpr uint64_t kFineSlopes = 1ull << 21;
+}
+
 struct sp_label_head {
     sp_context* ctx = nullptr;
     uint64_t labels = 0;
@@ -45,15 +49,16 @@ struct sp_label_head {
 
     uint32_t parts() const { return element == SP_F32 ? kParts : 1; }
     uint32_t products() const { return element == SP_F32 ? kPartProducts : 1; }
-    // Parts of the slopes: f32's three, and two for bf16 operands where the rows are few. One rounding to
-    // bf16 is then as much of the weight's gradient as its own last one (2.4e-3 of its norm in all, 1.7e-3 with
-    // two parts), and two parts cost the gradient of 128 x 65,536 x 512 13 of 88 us. With more rows a label's
-    // sums average it out, and a second part would double the bytes and half of the products. Not where the rows
-    // have factors of their own, which are in their slopes: the targets' slopes of rows of one factor, near
+    // Parts of the slopes: f32's three, and two for bf16 operands where that costs little, or matters most. One
+    // rounding to bf16 is nearly as much of the weight's gradient as its own last one (256 x 1000 x 64, features
+    // that lean towards their label: 2.1e-3 of its norm in all, 1.65e-3 with two parts). Two parts cost the
+    // gradient of 128 x 65,536 x 512 13 of 88 us, that of 2^21 slopes 1.4 to 3.5 us. With more rows a label's sums
+    // average the rounding out, and a second part would double the bytes and half of the products. Not where the
+    // rows have factors of their own, which are in their slopes: the targets' slopes of rows of one factor, near
     // minus that, are all rounded the same way (1.1e-3 of the weight's gradient at 20,000 x 32,768 x 512, which
     // takes 2.3 ms with two parts and 1.5 with one).
     uint32_t slope_parts(uint64_t rows, bool own_factors) const {
-        return element == SP_F32 ? kParts : rows <= kTile || own_factors ? 2 : 1;
+        return element == SP_F32 ? kParts : rows <= kTile || rows * labels <= kFineSlopes || own_factors ? 2 : 1;
     }
     uint64_t packed_stride() const { return ((uint64_t)dim + kBlockK - 1) / kBlockK * kBlockK; }
     uint64_t count_blocks() const { return (max_rows + 63) / 64; }

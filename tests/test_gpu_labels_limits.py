@@ -276,3 +276,22 @@ def test_weighted_rows_in_chunks(ctx, kind):
     again = head.gradient(features, weight, targets, loss.log_normalizers, 0.3, factors)
     assert torch.equal(again[0], to_features) and torch.equal(again[1], to_weight)
     head.check()
+
+
+@pytest.mark.parametrize("rows,labels,dim", [(129, 300, 64), (256, 1000, 64), (2000, 1000, 72), (1023, 2050, 40)])
+def test_bf16_weight_gradient_of_a_small_batch_is_rounded_once(ctx, rows, labels, dim):
+    """The mean's call, bounded as test_bf16_weight_gradient_of_weighted_rows_is_rounded_once."""
+    head = sb.LabelHead(ctx, labels, dim, torch.bfloat16, rows)
+    features, weight = matrix(rows, dim, torch.bfloat16, 1), matrix(labels, dim, torch.bfloat16, 2)
+    targets = tokens_for("all", rows, labels, torch.int64, 3)
+    loss = head.loss(features, weight, targets, 0.2)
+    _, to_weight = head.gradient(features, weight, targets, loss.log_normalizers, 0.2)
+    h, w = features.double(), weight.double()
+    logits = float(torch.tensor(0.2)) * h @ w.T
+    assert logits.abs().max() < 16
+    slopes = torch.softmax(logits, 1)
+    slopes[torch.arange(rows, device="cuda"), targets] -= 1
+    slopes *= float(torch.tensor(0.2)) / rows
+    want, terms = slopes.T @ h, slopes.T.abs() @ h.abs()
+    half = torch.ldexp(torch.ones_like(want), torch.frexp(want).exponent - 9)
+    assert (((to_weight.double() - want).abs() - half) <= (2.0**-15 + 2 * A * (2 * (rows / 16 + 1) + 8)) * terms).all()
