@@ -295,3 +295,21 @@ def test_bf16_weight_gradient_of_a_small_batch_is_rounded_once(ctx, rows, labels
     want, terms = slopes.T @ h, slopes.T.abs() @ h.abs()
     half = torch.ldexp(torch.ones_like(want), torch.frexp(want).exponent - 9)
     assert (((to_weight.double() - want).abs() - half) <= (2.0**-15 + 2 * A * (2 * (rows / 16 + 1) + 8)) * terms).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,training", PASSES)
+@pytest.mark.parametrize("dim", [64, 768, 4096, 65_536])
+def test_exact_logits_of_wide_features(ctx, rows, training, dim, dtype):
+    """Features of a single 1: each logit is a weight, as it is. What is given back for the truncation of sums, an
+    eighth of 2^-23 an addition of 16 columns, is not lost here; it stays bounded however wide the features are."""
+    head = sb.LabelHead(ctx, 1, dim, dtype, rows, training=training)
+    features, weight = torch.zeros(rows, dim, dtype=dtype, device="cuda"), matrix(1, dim, dtype, 2)
+    column = torch.arange(rows, device="cuda") * 977 % dim
+    features[torch.arange(rows, device="cuda"), column] = 1.0
+    targets = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    loss = head.loss(features, weight, targets)
+    want = weight[0, column].double()  # of one label, the normalizer is its logit
+    given = (min(dim // 16, 256) + 1) / 8
+    # f32 roundings of the scale and of the sums of three parts beside what is given back.
+    assert ((loss.log_normalizers - want).abs() <= want.abs() * (given + 3) * 2.0**-23).all()
