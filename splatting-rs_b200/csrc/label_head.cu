@@ -603,14 +603,19 @@ uint64_t chunk_for(const sp_label_head* h, uint64_t rows, uint32_t parts) {
     return best;
 }
 
-// Rows of f32 sums a gradient may need. plan_out: pieces times tiles stay within kOutWaves waves, or
-// there is one piece, which needs sums for the weight's gradient alone, over several chunks; or f32's
-// least pieces, of which a gradient of r rows over an inner n has at most n / (64 kLongestSum) + 1: r n
-// is at most the slope budget, and r at most the labels or, with more labels than one piece takes, the
-// budget over those.
-uint64_t sums_rows(const sp_label_head* h) {
-    const uint64_t f32 = h->parts() > 1 ? 2 * (kSlopeBudget / kParts / (kLongestSum * kBlockK)) : 0;
-    return std::max<uint64_t>((uint64_t)kOutWaves * h->sms * kTile, h->labels + f32);
+// Rows of f32 sums that a gradient of `rows` rows over an inner dimension of up to `inner` may need. plan_out:
+// pieces times tiles stay within kOutWaves waves, and a piece is 4 steps or longer; or f32's least pieces.
+uint64_t sums_rows(const sp_label_head* h, uint64_t rows, uint64_t inner) {
+    const uint64_t k = (inner + kBlockK - 1) / kBlockK, longest = h->parts() > 1 ? (k + kLongestSum - 1) / kLongestSum : 1;
+    const uint64_t chosen = k >= 8 ? std::min((uint64_t)kOutWaves * h->sms * kTile, rows * (k / 4)) : 0;
+    return std::max(chosen, longest > 1 ? rows * longest : 0);
+}
+// ... the features' gradient, and the weight's, which one piece of several chunks needs too.
+uint64_t feature_sums_rows(const sp_label_head* h) {
+    return sums_rows(h, std::min(h->max_rows, slope_rows(h)), h->labels);
+}
+uint64_t weight_sums_rows(const sp_label_head* h) {
+    return std::max(h->labels, sums_rows(h, h->labels, std::min(h->max_rows, slope_rows(h))));
 }
 
 uint64_t sums_stride(const sp_label_head* h) { return ((uint64_t)h->dim + 3) / 4 * 4; }
@@ -879,7 +884,7 @@ sp_status sp_label_head_create(sp_context* ctx, uint64_t labels, uint32_t dim, s
         SP_CHECK(allocate(h, &h->loss_sums, (max_rows * 32 + kThreads - 1) / kThreads));
         if (h->training) {
             SP_CHECK(allocate(h, &h->slopes, slope_rows(h) * h->slope_stride() * h->parts()));
-            SP_CHECK(allocate(h, &h->sums, sums_rows(h) * sums_stride(h) * 2));
+            SP_CHECK(allocate(h, &h->sums, (feature_sums_rows(h) + weight_sums_rows(h)) * sums_stride(h)));
         }
         return SP_OK;
     };
@@ -981,7 +986,7 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
     const OutPlan first = plan_out(h->sms, std::min(chunk, rows), h->labels, h->dim, h->parts(), chunks > 1);
     const bool weight_sums = first.weight > 1 || chunks > 1;
     float* weight_sum = h->sums;
-    float* feature_sum = h->sums + sums_rows(h) * sum_stride;
+    float* feature_sum = h->sums + weight_sums_rows(h) * sum_stride;
 
     for (uint64_t c = 0; c < chunks; ++c) {
         const uint64_t here = std::min(chunk, rows - c * chunk);
@@ -989,8 +994,8 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
         const OutPlan plan = c == 0 ? first
                                     : plan_out(h->sms, here, h->labels, h->dim, h->parts(), true, first.weight);
         const bool feature_sums = plan.features > 1;
-        SP_REQUIRE(ctx, (!feature_sums || plan.features * here <= sums_rows(h)) &&
-                            (!weight_sums || plan.weight * h->labels <= sums_rows(h)),
+        SP_REQUIRE(ctx, (!feature_sums || plan.features * here <= feature_sums_rows(h)) &&
+                            (!weight_sums || plan.weight * h->labels <= weight_sums_rows(h)),
                    SP_ERR_OVERFLOW, "the gradients' sums exceed their workspace");
         GemmArgs a = common_args(h, d_targets, wide, logit_scale);
         a.first_row = (uint32_t)(c * chunk);

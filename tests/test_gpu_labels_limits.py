@@ -313,3 +313,22 @@ def test_exact_logits_of_wide_features(ctx, rows, training, dim, dtype):
     given = (min(dim // 16, 256) + 1) / 8
     # f32 roundings of the scale and of the sums of three parts beside what is given back.
     assert ((loss.log_normalizers - want).abs() <= want.abs() * (given + 3) * 2.0**-23).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,labels,dim", [(1, 2, 16), (100, 100, 768), (300, 150, 1024), (60_000, 20, 512), (20, 60_000, 512)])
+def test_workspace_follows_the_sizes(ctx, rows, labels, dim, dtype):
+    """A head made for little holds little: copies of its operands, their slopes, and sums of the gradients in at
+    most as many pieces as their inner dimension has steps of 256 (f32: of 2048 at least), beside 32 MB."""
+    sb.LabelHead(ctx, 2, 16, dtype, 1).close()  # what the first head of a process loads
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    head = sb.LabelHead(ctx, labels, dim, dtype, rows)
+    used = before - torch.cuda.mem_get_info()[0]
+    up = lambda k, to: -(-k // to) * to  # noqa: E731
+    parts = 3 if dtype == torch.float32 else 1
+    operands = (up(rows, 256) + labels) * up(dim, 64) * 2 * parts
+    slopes = 2 * up(rows, 256) * up(labels, 256) * 2 * parts
+    sums = (rows * (1 + labels // 256) + labels * (1 + rows // 256)) * up(dim, 4) * 4
+    assert used <= operands + slopes + min(sums, 2 * (4 * 148 * 128 + rows + labels) * up(dim, 4) * 4) + (32 << 20)
+    head.close()
