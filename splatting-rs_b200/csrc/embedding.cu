@@ -538,7 +538,8 @@ __global__ void __launch_bounds__(kFewThreads)
                 for (uint32_t m = 1; m < team; ++m)
 #pragma unroll
                     for (int j = 0; j < N; ++j) acc[j] += s_part[(t + m * lanes) * N + j];
-                store_row<T, N>(out + (first_entry + e) * out_stride + column, acc, scale, out_packed);
+                // A row of nobody's is 0 whatever the scale, as where the sorted list's rows are zeroed.
+                store_row<T, N>(out + (first_entry + e) * out_stride + column, acc, n ? scale : 0.0f, out_packed);
             }
             if (team > 1) __syncthreads();
         }

@@ -332,3 +332,17 @@ def test_workspace_follows_the_sizes(ctx, rows, labels, dim, dtype):
     sums = (rows * (1 + labels // 256) + labels * (1 + rows // 256)) * up(dim, 4) * 4
     assert used <= operands + slopes + min(sums, 2 * (4 * 148 * 128 + rows + labels) * up(dim, 4) * 4) + (32 << 20)
     head.close()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [0, 9, 32_768, 32_769])
+@pytest.mark.parametrize("scale", [float("inf"), float("nan"), -2.0])
+def test_entries_without_tokens_have_zero_rows_whatever_the_scale(ctx, n, scale, dtype):
+    entries, dim = 50, 24
+    e = sb.Embedding(ctx, entries, dim, dtype, max(n, 1))
+    tokens = torch.arange(n, device="cuda") % 7
+    upstream = torch.ones(n, dim, dtype=dtype, device="cuda")
+    got = e.gradient(upstream, tokens, scale)
+    assert got[min(n, 7):].count_nonzero() == 0
+    count = torch.bincount(tokens, minlength=entries)[: min(n, 7), None].float() * scale
+    assert torch.equal(got[: min(n, 7)].nan_to_num(nan=7.0), count.to(dtype).expand(-1, dim).nan_to_num(nan=7.0))
