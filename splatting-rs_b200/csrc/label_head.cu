@@ -534,13 +534,12 @@ struct OutPlan {
 };
 
 OutPlan plan_out(uint32_t sms, uint64_t rows, uint64_t labels, uint32_t dim, uint32_t parts, bool sums_anyway,
-                 uint32_t weight_splits = 0, int pair_only = -1) {
+                 uint32_t weight_splits = 0) {
     OutPlan best{};
     best.us = 1e300;
     const uint32_t label_k = (uint32_t)((labels + kBlockK - 1) / kBlockK), row_k = (uint32_t)((rows + kBlockK - 1) / kBlockK);
     const double products = parts > 1 ? kPartProducts : 1;
     for (int pair = 0; pair < 2; ++pair) {
-        if (pair_only >= 0 && pair != pair_only) continue;
         const uint32_t workers = pair ? std::max(sms / 2, 1u) : sms;
         const uint32_t mf = tiles_of(rows, pair), mw = tiles_of(labels, pair), n = tiles_of(dim, pair);
         const double step_us = products * kStepUs * (pair ? kPairCost : 1.0);
