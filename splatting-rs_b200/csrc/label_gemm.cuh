@@ -4,7 +4,7 @@
 //   kStats   the logits' running sum of exponentials per row, and the target's logit or the
 //            largest one and its label
 //   kSlopes  the softmax slopes p - [target] (times c g of the row, if rows have their own), written as
-//            bf16 parts
+//            bf16 parts: f32's three, or one; kFineSlopes in two
 //   kOut     the tile itself, or a partial sum of it, of the two output gradients dH = G W and
 //            dW = G^T H, in one launch: the tiles of one fill the SMs the other's leave
 //
@@ -71,7 +71,8 @@ struct RowSet {
 
 constexpr uint32_t kNoTarget = 0xffffffffu;  // index_at's -1
 
-enum Ending { kStats = 0, kSlopes = 1, kOut = 2 };
+enum Ending { kStats = 0, kSlopes = 1, kOut = 2, kFineSlopes = 3 };
+constexpr bool makes_slopes(int ending) { return ending == kSlopes || ending == kFineSlopes; }
 
 // Warps that empty the accumulators: 8, or 16 for a pair's logits of bf16 operands, where the
 // exponentials take as long as the products up to some 256 columns and need more warps to overlap
@@ -81,8 +82,8 @@ template <int ENDING, bool PAIR, typename T>
 struct Shape {
     static constexpr int epilogue_warps = ENDING != kOut && PAIR && sizeof(T) == 2 ? 16 : 8;
     static constexpr int threads = 128 + 32 * epilogue_warps;
-    static constexpr int stages = ENDING == kSlopes && epilogue_warps == 16 ? 5 : 6;
-    static constexpr uint32_t store_bytes = ENDING == kSlopes ? epilogue_warps * kStoreBytes : 0;
+    static constexpr int stages = makes_slopes(ENDING) && epilogue_warps == 16 ? 5 : 6;
+    static constexpr uint32_t store_bytes = makes_slopes(ENDING) ? epilogue_warps * kStoreBytes : 0;
     static constexpr size_t smem = 1024 + (size_t)stages * kStageBytes + store_bytes + 256;
     static constexpr int column_parts = epilogue_warps / 4;  // of a tile, one per four warps
     static_assert(smem <= 227 * 1024, "shared memory of a block");
@@ -107,7 +108,6 @@ struct GemmArgs {
     uint32_t labels, dim;
     uint32_t products;     // 1, or more for operands in parts: those of the p-th product are the p-th hex
     uint32_t parts_a, parts_b;  // digits of these
-    uint32_t slope_parts;  // kSlopes
     uint32_t only_weight;  // kOut: so many first products are dW's alone
     uint32_t k_blocks;     // kStats, kSlopes: of the features' columns
     uint32_t n_tiles;      // kStats, kSlopes: of the labels
@@ -123,6 +123,7 @@ struct GemmArgs {
     float* target_logits;
     // kSlopes
     const double* log_normalizers;
+    double per_scale;      // log2(e) / scale2: a division in each tile's row took a tenth of a narrow pass
     const float* row_gradient;
     uint32_t panels;       // of 64 labels in a part of the slopes
     // bf16 operands: what rounding left of each row's target slope, by far the row's largest. dH takes it
@@ -320,9 +321,9 @@ __device__ __forceinline__ void add_logits(RowStats& s, float (&v)[W], uint32_t 
 }
 
 // The slopes of 32 logits of a row, in place (the target's only if PLACE); zeros past the labels and in rows that
-// do not count. The target's, if it is among them, also in `target_slope`: p - 1 from the difference of its logit and the
-// normalizer, since p itself may round to 1. The normalizer over the scale is `normalizer`, to f32's precision,
-// less shift_low / scale2.
+// do not count. The target's, if it is among them, also in `target_slope`: p - 1 from the difference of its logit
+// and the normalizer, since p itself may round to 1. The normalizer over the scale is `normalizer`, to f32's
+// precision, less shift_low / scale2.
 template <bool PLACE>
 __device__ __forceinline__ void to_slopes(float (&v)[32], uint32_t first, uint32_t labels, float scale2,
                                           float normalizer, float weight, uint32_t target, bool live,
@@ -610,8 +611,8 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
             if (ENDING != kOut && live) {
                 const uint32_t original = a.all_rows ? compact : a.row_of[compact];
                 if (a.targets) target = (uint32_t)index_at(a.targets, a.wide, original, a.labels);
-                if (ENDING == kSlopes) {
-                    const double exact = a.log_normalizers[original] * 1.4426950408889634 / a.scale2;
+                if (makes_slopes(ENDING)) {
+                    const double exact = a.log_normalizers[original] * a.per_scale;
                     normalizer = (float)exact;
                     shift_low = (float)(((double)normalizer - exact) * a.scale2);
                     weight = a.row_gradient ? a.scale * a.row_gradient[original] : 1.0f;
@@ -639,7 +640,7 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                         tc::barrier_arrive_cluster(PAIR ? tc::map_to_rank(drained + 8 * buffer, 0) : drained + 8 * buffer);
                 };
                 const uint32_t accumulator = tmem_at + buffer * kSide, columns_at = n * kSide + part * kSpan;
-                if constexpr (ENDING == kSlopes) {
+                if constexpr (makes_slopes(ENDING)) {
                     // 64 columns at a time: each part fills the warp's 32 x 64 tile, which a bulk copy
                     // writes out while the next is computed.
 #pragma unroll
@@ -655,16 +656,19 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                         };
                         if constexpr (sizeof(T) == 2) {
                             // A second part takes the slopes from the accumulator again: 64 of them and what
-                            // the first one left do not fit a thread's registers.
+                            // the first one left do not fit a thread's registers. A kernel of its own: as a
+                            // loop over an argument it made the pass with one part an eighth slower (9803 x
+                            // 12,379 x 28: 76 us, 67 without).
+                            constexpr int kSlopeParts = ENDING == kFineSlopes ? 2 : 1;
 #pragma unroll 1
-                            for (uint32_t p = 0; p < a.slope_parts; ++p) {
+                            for (int p = 0; p < kSlopeParts; ++p) {
 #pragma unroll
                                 for (int q = 0; q < 2; ++q) {
                                     float v[32];
                                     __syncwarp();
                                     tc::tmem_load32(accumulator + c + 32 * q, v);
                                     tc::tmem_load_wait();
-                                    if (q == 1 && c + 64 == kSpan && p + 1 == a.slope_parts) drain();
+                                    if (q == 1 && c + 64 == kSpan && p + 1 == kSlopeParts) drain();
                                     const uint32_t column = columns_at + c + 32 * q;
                                     float slope = 0.0f;
                                     to_slopes<false>(v, column, a.labels, a.scale2, normalizer, weight, target, live, shift_low, slope);
@@ -691,7 +695,7 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                             for (int q = 0; q < 2; ++q)
                                 to_slopes<true>(v[q], columns_at + c + 32 * q, a.labels, a.scale2, normalizer, weight, target,
                                                 live, shift_low, unused);
-                            for (int p = 0; p < (int)a.slope_parts; ++p) {
+                            for (int p = 0; p < (int)kParts; ++p) {
                                 reclaim();
                                 stage_part(stage_tile, lane, 0, v[0]);
                                 stage_part(stage_tile, lane, 1, v[1]);
@@ -761,7 +765,7 @@ __global__ void __launch_bounds__(Shape<ENDING, PAIR, T>::threads, 1)
                     a.target_logits[row] = stats.target_logit;
             }
         }
-        if (ENDING == kSlopes && lane == 0) tc::store_wait();
+        if (makes_slopes(ENDING) && lane == 0) tc::store_wait();
     }
     __syncwarp();
     if (!ok) {

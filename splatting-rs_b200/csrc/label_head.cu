@@ -23,7 +23,7 @@ using namespace splat;
 using namespace splat::label;
 
 namespace {
-constexpr uint64_t kFineSlopes = 1ull << 21;
+constexpr uint64_t kFewSlopes = 1ull << 21;
 }
 
 struct sp_label_head {
@@ -58,7 +58,7 @@ struct sp_label_head {
     // minus that, are all rounded the same way (1.1e-3 of the weight's gradient at 20,000 x 32,768 x 512, which
     // takes 2.3 ms with two parts and 1.5 with one).
     uint32_t slope_parts(uint64_t rows, bool own_factors) const {
-        return element == SP_F32 ? kParts : rows <= kTile || rows * labels <= kFineSlopes || own_factors ? 2 : 1;
+        return element == SP_F32 ? kParts : rows <= kTile || rows * labels <= kFewSlopes || own_factors ? 2 : 1;
     }
     uint64_t packed_stride() const { return ((uint64_t)dim + kBlockK - 1) / kBlockK * kBlockK; }
     uint64_t count_blocks() const { return (max_rows + 63) / 64; }
@@ -747,6 +747,7 @@ GemmArgs common_args(const sp_label_head* h, const void* targets, int wide, floa
     a.splits = 1;
     a.scale = scale;
     a.scale2 = scale2_for(scale, (h->dim + 15) / 16);
+    a.per_scale = 1.4426950408889634 / a.scale2;
     a.targets = targets;
     a.wide = wide;
     return a;
@@ -1005,13 +1006,13 @@ sp_status sp_label_head_gradient(sp_label_head* h, const void* d_features, int64
         a.log_normalizers = d_log_normalizers;
         a.row_gradient = d_row_gradient;
         a.panels = panels;
-        a.slope_parts = slope_parts;
         a.residuals = h->target_logits;  // free in a gradient
         const bool weight_here = in_place(h, d_weight, weight_stride);
         a.weight = weight_here ? static_cast<const bf16*>(d_weight) : h->packed_weight;
         a.weight_stride = weight_here ? weight_stride : (int64_t)h->packed_stride();
         SP_CUDA(ctx, h->element == SP_F32 ? (run_gemm<kSlopes, float>(h, logits.pair, logits.items(), op, slopes_out, a))
-                                          : (run_gemm<kSlopes, bf16>(h, logits.pair, logits.items(), op, slopes_out, a)));
+                     : slope_parts == 1   ? (run_gemm<kSlopes, bf16>(h, logits.pair, logits.items(), op, slopes_out, a))
+                                          : (run_gemm<kFineSlopes, bf16>(h, logits.pair, logits.items(), op, slopes_out, a)));
 
         if (slope_parts == 2) a.products = 2, a.only_weight = 1, a.parts_a = 0x01;  // the small part first
         OutArgs& f = a.out[0];
