@@ -4,6 +4,9 @@ workspace. Against plain 64-bit results, with the bounds of test_gpu_labels."""
 
 from __future__ import annotations
 
+import re
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -346,3 +349,44 @@ def test_entries_without_tokens_have_zero_rows_whatever_the_scale(ctx, n, scale,
     assert got[min(n, 7):].count_nonzero() == 0
     count = torch.bincount(tokens, minlength=entries)[: min(n, 7), None].float() * scale
     assert torch.equal(got[: min(n, 7)].nan_to_num(nan=7.0), count.to(dtype).expand(-1, dim).nan_to_num(nan=7.0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,labels,dim", [(5000, 150, 45), (3001, 4099, 64), (20_003, 257, 24), (700, 9000, 300)])
+def test_predict_of_many_rows(ctx, rows, labels, dim, dtype):
+    """As test_predict, at the sizes of a scene: several tiles of rows, labels cut into pieces or not."""
+    head = sb.LabelHead(ctx, labels, dim, dtype, rows, training=False)
+    features, weight = matrix(rows, dim, dtype, 1), matrix(labels, dim, dtype, 2)
+    b = Bounds(features, weight, None, 0.4)
+    got, log_probabilities = head.predict(features, weight, 0.4)
+    best = b.z.amax(1)
+    close(log_probabilities, best - b.normalizers, 2 * b.z_error + b.exp_error + 4 * A * b.normalizers.abs())
+    top = torch.topk(b.z, 2, 1).values
+    clear = top[:, 0] - top[:, 1] > 2 * b.z_error
+    assert clear.float().mean() > 0.9
+    assert torch.equal(got[clear].long(), b.z.argmax(1)[clear])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradient_beyond_the_budget_of_slopes(ctx, dtype):
+    """Rows past what the budget holds at once, whatever the budget is: the weight's gradient over the chunks."""
+    source = (Path(__file__).resolve().parents[1] / "splatting-rs_b200/csrc/label_head.cu").read_text()
+    factor, shift = re.search(r"kSlopeBudget = (\d+)ull << (\d+);", source).groups()
+    labels, dim, parts = 150_000, 16, 3 if dtype == torch.float32 else 1
+    limit = (int(factor) << int(shift)) // (-(-labels // 256) * 256 * parts) // 256 * 256
+    rows = limit + 300
+    head = sb.LabelHead(ctx, labels, dim, dtype, rows)
+    features, weight = matrix(rows, dim, dtype, 1), matrix(labels, dim, dtype, 2)
+    targets = tokens_for("some", rows, labels, torch.int32, 3)
+    loss = head.loss(features, weight, targets, 0.3)
+    to_features, to_weight = head.gradient(features, weight, targets, loss.log_normalizers, 0.3)
+    count = int(((targets >= 0) & (targets < labels)).sum())
+    want_weight = torch.zeros(labels, dim, dtype=torch.float64, device="cuda")
+    weight_error = torch.zeros_like(want_weight)
+    for first in range(0, rows, 500):
+        part = slice(first, min(rows, first + 500))
+        b = Bounds(features[part], weight, targets[part], 0.3, torch.full((part.stop - first,), 1.0 / count, device="cuda"))
+        want_weight += b.to_weight
+        weight_error += b.weight_error
+        close(to_features[part], b.to_features, b.features_error)
+    close(to_weight, want_weight, weight_error * 1.1)  # the chunks' sums add f32 roundings
