@@ -13,9 +13,9 @@
 // pair each block keeps 128 rows of A and of B and the accumulator of its A rows; the products are
 // issued by the first block and read B from both.
 //
-// Bound by the tensor cores: 20,000 rows x 32,768 labels x 512 bf16 take 380 us for the logits' sums (95 % of
-// the tensor pipe's cycles), 506 us for the slopes (71 %: 1.26 GB written, exponentials and roundings beside
-// the products) and 903 us for both gradients (93 %). Tiles of 256 x 256 per pair because a block's 128 x 128
+// Bound by the tensor cores: 20,000 rows x 32,768 labels x 512 bf16 take 397 us for the logits' sums (94 % of
+// the tensor pipe's cycles, at 1.50 GHz), 516 us for the slopes (71 %, at 1.52: 1.26 GB written, exponentials and
+// roundings beside the products) and 895 us for both gradients (92 %, at 1.35). Tiles of 256 x 256 per pair because a block's 128 x 128
 // reads twice the bytes per product from shared memory; the latter is for few rows or labels.
 #pragma once
 

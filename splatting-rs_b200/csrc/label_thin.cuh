@@ -5,7 +5,7 @@
 // its bf16 parts on the way into shared memory.
 //
 // One bf16 row against 65,536 labels of 512 takes 20 us, 67 MB at 3.3 TB/s: four tiles a block at most, so the
-// first copies' latency and the last tile's sums are a good part. 60 f32 rows against 20,011 labels of 768 take 32
+// first copies' latency and the last tile's sums are a good part. 60 f32 rows against 20,011 labels of 768 take 34
 // us for 62 MB: bound by the instructions of the conversion and its hand-over from stage to stage (without the
 // loads it takes 25).
 //
